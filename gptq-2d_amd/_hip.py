@@ -98,6 +98,19 @@ def lib() -> ctypes.CDLL:
         handle.gptq2d_trellis_pack.argtypes = [_P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P,
                                                _I64, _P, _P]
         handle.gptq2d_trellis_pack.restype = ctypes.c_int
+        cache = [_P, _I64, _I32, _I32, _I32]                       # pages, their count, heads, dim, page
+        tokens = [_P, _I64, _I64, _I64, _P, _P, _I64]              # table, seqs, width, row stride, lengths, offsets, tokens
+        for name in ("append", "read"):
+            fn = getattr(handle, f"gptq2d_kv_{name}")
+            fn.argtypes = [*cache, _P, _I64, _I64, _P, _I64, _I64, _I32, *tokens, _P]
+            fn.restype = ctypes.c_int
+        handle.gptq2d_kv_attend.argtypes = [*cache, _P, _I64, _I64, _I32, _I32, *tokens, _F64, _I64, _P, _I64, _I64, _P,
+                                            _P, _I64, _P]
+        handle.gptq2d_kv_attend.restype = ctypes.c_int
+        handle.gptq2d_kv_attend_workspace.argtypes = [_I64, _I64, _I32, _I32, _I32, _I64, _I64]
+        handle.gptq2d_kv_attend_workspace.restype = ctypes.c_int64
+        handle.gptq2d_kv_page_words.argtypes = [_I32, _I32, _I32]
+        handle.gptq2d_kv_page_words.restype = ctypes.c_int64
         handle.gptq2d_profile_start.argtypes = [_I64, ctypes.c_uint32]
         handle.gptq2d_profile_start.restype = ctypes.c_int
         handle.gptq2d_profile_read.argtypes = [_I32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),

@@ -1,0 +1,271 @@
+// Keys and values into the 4-bit cache (append) and back out of it (read).
+//
+// Both are bound by memory: a token's vectors are read (written) once, and 4.5 bits an element written (read).  A
+// workgroup takes one block of 32 tokens of one head, keys or values: the words of V hold eight tokens each, so the block
+// is the smallest part that no other workgroup of the call writes.  Eight threads take a token; codes go through LDS
+// into the words' order, so that whole blocks are written 16 bytes a thread in order.  In a block that is not all new
+// the words of K (one token each) and the scales of the new tokens are written alone, and in the words of V the new
+// tokens' nibbles replace the old.
+#include "kv_cache.h"
+
+namespace {
+
+constexpr int THREADS = 256;
+
+struct Rows {
+  void* k;
+  void* v;
+  int64_t k_token, k_head, v_token, v_head;  // strides in elements
+};
+
+struct BlockIds {
+  int64_t b, row0;  // row0: packed row of the block's token 0 (may be before the sequence's first)
+  int kb, first, last;  // block of the sequence, and its tokens [first, last) that the call takes
+  bool any;
+  int64_t t0, none0, none1, t1;  // rows of the sequence, those outside [none0, none1) without a place in the cache
+  bool leads;                    // the sequence's first slot
+};
+
+// Which block this workgroup takes; `back`: the lengths count the call's tokens already (read), else not (append).
+__device__ __forceinline__ BlockIds block_ids(const KvCache& c, int64_t slot, bool back) {
+  BlockIds id;
+  id.b = c.offsets ? kv_find(c, slot, 1, 32, 2) : slot;
+  const int64_t t0 = kv_offset(c, id.b), t1 = kv_offset(c, id.b + 1);
+  const int64_t most = (int64_t)c.width * c.page, n = t1 > t0 ? t1 - t0 : 0;
+  const int64_t held = c.lengths[id.b];
+  const int64_t start = back ? held - n : held;  // position of the first token
+  const int64_t begin = start < 0 ? 0 : start;
+  const int64_t end = start + n < most ? start + n : most;
+  const int64_t rel = c.offsets ? slot - kv_first_slot(c, id.b, 1, 32, 2) : 0;
+  const int64_t kb = begin / 32 + rel;
+  id.any = end > begin && kb * 32 < end;
+  id.kb = (int)kb;
+  id.first = (int)(begin > kb * 32 ? begin - kb * 32 : 0);
+  id.last = (int)(end < kb * 32 + 32 ? end - kb * 32 : 32);
+  id.row0 = t0 + kb * 32 - start;
+  id.t0 = t0, id.t1 = t0 + n;
+  id.none0 = end > begin ? t0 + begin - start : id.t1;
+  id.none1 = end > begin ? t0 + end - start : id.t1;
+  id.leads = rel == 0;
+  return id;
+}
+
+template <int TYPE, int ND>
+__global__ __launch_bounds__(THREADS) void append_kernel(KvCache c, Rows r) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr int DP = 64 * ND, PER = DP / 8;  // elements of a thread
+  alignas(16) __shared__ unsigned words[DP * 4];
+  __shared__ unsigned codes[32][DP / 4 + 1];  // V: codes of a token, a byte each
+  __shared__ unsigned affine[32];
+  const BlockIds id = block_ids(c, blockIdx.x, false);
+  if (!id.any) return;
+  const int h = blockIdx.y;
+  const bool value = blockIdx.z;
+  const int hw = (int)kv_head_words(ND, c.page);
+  int at;
+  unsigned* base = kv_head(c, id.b, id.kb, h, hw, at);
+  if (!base) return;
+  unsigned* out = base + (value ? (int64_t)c.page * 8 * ND : 0) + at * (DP * 4);
+  unsigned* out_affine = base + (int64_t)c.page * (16 * ND + (value ? 1 : 0)) + at * 32;
+
+  const int token = threadIdx.x >> 3, part = threadIdx.x & 7;
+  const bool mine = token >= id.first && token < id.last;
+  if (mine) {
+    const T* row = value ? (const T*)r.v + (id.row0 + token) * r.v_token + h * r.v_head
+                         : (const T*)r.k + (id.row0 + token) * r.k_token + h * r.k_head;
+    float x[PER];
+    load_row<TYPE, PER>(x, row, PER * part, c.dim);
+    // extremes; a NaN stays, and makes scale and zero NaN
+    float lo = PER * part < c.dim ? x[0] : __builtin_inff();
+    float hi = PER * part < c.dim ? x[0] : -__builtin_inff();
+#pragma unroll
+    for (int i = 1; i < PER; ++i) {
+      const bool in = PER * part + i < c.dim;
+      lo = in && (x[i] < lo || x[i] != x[i]) ? x[i] : lo;
+      hi = in && (x[i] > hi || x[i] != x[i]) ? x[i] : hi;
+    }
+#pragma unroll
+    for (int s = 1; s < 8; s *= 2) {
+      const float l2 = __shfl_xor(lo, s), h2 = __shfl_xor(hi, s);
+      lo = l2 < lo || l2 != l2 ? l2 : lo;
+      hi = h2 > hi || h2 != h2 ? h2 : hi;
+    }
+    float s = round_to_bf16((hi - lo) / 15.f);
+    s = s == 0.f ? 1.f : s;
+    const float z = round_to_bf16(lo);
+    if (part == 0) affine[token] = __float_as_uint(s) >> 16 | (__float_as_uint(z) & 0xffff0000u);
+    unsigned code[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      float q = round_even((x[i] - z) / s);
+      q = q > 0.f ? q : 0.f;  // also for a NaN
+      code[i] = (unsigned)(q < 15.f ? q : 15.f);
+    }
+    if (value) {
+#pragma unroll
+      for (int i = 0; i < PER; i += 4)
+        codes[token][(PER * part + i) / 4] = code[i] | code[i + 1] << 8 | code[i + 2] << 16 | code[i + 3] << 24;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; i += 8) {
+        const int d = PER * part + i, lane = token % 16 + 16 * (d / 8 % 4), W = 2 * ND * (token / 16) + d / 32;
+        unsigned w = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w |= code[i + e] << (e / 2 * 4 + e % 2 * 16);
+        words[W / 4 * 256 + lane * 4 + W % 4] = w;
+      }
+    }
+  }
+  __syncthreads();
+  const bool whole = id.first == 0 && id.last == 32;
+  if (threadIdx.x < 32 && (int)threadIdx.x >= id.first && (int)threadIdx.x < id.last)
+    out_affine[threadIdx.x] = affine[threadIdx.x];
+  if (!value) {
+    if (whole) {
+#pragma unroll
+      for (int i = threadIdx.x; i < DP; i += THREADS)
+        reinterpret_cast<uint4v*>(out)[i] = reinterpret_cast<const uint4v*>(words)[i];
+    } else {
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        const int i = THREADS * j + threadIdx.x, W = i / 256 * 4 + i % 4, key = W / (2 * ND) * 16 + i / 4 % 16;
+        if (key >= id.first && key < id.last) out[i] = words[i];
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < ND; ++j) {  // DP * 4 = THREADS * ND words
+    const int i = THREADS * j + threadIdx.x, lane = i / 4 % 64, d = 16 * (i / 256 * 4 + i % 4) + lane % 16, g = lane / 16;
+    unsigned w = 0, keep = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int token_e = 4 * g + e % 4 + e / 4 * 16, shift = e / 2 * 4 + e % 2 * 16;
+      const bool fresh = token_e >= id.first && token_e < id.last;
+      const unsigned code = codes[token_e][d / 4] >> (d % 4 * 8) & 15u;  // of an old token: whatever LDS holds
+      w |= (fresh ? code : 0u) << shift;
+      keep |= (fresh ? 0u : 15u) << shift;
+    }
+    const unsigned old = whole ? 0u : out[i];
+    out[i] = w | (old & keep);
+  }
+}
+
+template <int TYPE, int ND>
+__global__ __launch_bounds__(THREADS) void read_kernel(KvCache c, Rows r) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr int DP = 64 * ND;
+  const BlockIds id = block_ids(c, blockIdx.x, true);
+  const int h = blockIdx.y;
+  const bool value = blockIdx.z;
+  T* out = value ? (T*)r.v + h * r.v_head : (T*)r.k + h * r.k_head;
+  const int64_t stride = value ? r.v_token : r.k_token;
+  if (id.leads && (id.none0 > id.t0 || id.none1 < id.t1)) {  // tokens that the cache cannot hold: zeros
+    for (int64_t row = id.t0; row < id.t1; ++row)
+      if (row < id.none0 || row >= id.none1)
+        for (int d = threadIdx.x; d < c.dim; d += THREADS) out[row * stride + d] = from_f32<TYPE>(0.f);
+  }
+  if (!id.any) return;
+  const int hw = (int)kv_head_words(ND, c.page);
+  int at;
+  const unsigned* base = kv_head(c, id.b, id.kb, h, hw, at);
+  const unsigned* in = base + (value ? (int64_t)c.page * 8 * ND : 0) + at * (DP * 4);
+  const unsigned* in_affine = base + (int64_t)c.page * (16 * ND + (value ? 1 : 0)) + at * 32;
+#pragma unroll
+  for (int j = 0; j < ND; ++j) {  // a word a thread and turn; where the table's entry is no page, zeros
+    const int i = THREADS * j + threadIdx.x, W = i / 256 * 4 + i % 4, lane = i / 4 % 64, g = lane / 16;
+    const int key = W / (2 * ND) * 16 + lane % 16;
+    unsigned w = 0, a[8] = {};
+    if (base) {
+      w = in[i];
+      if (value) {
+        const uint4v a0 = *reinterpret_cast<const uint4v*>(in_affine + 4 * g);
+        const uint4v a1 = *reinterpret_cast<const uint4v*>(in_affine + 4 * g + 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = a0[e], a[e + 4] = a1[e];
+      } else {
+        a[0] = in_affine[key];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) a[e] = a[0];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int token = value ? 4 * g + e % 4 + e / 4 * 16 : key;
+      const int d = value ? 16 * W + lane % 16 : 32 * (W % (2 * ND)) + 8 * g + e;
+      const float x = __builtin_fmaf((float)(w >> (e / 2 * 4 + e % 2 * 16) & 15u), __uint_as_float(a[e] << 16),
+                                     __uint_as_float(a[e] & 0xffff0000u));
+      if (token >= id.first && token < id.last && d < c.dim) out[(id.row0 + token) * stride + d] = from_f32<TYPE>(x);
+    }
+  }
+}
+
+template <int TYPE>
+int launch(bool back, const KvCache& c, const Rows& r, int nd, hipStream_t st) {
+  const int64_t slots = c.offsets ? c.tokens / 32 + 2 * c.seqs : c.seqs;
+  if (slots > 0x7fffffff) return GPTQ2D_EUNSUPPORTED;
+  const dim3 grid((unsigned)slots, (unsigned)c.heads, 2);
+#define GPTQ2D_KV_CASE(ND)                                                             \
+  case ND:                                                                             \
+    if (back)                                                                          \
+      hipLaunchKernelGGL((read_kernel<TYPE, ND>), grid, dim3(THREADS), 0, st, c, r);   \
+    else                                                                               \
+      hipLaunchKernelGGL((append_kernel<TYPE, ND>), grid, dim3(THREADS), 0, st, c, r); \
+    break;
+  switch (nd) {
+    GPTQ2D_KV_CASE(1)
+    GPTQ2D_KV_CASE(2)
+    GPTQ2D_KV_CASE(3)
+    GPTQ2D_KV_CASE(4)
+  }
+#undef GPTQ2D_KV_CASE
+  return (int)hipGetLastError();
+}
+
+int run(bool back, int32_t type, const KvCache& c, const Rows& r, hipStream_t st) {
+  const int nd = (c.dim + 63) / 64;
+  switch (type) {
+    case TYPE_F32:
+      return launch<TYPE_F32>(back, c, r, nd, st);
+    case TYPE_BF16:
+      return launch<TYPE_BF16>(back, c, r, nd, st);
+    case TYPE_F16:
+      return launch<TYPE_F16>(back, c, r, nd, st);
+  }
+  return GPTQ2D_EINVAL;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t gptq2d_kv_page_words(int32_t heads, int32_t dim, int32_t page) {
+  if (heads < 1 || heads > 65535 || dim < 1 || dim > 256 || page < 32 || page > 4096 || page % 32) return -1;
+  return heads * kv_head_words((dim + 63) / 64, page);
+}
+
+int gptq2d_kv_append(void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, const void* k,
+                     int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int32_t type,
+                     const int32_t* table, int64_t seqs, int64_t width, int64_t table_stride, const int32_t* lengths,
+                     const int32_t* offsets, int64_t tokens, void* stream) {
+  KvCache c;
+  if (!make_cache(c, pages, page_count, heads, dim, page, table, seqs, width, table_stride, lengths, offsets, tokens))
+    return GPTQ2D_EINVAL;
+  if (tokens == 0 || seqs == 0 || width == 0 || page_count == 0) return 0;
+  const Rows r = {const_cast<void*>(k), const_cast<void*>(v), k_token, k_head, v_token, v_head};
+  return run(false, type, c, r, (hipStream_t)stream);
+}
+
+int gptq2d_kv_read(const void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, void* k,
+                   int64_t k_token, int64_t k_head, void* v, int64_t v_token, int64_t v_head, int32_t type,
+                   const int32_t* table, int64_t seqs, int64_t width, int64_t table_stride, const int32_t* lengths,
+                   const int32_t* offsets, int64_t tokens, void* stream) {
+  KvCache c;
+  if (!make_cache(c, pages, page_count, heads, dim, page, table, seqs, width, table_stride, lengths, offsets, tokens))
+    return GPTQ2D_EINVAL;
+  if (tokens == 0 || seqs == 0) return 0;
+  const Rows r = {k, v, k_token, k_head, v_token, v_head};
+  return run(true, type, c, r, (hipStream_t)stream);
+}
+
+}  // extern "C"

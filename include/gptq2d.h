@@ -304,6 +304,48 @@ GPTQ2D_DECLARE(double, f64)
 
 #undef GPTQ2D_DECLARE
 
+/* The paged cache of keys and values in 4 bits, and attention over it (no reference counterpart: the reference
+ * quantizes weights).  A token's key or value vector x of one head is held as codes c in 0..15 with s = bf16((max x -
+ * min x) / 15), 1 where that is 0, and z = bf16(min x): c = clamp(rint((x - z) / s), 0, 15), each step in fp32; it
+ * stands for c s + z (a vector with an infinity or a NaN for NaN).
+ *
+ * pages: page_count pages of gptq2d_kv_page_words(heads, dim, page) 32-bit words, 16-byte aligned, what they hold at
+ * first is never used.  heads: kv heads; dim: 1 to 256; page: tokens of a page, a multiple of 32, at most 4096.
+ * table[seqs][width] (rows table_stride apart): the pages of each sequence, in order; an entry that is no page holds
+ * no token (nothing is written there, read as zeros, attended to by nobody).  The page that a call appends to belongs
+ * to one sequence; full pages may be shared.  lengths[seqs]: tokens of each sequence, at most width page of which are
+ * there.  offsets[seqs + 1]: sequence b's tokens of the call are the packed rows offsets[b] .. offsets[b + 1] - 1 of
+ * `tokens`; NULL: one each (tokens == seqs).  Arrays are in device memory.  *_token and *_head: strides in elements of
+ * a packed [tokens, heads, dim] operand whose last axis is contiguous.  type 0: fp32, 1: bf16, 2: fp16. */
+int64_t gptq2d_kv_page_words(int32_t heads, int32_t dim, int32_t page); /* -1 for sizes it does not take */
+
+/* The call's keys and values into the cache, at positions lengths[b], lengths[b] + 1, ... */
+int gptq2d_kv_append(void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, const void* k,
+                     int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head, int32_t type,
+                     const int32_t* table, int64_t seqs, int64_t width, int64_t table_stride, const int32_t* lengths,
+                     const int32_t* offsets, int64_t tokens, void* stream);
+
+/* The values that the last tokens of each sequence stand for: those up to lengths[b] - 1.  Rows without a token in the
+ * cache (more than the sequence holds) are zeros. */
+int gptq2d_kv_read(const void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, void* k,
+                   int64_t k_token, int64_t k_head, void* v, int64_t v_token, int64_t v_head, int32_t type,
+                   const int32_t* table, int64_t seqs, int64_t width, int64_t table_stride, const int32_t* lengths,
+                   const int32_t* offsets, int64_t tokens, void* stream);
+
+/* Attention of the call's tokens, the last ones of each sequence (query i of T_b is at position lengths[b] - T_b + i):
+ *   out = sum_j softmax_j(scale q . k_j) v_j over the tokens j <= its position and, with window > 0, j > position - window.
+ * q, out: [tokens, heads group, dim], query head h on kv head h / group.  lse (optional, [tokens, heads group]): the
+ * natural logarithm of sum_j exp(scale q . k_j).  A query that sees no token gives zeros and -inf.  work: 16-byte aligned,
+ * gptq2d_kv_attend_workspace bytes (`most`: width page), its contents of no use afterwards; GPTQ2D_ESCRATCH where it is
+ * smaller. */
+int64_t gptq2d_kv_attend_workspace(int64_t tokens, int64_t seqs, int32_t heads, int32_t group, int32_t dim, int64_t most,
+                                   int64_t window);
+int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, const void* q,
+                     int64_t q_token, int64_t q_head, int32_t group, int32_t type, const int32_t* table, int64_t seqs,
+                     int64_t width, int64_t table_stride, const int32_t* lengths, const int32_t* offsets, int64_t tokens,
+                     double scale, int64_t window, void* out, int64_t out_token, int64_t out_head, float* lse, void* work,
+                     int64_t work_bytes, void* stream);
+
 /* Launch profiler (no reference counterpart; the reference times with host clocks, demo.ipynb:109-118).
  * While on, every launch of a profiled kernel class is bracketed with HIP events on its stream.
  * Process-global, not thread-safe, not for use under stream capture.

@@ -1,0 +1,375 @@
+"""GPU tests of the 4-bit cache of keys and values (kv_cache.py over csrc/kv_append.hip and csrc/kv_attend.hip) against
+its definition in 64 bits on the CPU.
+
+Append and read: the values read back equal the definition's bit for bit (every step of it is a single fp32 operation).
+Attention: head sizes that fill their tiles and not, one query to many, shared heads, windows, ragged lengths, lengths
+of 0 and 1, fewer tokens held than asked, pages in any order; stale pages, infinities and NaN where nothing may look.
+
+Tolerance of attention, from the kernel's roundings: the result's own (half a unit in the last place is at most 2^-8 of it
+for bf16, 2^-11 fp16, 2^-24 fp32), plus, of the largest value held: 2^-11 for bf16 (weights held to 11 bits are off by at
+most 2^-11 of p s |c - 8|, and s |c - 8| is at most 8/15 of the values' spread, itself at most twice the largest; all of
+them off by as much in one direction does not happen), and 3e-5 otherwise (scores of up to
+about 16 as sums of `dim` <= 256 terms in fp32: 16 x 2^-24 x sqrt(256) x 2 = 3e-5 of relative change in a weight)."""
+
+import math
+
+import pytest
+import torch
+
+import _hip
+from kv_cache import KVCache4
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+OWN = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+OF_VALUES = {torch.float32: 3e-5, torch.bfloat16: 2.0 ** -11, torch.float16: 3e-5}
+
+
+def held_values(x):
+    """What x [..., dim] is held as: (c s + z) in 64 bits, from its definition."""
+    x = x.float()
+    lo, hi = x.amin(-1, keepdim=True), x.amax(-1, keepdim=True)
+    s = ((hi - lo) / torch.tensor(15.)).to(torch.bfloat16).float()
+    s = torch.where(s == 0, torch.ones_like(s), s)
+    z = lo.to(torch.bfloat16).float()
+    c = ((x - z) / s).round().clamp(0, 15)
+    return c.double() * s.double() + z.double()
+
+
+class Sequences:
+    """Ragged sequences on the host, their cache on the GPU, filled by appends of the given pieces."""
+
+    def __init__(self, held, hkv, dim, dtype, page=32, seed=0, spare=2, pieces=1, k=None, v=None):
+        g = torch.Generator().manual_seed(seed)
+        self.held, self.hkv, self.dim, self.dtype, self.page, self.g = held, hkv, dim, dtype, page, g
+        total = sum(held)
+        mix = torch.randn(hkv, dim, generator=g)
+        self.k = ((torch.randn(total, hkv, dim, generator=g) + mix) if k is None else k).to(dtype)
+        self.v = ((torch.randn(total, hkv, dim, generator=g) - mix) if v is None else v).to(dtype)
+        blocks = [-(-h // page) for h in held]
+        self.pages = sum(blocks) + spare
+        order = torch.randperm(self.pages, generator=g).to(torch.int32)
+        self.table = torch.full((len(held), max(max(blocks), 1)), -7, dtype=torch.int32)
+        at = 0
+        for b, n in enumerate(blocks):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+        self.cache = KVCache4(self.pages, hkv, dim, page_size=page, device=DEV)
+        self.cache.pages.fill_(-1)  # every stale scale and zero a NaN
+        self.starts = [0]
+        for h in held:
+            self.starts.append(self.starts[-1] + h)
+        self.dev_table = self.table.to(DEV)
+        for piece in range(pieces):
+            lo = [h * piece // pieces for h in held]
+            hi = [h * (piece + 1) // pieces for h in held]
+            rows = torch.cat([torch.arange(s + a, s + e) for s, a, e in zip(self.starts, lo, hi)])
+            counts = torch.tensor([0] + [e - a for a, e in zip(lo, hi)]).cumsum(0).to(torch.int32)
+            self.cache.append(self.k[rows].to(DEV), self.v[rows].to(DEV), self.dev_table,
+                              torch.tensor(lo, dtype=torch.int32, device=DEV), counts.to(DEV))
+
+    def lengths(self):
+        return torch.tensor(self.held, dtype=torch.int32, device=DEV)
+
+    def reference(self, q, new, scale, window):
+        """(out, lse) in 64 bits."""
+        kv, vv = held_values(self.k), held_values(self.v)
+        group = q.size(1) // self.hkv
+        out = torch.zeros(q.shape, dtype=torch.float64)
+        lse = torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
+        r = 0
+        for b, t in enumerate(new):
+            h, s = self.held[b], self.starts[b]
+            for i in range(t):
+                p = h - t + i
+                first = max(0, p - window + 1) if window else 0
+                if p >= first and p >= 0:
+                    kk = kv[s + first:s + p + 1].repeat_interleave(group, 1)
+                    vw = vv[s + first:s + p + 1].repeat_interleave(group, 1)
+                    z = torch.einsum("hd,nhd->hn", q[r].double(), kk) * scale
+                    lse[r] = torch.logsumexp(z, -1)
+                    out[r] = torch.einsum("hn,nhd->hd", torch.softmax(z, -1), vw)
+                r += 1
+        return out, lse
+
+
+def check(got, want, biggest, dtype):
+    allowed = want.abs() * OWN[dtype] * 1.01 + torch.finfo(dtype).tiny + OF_VALUES[dtype] * biggest
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= allowed).all()), f"off by {float((off / allowed).max()):.3g} of what is allowed"
+
+
+def starts(counts):
+    return torch.tensor([0] + counts).cumsum(0).to(torch.int32).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,hkv,page", [(128, 2, 32), (64, 1, 64), (80, 3, 96), (256, 1, 32), (192, 2, 64), (1, 2, 32),
+                                          (33, 1, 32), (250, 1, 128)])
+def test_append_and_read(dtype, dim, hkv, page):
+    print(f"append {dtype} dim {dim} heads {hkv} page {page}", flush=True)
+    held = [0, 1, 31, 32, 33, 100, 257, 64]
+    for pieces in (1, 5):
+        s = Sequences(held, hkv, dim, TYPES[dtype], page, seed=dim, pieces=pieces)
+        k, v = s.cache.read(s.dev_table, s.lengths(), starts(held), tokens=sum(held))
+        assert torch.equal(k.cpu().double(), held_values(s.k))
+        assert torch.equal(v.cpu().double(), held_values(s.v))
+
+
+def test_append_one_token_each_and_neighbours_stay():
+    """Decode steps: a token a sequence, without offsets; what was there stays as it is."""
+    held = [5, 31, 32, 63, 0]
+    s = Sequences(held, 2, 128, torch.bfloat16, 32, seed=3, spare=20)
+    table = torch.cat([s.table, torch.full((5, 2), -1, dtype=torch.int32)], 1)
+    free = [p for p in range(s.pages) if p not in set(s.table.flatten().tolist())]
+    for b, h in enumerate(held):
+        for w in range(-(-h // 32), -(-(h + 8) // 32)):
+            table[b, w] = free.pop()
+    table = table.to(DEV)
+    ks = [list(s.k[a:b]) for a, b in zip(s.starts, s.starts[1:])]
+    vs = [list(s.v[a:b]) for a, b in zip(s.starts, s.starts[1:])]
+    g = torch.Generator().manual_seed(1)
+    lengths = s.lengths()
+    for step in range(8):
+        k, v = (torch.randn(5, 2, 128, generator=g).bfloat16() for _ in range(2))
+        s.cache.append(k.to(DEV), v.to(DEV), table, lengths)
+        lengths += 1
+        for b in range(5):
+            ks[b].append(k[b])
+            vs[b].append(v[b])
+    counts = [len(x) for x in ks]
+    k, v = s.cache.read(table, lengths, starts(counts), tokens=sum(counts))
+    assert torch.equal(k.cpu().double(), held_values(torch.stack(sum(ks, []))))
+    assert torch.equal(v.cpu().double(), held_values(torch.stack(sum(vs, []))))
+
+
+def test_append_special_vectors():
+    """Constant vectors, zeros, the type's extremes; infinities and NaN make their own vector NaN and no other."""
+    rows = torch.randn(12, 1, 64, generator=torch.Generator().manual_seed(0))
+    rows[1] = 0.
+    rows[2] = 3.25
+    rows[3] = -1e-30
+    rows[4, 0, 5] = 3e38
+    rows[5] *= 1e-38
+    rows[6, 0, 7] = math.inf
+    rows[7, 0, 0] = math.nan
+    rows[8, 0, 63] = -math.inf
+    rows[9, 0, 63] = math.nan
+    s = Sequences([12], 1, 64, torch.float32, 32, k=rows, v=rows.flip(0))
+    k, v = s.cache.read(s.dev_table, s.lengths(), starts([12]), tokens=12)
+    want = held_values(rows)
+    bad = torch.tensor([6, 7, 8, 9])
+    good = torch.tensor([0, 1, 2, 3, 4, 5, 10, 11])
+    assert torch.equal(k.cpu().double()[good], want[good]) and torch.equal(v.cpu().flip(0).double()[good], want[good])
+    assert bool(k.cpu()[bad].isnan().all()) and bool(v.cpu().flip(0)[bad].isnan().all())
+
+
+def test_read_rows_without_a_token():
+    s = Sequences([3, 40, 0], 2, 64, torch.float16, 32, seed=4)
+    k, v = s.cache.read(s.dev_table, s.lengths(), starts([5, 2, 3]), tokens=10, dtype=torch.float16)
+    for got, x in ((k, s.k), (v, s.v)):
+        want = held_values(x).to(torch.float16)
+        assert torch.equal(got.cpu()[2:5], want[:3]) and torch.equal(got.cpu()[5:7], want[41:43])
+        assert not got.cpu()[[0, 1, 7, 8, 9]].any()
+
+
+CASES = [  # held, new, kv heads, group, dim, page, window
+    ([1000], [1], 2, 4, 128, 64, None),
+    ([0, 1, 31, 32, 33, 500, 1025], [1] * 7, 2, 8, 128, 32, None),
+    ([0, 1, 31, 32, 33, 500, 1025], [1] * 7, 1, 1, 64, 32, None),
+    ([40, 300, 2], [5, 5, 5], 2, 3, 80, 32, None),          # fewer tokens held than asked in the last
+    ([700, 64, 129], [3, 64, 40], 2, 2, 128, 96, None),
+    ([700, 64, 129, 0], [3, 64, 40, 2], 1, 5, 96, 32, 17),
+    ([900, 33], [1, 1], 1, 16, 256, 32, 33),
+    ([900, 33], [20, 2], 1, 20, 128, 32, 1),
+    ([600], [1], 1, 71, 64, 32, None),                       # more heads than a tile has columns
+    ([300, 2, 4000], [0, 1, 1], 2, 2, 192, 32, 1000),        # a sequence without a query
+    ([257], [257], 2, 2, 128, 32, None),
+    ([77, 12], [3, 2], 3, 1, 33, 32, None),
+    ([40000, 700], [1, 1], 1, 4, 128, 128, None),            # chunks that are joined
+    ([3000], [150], 1, 8, 128, 64, 500),
+]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attend(case, dtype):
+    held, new, hkv, group, dim, page, window = CASES[case]
+    print(f"attend case {case} {dtype}", flush=True)
+    dt = TYPES[dtype]
+    s = Sequences(held, hkv, dim, dt, page, seed=case)
+    q = torch.randn(sum(new), hkv * group, dim, generator=s.g).to(dt)
+    scale = dim ** -0.5
+    want, want_lse = s.reference(q, new, scale, window)
+    offsets = None if new == [1] * len(new) else starts(new)
+    got, lse = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), offsets, window=window, return_lse=True)
+    assert got.dtype is dt and got.shape == q.shape
+    check(want.to(dt), want, 0., dt)  # the tolerance admits the result itself, rounded once
+    check(got, want, float(held_values(s.v).abs().max()), dt)
+    empty = want_lse == -math.inf
+    assert torch.equal(lse.cpu() == -math.inf, empty) and not got.cpu()[empty].any()
+    off = (lse.cpu().double() - want_lse)[~empty].abs()
+    assert off.numel() == 0 or float(off.max()) < 1e-4
+
+
+def test_attend_large_scores_and_scales():
+    """Scores of hundreds, values whose scales differ by 2^40, tiny and large queries."""
+    g = torch.Generator().manual_seed(8)
+    k = torch.randn(700, 1, 128, generator=g) * 4
+    v = torch.randn(700, 1, 128, generator=g) * torch.logspace(-6, 6, 700).view(-1, 1, 1)
+    for size in (1e-20, 1e-3, 8., 1e4):
+        s = Sequences([700], 1, 128, torch.float32, 32, k=k, v=v)
+        q = torch.randn(1, 4, 128, generator=g) * size
+        want, _ = s.reference(q, [1], 128 ** -0.5, None)
+        got = s.cache.attend(q.to(DEV), s.dev_table, s.lengths())
+        # a weight is off by its score's error: fp32 sums of terms as large as the scores themselves
+        top = float((q.double().abs().max() * 4 * 4 * 128 ** 0.5))
+        allowed = want.abs() * 2e-6 + float(held_values(s.v).abs().max()) * min(1., max(3e-5, top * 3e-6))
+        assert bool(((got.cpu().double() - want).abs() <= allowed).all())
+
+
+def test_nan_and_infinity_where_nothing_looks():
+    """A token whose key or value is NaN or infinite changes the queries that see it and no others."""
+    for what in (math.nan, math.inf, -math.inf):
+        for which in ("k", "v"):
+            g = torch.Generator().manual_seed(2)
+            k, v = torch.randn(400, 2, 128, generator=g), torch.randn(400, 2, 128, generator=g)
+            clean = Sequences([400], 2, 128, torch.bfloat16, 32, k=k.clone(), v=v.clone())
+            bad = {"k": k, "v": v}[which]
+            bad[390, 1, 17] = what
+            dirty = Sequences([400], 2, 128, torch.bfloat16, 32, k=k, v=v)
+            q = torch.randn(60, 8, 128, generator=g).bfloat16().to(DEV)
+            for window in (None, 4):
+                a = clean.cache.attend(q, clean.dev_table, clean.lengths(), starts([60]), window=window).cpu()
+                b = dirty.cache.attend(q, dirty.dev_table, dirty.lengths(), starts([60]), window=window).cpu()
+                sees = torch.zeros(60, dtype=torch.bool)
+                sees[50:54 if window else 60] = True
+                assert torch.equal(a[:, :4], b[:, :4]), "the other kv head"
+                assert torch.equal(a[~sees], b[~sees]), "queries that do not see the token"
+                assert bool(b[sees][:, 4:].isnan().all())
+
+
+def test_pages_that_are_none_and_lengths_past_the_table():
+    """Entries outside the pool hold no token; lengths beyond the table's pages end there."""
+    s = Sequences([96, 64], 1, 64, torch.float32, 32, seed=5)
+    q = torch.randn(2, 2, 64, generator=s.g)
+    table = s.table.clone()
+    table[0, 1] = s.pages + 5
+    table[1, 2] = -1
+    got = s.cache.attend(q.to(DEV), table.to(DEV), torch.tensor([96, 500], dtype=torch.int32, device=DEV))
+    kv, vv = held_values(s.k), held_values(s.v)
+    keep = torch.cat([torch.arange(32), torch.arange(64, 96)])
+    for b, rows in ((0, keep), (1, torch.arange(96, 160))):
+        z = q[b].double() @ kv[rows, 0].t() / 8
+        check(got[b], torch.softmax(z, -1) @ vv[rows, 0], float(vv.abs().max()), torch.float32)
+    before = s.cache.pages.clone()
+    new = torch.randn(2, 1, 64)
+    s.cache.append(new.to(DEV), new.to(DEV), table.to(DEV), torch.tensor([40, 96], dtype=torch.int32, device=DEV))
+    assert torch.equal(before, s.cache.pages), "appends without a page write nothing"
+
+
+def test_strided_operands():
+    """q, k, v as slices of one projection's output, and with heads and tokens in the other order."""
+    g = torch.Generator().manual_seed(6)
+    t, hq, hkv, dim = 37, 6, 2, 72
+    qkv = torch.randn(t, (hq + 2 * hkv) * dim + 3, generator=g).bfloat16().to(DEV)[:, 1:-2]
+    q = qkv[:, :hq * dim].view(t, hq, dim)
+    k = qkv[:, hq * dim:(hq + hkv) * dim].view(t, hkv, dim)
+    v = qkv[:, (hq + hkv) * dim:].view(t, hkv, dim).transpose(0, 1).contiguous().transpose(0, 1)
+    table = torch.tensor([[2, 0]], dtype=torch.int32, device=DEV)
+    none, held = torch.zeros(1, dtype=torch.int32, device=DEV), torch.full((1,), t, dtype=torch.int32, device=DEV)
+    outs = []
+    for dense in (False, True):
+        cache = KVCache4(3, hkv, dim, page_size=32, device=DEV)
+        a, b, c = (x.contiguous() if dense else x for x in (q, k, v))
+        cache.append(b, c, table, none, starts([t]))
+        outs.append(cache.attend(a, table, held, starts([t])))
+    assert torch.equal(*outs)
+
+
+def test_other_stream_and_graph():
+    """On a stream of the caller's, and in a graph replayed with other lengths (over tokens that are held) and other tokens, eager work between."""
+    s = Sequences([200, 90], 2, 128, torch.float16, 32, seed=7, spare=4)
+    table = torch.cat([s.table, torch.zeros(2, 1, dtype=torch.int32)], 1)
+    free = [p for p in range(s.pages) if p not in set(s.table.flatten().tolist())]
+    table[0, 7], table[1, 3] = free[0], free[1]
+    table = table.to(DEV)
+    g = torch.Generator().manual_seed(3)
+    k, v, q = (torch.randn(2, h, 128, generator=g).half().to(DEV) for h in (2, 2, 8))
+    held = s.lengths()
+    after = held + 1
+    start = s.cache.pages.clone()
+
+    def step():
+        s.cache.append(k, v, table, held)
+        return s.cache.attend(q, table, after)
+
+    want = step().clone()
+    s.cache.pages.copy_(start)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for turn in range(4):
+        k.normal_(), v.normal_(), q.normal_()
+        held.sub_(3), after.sub_(3)
+        s.cache.pages.copy_(start)
+        want = step().clone()
+        s.cache.pages.copy_(start)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), turn
+
+
+def test_nothing_to_do():
+    cache = KVCache4(2, 1, 64, page_size=32, device=DEV)
+    table = torch.zeros(0, 1, dtype=torch.int32, device=DEV)
+    none = torch.zeros(0, dtype=torch.int32, device=DEV)
+    empty = torch.empty(0, 1, 64, device=DEV)
+    cache.append(empty, empty, table, none)
+    assert cache.attend(empty, table, none).shape == (0, 1, 64)
+    assert cache.read(table, none)[0].shape == (0, 1, 64)
+    out = cache.attend(torch.ones(1, 1, 64, device=DEV), torch.zeros(1, 0, dtype=torch.int32, device=DEV),
+                       torch.ones(1, dtype=torch.int32, device=DEV))
+    assert not out.any()
+
+
+def test_refusals():
+    with pytest.raises(ValueError):
+        KVCache4(4, 1, 64, page_size=48, device=DEV)
+    with pytest.raises(ValueError):
+        KVCache4(4, 1, 257, device=DEV)
+    with pytest.raises(_hip.GPTQ2DError):
+        KVCache4(4, 1, 64, device="cpu")
+    cache = KVCache4(4, 2, 64, page_size=32, device=DEV)
+    table = torch.zeros(3, 2, dtype=torch.int32, device=DEV)
+    lengths = torch.zeros(3, dtype=torch.int32, device=DEV)
+    k = torch.zeros(3, 2, 64, device=DEV)
+    bad = [
+        lambda: cache.append(k, k[:2], table, lengths),
+        lambda: cache.append(k, k.half(), table, lengths),
+        lambda: cache.append(k.double(), k.double(), table, lengths),
+        lambda: cache.append(k[:, :1], k[:, :1], table, lengths),
+        lambda: cache.append(k, k, table.long(), lengths),
+        lambda: cache.append(k, k, table, lengths[:2]),
+        lambda: cache.append(k, k, table, lengths.cpu()),
+        lambda: cache.append(k[:2], k[:2], table, lengths),                       # two tokens, three sequences
+        lambda: cache.append(k, k, table, lengths, lengths),                      # three offsets for three sequences
+        lambda: cache.append(k, k, table.t().contiguous().t(), lengths),
+        lambda: cache.attend(torch.zeros(3, 3, 64, device=DEV), table, lengths),  # three heads on two
+        lambda: cache.attend(torch.zeros(3, 4, 65, device=DEV), table, lengths),
+        lambda: cache.attend(torch.zeros(3, 4, 64, device=DEV), table, lengths, window=0),
+        lambda: cache.attend(torch.zeros(3, 4, 64), table, lengths),
+        lambda: cache.read(table, lengths, torch.zeros(4, dtype=torch.int32, device=DEV)),
+        lambda: cache.read(table, lengths, dtype=torch.float64),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
