@@ -98,6 +98,12 @@ def lib() -> ctypes.CDLL:
         handle.gptq2d_trellis_pack.argtypes = [_P, _I64, _I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _P,
                                                _I64, _P, _P]
         handle.gptq2d_trellis_pack.restype = ctypes.c_int
+        handle.gptq2d_packed_linear.argtypes = [_P, _I64, _I32, _I64, _P, _I64, _I64, _I64, _I32, _P, _I64, _I64, _P,
+                                                _I64, _I64, _F64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _P,
+                                                _I64, _P]
+        handle.gptq2d_packed_linear.restype = ctypes.c_int
+        handle.gptq2d_packed_linear_workspace.argtypes = [_I64, _I64, _I64, _I32, _I64, _I32, _I64, _I64]
+        handle.gptq2d_packed_linear_workspace.restype = ctypes.c_int64
         cache = [_P, _I64, _I32, _I32, _I32]                       # pages, their count, heads, dim, page
         tokens = [_P, _I64, _I64, _I64, _P, _P, _I64]              # table, seqs, width, row stride, lengths, offsets, tokens
         for name in ("append", "read"):

@@ -78,11 +78,6 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Exponent e with 2^e <= x < 2^(e + 1) of a finite x > 0 (0 for anything else).
-__device__ __forceinline__ int exponent_of(float x) {
-  return x > 0.f && x < __builtin_inff() ? (int)__builtin_amdgcn_frexp_expf(x) - 1 : 0;
-}
-
 // A column's query as B operands, QP pieces; `factor` takes the products' sums back to scores, `sum` is the sum of what
 // the operands hold.
 template <int TYPE, int ND, int QP>

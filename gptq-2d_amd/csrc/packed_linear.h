@@ -1,0 +1,264 @@
+// Products with a packed INT layer: what the kernels of packed_linear.hip share.
+//
+//   y[t, i] = sum_k x[t, k] (u[i, k] - w[i, k / group]) s[i, k / group],  w = zero point - qmin,
+// u the code in the layer's bit field (pack.hip).  The matrix cores multiply fp16 activations by u - 2^(bits - 1), which
+// fp16 holds exactly; a group's products are summed in fp32 and then multiplied by its scale, and what w differs from
+// 2^(bits - 1) is taken off through the sum of the group's activations.  Activations are scaled by a power of two per token
+// (the largest element to 2^14..2^15): bf16 and fp16 elements down to 2^-30 of the largest stay as they are, fp32 ones
+// are two pieces of together 22 bits.  So no weight is rounded, whatever its scale.
+#pragma once
+
+#include "elements.h"
+#include "lds_dma.h"
+#include "split_mma.h"
+
+namespace {
+
+// Order of a run of eight activations in memory: element j and j + 4 side by side, as the codes' pairs come out.
+// Operands: lane l holds row (token) or column (row of W) l % 16 and the eight k of its part g = l / 16 of a step.
+// WIDE (groups that a block of 128 columns does not cut): in step i part g holds k = 32 g + 8 i .. + 7 of the block, so that a
+// lane's 32 codes are one run of its row.  Otherwise k = 32 i + 8 g .. + 7, so that a step stays inside a group; the
+// words change places between the four parts for that (four permlane swaps for 32 codes).
+
+// The codes of 128 columns of 16 rows, as loaded: this lane's 32 (BITS words).
+template <int BITS>
+struct Codes {
+  unsigned w[BITS];
+};
+
+template <int BITS>
+__device__ __forceinline__ void load_codes(Codes<BITS>& c, const unsigned* row, int at, int row_words) {
+  typedef unsigned vec4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef unsigned vec3 __attribute__((ext_vector_type(3), aligned(4)));
+  typedef unsigned vec2 __attribute__((ext_vector_type(2), aligned(4)));
+  if (at + BITS <= row_words) {
+    if constexpr (BITS == 2) {
+      const vec2 v = *reinterpret_cast<const vec2*>(row + at);
+      c.w[0] = v[0], c.w[1] = v[1];
+    } else if constexpr (BITS == 3) {
+      const vec3 v = *reinterpret_cast<const vec3*>(row + at);
+      c.w[0] = v[0], c.w[1] = v[1], c.w[2] = v[2];
+    } else {
+#pragma unroll
+      for (int i = 0; i < BITS; i += 4) {
+        const vec4 v = *reinterpret_cast<const vec4*>(row + at + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c.w[i + j] = v[j];
+      }
+    }
+  } else {  // the row's end: the activations there are zeros
+#pragma unroll
+    for (int i = 0; i < BITS; ++i) c.w[i] = at + i < row_words ? row[at + i] : 0u;
+  }
+}
+
+// Step i's eight codes of the lane, as they lie: 8 BITS bits in one word (two for 8 bits).
+template <int BITS>
+struct Run {
+  unsigned w[BITS == 8 ? 2 : 1];
+};
+
+template <int BITS>
+__device__ __forceinline__ void split_runs(Run<BITS> (&r)[4], const Codes<BITS>& c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (BITS == 8) {
+      r[i].w[0] = c.w[2 * i], r[i].w[1] = c.w[2 * i + 1];
+    } else if constexpr (BITS == 4) {
+      r[i].w[0] = c.w[i];
+    } else if constexpr (BITS == 3) {
+      r[i].w[0] = i == 0 ? c.w[0]
+                         : i == 1 ? __builtin_amdgcn_alignbit(c.w[1], c.w[0], 24)
+                                  : i == 2 ? __builtin_amdgcn_alignbit(c.w[2], c.w[1], 16) : c.w[2] >> 8;
+    } else {
+      r[i].w[0] = i % 2 ? c.w[i / 2] >> 16 : c.w[i / 2];
+    }
+  }
+}
+
+// r[i] of part g becomes r[g] of part i: 4 x 4 words exchanged between the lanes l, l + 16, l + 32, l + 48.
+__device__ __forceinline__ void swap_parts(unsigned& a, unsigned& b, unsigned& c, unsigned& d) {
+  typedef unsigned pair __attribute__((ext_vector_type(2)));
+  pair p = __builtin_amdgcn_permlane32_swap(a, c, false, false);
+  a = p[0], c = p[1];
+  p = __builtin_amdgcn_permlane32_swap(b, d, false, false);
+  b = p[0], d = p[1];
+  p = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = p[0], b = p[1];
+  p = __builtin_amdgcn_permlane16_swap(c, d, false, false);
+  c = p[0], d = p[1];
+}
+
+__device__ __forceinline__ half2v as_half2(unsigned u) { return __builtin_bit_cast(half2v, u); }
+__device__ __forceinline__ half2v both(float x) { return (half2v){(_Float16)x, (_Float16)x}; }
+
+// The eight codes of a run, less 2^(BITS - 1), in fp16 in the activations' order.  1024 + c 2^p is an fp16 number with the
+// code in its low bits: a mask brings two codes of a word whose halves hold four each, one packed operation takes
+// 1024 and the factor away, exactly.
+template <int BITS>
+__device__ __forceinline__ half8 centred(const Run<BITS>& r) {
+  union {
+    half2v h[4];
+    half8 v;
+  } o;
+  constexpr unsigned ONE = 0x64006400u;
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o.h[j] = as_half2(__builtin_amdgcn_perm(r.w[1], r.w[0], 0x0c040c00u + j * 0x00010001u) | ONE) + both(-1152.f);
+  } else if constexpr (BITS == 4) {
+    const unsigned a = r.w[0], b = a >> 8;
+    o.h[0] = as_half2((a & 0x000f000fu) | ONE) + both(-1032.f);
+    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00f000f0u) | ONE), both(0.0625f), both(-72.f));
+    o.h[2] = as_half2((b & 0x000f000fu) | ONE) + both(-1032.f);
+    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x00f000f0u) | ONE), both(0.0625f), both(-72.f));
+  } else if constexpr (BITS == 3) {
+    const unsigned a = (r.w[0] & 0xfffu) | (r.w[0] << 4 & 0x0fff0000u), b = a >> 3;
+    o.h[0] = as_half2((a & 0x00070007u) | ONE) + both(-1028.f);
+    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00380038u) | ONE), both(0.125f), both(-132.f));
+    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x01c001c0u) | ONE), both(0.015625f), both(-20.f));
+    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x01c001c0u) | ONE), both(0.015625f), both(-20.f));
+  } else {
+    const unsigned a = (r.w[0] & 0xffu) | (r.w[0] << 8 & 0x00ff0000u);
+    o.h[0] = as_half2((a & 0x00030003u) | ONE) + both(-1026.f);
+    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x000c000cu) | ONE), both(0.25f), both(-258.f));
+    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x00300030u) | ONE), both(0.0625f), both(-66.f));
+    o.h[3] = __builtin_elementwise_fma(as_half2((a & 0x00c000c0u) | ONE), both(0.015625f), both(-18.f));
+  }
+  return o.v;
+}
+
+// The four steps' operands of a block of 128 columns.
+template <int BITS, bool WIDE>
+__device__ __forceinline__ void operands(half8 (&o)[4], const Codes<BITS>& c) {
+  Run<BITS> r[4];
+  split_runs<BITS>(r, c);
+  if constexpr (!WIDE) {
+    swap_parts(r[0].w[0], r[1].w[0], r[2].w[0], r[3].w[0]);
+    if constexpr (BITS == 8) swap_parts(r[0].w[1], r[1].w[1], r[2].w[1], r[3].w[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = centred<BITS>(r[i]);
+}
+
+__device__ __forceinline__ floatx4 mma(half8 a, half8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mma(bf16x8 a, bf16x8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// A call, as its kernels take it.
+struct Linear {
+  int tokens, m, n, blocks;  // blocks of 128 columns
+  // layer
+  const unsigned* words;
+  int64_t row_words;
+  const float* scale;
+  const float* zero;  // or none: `offset` everywhere
+  int64_t scale_row, scale_col, zero_row, zero_col;
+  float qmin, offset;  // offset: -qmin - 2^(bits - 1)
+  int group;       // columns of a group, a multiple of 32 (whole rows: 128 blocks)
+  unsigned steps;  // group / 32 (not WIDE: steps of 32 columns of a group) or group / 128
+  unsigned mag;    // of the division by `steps`
+  bool corrected;  // offset or zero points not 0
+  // activations
+  const void* x;
+  int64_t x_token;
+  int type;
+  _Float16* xp;  // [pieces][tokens][128 blocks], their factor back [tokens], sums of groups [groups][tokens to 16]
+  int64_t piece;
+  float* factor;
+  float* sums;
+  int64_t sums_row;
+  int groups;
+  // adapters, or none (index null)
+  const void* a;
+  const void* b;
+  const float* scaling;
+  const int32_t* index;
+  int adapters, rank, rank_pad, chunks, chunk;  // v: [chunks][tokens][rank_pad]; columns of a chunk
+  float* v;
+  // result
+  void* y;
+  int64_t y_token;
+  const void* bias;
+  int splits, split_blocks;
+  float* part;  // [splits][tokens][m] where splits > 1
+};
+
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int type) {
+  if (type == TYPE_F32) return static_cast<const float*>(p)[i];
+  if (type == TYPE_BF16) return to_f32<TYPE_BF16>(static_cast<const uint16_t*>(p)[i]);
+  return (float)static_cast<const _Float16*>(p)[i];
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, int type, float x) {
+  if (type == TYPE_F32)
+    static_cast<float*>(p)[i] = x;
+  else if (type == TYPE_BF16)
+    static_cast<uint16_t*>(p)[i] = from_f32<TYPE_BF16>(x);
+  else
+    static_cast<_Float16*>(p)[i] = (_Float16)x;
+}
+__device__ __forceinline__ void load_any8(float (&x)[8], const void* p, int64_t row, int d, int dim, int type) {
+  if (type == TYPE_F32)
+    load_row<TYPE_F32, 8>(x, static_cast<const float*>(p) + row, d, dim);
+  else if (type == TYPE_BF16)
+    load_row<TYPE_BF16, 8>(x, static_cast<const uint16_t*>(p) + row, d, dim);
+  else
+    load_row<TYPE_F16, 8>(x, static_cast<const _Float16*>(p) + row, d, dim);
+}
+
+// The index of the adapter of token t, -1 for none.
+__device__ __forceinline__ int adapter_of(const Linear& p, int t) {
+  const int a = t < p.tokens ? p.index[t] : -1;
+  return a >= 0 && a < p.adapters ? a : -1;
+}
+
+// acc[j] += V B^T for the 16 tokens from t0 and the 16 rows of W from r0 + 16 j, one distinct adapter of the tokens after
+// the other, the others' rows of V zeros.  V (fp32) and B are taken in bf16 pieces: six products, 2^-23 of the result; of
+// bf16 adapters B is one piece, and two of V leave out 2^-17.
+template <int MR>
+__device__ __forceinline__ void add_adapters(floatx4 (&acc)[MR], const Linear& p, int t0, int r0) {
+  const int lane = threadIdx.x & 63, g = lane >> 4, t = t0 + (lane & 15);
+  const int mine = adapter_of(p, t);
+  unsigned pending = (unsigned)__builtin_amdgcn_ballot_w64(mine >= 0) & 0xffffu;
+  while (pending) {
+    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctz(pending));
+    pending &= ~(unsigned)__builtin_amdgcn_ballot_w64(mine == a);
+    const float c = p.scaling ? p.scaling[a] : 1.f;
+    for (int j0 = 0; j0 < p.rank_pad; j0 += 32) {
+      float v[8] = {};
+      if (mine == a) {
+        const float* row = p.v + (int64_t)t * p.rank_pad + j0 + 8 * g;
+        for (int k = 0; k < p.chunks; ++k) {
+          const float4 lo = *reinterpret_cast<const float4*>(row), hi = *reinterpret_cast<const float4*>(row + 4);
+          v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+          v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+          row += (int64_t)p.tokens * p.rank_pad;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= c;
+      }
+      bf16x8 vp[3];
+      split8(v, vp);
+#pragma unroll
+      for (int j = 0; j < MR; ++j) {
+        const int r = r0 + 16 * j + (lane & 15);
+        float b[8];
+        load_any8(b, p.b, ((int64_t)a * p.m + (r < p.m ? r : p.m - 1)) * p.rank, j0 + 8 * g, p.rank, p.type);
+        bf16x8 bp[3];
+        split8(b, bp);
+        if (p.type == TYPE_BF16) {
+          acc[j] = mma(vp[1], bp[0], acc[j]);
+          acc[j] = mma(vp[0], bp[0], acc[j]);
+        } else {
+#pragma unroll
+          for (int q = 0; q < NPROD; ++q) acc[j] = mma(vp[prod_a[q]], bp[prod_b[q]], acc[j]);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace

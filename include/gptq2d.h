@@ -346,6 +346,25 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
                      double scale, int64_t window, void* out, int64_t out_token, int64_t out_head, float* lse, void* work,
                      int64_t work_bytes, void* stream);
 
+/* Product with a packed INT layer, beside it the low-rank adapters of many requests (no reference counterpart: the
+ * reference returns dequantized weights):
+ *   y[t, i] = sum_k x[t, k] (u[i, k] + qmin - zero[i, k / group]) scale[i, k / group] + bias[i]
+ *             + scaling[e] sum_j (sum_k x[t, k] a[e, j, k]) b[e, i, j],  e = index[t].
+ * x: [tokens, n] of `type` (0: fp32, 1: bf16, 2: fp16), rows x_token elements apart; y, bias, a [adapters, rank, n] and
+ * b [adapters, m, rank] of the same type.  words: the codes u of gptq2d_pack_int (m rows of row_words words, bits 2, 3, 4
+ * or 8).  scale and zero (NULL: 0) are fp32, read at row *_row + group *_col elements; group: a multiple of 32 columns, 0
+ * for whole rows.  index (int32, NULL or adapters 0: none): a token whose index is no adapter has none.  scaling NULL: 1.
+ * n below 2^21.  work: 16-byte aligned, gptq2d_packed_linear_workspace bytes, of no use afterwards; GPTQ2D_ESCRATCH where it
+ * is smaller.  adapters and rank: 0 where index is NULL. */
+int64_t gptq2d_packed_linear_workspace(int64_t tokens, int64_t m, int64_t n, int32_t bits, int64_t group, int32_t type,
+                                       int64_t adapters, int64_t rank); /* -1 for sizes it does not take */
+int gptq2d_packed_linear(const void* x, int64_t x_token, int32_t type, int64_t tokens, const uint32_t* words, int64_t m,
+                         int64_t n, int64_t row_words, int32_t bits, const float* scale, int64_t scale_row,
+                         int64_t scale_col, const float* zero, int64_t zero_row, int64_t zero_col, double qmin,
+                         int64_t group, const void* bias, const void* a, const void* b, const float* scaling,
+                         const int32_t* index, int64_t adapters, int64_t rank, void* y, int64_t y_token, void* work,
+                         int64_t work_bytes, void* stream);
+
 /* Launch profiler (no reference counterpart; the reference times with host clocks, demo.ipynb:109-118).
  * While on, every launch of a profiled kernel class is bracketed with HIP events on its stream.
  * Process-global, not thread-safe, not for use under stream capture.
