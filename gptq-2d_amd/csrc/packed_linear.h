@@ -2,10 +2,11 @@
 //
 //   y[t, i] = sum_k x[t, k] (u[i, k] - w[i, k / group]) s[i, k / group],  w = zero point - qmin,
 // u the code in the layer's bit field (pack.hip).  The matrix cores multiply fp16 activations by u - 2^(bits - 1), which
-// fp16 holds exactly; a group's products are summed in fp32 and then multiplied by its scale, and what w differs from
-// 2^(bits - 1) is taken off through the sum of the group's activations.  Activations are scaled by a power of two per token
+// fp16 holds exactly, less the nearest whole number to what w differs from that; a group's products are summed in fp32 and
+// then multiplied by its scale, and the rest of w (0 for whole zero points) is taken off through the sum of the group's
+// activations.  Activations are scaled by a power of two per token
 // (the largest element to 2^14..2^15): bf16 and fp16 elements down to 2^-30 of the largest stay as they are, fp32 ones
-// are two pieces of together 22 bits.  So no weight is rounded, whatever its scale.
+// are two pieces of together 22 bits.  So no weight is rounded, whatever its scale, and a whole zero point costs nothing.
 #pragma once
 
 #include "elements.h"
@@ -26,29 +27,32 @@ struct Codes {
   unsigned w[BITS];
 };
 
-template <int BITS>
+// Words at .. at + BITS - 1 of a row (vector loads need only a word's own alignment); GUARD: zeros past the row's end, where
+// the activations are zeros.
+template <int BITS, bool GUARD>
 __device__ __forceinline__ void load_codes(Codes<BITS>& c, const unsigned* row, int at, int row_words) {
   typedef unsigned vec4 __attribute__((ext_vector_type(4), aligned(4)));
   typedef unsigned vec3 __attribute__((ext_vector_type(3), aligned(4)));
   typedef unsigned vec2 __attribute__((ext_vector_type(2), aligned(4)));
-  if (at + BITS <= row_words) {
-    if constexpr (BITS == 2) {
-      const vec2 v = *reinterpret_cast<const vec2*>(row + at);
-      c.w[0] = v[0], c.w[1] = v[1];
-    } else if constexpr (BITS == 3) {
-      const vec3 v = *reinterpret_cast<const vec3*>(row + at);
-      c.w[0] = v[0], c.w[1] = v[1], c.w[2] = v[2];
-    } else {
+  if constexpr (GUARD) {
 #pragma unroll
-      for (int i = 0; i < BITS; i += 4) {
-        const vec4 v = *reinterpret_cast<const vec4*>(row + at + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) c.w[i + j] = v[j];
-      }
+    for (int i = 0; i < BITS; ++i) {
+      c.w[i] = 0;
+      if (at + i < row_words) c.w[i] = row[at + i];
     }
-  } else {  // the row's end: the activations there are zeros
+  } else if constexpr (BITS == 2) {
+    const vec2 v = *reinterpret_cast<const vec2*>(row + at);
+    c.w[0] = v[0], c.w[1] = v[1];
+  } else if constexpr (BITS == 3) {
+    const vec3 v = *reinterpret_cast<const vec3*>(row + at);
+    c.w[0] = v[0], c.w[1] = v[1], c.w[2] = v[2];
+  } else {
 #pragma unroll
-    for (int i = 0; i < BITS; ++i) c.w[i] = at + i < row_words ? row[at + i] : 0u;
+    for (int i = 0; i < BITS; i += 4) {
+      const vec4 v = *reinterpret_cast<const vec4*>(row + at + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) c.w[i + j] = v[j];
+    }
   }
 }
 
@@ -92,11 +96,35 @@ __device__ __forceinline__ void swap_parts(unsigned& a, unsigned& b, unsigned& c
 __device__ __forceinline__ half2v as_half2(unsigned u) { return __builtin_bit_cast(half2v, u); }
 __device__ __forceinline__ half2v both(float x) { return (half2v){(_Float16)x, (_Float16)x}; }
 
-// The eight codes of a run, less 2^(BITS - 1), in fp16 in the activations' order.  1024 + c 2^p is an fp16 number with the
-// code in its low bits: a mask brings two codes of a word whose halves hold four each, one packed operation takes
-// 1024 and the factor away, exactly.
+// What is taken off the codes of a row's group: 2^(BITS - 1) and, where the zero point is that far from it, the whole number
+// nearest to the rest; the rest of the rest (0 for zero points that are whole) goes through the activations' sum.
 template <int BITS>
-__device__ __forceinline__ half8 centred(const Run<BITS>& r) {
+struct Middle {
+  half2v k[BITS == 8 ? 1 : BITS == 4 ? 2 : BITS == 3 ? 3 : 4];
+};
+
+template <int BITS>
+__device__ __forceinline__ float split_shift(Middle<BITS>& m, float shift) {
+  float whole = round_even(shift);
+  whole = __builtin_fabsf(whole) <= 512.f ? whole : 0.f;  // fp16 holds 1024 + 128 + 512; also for a NaN
+  const half2v w = both(whole);
+  if constexpr (BITS == 8) {
+    m.k[0] = both(-1152.f) - w;
+  } else if constexpr (BITS == 4) {
+    m.k[0] = both(-1032.f) - w, m.k[1] = both(-72.f) - w;
+  } else if constexpr (BITS == 3) {
+    m.k[0] = both(-1028.f) - w, m.k[1] = both(-132.f) - w, m.k[2] = both(-20.f) - w;
+  } else {
+    m.k[0] = both(-1026.f) - w, m.k[1] = both(-258.f) - w, m.k[2] = both(-66.f) - w, m.k[3] = both(-18.f) - w;
+  }
+  return shift - whole;
+}
+
+// The eight codes of a run less their middle, in fp16 in the activations' order.  1024 + c 2^p is an fp16 number with the
+// code in its low bits: a mask brings two codes of a word whose halves hold four each, one packed operation takes 1024,
+// the factor and the middle away, exactly: nine instructions for eight 4-bit codes.
+template <int BITS>
+__device__ __forceinline__ half8 centred(const Run<BITS>& r, const Middle<BITS>& m) {
   union {
     half2v h[4];
     half8 v;
@@ -105,40 +133,37 @@ __device__ __forceinline__ half8 centred(const Run<BITS>& r) {
   if constexpr (BITS == 8) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      o.h[j] = as_half2(__builtin_amdgcn_perm(r.w[1], r.w[0], 0x0c040c00u + j * 0x00010001u) | ONE) + both(-1152.f);
+      o.h[j] = as_half2(__builtin_amdgcn_perm(r.w[1], r.w[0], 0x0c040c00u + j * 0x00010001u) | ONE) + m.k[0];
   } else if constexpr (BITS == 4) {
     const unsigned a = r.w[0], b = a >> 8;
-    o.h[0] = as_half2((a & 0x000f000fu) | ONE) + both(-1032.f);
-    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00f000f0u) | ONE), both(0.0625f), both(-72.f));
-    o.h[2] = as_half2((b & 0x000f000fu) | ONE) + both(-1032.f);
-    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x00f000f0u) | ONE), both(0.0625f), both(-72.f));
+    o.h[0] = as_half2((a & 0x000f000fu) | ONE) + m.k[0];
+    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00f000f0u) | ONE), both(0.0625f), m.k[1]);
+    o.h[2] = as_half2((b & 0x000f000fu) | ONE) + m.k[0];
+    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x00f000f0u) | ONE), both(0.0625f), m.k[1]);
   } else if constexpr (BITS == 3) {
     const unsigned a = (r.w[0] & 0xfffu) | (r.w[0] << 4 & 0x0fff0000u), b = a >> 3;
-    o.h[0] = as_half2((a & 0x00070007u) | ONE) + both(-1028.f);
-    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00380038u) | ONE), both(0.125f), both(-132.f));
-    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x01c001c0u) | ONE), both(0.015625f), both(-20.f));
-    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x01c001c0u) | ONE), both(0.015625f), both(-20.f));
+    o.h[0] = as_half2((a & 0x00070007u) | ONE) + m.k[0];
+    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00380038u) | ONE), both(0.125f), m.k[1]);
+    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x01c001c0u) | ONE), both(0.015625f), m.k[2]);
+    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x01c001c0u) | ONE), both(0.015625f), m.k[2]);
   } else {
     const unsigned a = (r.w[0] & 0xffu) | (r.w[0] << 8 & 0x00ff0000u);
-    o.h[0] = as_half2((a & 0x00030003u) | ONE) + both(-1026.f);
-    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x000c000cu) | ONE), both(0.25f), both(-258.f));
-    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x00300030u) | ONE), both(0.0625f), both(-66.f));
-    o.h[3] = __builtin_elementwise_fma(as_half2((a & 0x00c000c0u) | ONE), both(0.015625f), both(-18.f));
+    o.h[0] = as_half2((a & 0x00030003u) | ONE) + m.k[0];
+    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x000c000cu) | ONE), both(0.25f), m.k[1]);
+    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x00300030u) | ONE), both(0.0625f), m.k[2]);
+    o.h[3] = __builtin_elementwise_fma(as_half2((a & 0x00c000c0u) | ONE), both(0.015625f), m.k[3]);
   }
   return o.v;
 }
 
-// The four steps' operands of a block of 128 columns.
+// The four steps' runs of a block of 128 columns.
 template <int BITS, bool WIDE>
-__device__ __forceinline__ void operands(half8 (&o)[4], const Codes<BITS>& c) {
-  Run<BITS> r[4];
+__device__ __forceinline__ void step_runs(Run<BITS> (&r)[4], const Codes<BITS>& c) {
   split_runs<BITS>(r, c);
   if constexpr (!WIDE) {
     swap_parts(r[0].w[0], r[1].w[0], r[2].w[0], r[3].w[0]);
     if constexpr (BITS == 8) swap_parts(r[0].w[1], r[1].w[1], r[2].w[1], r[3].w[1]);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = centred<BITS>(r[i]);
 }
 
 __device__ __forceinline__ floatx4 mma(half8 a, half8 b, floatx4 c) {
@@ -151,6 +176,8 @@ __device__ __forceinline__ floatx4 mma(bf16x8 a, bf16x8 b, floatx4 c) {
 // A call, as its kernels take it.
 struct Linear {
   int tokens, m, n, blocks;  // blocks of 128 columns
+  int whole;                 // of which a row's words hold all
+  int64_t need_words;        // of a row
   // layer
   const unsigned* words;
   int64_t row_words;
@@ -161,7 +188,7 @@ struct Linear {
   int group;       // columns of a group, a multiple of 32 (whole rows: 128 blocks)
   unsigned steps;  // group / 32 (not WIDE: steps of 32 columns of a group) or group / 128
   unsigned mag;    // of the division by `steps`
-  bool corrected;  // offset or zero points not 0
+  bool corrected;  // zero points, or an offset that is no whole number
   // activations
   const void* x;
   int64_t x_token;
@@ -177,7 +204,7 @@ struct Linear {
   const void* b;
   const float* scaling;
   const int32_t* index;
-  int adapters, rank, rank_pad, chunks, chunk;  // v: [chunks][tokens][rank_pad]; columns of a chunk
+  int adapters, rank, rank_pad, slots, chunks, chunk;  // v: [chunks][tokens][rank_pad]; columns of a chunk
   float* v;
   // result
   void* y;
@@ -217,7 +244,7 @@ __device__ __forceinline__ int adapter_of(const Linear& p, int t) {
 
 // acc[j] += V B^T for the 16 tokens from t0 and the 16 rows of W from r0 + 16 j, one distinct adapter of the tokens after
 // the other, the others' rows of V zeros.  V (fp32) and B are taken in bf16 pieces: six products, 2^-23 of the result; of
-// bf16 adapters B is one piece, and two of V leave out 2^-17.
+// bf16 adapters B is one piece, and two of V leave out 2^-17.  For long batches, where 16 tokens have one or two adapters.
 template <int MR>
 __device__ __forceinline__ void add_adapters(floatx4 (&acc)[MR], const Linear& p, int t0, int r0) {
   const int lane = threadIdx.x & 63, g = lane >> 4, t = t0 + (lane & 15);
@@ -231,6 +258,7 @@ __device__ __forceinline__ void add_adapters(floatx4 (&acc)[MR], const Linear& p
       float v[8] = {};
       if (mine == a) {
         const float* row = p.v + (int64_t)t * p.rank_pad + j0 + 8 * g;
+#pragma unroll 4
         for (int k = 0; k < p.chunks; ++k) {
           const float4 lo = *reinterpret_cast<const float4*>(row), hi = *reinterpret_cast<const float4*>(row + 4);
           v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
@@ -258,6 +286,47 @@ __device__ __forceinline__ void add_adapters(floatx4 (&acc)[MR], const Linear& p
         }
       }
     }
+  }
+}
+
+// acc[n] += V B^T for the tokens t0 + 16 n + 4 g .. + 3 and the lane's row r of W, each token with its own adapter: for short
+// batches, where every token may have another one.  Eight ranks at a time, dealt to `shares` waves that sum apart.
+template <int NT>
+__device__ __forceinline__ void add_own_adapters(floatx4 (&acc)[NT], const Linear& p, int t0, int r, int share, int shares) {
+  const int g = threadIdx.x >> 4 & 3, row = r < p.m ? r : p.m - 1;
+  if (8 * share >= p.rank) return;
+#pragma unroll 1
+  for (int n = 0; n < NT; ++n) {
+    const int t = t0 + 16 * n + 4 * g;
+    int a[4];
+    floatx4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = adapter_of(p, t + i);
+    for (int j = 8 * share; j < p.rank; j += 8 * shares) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (a[i] >= 0) {
+          float b[8], v[8] = {};
+          load_any8(b, p.b, ((int64_t)a[i] * p.m + row) * p.rank, j, p.rank, p.type);
+          const float* at = p.v + (int64_t)(t + i) * p.rank_pad + j;
+#pragma unroll 2
+          for (int k = 0; k < p.chunks; ++k) {
+            const float4 lo = *reinterpret_cast<const float4*>(at), hi = *reinterpret_cast<const float4*>(at + 4);
+            v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+            v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+            at += (int64_t)p.tokens * p.rank_pad;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum[i] = __builtin_fmaf(v[e], b[e], sum[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (a[i] >= 0 && p.scaling) sum[i] *= p.scaling[a[i]];
+#pragma unroll
+    for (int m = 0; m < NT; ++m)
+      if (m == n) acc[m] += sum;
   }
 }
 
