@@ -67,4 +67,15 @@ __device__ __forceinline__ int exponent_of(float x) {
   return x > 0.f && x < __builtin_inff() ? (int)__builtin_amdgcn_frexp_expf(x) - 1 : 0;
 }
 
+__device__ __forceinline__ half2v as_half2(unsigned u) { return __builtin_bit_cast(half2v, u); }
+__device__ __forceinline__ half2v both(float x) { return (half2v){(_Float16)x, (_Float16)x}; }
+
+// x & mask | 0x64006400 (two fp16 numbers of 1024 and up) in one instruction: with literals the compiler takes two, since
+// an instruction holds one constant.
+__device__ __forceinline__ half2v codes_at(unsigned x, unsigned mask) {
+  unsigned r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(0x64006400u));
+  return as_half2(r);
+}
+
 }  // namespace

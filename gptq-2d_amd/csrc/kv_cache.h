@@ -28,21 +28,14 @@ namespace {
 // bits; one subtraction (or multiplication by 1/16 and subtraction) leaves c - 8, exactly: nine instructions a word.
 __device__ __forceinline__ half8 centred_codes(unsigned w) {
   union {
-    unsigned u[4];
     half2v h[4];
     half8 v;
   } r;
   const unsigned x = w >> 8;
-  r.u[0] = (w & 0x000f000fu) | 0x64006400u;
-  r.u[1] = (w & 0x00f000f0u) | 0x64006400u;
-  r.u[2] = (x & 0x000f000fu) | 0x64006400u;
-  r.u[3] = (x & 0x00f000f0u) | 0x64006400u;
-  const half2v k1032 = {(_Float16)-1032.f, (_Float16)-1032.f}, k16 = {(_Float16)0.0625f, (_Float16)0.0625f},
-               k72 = {(_Float16)-72.f, (_Float16)-72.f};
-  r.h[0] += k1032;
-  r.h[2] += k1032;
-  r.h[1] = __builtin_elementwise_fma(r.h[1], k16, k72);
-  r.h[3] = __builtin_elementwise_fma(r.h[3], k16, k72);
+  r.h[0] = codes_at(w, 0x000f000fu) + both(-1032.f);
+  r.h[1] = __builtin_elementwise_fma(codes_at(w, 0x00f000f0u), both(0.0625f), both(-72.f));
+  r.h[2] = codes_at(x, 0x000f000fu) + both(-1032.f);
+  r.h[3] = __builtin_elementwise_fma(codes_at(x, 0x00f000f0u), both(0.0625f), both(-72.f));
   return r.v;
 }
 

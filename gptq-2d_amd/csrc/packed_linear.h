@@ -93,9 +93,6 @@ __device__ __forceinline__ void swap_parts(unsigned& a, unsigned& b, unsigned& c
   c = p[0], d = p[1];
 }
 
-__device__ __forceinline__ half2v as_half2(unsigned u) { return __builtin_bit_cast(half2v, u); }
-__device__ __forceinline__ half2v both(float x) { return (half2v){(_Float16)x, (_Float16)x}; }
-
 // What is taken off the codes of a row's group: 2^(BITS - 1) and, where the zero point is that far from it, the whole number
 // nearest to the rest; the rest of the rest (0 for zero points that are whole) goes through the activations' sum.
 template <int BITS>
@@ -129,29 +126,28 @@ __device__ __forceinline__ half8 centred(const Run<BITS>& r, const Middle<BITS>&
     half2v h[4];
     half8 v;
   } o;
-  constexpr unsigned ONE = 0x64006400u;
   if constexpr (BITS == 8) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      o.h[j] = as_half2(__builtin_amdgcn_perm(r.w[1], r.w[0], 0x0c040c00u + j * 0x00010001u) | ONE) + m.k[0];
+      o.h[j] = as_half2(__builtin_amdgcn_perm(r.w[1], r.w[0], 0x0c040c00u + j * 0x00010001u) | 0x64006400u) + m.k[0];
   } else if constexpr (BITS == 4) {
     const unsigned a = r.w[0], b = a >> 8;
-    o.h[0] = as_half2((a & 0x000f000fu) | ONE) + m.k[0];
-    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00f000f0u) | ONE), both(0.0625f), m.k[1]);
-    o.h[2] = as_half2((b & 0x000f000fu) | ONE) + m.k[0];
-    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x00f000f0u) | ONE), both(0.0625f), m.k[1]);
+    o.h[0] = codes_at(a, 0x000f000fu) + m.k[0];
+    o.h[1] = __builtin_elementwise_fma(codes_at(a, 0x00f000f0u), both(0.0625f), m.k[1]);
+    o.h[2] = codes_at(b, 0x000f000fu) + m.k[0];
+    o.h[3] = __builtin_elementwise_fma(codes_at(b, 0x00f000f0u), both(0.0625f), m.k[1]);
   } else if constexpr (BITS == 3) {
     const unsigned a = (r.w[0] & 0xfffu) | (r.w[0] << 4 & 0x0fff0000u), b = a >> 3;
-    o.h[0] = as_half2((a & 0x00070007u) | ONE) + m.k[0];
-    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x00380038u) | ONE), both(0.125f), m.k[1]);
-    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x01c001c0u) | ONE), both(0.015625f), m.k[2]);
-    o.h[3] = __builtin_elementwise_fma(as_half2((b & 0x01c001c0u) | ONE), both(0.015625f), m.k[2]);
+    o.h[0] = codes_at(a, 0x00070007u) + m.k[0];
+    o.h[1] = __builtin_elementwise_fma(codes_at(a, 0x00380038u), both(0.125f), m.k[1]);
+    o.h[2] = __builtin_elementwise_fma(codes_at(a, 0x01c001c0u), both(0.015625f), m.k[2]);
+    o.h[3] = __builtin_elementwise_fma(codes_at(b, 0x01c001c0u), both(0.015625f), m.k[2]);
   } else {
     const unsigned a = (r.w[0] & 0xffu) | (r.w[0] << 8 & 0x00ff0000u);
-    o.h[0] = as_half2((a & 0x00030003u) | ONE) + m.k[0];
-    o.h[1] = __builtin_elementwise_fma(as_half2((a & 0x000c000cu) | ONE), both(0.25f), m.k[1]);
-    o.h[2] = __builtin_elementwise_fma(as_half2((a & 0x00300030u) | ONE), both(0.0625f), m.k[2]);
-    o.h[3] = __builtin_elementwise_fma(as_half2((a & 0x00c000c0u) | ONE), both(0.015625f), m.k[3]);
+    o.h[0] = codes_at(a, 0x00030003u) + m.k[0];
+    o.h[1] = __builtin_elementwise_fma(codes_at(a, 0x000c000cu), both(0.25f), m.k[1]);
+    o.h[2] = __builtin_elementwise_fma(codes_at(a, 0x00300030u), both(0.0625f), m.k[2]);
+    o.h[3] = __builtin_elementwise_fma(codes_at(a, 0x00c000c0u), both(0.015625f), m.k[3]);
   }
   return o.v;
 }
@@ -290,9 +286,11 @@ __device__ __forceinline__ void add_adapters(floatx4 (&acc)[MR], const Linear& p
 }
 
 // acc[n] += V B^T for the tokens t0 + 16 n + 4 g .. + 3 and the lane's row r of W, each token with its own adapter: for short
-// batches, where every token may have another one.  Eight ranks at a time, dealt to `shares` waves that sum apart.
-template <int NT>
+// batches, where every token may have another one.  Eight ranks at a time, dealt to `shares` waves that sum apart; the
+// loads of four tokens are in flight together.  NP: fp32 elements where 2.
+template <int NT, int NP>
 __device__ __forceinline__ void add_own_adapters(floatx4 (&acc)[NT], const Linear& p, int t0, int r, int share, int shares) {
+  typedef unsigned vec __attribute__((ext_vector_type(4), aligned(2)));
   const int g = threadIdx.x >> 4 & 3, row = r < p.m ? r : p.m - 1;
   if (8 * share >= p.rank) return;
 #pragma unroll 1
@@ -302,23 +300,61 @@ __device__ __forceinline__ void add_own_adapters(floatx4 (&acc)[NT], const Linea
     floatx4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) a[i] = adapter_of(p, t + i);
+    if (!__builtin_amdgcn_ballot_w64(a[0] >= 0 || a[1] >= 0 || a[2] >= 0 || a[3] >= 0)) continue;
     for (int j = 8 * share; j < p.rank; j += 8 * shares) {
+      vec b[4][NP];
+      const bool whole = j + 8 <= p.rank;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (a[i] >= 0) {
-          float b[8], v[8] = {};
-          load_any8(b, p.b, ((int64_t)a[i] * p.m + row) * p.rank, j, p.rank, p.type);
-          const float* at = p.v + (int64_t)(t + i) * p.rank_pad + j;
-#pragma unroll 2
-          for (int k = 0; k < p.chunks; ++k) {
-            const float4 lo = *reinterpret_cast<const float4*>(at), hi = *reinterpret_cast<const float4*>(at + 4);
-            v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-            v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
-            at += (int64_t)p.tokens * p.rank_pad;
-          }
+        const char* at = static_cast<const char*>(p.b) + (((int64_t)(a[i] < 0 ? 0 : a[i]) * p.m + row) * p.rank + j) * (2 * NP);
+        if (whole) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) sum[i] = __builtin_fmaf(v[e], b[e], sum[i]);
+          for (int q = 0; q < NP; ++q) b[i][q] = *reinterpret_cast<const vec*>(at + 16 * q);
+        } else {
+          typedef typename std::conditional<NP == 2, unsigned, uint16_t>::type E;
+          union {
+            E e[8];
+            unsigned u[4 * NP];
+          } x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x.e[e] = j + e < p.rank ? reinterpret_cast<const E*>(at)[e] : (E)0;
+#pragma unroll
+          for (int e = 0; e < 4 * NP; ++e) b[i][e / 4][e % 4] = x.u[e];
         }
+      }
+      float v[4][8] = {};
+      const float* at[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) at[i] = p.v + (int64_t)(a[i] < 0 ? 0 : t + i) * p.rank_pad + j;
+#pragma unroll 1
+      for (int k = 0; k < p.chunks; ++k) {
+        float4 x[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i][0] = *reinterpret_cast<const float4*>(at[i]), x[i][1] = *reinterpret_cast<const float4*>(at[i] + 4);
+          at[i] += (int64_t)p.tokens * p.rank_pad;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            v[i][4 * h] += x[i][h].x, v[i][4 * h + 1] += x[i][h].y, v[i][4 * h + 2] += x[i][h].z, v[i][4 * h + 3] += x[i][h].w;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float add = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float w;
+          if constexpr (NP == 2) {
+            w = __uint_as_float(b[i][e / 4][e % 4]);
+          } else {
+            const unsigned u = b[i][0][e / 2] >> (e % 2 * 16) & 0xffffu;
+            w = p.type == TYPE_BF16 ? __uint_as_float(u << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)u);
+          }
+          add = __builtin_fmaf(v[i][e], w, add);
+        }
+        sum[i] += a[i] < 0 ? 0.f : add;  // without an adapter whatever was read
       }
     }
 #pragma unroll
@@ -330,4 +366,25 @@ __device__ __forceinline__ void add_own_adapters(floatx4 (&acc)[NT], const Linea
   }
 }
 
+// Groups: whole rows, multiples of 128 columns, other multiples of 32; the last two with zero points or without.
+enum { ROWS = 0, WIDE = 1, NARROW = 2, ZEROS = 4 };
+__host__ __device__ constexpr bool narrow(int mode) { return (mode & 3) == NARROW; }
+__host__ __device__ constexpr bool wide(int mode) { return (mode & 3) == WIDE; }
+__host__ __device__ constexpr bool zeros(int mode) { return mode & ZEROS; }
+
+// How a call is computed: tile (tokens of a workgroup; up to 64 stream_kernel, 128 tile_kernel), rows of a workgroup, splits
+// of the columns, and where its workspace holds what (floats).
+struct Plan {
+  int pieces, tile, rows, splits, split_blocks, mode, bits, rank_pad, slots, chunks, chunk;
+  int64_t groups, sums_row, xp, factor, sums, v, part, total;  // offsets; total: floats
+};
+
 }  // namespace
+
+// launch_mode<BITS> of a Linear and a Plan, one source file each.
+#define GPTQ2D_PACKED_PRODUCT(BITS) \
+  __attribute__((visibility("hidden"))) int packed_product_bits##BITS(const void* linear, const void* plan, hipStream_t st)
+GPTQ2D_PACKED_PRODUCT(2);
+GPTQ2D_PACKED_PRODUCT(3);
+GPTQ2D_PACKED_PRODUCT(4);
+GPTQ2D_PACKED_PRODUCT(8);
