@@ -41,8 +41,7 @@ struct Tile {
   int chunks;          // workgroups that share the blocks
 };
 
-template <int CT>
-__device__ __forceinline__ Tile make_tile(const KvCache& c, const Attend& a, int64_t b, int col0) {
+__device__ __forceinline__ Tile make_tile(const KvCache& c, const Attend& a, int64_t b, int col0, int CT) {
   Tile t;
   t.b = b;
   const int64_t t0 = kv_offset(c, b), t1 = kv_offset(c, b + 1);
@@ -267,7 +266,7 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
   const int64_t seq = kv_find(c, slot, a.group, CT, 1);
   const int64_t col0 = (slot - kv_first_slot(c, seq, a.group, CT, 1)) * CT;
   if (col0 > 0x7fffff00) return;
-  const Tile t = make_tile<CT>(c, a, seq, (int)col0);
+  const Tile t = make_tile(c, a, seq, (int)col0, CT);
   if (t.col0 >= t.cols || chunk >= t.chunks) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
 
@@ -401,11 +400,311 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
   }
 }
 
-// Joins the chunks' results: a wave a (token, query head), whose chunks are added in their order.
-template <int TYPE, int ND, int NQ>
-__global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a) {
+// Many columns (a prompt's tokens times the heads that share a kv head).  A workgroup takes 32 columns a wave and `chunk` blocks of
+// 32 keys; the block's codes are brought to fp16 once, by all waves, into LDS, where they lie as operands (two blocks in
+// turn, one barrier a block; the next one's words are in flight meanwhile), and its scales and zeros in fp32 with what all
+// columns share already in them.  Bound by the vector instructions of the softmax, so a score takes few: its exponent is
+// two fused multiply-adds off a reference that is the maximum of some block before, not of this one -- it moves when a score
+// exceeds it by 2^8, which needs no maximum over the lanes to be seen --, then one each for the exponential, its product
+// with the value's scale, the two sums, and half of one each for the comparison and the conversion.
+constexpr int PQ = 2, PWAVES = 4;  // columns of a wave: 16 PQ
+constexpr int AHEAD = 8;           // log2 of how far weights may exceed 1
+constexpr int PROOM = 7;           // weights times scales are held as p s 2^(PROOM - shift), at most 2^(PROOM + AHEAD)
+
+template <int ND, int PP>
+struct PromptState {
+  floatx4 o[PQ][4 * ND];
+  float top[PQ], l[PQ], z[PQ];
+  bool fresh[PQ];  // a column that has not seen a key: its reference is still to be taken, however low
+  int shift;
+};
+
+template <int ND, int QP, int PP, bool MASK>
+__device__ __forceinline__ void prompt_block(PromptState<ND, PP>& st, const half8 (&q)[PQ][2 * ND][QP],
+                                             const float (&qsum)[PQ], const half8 (*kop)[64], const half8 (*vop)[64],
+                                             const float (*aff)[32], int lane, int key0, const int (&pos)[PQ], int window) {
+  const int g = lane >> 4;
+  float e[PQ][8], most[PQ];
+#pragma unroll
+  for (int n = 0; n < PQ; ++n) most[n] = -__builtin_inff();
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    floatx4 s[PQ];
+#pragma unroll
+    for (int n = 0; n < PQ; ++n) s[n] = (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 2 * ND; ++i) {
+      const half8 k = kop[2 * ND * t + i][lane];
+#pragma unroll
+      for (int n = 0; n < PQ; ++n)
+#pragma unroll
+        for (int p = 0; p < QP; ++p) s[n] = mfma(k, q[n][i][p], s[n]);
+    }
+    const floatx4 ks = *reinterpret_cast<const floatx4*>(&aff[0][16 * t + 4 * g]);
+    const floatx4 kz = *reinterpret_cast<const floatx4*>(&aff[1][16 * t + 4 * g]);
+#pragma unroll
+    for (int n = 0; n < PQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = __builtin_fmaf(ks[i], s[n][i], __builtin_fmaf(kz[i], qsum[n], -st.top[n]));
+        if constexpr (MASK) {
+          const int key = key0 + 16 * t + i;
+          if (key > pos[n] || (window && key <= pos[n] - window)) x = -__builtin_inff();
+        }
+        e[n][4 * t + i] = x;
+        most[n] = fmaxf(most[n], x);
+      }
+  }
+  bool move = false;
+#pragma unroll
+  for (int n = 0; n < PQ; ++n) move |= most[n] > (st.fresh[n] ? -__builtin_inff() : (float)AHEAD);
+  if (__builtin_amdgcn_ballot_w64(move)) {  // the reference moves up to this block's maximum
+#pragma unroll
+    for (int n = 0; n < PQ; ++n) {
+      const float m = quad_max(most[n]);
+      const float up = st.fresh[n] ? (m == -__builtin_inff() ? 0.f : m) : fmaxf(m, 0.f);
+      const float f = st.fresh[n] ? 1.f : __builtin_amdgcn_exp2f(-up);  // sums of 0 stay, however far down it goes
+      st.fresh[n] = st.fresh[n] && m == -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[n][i] -= up;
+      st.top[n] += up;
+      st.l[n] *= f;
+      st.z[n] *= f;
+#pragma unroll
+      for (int d = 0; d < 4 * ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[n][d][i] *= f;
+    }
+  }
+  half8 p[PQ][PP];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const floatx4 vs = *reinterpret_cast<const floatx4*>(&aff[2][16 * t + 4 * g]);
+    const floatx4 vz = *reinterpret_cast<const floatx4*>(&aff[3][16 * t + 4 * g]);
+#pragma unroll
+    for (int n = 0; n < PQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = e[n][4 * t + i], w = __builtin_amdgcn_exp2f(x);
+        float ps = w * vs[i], pz = w * vz[i];
+        if constexpr (MASK) {  // a scale that is no number must not reach columns that do not see its key
+          ps = x == -__builtin_inff() ? 0.f : ps;
+          pz = x == -__builtin_inff() ? 0.f : pz;
+        }
+        st.l[n] += w;
+        st.z[n] += pz;
+        const _Float16 h = (_Float16)ps;
+        p[n][0][4 * t + i] = h;
+        if constexpr (PP == 2) p[n][1][4 * t + i] = (_Float16)(ps - (float)h);
+      }
+  }
+#pragma unroll
+  for (int W = 0; W < 4 * ND; ++W) {
+    const half8 v = vop[W][lane];
+#pragma unroll
+    for (int n = 0; n < PQ; ++n)
+#pragma unroll
+      for (int r = 0; r < PP; ++r) st.o[n][W] = mfma(v, p[n][r], st.o[n][W]);
+  }
+}
+
+template <int TYPE, int ND>
+__global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int CT = 16 * NQ, DP = 64 * ND;
+  constexpr int CT = 16 * PQ * PWAVES, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2;
+  constexpr int CH = (2 * ND + PWAVES - 1) / PWAVES;  // chunks of 1 KB of words of a block that a wave brings
+  __shared__ half8 ops[2][8 * ND][64];                // K's operands, then V's
+  __shared__ float aff[2][4][32];                     // scale and zero of keys (times what scores share), of values
+  __shared__ int shifts[2];
+  __shared__ float tops[PWAVES];
+  const int head = blockIdx.x, chunk = blockIdx.z;
+  const int64_t slot = blockIdx.y + (int64_t)gridDim.y * (blockIdx.z / a.chunks);
+  const int part = chunk % a.chunks;
+  const int64_t seq = kv_find(c, slot, a.group, CT, 1);
+  const int64_t first = kv_first_slot(c, seq, a.group, CT, 1);
+  if (slot < first || (slot - first) * CT > 0x7fffff00) return;
+  const Tile t = make_tile(c, a, seq, (int)((slot - first) * CT), CT);
+  if (t.col0 >= t.cols || part >= t.chunks) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
+
+  // the columns' queries, scaled by one power of two for all of the workgroup's
+  int pos[PQ], row_of[PQ], head_of[PQ];
+  bool valid[PQ];
+  float top = 0.f;
+  half8 q[PQ][2 * ND][QP];
+  float qsum[PQ];
+  int ex = 0;
+#pragma unroll
+  for (int turn = 0; turn < 2; ++turn) {
+#pragma unroll
+    for (int n = 0; n < PQ; ++n) {
+      const int col = t.col0 + 16 * (PQ * wave + n) + (lane & 15), token = col / a.group;
+      valid[n] = col < t.cols;
+      pos[n] = valid[n] ? t.pos0 + token : t.pos_hi;
+      row_of[n] = token, head_of[n] = head * a.group + col % a.group;
+      const T* row = (const T*)a.q + (t.row + (valid[n] ? token : 0)) * a.q_token + head_of[n] * a.q_head;
+      float total = 0.f;
+#pragma unroll
+      for (int s = 0; s < 2 * ND; ++s) {
+        float x[8];
+        load_row<TYPE, 8>(x, row, 32 * s + 8 * g, valid[n] ? c.dim : 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (turn == 0) {
+            const float v = __builtin_fabsf(x[e]);
+            top = v < __builtin_inff() && v > top ? v : top;  // infinities and NaN stay what they are in fp16
+          } else {
+            const float v = __builtin_ldexpf(x[e], -ex);
+            const _Float16 h = (_Float16)v;
+            q[n][s][0][e] = h;
+            total += (float)h;
+            if constexpr (QP == 2) {
+              const _Float16 l = (_Float16)(v - (float)h);
+              q[n][s][1][e] = l;
+              total += (float)l;
+            }
+          }
+        }
+      }
+      if (turn == 1) qsum[n] = quad_sum(total);
+    }
+    if (turn == 0) {
+#pragma unroll
+      for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
+      if (lane == 0) tops[wave] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < PWAVES; ++w) top = fmaxf(top, tops[w]);
+      ex = __builtin_amdgcn_readfirstlane(exponent_of(top) - 14);
+    }
+  }
+  const float factor = __builtin_ldexpf(a.scale, ex);
+
+  PromptState<ND, PP> st;
+  st.shift = -1000;
+#pragma unroll
+  for (int n = 0; n < PQ; ++n) {
+    st.top[n] = st.l[n] = st.z[n] = 0.f;
+    st.fresh[n] = true;
+#pragma unroll
+    for (int d = 0; d < 4 * ND; ++d) st.o[n][d] = (floatx4){0.f, 0.f, 0.f, 0.f};
+  }
+  const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + part * a.chunk);
+  const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
+  const int pos_lo = __builtin_amdgcn_readfirstlane(t.pos_lo), pos_hi = __builtin_amdgcn_readfirstlane(t.pos_hi);
+  const int hw = (int)kv_head_words(ND, c.page), len = t.len;
+  const int64_t b = t.b;
+  uint4v words[CH];
+  unsigned affine = 0;
+  int held = -1000;  // the shift that values are staged with
+  auto load = [&](const unsigned* base, int at) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int ch = wave + PWAVES * i;  // K's chunks, then V's
+      if (ch < 2 * ND)
+        words[i] = *reinterpret_cast<const uint4v*>(base + (ch < ND ? 0 : c.page * (8 * ND)) + at * (256 * ND) +
+                                                    (ch < ND ? ch : ch - ND) * 256 + lane * 4);
+    }
+    if (wave == 0) affine = base[c.page * (16 * ND + (lane >> 5)) + at * 32 + (lane & 31)];
+  };
+  auto put = [&](int kb, int buf) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int ch = wave + PWAVES * i;
+      if (ch < 2 * ND) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) ops[buf][4 * ch + w][lane] = centred_codes(words[i][w]);
+      }
+    }
+    if (wave == 0) {  // lanes 0..31 the keys, 32..63 the values
+      unsigned w = kb * 32 + (lane & 31) < len ? affine : 0u;  // beyond the sequence: whatever the page holds
+      const float s = __uint_as_float(w << 16), z = __builtin_fmaf(8.f, s, __uint_as_float(w & 0xffff0000u));
+      int big = lane >= 32 && (w >> 7 & 255u) != 255u ? (int)(w >> 7 & 255u) - 126 : -126;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int x = __shfl_xor(big, d);
+        big = x > big ? x : big;
+      }
+      big = __builtin_amdgcn_readfirstlane(big);
+      if (big > held) held = big + 2;  // room for scales four times as large
+      aff[buf][lane >> 5 << 1][lane & 31] = lane < 32 ? s * factor : __builtin_ldexpf(s, PROOM - held);
+      aff[buf][(lane >> 5 << 1) + 1][lane & 31] = lane < 32 ? z * factor : z;
+      if (lane == 0) shifts[buf] = held;
+    }
+  };
+  int at = 0, at2 = 0;
+  const unsigned* base = begin < end ? kv_head(c, b, begin, head, hw, at) : nullptr;
+  if (base) load(base, at);
+  const unsigned* next = begin + 1 < end ? kv_head(c, b, begin + 1, head, hw, at2) : nullptr;
+  if (base) put(begin, 0);
+  __syncthreads();
+  for (int kb = begin; kb < end; ++kb) {
+    const int buf = (kb - begin) & 1;
+    if (next) load(next, at2);
+    int at3 = 0;
+    const unsigned* after = kb + 2 < end ? kv_head(c, b, kb + 2, head, hw, at3) : nullptr;
+    if (base) {
+      const int shift = __builtin_amdgcn_readfirstlane(shifts[buf]);
+      if (shift != st.shift) {
+#pragma unroll
+        for (int n = 0; n < PQ; ++n)
+#pragma unroll
+          for (int d = 0; d < 4 * ND; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) st.o[n][d][i] = __builtin_ldexpf(st.o[n][d][i], st.shift - shift);
+        st.shift = shift;
+      }
+      const int key0 = kb * 32 + 4 * g;
+      if (kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window))
+        prompt_block<ND, QP, PP, false>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], lane, key0, pos, a.window);
+      else
+        prompt_block<ND, QP, PP, true>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], lane, key0, pos, a.window);
+    }
+    if (next) put(kb + 1, 1 - buf);
+    __syncthreads();
+    base = next, next = after, at2 = at3;
+  }
+#pragma unroll
+  for (int n = 0; n < PQ; ++n) {
+    const float l = quad_sum(st.l[n]), z = quad_sum(st.z[n]);
+    const int in = 16 * (PQ * wave + n) + (lane & 15);
+    const bool none = l == 0.f;
+    if (t.chunks > 1) {
+      float* out = a.part + ((slot * c.heads + head) * a.chunks + part) * (int64_t)(CT * (DP + 2));
+#pragma unroll
+      for (int d = 0; d < 4 * ND; ++d) {
+        floatx4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(st.o[n][d][i], st.shift - PROOM) + z;
+        if (valid[n]) *reinterpret_cast<floatx4*>(out + in * DP + 16 * d + 4 * g) = v;
+      }
+      if (valid[n] && g == 0) {
+        out[CT * DP + in] = none ? -__builtin_inff() : st.top[n];
+        out[CT * (DP + 1) + in] = l;
+      }
+    } else {
+      const int64_t row = t.row + row_of[n];
+      const float f = none ? 0.f : 1.f / l;
+      T* out = (T*)a.out + row * a.out_token + head_of[n] * a.out_head;
+#pragma unroll
+      for (int d = 0; d < 4 * ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = (__builtin_ldexpf(st.o[n][d][i], st.shift - PROOM) + z) * f;
+          const T x = from_f32<TYPE>(none ? 0.f : v);
+          if (valid[n] && 16 * d + 4 * g + i < c.dim) out[16 * d + 4 * g + i] = x;
+        }
+      if (valid[n] && a.lse && g == 0)
+        a.lse[row * (int64_t)(c.heads * a.group) + head_of[n]] = none ? -__builtin_inff() : (st.top[n] + __builtin_log2f(l)) * LN2;
+    }
+  }
+}
+
+// Joins the chunks' results: a wave a (token, query head), whose chunks are added in their order.
+template <int TYPE, int ND>
+__global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a, int CT) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr int DP = 64 * ND;
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = c.heads * a.group;
@@ -414,7 +713,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a) {
   const int hq = (int)(item - row * heads), head = hq / a.group;
   const int64_t seq = kv_find(c, row, 1, 1, 0);
   const int col = (int)(row - kv_offset(c, seq)) * a.group + hq % a.group;
-  const Tile t = make_tile<CT>(c, a, seq, col / CT * CT);
+  const Tile t = make_tile(c, a, seq, col / CT * CT, CT);
   if (t.chunks <= 1) return;
   const int64_t slot = kv_first_slot(c, seq, a.group, CT, 1) + col / CT;
   const int in = col % CT;
@@ -452,34 +751,47 @@ __global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a) {
 
 // How a call is split: columns of a workgroup and blocks of 32 keys of a chunk.
 struct Plan {
-  int nq, nd, chunk, chunks;
+  int nq, nd, ct, chunk, chunks;  // nq 0: prompt_kernel; ct: columns of a workgroup
   int64_t slots, part;  // part: floats of the partial results
 };
 
 inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int dim, int64_t most, int64_t window) {
   Plan p;
   p.nd = (dim + 63) / 64;
-  p.nq = p.nd > 2 || tokens * group <= 16 * seqs ? 1 : 2;
-  const int ct = 16 * p.nq;
-  p.slots = tokens * group / ct + seqs;
+  const int64_t columns = tokens * group;
+  p.nq = columns >= 64 * seqs ? 0 : p.nd > 2 || columns <= 16 * seqs ? 1 : 2;
+  p.ct = p.nq ? 16 * p.nq : 16 * PQ * PWAVES;
+  p.slots = columns / p.ct + seqs;
   int64_t range = most;
-  if (window && window + ct < range) range = window + ct;
+  if (window && window + p.ct < range) range = window + p.ct;
   const int64_t blocks = range / 32 + 2;
   const int64_t want = (blocks * p.slots * heads + 1023) / 1024;
-  p.chunk = (int)(want < 4 ? 4 : want > 64 ? 64 : want);
+  if (p.nq)
+    p.chunk = (int)(want < 4 ? 4 : want > 64 ? 64 : want);
+  else  // as many as fill the chip, no more: each writes its columns' sums
+    p.chunk = (int)(p.slots * heads >= 256 ? blocks : want < 16 ? 16 : want);
   p.chunks = (int)((blocks + p.chunk - 1) / p.chunk);
   if (p.chunks <= 1) p.chunks = 1;
-  p.part = p.chunks > 1 ? p.slots * heads * p.chunks * (int64_t)(ct * (64 * p.nd + 2)) : 0;
+  p.part = p.chunks > 1 ? p.slots * heads * p.chunks * (int64_t)(p.ct * (64 * p.nd + 2)) : 0;
   return p;
 }
 
-template <int TYPE, int ND, int NQ>
+template <int TYPE, int ND>
 int launch(const KvCache& c, const Attend& a, const Plan& p, hipStream_t st) {
-  hipLaunchKernelGGL((attend_kernel<TYPE, ND, NQ>), dim3((unsigned)p.slots, (unsigned)c.heads, (unsigned)p.chunks),
-                     dim3(THREADS), 0, st, c, a);
+  const dim3 grid((unsigned)p.slots, (unsigned)c.heads, (unsigned)p.chunks), block(THREADS);
+  if (p.nq == 0) {  // heads first: the workgroups of one XCD (every eighth) then read few heads' keys and values
+    const int64_t turns = cdiv(p.slots, 65535);
+    hipLaunchKernelGGL((prompt_kernel<TYPE, ND>),
+                       dim3((unsigned)c.heads, (unsigned)cdiv(p.slots, turns), (unsigned)(p.chunks * turns)),
+                       dim3(64 * PWAVES), 0, st, c, a);
+  } else if (p.nq == 1) {
+    hipLaunchKernelGGL((attend_kernel<TYPE, ND, 1>), grid, block, 0, st, c, a);
+  } else {
+    if constexpr (ND <= 2) hipLaunchKernelGGL((attend_kernel<TYPE, ND, 2>), grid, block, 0, st, c, a);
+  }
   if (p.chunks > 1)
-    hipLaunchKernelGGL((join_kernel<TYPE, ND, NQ>), dim3((unsigned)cdiv(c.tokens * c.heads * a.group, WAVES)),
-                       dim3(THREADS), 0, st, c, a);
+    hipLaunchKernelGGL((join_kernel<TYPE, ND>), dim3((unsigned)cdiv(c.tokens * c.heads * a.group, WAVES)), block, 0, st, c, a,
+                       p.ct);
   return (int)hipGetLastError();
 }
 
@@ -487,13 +799,13 @@ template <int TYPE>
 int launch_type(const KvCache& c, const Attend& a, const Plan& p, hipStream_t st) {
   switch (p.nd) {
     case 1:
-      return p.nq == 1 ? launch<TYPE, 1, 1>(c, a, p, st) : launch<TYPE, 1, 2>(c, a, p, st);
+      return launch<TYPE, 1>(c, a, p, st);
     case 2:
-      return p.nq == 1 ? launch<TYPE, 2, 1>(c, a, p, st) : launch<TYPE, 2, 2>(c, a, p, st);
+      return launch<TYPE, 2>(c, a, p, st);
     case 3:
-      return launch<TYPE, 3, 1>(c, a, p, st);
+      return launch<TYPE, 3>(c, a, p, st);
     case 4:
-      return launch<TYPE, 4, 1>(c, a, p, st);
+      return launch<TYPE, 4>(c, a, p, st);
   }
   return GPTQ2D_EINVAL;
 }
@@ -525,7 +837,7 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
     return GPTQ2D_EINVAL;
   if (tokens == 0 || seqs == 0) return 0;
   const Plan p = make_plan(tokens, seqs, heads, group, dim, width * page, window);
-  if (p.slots > 0x7fffffff || p.chunks > 65535) return GPTQ2D_EUNSUPPORTED;
+  if (p.slots > 0x7fffffff || p.chunks * (p.nq ? 1 : cdiv(p.slots, 65535)) > 65535) return GPTQ2D_EUNSUPPORTED;
   if (work_bytes < 4 * p.part || (p.part && (!work || (uintptr_t)work % 16))) return GPTQ2D_ESCRATCH;
   Attend a;
   a.q = q, a.q_token = q_token, a.q_head = q_head;

@@ -189,6 +189,11 @@ CASES = [  # held, new, kv heads, group, dim, page, window
     ([77, 12], [3, 2], 3, 1, 33, 32, None),
     ([40000, 700], [1, 1], 1, 4, 128, 128, None),            # chunks that are joined
     ([3000], [150], 1, 8, 128, 64, 500),
+    ([300, 90, 0, 70], [200, 90, 5, 70], 2, 3, 80, 32, None),  # many columns: prompts, ragged, one longer than what is held
+    ([500], [300], 1, 2, 256, 96, 70),
+    ([257, 31], [131, 31], 1, 5, 192, 32, None),
+    ([200], [70], 3, 1, 33, 32, 1),
+    ([9000], [70], 1, 1, 64, 128, None),                         # few columns of long keys: chunks of a prompt
 ]
 
 
@@ -229,7 +234,23 @@ def test_attend_large_scores_and_scales():
         assert bool(((got.cpu().double() - want).abs() <= allowed).all())
 
 
-def test_nan_and_infinity_where_nothing_looks():
+@pytest.mark.parametrize("sign", [-1., 1.])
+@pytest.mark.parametrize("new", [1, 5, 80])
+def test_scores_all_far_from_zero(new, sign):
+    """All scores near -3000 or 3000 (far below or above any fixed reference), rising along the keys by 400."""
+    g = torch.Generator().manual_seed(new)
+    k = 0.05 * torch.randn(300, 1, 64, generator=g) + torch.linspace(85., 95., 300).view(-1, 1, 1) * sign
+    s = Sequences([300], 1, 64, torch.float32, 32, k=k, seed=1)
+    q = 4.2 + 0.05 * torch.randn(new, 2, 64, generator=g)
+    want, want_lse = s.reference(q, [new], 0.125, None)
+    got, lse = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), starts([new]), scale=0.125, return_lse=True)
+    # scores of 3000 in fp32: off by 3000 x 2^-24 x sqrt(64) x 2 = 3e-3 at most
+    assert float((got.cpu().double() - want).abs().max()) < 3e-3 * float(held_values(s.v).abs().max())
+    assert float((lse.cpu().double() - want_lse).abs().max()) < 3e-3
+
+
+@pytest.mark.parametrize("new", [15, 60])
+def test_nan_and_infinity_where_nothing_looks(new):
     """A token whose key or value is NaN or infinite changes the queries that see it and no others."""
     for what in (math.nan, math.inf, -math.inf):
         for which in ("k", "v"):
@@ -239,12 +260,12 @@ def test_nan_and_infinity_where_nothing_looks():
             bad = {"k": k, "v": v}[which]
             bad[390, 1, 17] = what
             dirty = Sequences([400], 2, 128, torch.bfloat16, 32, k=k, v=v)
-            q = torch.randn(60, 8, 128, generator=g).bfloat16().to(DEV)
+            q = torch.randn(new, 8, 128, generator=g).bfloat16().to(DEV)
             for window in (None, 4):
-                a = clean.cache.attend(q, clean.dev_table, clean.lengths(), starts([60]), window=window).cpu()
-                b = dirty.cache.attend(q, dirty.dev_table, dirty.lengths(), starts([60]), window=window).cpu()
-                sees = torch.zeros(60, dtype=torch.bool)
-                sees[50:54 if window else 60] = True
+                a = clean.cache.attend(q, clean.dev_table, clean.lengths(), starts([new]), window=window).cpu()
+                b = dirty.cache.attend(q, dirty.dev_table, dirty.lengths(), starts([new]), window=window).cpu()
+                sees = torch.zeros(new, dtype=torch.bool)
+                sees[new - 10:new - 6 if window else new] = True
                 assert torch.equal(a[:, :4], b[:, :4]), "the other kv head"
                 assert torch.equal(a[~sees], b[~sees]), "queries that do not see the token"
                 assert bool(b[sees][:, 4:].isnan().all())
