@@ -94,12 +94,19 @@ __global__ __launch_bounds__(THREADS) void append_kernel(KvCache c, Rows r) {
     s = s == 0.f ? 1.f : s;
     const float z = round_to_bf16(lo);
     if (part == 0) affine[token] = __float_as_uint(s) >> 16 | (__float_as_uint(z) & 0xffff0000u);
+    // The quotient (x - z) / s as IEEE rounds it, from the correctly rounded 1 / s and one correction with the exact
+    // remainder (Markstein's method), where s is in a range in which nothing on the way leaves the normal numbers (the
+    // differences are below 2^5 s, and below 2^-24 of s they round to code 0 whatever the remainder); a division otherwise.
+    const float rcp = 1.f / s;
+    const bool plain = s >= 0x1p-60f && s <= 0x1p60f;
     unsigned code[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      float q = round_even((x[i] - z) / s);
-      q = q > 0.f ? q : 0.f;  // also for a NaN
-      code[i] = (unsigned)(q < 15.f ? q : 15.f);
+      const float y = x[i] - z, q0 = y * rcp;
+      float q = __builtin_fmaf(__builtin_fmaf(-q0, s, y), rcp, q0);
+      if (!plain) q = y / s;
+      q = __builtin_amdgcn_fmed3f(round_even(q), 0.f, 15.f);
+      code[i] = q == q ? (unsigned)q : 0u;
     }
     if (value) {
 #pragma unroll
@@ -151,10 +158,15 @@ __global__ __launch_bounds__(THREADS) void append_kernel(KvCache c, Rows r) {
   }
 }
 
+// A block's words go through LDS, so that both they and the values lie in order in memory: a thread gives eight elements
+// of one token, from one word of K or from one nibble each of eight words of V.
 template <int TYPE, int ND>
 __global__ __launch_bounds__(THREADS) void read_kernel(KvCache c, Rows r) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int DP = 64 * ND;
+  constexpr int DP = 64 * ND, V = 16 / (int)sizeof(T);  // elements of a 16-byte store
+  typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  alignas(16) __shared__ unsigned words[DP * 4];
+  __shared__ unsigned affine[32];
   const BlockIds id = block_ids(c, blockIdx.x, true);
   const int h = blockIdx.y;
   const bool value = blockIdx.z;
@@ -169,33 +181,53 @@ __global__ __launch_bounds__(THREADS) void read_kernel(KvCache c, Rows r) {
   const int hw = (int)kv_head_words(ND, c.page);
   int at;
   const unsigned* base = kv_head(c, id.b, id.kb, h, hw, at);
-  const unsigned* in = base + (value ? (int64_t)c.page * 8 * ND : 0) + at * (DP * 4);
-  const unsigned* in_affine = base + (int64_t)c.page * (16 * ND + (value ? 1 : 0)) + at * 32;
+  if (base) {
+    const unsigned* in = base + (value ? (int64_t)c.page * 8 * ND : 0) + at * (DP * 4);
+    if (ND % 4 == 0 || threadIdx.x < DP) {
 #pragma unroll
-  for (int j = 0; j < ND; ++j) {  // a word a thread and turn; where the table's entry is no page, zeros
-    const int i = THREADS * j + threadIdx.x, W = i / 256 * 4 + i % 4, lane = i / 4 % 64, g = lane / 16;
-    const int key = W / (2 * ND) * 16 + lane % 16;
-    unsigned w = 0, a[8] = {};
-    if (base) {
-      w = in[i];
-      if (value) {
-        const uint4v a0 = *reinterpret_cast<const uint4v*>(in_affine + 4 * g);
-        const uint4v a1 = *reinterpret_cast<const uint4v*>(in_affine + 4 * g + 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = a0[e], a[e + 4] = a1[e];
-      } else {
-        a[0] = in_affine[key];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) a[e] = a[0];
-      }
+      for (int j = 0; j < (ND + 3) / 4; ++j)
+        reinterpret_cast<uint4v*>(words)[THREADS * j + threadIdx.x] = reinterpret_cast<const uint4v*>(in)[THREADS * j + threadIdx.x];
     }
+    if (threadIdx.x < 32) affine[threadIdx.x] = base[(int64_t)c.page * (16 * ND + (value ? 1 : 0)) + at * 32 + threadIdx.x];
+  } else {  // the table's entry is no page: zeros
+    for (int i = threadIdx.x; i < DP * 4; i += THREADS) words[i] = 0;
+    if (threadIdx.x < 32) affine[threadIdx.x] = 0;
+  }
+  __syncthreads();
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int token = value ? 4 * g + e % 4 + e / 4 * 16 : key;
-      const int d = value ? 16 * W + lane % 16 : 32 * (W % (2 * ND)) + 8 * g + e;
-      const float x = __builtin_fmaf((float)(w >> (e / 2 * 4 + e % 2 * 16) & 15u), __uint_as_float(a[e] << 16),
-                                     __uint_as_float(a[e] & 0xffff0000u));
-      if (token >= id.first && token < id.last && d < c.dim) out[(id.row0 + token) * stride + d] = from_f32<TYPE>(x);
+  for (int j = 0; j < ND; ++j) {
+    const int i = THREADS * j + threadIdx.x, token = i / (8 * ND), d = i % (8 * ND) * 8;
+    const unsigned a = affine[token];
+    const float s = __uint_as_float(a << 16), z = __uint_as_float(a & 0xffff0000u);
+    unsigned w[8];
+    int shift[8];
+    if (value) {
+      const int e = token % 4 + token / 16 * 4, lane = d % 16 + 16 * (token / 4 % 4), W = d / 16;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = words[W / 4 * 256 + (lane + k) * 4 + W % 4], shift[k] = e / 2 * 4 + e % 2 * 16;
+    } else {
+      const int W = 2 * ND * (token / 16) + d / 32;
+      w[0] = words[W / 4 * 256 + (token % 16 + 16 * (d / 8 % 4)) * 4 + W % 4];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = w[0], shift[k] = k / 2 * 4 + k % 2 * 16;
+    }
+    T x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = from_f32<TYPE>(__builtin_fmaf((float)(w[k] >> shift[k] & 15u), s, z));
+    T* to = out + (id.row0 + token) * stride + d;
+    const bool in = token >= id.first && token < id.last;
+    if (in && d + 8 <= c.dim) {
+#pragma unroll
+      for (int k = 0; k < 8; k += V) {
+        vec v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = x[k + e];
+        *reinterpret_cast<vec*>(to + k) = v;
+      }
+    } else if (in) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (d + k < c.dim) to[k] = x[k];
     }
   }
 }

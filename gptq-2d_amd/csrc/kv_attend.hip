@@ -77,165 +77,253 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// A column's query as B operands, QP pieces; `factor` takes the products' sums back to scores, `sum` is the sum of what
-// the operands hold.
-template <int TYPE, int ND, int QP>
-__device__ __forceinline__ void load_query(half8 (&q)[2 * ND][QP], float& factor, float& sum,
-                                           const typename Elem<TYPE>::T* row, bool valid, int dim, int g, float scale) {
-  float x[2 * ND][8];
+// The queries of NQ x 16 columns as B operands, QP pieces, scaled by one power of two for all columns of the workgroup (its
+// largest element to 2^14..2^15, found by the first pass over them; `tops`: LDS for WV waves); `sum` is the sum of what a
+// column's operands hold.  Returns the exponent that takes the products back.
+template <int TYPE, int ND, int NQ, int QP, int WV>
+__device__ __forceinline__ int load_queries(half8 (&q)[NQ][2 * ND][QP], float (&sum)[NQ],
+                                            const typename Elem<TYPE>::T* const (&row)[NQ], const bool (&valid)[NQ], int dim,
+                                            float* tops) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
   float top = 0.f;
+#pragma unroll 1
+  for (int s = 0; s < 2 * ND; ++s)
 #pragma unroll
-  for (int s = 0; s < 2 * ND; ++s) {
-    if (valid) {
-      load_row<TYPE, 8>(x[s], row, 32 * s + 8 * g, dim);
-    } else {
+    for (int n = 0; n < NQ; ++n) {
+      float x[8];
+      load_row<TYPE, 8>(x, row[n], 32 * s + 8 * g, valid[n] ? dim : 0);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = __builtin_fabsf(x[s][e]);
-      top = v < __builtin_inff() && v > top ? v : top;  // infinities and NaN stay what they are in fp16
-    }
-  }
-  top = quad_max(top);
-  const int ex = exponent_of(top) - 14;
-  float total = 0.f;
-#pragma unroll
-  for (int s = 0; s < 2 * ND; ++s) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = __builtin_ldexpf(x[s][e], -ex);
-      const _Float16 h = (_Float16)v;
-      q[s][0][e] = h;
-      total += (float)h;
-      if constexpr (QP == 2) {
-        const _Float16 l = (_Float16)(v - (float)h);
-        q[s][1][e] = l;
-        total += (float)l;
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_fabsf(x[e]);
+        top = v < __builtin_inff() && v > top ? v : top;  // infinities and NaN stay what they are in fp16
       }
     }
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
+  if (WV > 1) {
+    if (lane == 0) tops[wave] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WV; ++w) top = fmaxf(top, tops[w]);
   }
-  sum = quad_sum(total);
-  factor = __builtin_ldexpf(scale, ex);
-}
-
-// Running state of a wave's columns over its keys.
-template <int ND, int NQ>
-struct State {
-  floatx4 o[NQ][4 * ND];  // elements 16 t + 4 g .. + 3 of column l % 16, times 2^(ROOM - shift)
-  float top[NQ], l[NQ], z[NQ];  // maximum (all lanes of the column), this lane's sums of p and of p (z + 8 s)
-  int shift;                    // p s is held as p s 2^-shift in fp16
-};
-
-// p s 2^(ROOM - shift) <= 2^ROOM in fp16: the smaller ones keep their 11 bits down to 2^-28 of that.
-constexpr int ROOM = 14;
-
-// One block of 32 keys: kw, vw its codes' words, ka, va its scales and zeros (key 16 t + 4 g + i of this lane).
-template <int ND, int NQ, int QP, int PP, bool MASK>
-__device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)[NQ][2 * ND][QP], const float (&factor)[NQ],
-                                             const float (&qsum)[NQ], const uint4v (&kw)[ND], const uint4v (&vw)[ND],
-                                             const uint4v (&ka)[2], const uint4v (&va)[2], int key0, int len,
-                                             const int (&pos)[NQ], int window) {
-  floatx4 s[NQ][2];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = (floatx4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int W = 0; W < 4 * ND; ++W) {
-    const half8 k = centred_codes(kw[W / 4][W % 4]);
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int p = 0; p < QP; ++p) s[n][W / (2 * ND)] = mfma(k, q[n][W % (2 * ND)][p], s[n][W / (2 * ND)]);
-  }
-  float vs[8], vz[8];
-  int big = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    unsigned w = va[i / 4][i % 4];
-    if (MASK && key0 + 16 * (i / 4) + i % 4 >= len) w = 0;  // beyond the sequence: whatever the page holds
-    const int ex = (int)(w >> 7 & 255u);
-    if (ex != 255) big = ex > big ? ex : big;
-    vs[i] = __uint_as_float(w << 16);
-    vz[i] = __builtin_fmaf(8.f, vs[i], __uint_as_float(w & 0xffff0000u));
-  }
-  // a larger scale than any before: the sums so far move to its range (with room for twice four more)
-  if (__builtin_amdgcn_ballot_w64(big - 126 > st.shift)) {
-    int most = __shfl_xor(big, 16);
-    most = most > big ? most : big;
-    const int other = __shfl_xor(most, 32);
-    most = most > other ? most : other;
-    most = __builtin_amdgcn_readfirstlane(most) - 126 + 2;
-#pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int t = 0; t < 4 * ND; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[n][t][i] = __builtin_ldexpf(st.o[n][t][i], st.shift - most);
-    st.shift = most;
-  }
-  half8 p[NQ][PP];
+  const int ex = __builtin_amdgcn_readfirstlane(exponent_of(top) - 14);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
-    float t[8];
-    float top = -__builtin_inff();
+    float total = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned w = ka[i / 4][i % 4];
-      const float ks = __uint_as_float(w << 16), kz = __builtin_fmaf(8.f, ks, __uint_as_float(w & 0xffff0000u));
-      t[i] = __builtin_fmaf(ks, s[n][i / 4][i % 4], kz * qsum[n]) * factor[n];
-      if constexpr (MASK) {
+    for (int s = 0; s < 2 * ND; ++s) {
+      float x[8];
+      load_row<TYPE, 8>(x, row[n], 32 * s + 8 * g, valid[n] ? dim : 0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = __builtin_ldexpf(x[e], -ex);
+        const _Float16 h = (_Float16)v;
+        q[n][s][0][e] = h;
+        total += (float)h;
+        if constexpr (QP == 2) {
+          const _Float16 l = (_Float16)(v - (float)h);
+          q[n][s][1][e] = l;
+          total += (float)l;
+        }
+      }
+    }
+    sum[n] = quad_sum(total);
+  }
+  return ex;
+}
+
+// Softmax over a wave's columns, a block of 32 keys at a time.  Bound by vector instructions, so a score takes few: its
+// exponent is two fused multiply-adds off a reference that is the maximum of some block before, not of this one -- it moves
+// when a score exceeds it by 2^AHEAD, which needs no maximum over the lanes to be seen --, then one each for the exponential,
+// its product with the value's scale and the two sums, and half of one each for the comparison and the conversion.
+constexpr int AHEAD = 8;  // log2 of how far weights may exceed 1
+constexpr int ROOM = 7;   // weights times scales are held as p s 2^(ROOM - shift) <= 2^(ROOM + AHEAD) in fp16: s < 2^shift
+
+template <int ND, int NQ>
+struct State {
+  floatx4 o[NQ][4 * ND];        // elements 16 t + 4 g .. + 3 of column l % 16, times 2^(ROOM - shift)
+  float top[NQ], l[NQ], z[NQ];  // reference; this lane's sums of p and of p (z + 8 s)
+  bool fresh[NQ];               // the column has not seen a key: its reference is still to be taken, however low
+  int shift;
+};
+
+template <int ND, int NQ>
+__device__ __forceinline__ void clear(State<ND, NQ>& st) {
+  st.shift = -1000;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    st.top[n] = st.l[n] = st.z[n] = 0.f;
+    st.fresh[n] = true;
+#pragma unroll
+    for (int d = 0; d < 4 * ND; ++d) st.o[n][d] = (floatx4){0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// Exponents e of a block's scores off the reference, and the sums so far brought to the values' new `shift` and, where a
+// column's reference moves, to it -- in one place, so that the sums stay in their registers.  key0: this lane's first key
+// (keys key0 + 16 (i / 4) + i % 4); ks, kz: scales and zeros with what all columns share in them.
+template <int ND, int NQ>
+__device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], const floatx4 (&s)[NQ][2], const float (&ks)[8],
+                                          const float (&kz)[8], const float (&qsum)[NQ], bool mask, int key0,
+                                          const int (&pos)[NQ], int window, int shift) {
+  float most[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      e[n][i] = __builtin_fmaf(ks[i], s[n][i / 4][i % 4], __builtin_fmaf(kz[i], qsum[n], -st.top[n]));
+  if (mask) {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const int from = window ? pos[n] - window : -1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
         const int key = key0 + 16 * (i / 4) + i % 4;
-        if (key > pos[n] || (window && key <= pos[n] - window)) t[i] = -__builtin_inff();
+        e[n][i] = key > pos[n] || key <= from ? -__builtin_inff() : e[n][i];
       }
-      top = t[i] > top || t[i] != t[i] ? t[i] : top;
-    }
-    {
-      const float a = __shfl_xor(top, 16);
-      top = a > top || a != a ? a : top;
-      const float b = __shfl_xor(top, 32);
-      top = b > top || b != b ? b : top;
-    }
-    if (__builtin_amdgcn_ballot_w64(top > st.top[n] || top != top)) {
-      const float now = top > st.top[n] || top != top ? top : st.top[n];
-      const float f = now == st.top[n] ? 1.f : __builtin_amdgcn_exp2f(st.top[n] - now);
-      st.top[n] = now;
-      st.l[n] *= f;
-      st.z[n] *= f;
-#pragma unroll
-      for (int d = 0; d < 4 * ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[n][d][i] *= f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float w = __builtin_amdgcn_exp2f(t[i] - st.top[n]);
-      float ps = __builtin_ldexpf(w * vs[i], ROOM - st.shift), pz = w * vz[i];
-      if constexpr (MASK) {
-        const bool hidden = t[i] == -__builtin_inff();
-        w = hidden ? 0.f : w, ps = hidden ? 0.f : ps, pz = hidden ? 0.f : pz;
-      }
-      st.l[n] += w;
-      st.z[n] += pz;
-      const _Float16 h = (_Float16)ps;
-      p[n][0][i] = h;
-      if constexpr (PP == 2) p[n][1][i] = (_Float16)(ps - (float)h);
     }
   }
+  bool move = shift != st.shift;
 #pragma unroll
-  for (int W = 0; W < 4 * ND; ++W) {
-    const half8 v = centred_codes(vw[W / 4][W % 4]);
+  for (int n = 0; n < NQ; ++n) {
+    most[n] = e[n][0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most[n] = fmaxf(most[n], e[n][i]);
+    move |= most[n] > (st.fresh[n] ? -__builtin_inff() : (float)AHEAD);
+  }
+  if (__builtin_amdgcn_ballot_w64(move)) {
+    const int less = st.shift - shift;
+    st.shift = shift;
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      const float m = quad_max(most[n]);
+      const float up = st.fresh[n] ? (m == -__builtin_inff() ? 0.f : m) : m > (float)AHEAD ? m : 0.f;
+      const float f = st.fresh[n] ? 1.f : __builtin_amdgcn_exp2f(-up);  // sums of 0 stay, however far down it goes
+      st.fresh[n] = st.fresh[n] && m == -__builtin_inff();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[n][i] -= up;
+      st.top[n] += up;
+      st.l[n] *= f;
+      st.z[n] *= f;
+      const float f2 = __builtin_ldexpf(f, less);
+#pragma unroll
+      for (int d = 0; d < 4 * ND; ++d) st.o[n][d] *= f2;
+    }
+  }
+}
+
+// The block's weights: p s as B operands in PP pieces, and the sums of p and p (z + 8 s).
+template <int ND, int NQ, int PP>
+__device__ __forceinline__ void weights(State<ND, NQ>& st, half8 (&p)[NQ][PP], const float (&e)[NQ][8], const float (&vs)[8],
+                                        const float (&vz)[8], bool mask) {
+  float ps[NQ][8];
+  if (mask) {  // a scale or zero that is no number must not reach columns that do not see its key
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
-      for (int r = 0; r < PP; ++r) st.o[n][W] = mfma(v, p[n][r], st.o[n][W]);
+      for (int i = 0; i < 8; ++i) {
+        const bool hidden = e[n][i] == -__builtin_inff();
+        const float w = __builtin_amdgcn_exp2f(e[n][i]), z = w * vz[i];
+        ps[n][i] = hidden ? 0.f : w * vs[i];
+        st.l[n] += w;
+        st.z[n] += hidden ? 0.f : z;
+      }
+  } else {
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float w = __builtin_amdgcn_exp2f(e[n][i]);
+        ps[n][i] = w * vs[i];
+        st.l[n] += w;
+        st.z[n] = __builtin_fmaf(w, vz[i], st.z[n]);
+      }
   }
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const _Float16 h = (_Float16)ps[n][i];
+      p[n][0][i] = h;
+      if constexpr (PP == 2) p[n][1][i] = (_Float16)(ps[n][i] - (float)h);
+    }
+}
+
+// The shift that admits the scales whose largest bits (of 32) this lane found to be `bits`: the present one where it does.
+__device__ __forceinline__ int admit(int shift, unsigned bits, const float (&s)[8]) {
+  const int limit = shift < -126 ? 0 : (shift + 127) << 23;  // bits of 2^shift
+  if (!__builtin_amdgcn_ballot_w64((int)bits >= limit)) return shift;
+  int big = -126;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {  // infinities and NaN apart
+    const int ex = (int)(__float_as_uint(s[i]) >> 23 & 255u);
+    big = ex != 255 && ex - 126 > big ? ex - 126 : big;
+  }
+  int x = __shfl_xor(big, 16);
+  big = x > big ? x : big;
+  x = __shfl_xor(big, 32);
+  big = __builtin_amdgcn_readfirstlane(x > big ? x : big);
+  return big > shift ? big + 2 : shift;  // with room for scales four times as large
 }
 
 template <int ND>
 struct Words {
   uint4v kw[ND], vw[ND], ka[2], va[2];
 };
+
+// Scales and zeros of this lane's eight keys: s and z + 8 s; keys from `left` on are beyond the sequence, whatever the page
+// holds (left: 8 where none is).
+__device__ __forceinline__ void unpack_affine(float (&s)[8], float (&z)[8], const uint4v (&w)[2], bool mask, int key0, int len) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    unsigned u = w[i / 4][i % 4];
+    if (mask) u = key0 + 16 * (i / 4) + i % 4 < len ? u : 0u;
+    s[i] = __uint_as_float(u << 16);
+    z[i] = __builtin_fmaf(8.f, s[i], __uint_as_float(u & 0xffff0000u));
+  }
+}
+
+template <int ND, int NQ, int QP, int PP>
+__device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)[NQ][2 * ND][QP], const float (&qsum)[NQ],
+                                             const Words<ND>& w, float factor, bool mask, int key0, int len,
+                                             const int (&pos)[NQ], int window) {
+  floatx4 s[NQ][2];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4 * ND; ++i) {
+    const int W = i / 2 + i % 2 * (2 * ND);  // the two tiles of keys in turn
+    const half8 k = centred_codes(w.kw[W / 4][W % 4]);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int p = 0; p < QP; ++p) s[n][i % 2] = mfma(k, q[n][i / 2][p], s[n][i % 2]);
+  }
+  float ks[8], kz[8], vs[8], vz[8], e[NQ][8];
+  unpack_affine(ks, kz, w.ka, mask, key0, len);
+  unpack_affine(vs, vz, w.va, mask, key0, len);
+  unsigned bits = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const unsigned u = __float_as_uint(vs[i]) & 0x7fffffffu;  // a NaN may have any sign
+    bits = u > bits ? u : bits;
+    ks[i] *= factor, kz[i] *= factor;
+  }
+  const int shift = admit(st.shift, bits, vs);
+  exponents<ND, NQ>(st, e, s, ks, kz, qsum, mask, key0, pos, window, shift);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) vs[i] = __builtin_ldexpf(vs[i], ROOM - shift);
+  half8 p[NQ][PP];
+  weights<ND, NQ, PP>(st, p, e, vs, vz, mask);
+#pragma unroll
+  for (int W = 0; W < 4 * ND; ++W) {
+    const half8 v = centred_codes(w.vw[W / 4][W % 4]);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int r = 0; r < PP; ++r) st.o[n][W] = mfma(v, p[n][r], st.o[n][W]);
+  }
+}
 
 template <int ND>
 __device__ __forceinline__ void load_block(Words<ND>& w, const unsigned* base, int at, int page, int lane) {
@@ -271,25 +359,20 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
 
   half8 q[NQ][2 * ND][QP];
-  float factor[NQ], qsum[NQ];
+  float qsum[NQ];
   int pos[NQ];
+  bool valid[NQ];
+  const T* rows[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int col = t.col0 + 16 * n + (lane & 15), token = col / a.group, hq = head * a.group + col % a.group;
-    const bool valid = col < t.cols;
-    pos[n] = valid ? t.pos0 + token : t.pos_hi;
-    load_query<TYPE, ND, QP>(q[n], factor[n], qsum[n],
-                             (const T*)a.q + (t.row + token) * a.q_token + hq * a.q_head, valid, c.dim, g, a.scale);
+    valid[n] = col < t.cols;
+    pos[n] = valid[n] ? t.pos0 + token : t.pos_hi;
+    rows[n] = (const T*)a.q + (t.row + (valid[n] ? token : 0)) * a.q_token + hq * a.q_head;
   }
+  const float factor = __builtin_ldexpf(a.scale, load_queries<TYPE, ND, NQ, QP, 1>(q, qsum, rows, valid, c.dim, nullptr));
   State<ND, NQ> st;
-  st.shift = -1000;
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    st.top[n] = -__builtin_inff();
-    st.l[n] = st.z[n] = 0.f;
-#pragma unroll
-    for (int d = 0; d < 4 * ND; ++d) st.o[n][d] = (floatx4){0.f, 0.f, 0.f, 0.f};
-  }
+  clear(st);
   const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + chunk * a.chunk);
   const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
   const int pos_lo = __builtin_amdgcn_readfirstlane(t.pos_lo), pos_hi = __builtin_amdgcn_readfirstlane(t.pos_hi);
@@ -308,11 +391,8 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
     int at3 = 0;
     const unsigned* after = kb + 2 * WAVES < end ? kv_head(c, b, kb + 2 * WAVES, head, hw, at3) : nullptr;
     if (base) {
-      const int key0 = kb * 32 + 4 * g;
-      if (kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window))
-        attend_block<ND, NQ, QP, PP, false>(st, q, factor, qsum, cur.kw, cur.vw, cur.ka, cur.va, key0, t.len, pos, a.window);
-      else
-        attend_block<ND, NQ, QP, PP, true>(st, q, factor, qsum, cur.kw, cur.vw, cur.ka, cur.va, key0, t.len, pos, a.window);
+      const bool mask = !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
+      attend_block<ND, NQ, QP, PP>(st, q, qsum, cur, factor, mask, kb * 32 + 4 * g, t.len, pos, a.window);
     }
     cur = ahead;
     base = next;
@@ -323,6 +403,7 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
   for (int n = 0; n < NQ; ++n) {
     st.l[n] = quad_sum(st.l[n]);
     st.z[n] = quad_sum(st.z[n]);
+    if (st.fresh[n]) st.top[n] = -__builtin_inff();
     if (g == 0) {
       tops[wave][16 * n + lane] = st.top[n];
       ls[wave][16 * n + lane] = st.l[n];
@@ -403,101 +484,44 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
 // Many columns (a prompt's tokens times the heads that share a kv head).  A workgroup takes 32 columns a wave and `chunk` blocks of
 // 32 keys; the block's codes are brought to fp16 once, by all waves, into LDS, where they lie as operands (two blocks in
 // turn, one barrier a block; the next one's words are in flight meanwhile), and its scales and zeros in fp32 with what all
-// columns share already in them.  Bound by the vector instructions of the softmax, so a score takes few: its exponent is
-// two fused multiply-adds off a reference that is the maximum of some block before, not of this one -- it moves when a score
-// exceeds it by 2^8, which needs no maximum over the lanes to be seen --, then one each for the exponential, its product
-// with the value's scale, the two sums, and half of one each for the comparison and the conversion.
+// columns share already in them.
 constexpr int PQ = 2, PWAVES = 4;  // columns of a wave: 16 PQ
-constexpr int AHEAD = 8;           // log2 of how far weights may exceed 1
-constexpr int PROOM = 7;           // weights times scales are held as p s 2^(PROOM - shift), at most 2^(PROOM + AHEAD)
 
-template <int ND, int PP>
-struct PromptState {
-  floatx4 o[PQ][4 * ND];
-  float top[PQ], l[PQ], z[PQ];
-  bool fresh[PQ];  // a column that has not seen a key: its reference is still to be taken, however low
-  int shift;
-};
-
-template <int ND, int QP, int PP, bool MASK>
-__device__ __forceinline__ void prompt_block(PromptState<ND, PP>& st, const half8 (&q)[PQ][2 * ND][QP],
-                                             const float (&qsum)[PQ], const half8 (*kop)[64], const half8 (*vop)[64],
-                                             const float (*aff)[32], int lane, int key0, const int (&pos)[PQ], int window) {
-  const int g = lane >> 4;
-  float e[PQ][8], most[PQ];
-#pragma unroll
-  for (int n = 0; n < PQ; ++n) most[n] = -__builtin_inff();
+template <int ND, int QP, int PP>
+__device__ __forceinline__ void prompt_block(State<ND, PQ>& st, const half8 (&q)[PQ][2 * ND][QP], const float (&qsum)[PQ],
+                                             const half8 (*kop)[64], const half8 (*vop)[64], const float (*aff)[32], bool mask,
+                                             int key0, const int (&pos)[PQ], int window, int shift) {
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  floatx4 s[PQ][2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    floatx4 s[PQ];
 #pragma unroll
-    for (int n = 0; n < PQ; ++n) s[n] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < PQ; ++n) s[n][t] = (floatx4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 2 * ND; ++i) {
       const half8 k = kop[2 * ND * t + i][lane];
 #pragma unroll
       for (int n = 0; n < PQ; ++n)
 #pragma unroll
-        for (int p = 0; p < QP; ++p) s[n] = mfma(k, q[n][i][p], s[n]);
-    }
-    const floatx4 ks = *reinterpret_cast<const floatx4*>(&aff[0][16 * t + 4 * g]);
-    const floatx4 kz = *reinterpret_cast<const floatx4*>(&aff[1][16 * t + 4 * g]);
-#pragma unroll
-    for (int n = 0; n < PQ; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x = __builtin_fmaf(ks[i], s[n][i], __builtin_fmaf(kz[i], qsum[n], -st.top[n]));
-        if constexpr (MASK) {
-          const int key = key0 + 16 * t + i;
-          if (key > pos[n] || (window && key <= pos[n] - window)) x = -__builtin_inff();
-        }
-        e[n][4 * t + i] = x;
-        most[n] = fmaxf(most[n], x);
-      }
-  }
-  bool move = false;
-#pragma unroll
-  for (int n = 0; n < PQ; ++n) move |= most[n] > (st.fresh[n] ? -__builtin_inff() : (float)AHEAD);
-  if (__builtin_amdgcn_ballot_w64(move)) {  // the reference moves up to this block's maximum
-#pragma unroll
-    for (int n = 0; n < PQ; ++n) {
-      const float m = quad_max(most[n]);
-      const float up = st.fresh[n] ? (m == -__builtin_inff() ? 0.f : m) : fmaxf(m, 0.f);
-      const float f = st.fresh[n] ? 1.f : __builtin_amdgcn_exp2f(-up);  // sums of 0 stay, however far down it goes
-      st.fresh[n] = st.fresh[n] && m == -__builtin_inff();
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[n][i] -= up;
-      st.top[n] += up;
-      st.l[n] *= f;
-      st.z[n] *= f;
-#pragma unroll
-      for (int d = 0; d < 4 * ND; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st.o[n][d][i] *= f;
+        for (int p = 0; p < QP; ++p) s[n][t] = mfma(k, q[n][i][p], s[n][t]);
     }
   }
+  float a0[8], a1[8], e[PQ][8];
+  auto read = [&](float (&x)[8], int i) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const floatx4 v = *reinterpret_cast<const floatx4*>(&aff[i][16 * t + 4 * g]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * t + j] = v[j];
+    }
+  };
+  read(a0, 0);
+  read(a1, 1);
+  exponents<ND, PQ>(st, e, s, a0, a1, qsum, mask, key0, pos, window, shift);
   half8 p[PQ][PP];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const floatx4 vs = *reinterpret_cast<const floatx4*>(&aff[2][16 * t + 4 * g]);
-    const floatx4 vz = *reinterpret_cast<const floatx4*>(&aff[3][16 * t + 4 * g]);
-#pragma unroll
-    for (int n = 0; n < PQ; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = e[n][4 * t + i], w = __builtin_amdgcn_exp2f(x);
-        float ps = w * vs[i], pz = w * vz[i];
-        if constexpr (MASK) {  // a scale that is no number must not reach columns that do not see its key
-          ps = x == -__builtin_inff() ? 0.f : ps;
-          pz = x == -__builtin_inff() ? 0.f : pz;
-        }
-        st.l[n] += w;
-        st.z[n] += pz;
-        const _Float16 h = (_Float16)ps;
-        p[n][0][4 * t + i] = h;
-        if constexpr (PP == 2) p[n][1][4 * t + i] = (_Float16)(ps - (float)h);
-      }
-  }
+  read(a0, 2);
+  read(a1, 3);
+  weights<ND, PQ, PP>(st, p, e, a0, a1, mask);
 #pragma unroll
   for (int W = 0; W < 4 * ND; ++W) {
     const half8 v = vop[W][lane];
@@ -527,68 +551,22 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   if (t.col0 >= t.cols || part >= t.chunks) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
 
-  // the columns' queries, scaled by one power of two for all of the workgroup's
   int pos[PQ], row_of[PQ], head_of[PQ];
   bool valid[PQ];
-  float top = 0.f;
+  const T* rows[PQ];
   half8 q[PQ][2 * ND][QP];
   float qsum[PQ];
-  int ex = 0;
-#pragma unroll
-  for (int turn = 0; turn < 2; ++turn) {
-#pragma unroll
-    for (int n = 0; n < PQ; ++n) {
-      const int col = t.col0 + 16 * (PQ * wave + n) + (lane & 15), token = col / a.group;
-      valid[n] = col < t.cols;
-      pos[n] = valid[n] ? t.pos0 + token : t.pos_hi;
-      row_of[n] = token, head_of[n] = head * a.group + col % a.group;
-      const T* row = (const T*)a.q + (t.row + (valid[n] ? token : 0)) * a.q_token + head_of[n] * a.q_head;
-      float total = 0.f;
-#pragma unroll
-      for (int s = 0; s < 2 * ND; ++s) {
-        float x[8];
-        load_row<TYPE, 8>(x, row, 32 * s + 8 * g, valid[n] ? c.dim : 0);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (turn == 0) {
-            const float v = __builtin_fabsf(x[e]);
-            top = v < __builtin_inff() && v > top ? v : top;  // infinities and NaN stay what they are in fp16
-          } else {
-            const float v = __builtin_ldexpf(x[e], -ex);
-            const _Float16 h = (_Float16)v;
-            q[n][s][0][e] = h;
-            total += (float)h;
-            if constexpr (QP == 2) {
-              const _Float16 l = (_Float16)(v - (float)h);
-              q[n][s][1][e] = l;
-              total += (float)l;
-            }
-          }
-        }
-      }
-      if (turn == 1) qsum[n] = quad_sum(total);
-    }
-    if (turn == 0) {
-#pragma unroll
-      for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
-      if (lane == 0) tops[wave] = top;
-      __syncthreads();
-#pragma unroll
-      for (int w = 0; w < PWAVES; ++w) top = fmaxf(top, tops[w]);
-      ex = __builtin_amdgcn_readfirstlane(exponent_of(top) - 14);
-    }
-  }
-  const float factor = __builtin_ldexpf(a.scale, ex);
-
-  PromptState<ND, PP> st;
-  st.shift = -1000;
 #pragma unroll
   for (int n = 0; n < PQ; ++n) {
-    st.top[n] = st.l[n] = st.z[n] = 0.f;
-    st.fresh[n] = true;
-#pragma unroll
-    for (int d = 0; d < 4 * ND; ++d) st.o[n][d] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    const int col = t.col0 + 16 * (PQ * wave + n) + (lane & 15), token = col / a.group;
+    valid[n] = col < t.cols;
+    pos[n] = valid[n] ? t.pos0 + token : t.pos_hi;
+    row_of[n] = token, head_of[n] = head * a.group + col % a.group;
+    rows[n] = (const T*)a.q + (t.row + (valid[n] ? token : 0)) * a.q_token + head_of[n] * a.q_head;
   }
+  const float factor = __builtin_ldexpf(a.scale, load_queries<TYPE, ND, PQ, QP, PWAVES>(q, qsum, rows, valid, c.dim, tops));
+  State<ND, PQ> st;
+  clear(st);
   const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + part * a.chunk);
   const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
   const int pos_lo = __builtin_amdgcn_readfirstlane(t.pos_lo), pos_hi = __builtin_amdgcn_readfirstlane(t.pos_hi);
@@ -627,7 +605,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
       }
       big = __builtin_amdgcn_readfirstlane(big);
       if (big > held) held = big + 2;  // room for scales four times as large
-      aff[buf][lane >> 5 << 1][lane & 31] = lane < 32 ? s * factor : __builtin_ldexpf(s, PROOM - held);
+      aff[buf][lane >> 5 << 1][lane & 31] = lane < 32 ? s * factor : __builtin_ldexpf(s, ROOM - held);
       aff[buf][(lane >> 5 << 1) + 1][lane & 31] = lane < 32 ? z * factor : z;
       if (lane == 0) shifts[buf] = held;
     }
@@ -645,20 +623,8 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
     const unsigned* after = kb + 2 < end ? kv_head(c, b, kb + 2, head, hw, at3) : nullptr;
     if (base) {
       const int shift = __builtin_amdgcn_readfirstlane(shifts[buf]);
-      if (shift != st.shift) {
-#pragma unroll
-        for (int n = 0; n < PQ; ++n)
-#pragma unroll
-          for (int d = 0; d < 4 * ND; ++d)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) st.o[n][d][i] = __builtin_ldexpf(st.o[n][d][i], st.shift - shift);
-        st.shift = shift;
-      }
-      const int key0 = kb * 32 + 4 * g;
-      if (kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window))
-        prompt_block<ND, QP, PP, false>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], lane, key0, pos, a.window);
-      else
-        prompt_block<ND, QP, PP, true>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], lane, key0, pos, a.window);
+      const bool mask = !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
+      prompt_block<ND, QP, PP>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], mask, kb * 32 + 4 * g, pos, a.window, shift);
     }
     if (next) put(kb + 1, 1 - buf);
     __syncthreads();
@@ -668,14 +634,14 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   for (int n = 0; n < PQ; ++n) {
     const float l = quad_sum(st.l[n]), z = quad_sum(st.z[n]);
     const int in = 16 * (PQ * wave + n) + (lane & 15);
-    const bool none = l == 0.f;
+    const bool none = st.fresh[n];
     if (t.chunks > 1) {
       float* out = a.part + ((slot * c.heads + head) * a.chunks + part) * (int64_t)(CT * (DP + 2));
 #pragma unroll
       for (int d = 0; d < 4 * ND; ++d) {
         floatx4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(st.o[n][d][i], st.shift - PROOM) + z;
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(st.o[n][d][i], st.shift - ROOM) + z;
         if (valid[n]) *reinterpret_cast<floatx4*>(out + in * DP + 16 * d + 4 * g) = v;
       }
       if (valid[n] && g == 0) {
@@ -690,7 +656,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
       for (int d = 0; d < 4 * ND; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v = (__builtin_ldexpf(st.o[n][d][i], st.shift - PROOM) + z) * f;
+          const float v = (__builtin_ldexpf(st.o[n][d][i], st.shift - ROOM) + z) * f;
           const T x = from_f32<TYPE>(none ? 0.f : v);
           if (valid[n] && 16 * d + 4 * g + i < c.dim) out[16 * d + 4 * g + i] = x;
         }
