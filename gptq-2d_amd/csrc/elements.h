@@ -62,6 +62,25 @@ __device__ __forceinline__ void load_row(float (&x)[N], const typename Elem<TYPE
   }
 }
 
+// Eight consecutive elements as they lie, 0 past the row's end; loads only, so that several can be in flight.
+template <int TYPE>
+struct Raw8 {
+  typedef typename Elem<TYPE>::T T;
+  static constexpr int V = 16 / (int)sizeof(T);  // elements of a 16-byte load
+  typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  vec v[8 / V];
+  __device__ __forceinline__ void load(const T* __restrict__ row, int d, int n) {
+    if (d + 8 <= n) {
+#pragma unroll
+      for (int i = 0; i < 8 / V; ++i) v[i] = *reinterpret_cast<const vec*>(row + d + V * i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i / V][i % V] = d + i < n ? row[d + i] : (T)0;
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const { return to_f32<TYPE>(v[i / V][i % V]); }
+};
+
 // Exponent e with 2^e <= x < 2^(e + 1) of a finite x > 0 (0 for anything else).
 __device__ __forceinline__ int exponent_of(float x) {
   return x > 0.f && x < __builtin_inff() ? (int)__builtin_amdgcn_frexp_expf(x) - 1 : 0;

@@ -10,6 +10,7 @@
 // bits.  p_j s_j is brought to fp16's range by a power of two above the largest s seen, and rounded to 11 bits for
 // bf16 results (which have 8), in two pieces otherwise.  Sums, maxima and rescaling are fp32.
 #include "kv_cache.h"
+#include "lds_dma.h"
 
 namespace {
 
@@ -85,19 +86,21 @@ __device__ __forceinline__ int load_queries(half8 (&q)[NQ][2 * ND][QP], float (&
                                             const typename Elem<TYPE>::T* const (&row)[NQ], const bool (&valid)[NQ], int dim,
                                             float* tops) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+  Raw8<TYPE> x[NQ][2 * ND];
   float top = 0.f;
-#pragma unroll 1
-  for (int s = 0; s < 2 * ND; ++s)
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float x[8];
-      load_row<TYPE, 8>(x, row[n], 32 * s + 8 * g, valid[n] ? dim : 0);
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int s = 0; s < 2 * ND; ++s) x[n][s].load(row[n], 32 * s + 8 * g, valid[n] ? dim : 0);
+#pragma unroll
+  for (int n = 0; n < NQ; ++n)
+#pragma unroll
+    for (int s = 0; s < 2 * ND; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_fabsf(x[e]);
+        const float v = __builtin_fabsf(x[n][s][e]);
         top = v < __builtin_inff() && v > top ? v : top;  // infinities and NaN stay what they are in fp16
       }
-    }
 #pragma unroll
   for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
   if (WV > 1) {
@@ -112,11 +115,9 @@ __device__ __forceinline__ int load_queries(half8 (&q)[NQ][2 * ND][QP], float (&
     float total = 0.f;
 #pragma unroll
     for (int s = 0; s < 2 * ND; ++s) {
-      float x[8];
-      load_row<TYPE, 8>(x, row[n], 32 * s + 8 * g, valid[n] ? dim : 0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_ldexpf(x[e], -ex);
+        const float v = __builtin_ldexpf(x[n][s][e], -ex);
         const _Float16 h = (_Float16)v;
         q[n][s][0][e] = h;
         total += (float)h;
@@ -173,6 +174,7 @@ __device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], 
     for (int i = 0; i < 8; ++i)
       e[n][i] = __builtin_fmaf(ks[i], s[n][i / 4][i % 4], __builtin_fmaf(kz[i], qsum[n], -st.top[n]));
   if (mask) {
+    asm volatile("");  // a branch, not sixteen selects for every block
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const int from = window ? pos[n] - window : -1;
@@ -218,6 +220,7 @@ __device__ __forceinline__ void weights(State<ND, NQ>& st, half8 (&p)[NQ][PP], c
                                         const float (&vz)[8], bool mask) {
   float ps[NQ][8];
   if (mask) {  // a scale or zero that is no number must not reach columns that do not see its key
+    asm volatile("");
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
 #pragma unroll
@@ -271,13 +274,11 @@ struct Words {
   uint4v kw[ND], vw[ND], ka[2], va[2];
 };
 
-// Scales and zeros of this lane's eight keys: s and z + 8 s; keys from `left` on are beyond the sequence, whatever the page
-// holds (left: 8 where none is).
-__device__ __forceinline__ void unpack_affine(float (&s)[8], float (&z)[8], const uint4v (&w)[2], bool mask, int key0, int len) {
+// Scales and zeros of this lane's eight keys: s and z + 8 s.
+__device__ __forceinline__ void unpack_affine(float (&s)[8], float (&z)[8], const uint4v (&w)[2]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    unsigned u = w[i / 4][i % 4];
-    if (mask) u = key0 + 16 * (i / 4) + i % 4 < len ? u : 0u;
+    const unsigned u = w[i / 4][i % 4];
     s[i] = __uint_as_float(u << 16);
     z[i] = __builtin_fmaf(8.f, s[i], __uint_as_float(u & 0xffff0000u));
   }
@@ -285,7 +286,7 @@ __device__ __forceinline__ void unpack_affine(float (&s)[8], float (&z)[8], cons
 
 template <int ND, int NQ, int QP, int PP>
 __device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)[NQ][2 * ND][QP], const float (&qsum)[NQ],
-                                             const Words<ND>& w, float factor, bool mask, int key0, int len,
+                                             Words<ND>& w, float factor, bool mask, int key0, int len,
                                              const int (&pos)[NQ], int window) {
   floatx4 s[NQ][2];
 #pragma unroll
@@ -300,8 +301,13 @@ __device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)
       for (int p = 0; p < QP; ++p) s[n][i % 2] = mfma(k, q[n][i / 2][p], s[n][i % 2]);
   }
   float ks[8], kz[8], vs[8], vz[8], e[NQ][8];
-  unpack_affine(ks, kz, w.ka, mask, key0, len);
-  unpack_affine(vs, vz, w.va, mask, key0, len);
+  if (mask) {  // beyond the sequence: whatever the page holds
+    asm volatile("");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w.va[i / 4][i % 4] = key0 + 16 * (i / 4) + i % 4 < len ? w.va[i / 4][i % 4] : 0u;
+  }
+  unpack_affine(ks, kz, w.ka);
+  unpack_affine(vs, vz, w.va);
   unsigned bits = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -325,29 +331,60 @@ __device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)
   }
 }
 
+// A wave's ring of blocks in LDS, each loaded there straight from memory S - 1 blocks ahead: K's and V's words (1 KB a chunk, as the
+// lanes read them), then the scales and zeros of 32 keys and 32 values.  Two workgroups of four waves a CU have some 100 KB
+// on their way.
 template <int ND>
-__device__ __forceinline__ void load_block(Words<ND>& w, const unsigned* base, int at, int page, int lane) {
-  const unsigned* k = base + at * (256 * ND) + lane * 4;
-  const unsigned* v = k + page * (8 * ND);
-  const unsigned* ka = base + page * (16 * ND) + at * 32 + lane / 16 * 4;
-  const unsigned* va = ka + page;
-#pragma unroll
-  for (int i = 0; i < ND; ++i) w.kw[i] = *reinterpret_cast<const uint4v*>(k + 256 * i);
-#pragma unroll
-  for (int t = 0; t < 2; ++t) w.ka[t] = *reinterpret_cast<const uint4v*>(ka + 16 * t);
-#pragma unroll
-  for (int i = 0; i < ND; ++i) w.vw[i] = *reinterpret_cast<const uint4v*>(v + 256 * i);
-#pragma unroll
-  for (int t = 0; t < 2; ++t) w.va[t] = *reinterpret_cast<const uint4v*>(va + 16 * t);
+struct Ring {
+  static constexpr int STAGE = 2048 * ND + 256, LOADS = 2 * ND + 1;
+  static constexpr int S = 20480 / STAGE < 8 ? 20480 / STAGE : 8;
+};
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt has six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// A workgroup takes 16 NQ columns and `chunk` blocks of 32 keys, its waves every fourth block each, the next block's
-// words in flight while one is computed; the waves' results are joined through LDS.
+// Block `at` of the head's part of a page at `base`; without a page zeros.
+template <int ND>
+__device__ __forceinline__ void stage_block(char* to, const unsigned* base, int at, int page, int lane) {
+  const int words = base ? 1 : 0;
+  const auto rsrc = [&](int first, int count) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned*>(base + (base ? first : 0)), (short)0, words * count * 4, 0x00020000);
+  };
+  const __amdgpu_buffer_rsrc_t k = rsrc(at * (256 * ND), 256 * ND), v = rsrc(page * (8 * ND) + at * (256 * ND), 256 * ND);
+#pragma unroll
+  for (int i = 0; i < ND; ++i) dma_load<4>(k, reinterpret_cast<float*>(to + 1024 * i), 1024 * i + 16 * lane);
+#pragma unroll
+  for (int i = 0; i < ND; ++i) dma_load<4>(v, reinterpret_cast<float*>(to + 1024 * (ND + i)), 1024 * i + 16 * lane);
+  const __amdgpu_buffer_rsrc_t a = rsrc(page * (16 * ND) + at * 32, page + 32);
+  dma_load<1>(a, reinterpret_cast<float*>(to + 2048 * ND), (lane < 32 ? lane : page + lane - 32) * 4);
+}
+
+template <int ND>
+__device__ __forceinline__ void read_block(Words<ND>& w, const char* from, int lane) {
+#pragma unroll
+  for (int i = 0; i < ND; ++i) w.kw[i] = *reinterpret_cast<const uint4v*>(from + 1024 * i + 16 * lane);
+#pragma unroll
+  for (int i = 0; i < ND; ++i) w.vw[i] = *reinterpret_cast<const uint4v*>(from + 1024 * (ND + i) + 16 * lane);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    w.ka[t] = *reinterpret_cast<const uint4v*>(from + 2048 * ND + 64 * t + lane / 16 * 16);
+    w.va[t] = *reinterpret_cast<const uint4v*>(from + 2048 * ND + 128 + 64 * t + lane / 16 * 16);
+  }
+}
+
+// A workgroup takes 16 NQ columns and `chunk` blocks of 32 keys, its waves every fourth block each; the waves' results are
+// joined through LDS.
 template <int TYPE, int ND, int NQ>
 __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
   constexpr int CT = 16 * NQ, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2;
-  __shared__ floatx4 sums[NQ][4 * ND][64];
+  typedef Ring<ND> R;
+  constexpr int S = R::S;
+  static_assert(S * R::STAGE >= NQ * 4 * ND * 1024, "a wave's sums fit where its blocks were");
+  alignas(16) __shared__ char ring[WAVES][S][R::STAGE];
   __shared__ float tops[WAVES][CT], ls[WAVES][CT];
   const int64_t slot = blockIdx.x;
   const int head = blockIdx.y, chunk = blockIdx.z;
@@ -358,6 +395,23 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
   if (t.col0 >= t.cols || chunk >= t.chunks) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
 
+  const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + chunk * a.chunk);
+  const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
+  const int pos_lo = __builtin_amdgcn_readfirstlane(t.pos_lo), pos_hi = __builtin_amdgcn_readfirstlane(t.pos_hi);
+  const int hw = (int)kv_head_words(ND, c.page);
+  const int64_t b = t.b;
+  const int first = begin + wave, count = end > first ? (end - first + WAVES - 1) / WAVES : 0;
+  unsigned there = 0;  // bit per stage: the block has a page
+  int at = 0;
+  const unsigned* base = nullptr;
+#pragma unroll
+  for (int i = 0; i < S - 1; ++i)
+    if (i < count) {
+      base = kv_head(c, b, first + WAVES * i, head, hw, at);
+      there |= (base ? 1u : 0u) << i;
+      stage_block<ND>(ring[wave][i], base, at, c.page, lane);
+    }
+  base = S - 1 < count ? kv_head(c, b, first + WAVES * (S - 1), head, hw, at) : nullptr;
   half8 q[NQ][2 * ND][QP];
   float qsum[NQ];
   int pos[NQ];
@@ -373,110 +427,90 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
   const float factor = __builtin_ldexpf(a.scale, load_queries<TYPE, ND, NQ, QP, 1>(q, qsum, rows, valid, c.dim, nullptr));
   State<ND, NQ> st;
   clear(st);
-  const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + chunk * a.chunk);
-  const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
-  const int pos_lo = __builtin_amdgcn_readfirstlane(t.pos_lo), pos_hi = __builtin_amdgcn_readfirstlane(t.pos_hi);
-  const int hw = (int)kv_head_words(ND, c.page);
-  const int64_t b = t.b;
-  Words<ND> cur;
-  int at = 0;
-  int kb = begin + wave;
-  const unsigned* base = kb < end ? kv_head(c, b, kb, head, hw, at) : nullptr;
-  if (base) load_block<ND>(cur, base, at, c.page, lane);
-  int at2 = 0;
-  const unsigned* next = kb + WAVES < end ? kv_head(c, b, kb + WAVES, head, hw, at2) : nullptr;
-  for (; kb < end; kb += WAVES) {
-    Words<ND> ahead;
-    if (next) load_block<ND>(ahead, next, at2, c.page, lane);
-    int at3 = 0;
-    const unsigned* after = kb + 2 * WAVES < end ? kv_head(c, b, kb + 2 * WAVES, head, hw, at3) : nullptr;
-    if (base) {
-      const bool mask = !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
-      attend_block<ND, NQ, QP, PP>(st, q, qsum, cur, factor, mask, kb * 32 + 4 * g, t.len, pos, a.window);
+  int buf = 0;
+  for (int i = 0; i < count; ++i) {
+    if (i + S - 1 <= count)
+      wait_loads<(S - 2) * R::LOADS>();
+    else
+      wait_loads<0>();
+    const int ahead = buf ? buf - 1 : S - 1;
+    if (i + S - 1 < count) {
+      there = (there & ~(1u << ahead)) | (base ? 1u : 0u) << ahead;
+      stage_block<ND>(ring[wave][ahead], base, at, c.page, lane);
+      if (i + S < count) base = kv_head(c, b, first + WAVES * (i + S), head, hw, at);
     }
-    cur = ahead;
-    base = next;
-    next = after;
-    at2 = at3;
+    Words<ND> w;
+    read_block<ND>(w, ring[wave][buf], lane);
+    const int kb = first + WAVES * i;
+    const bool page = there >> buf & 1u;
+    const bool mask = !page || !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
+    int seen[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) seen[n] = page ? pos[n] : -1;  // without a page nobody sees its keys
+    attend_block<ND, NQ, QP, PP>(st, q, qsum, w, factor, mask, kb * 32 + 4 * g, page ? t.len : 0, seen, a.window);
+    buf = buf + 1 < S ? buf + 1 : 0;
   }
+  // the waves' results, brought to one reference, in the place of their own blocks; then every thread adds four elements
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     st.l[n] = quad_sum(st.l[n]);
     st.z[n] = quad_sum(st.z[n]);
-    if (st.fresh[n]) st.top[n] = -__builtin_inff();
+    if (st.fresh[n] && st.l[n] == 0.f) st.top[n] = -__builtin_inff();  // saw no key; scores that are no numbers stay such
     if (g == 0) {
       tops[wave][16 * n + lane] = st.top[n];
       ls[wave][16 * n + lane] = st.l[n];
     }
   }
   __syncthreads();
-  float top[NQ], l[NQ];
+  floatx4* const mine = reinterpret_cast<floatx4*>(&ring[wave][0][0]);
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float m = -__builtin_inff();
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float x = tops[w][16 * n + (lane & 15)];
-      m = x > m || x != x ? x : m;
-    }
-    top[n] = m;
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const float x = tops[w][16 * n + (lane & 15)];
-      sum += (x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - m)) * ls[w][16 * n + (lane & 15)];
-    }
-    l[n] = sum;
+    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, tops[w][16 * n + (lane & 15)]);
     const float f = st.top[n] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.top[n] - m);
+    const float f2 = __builtin_ldexpf(f, st.shift - ROOM), z = f * st.z[n];
 #pragma unroll
     for (int d = 0; d < 4 * ND; ++d)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        st.o[n][d][i] = f * (__builtin_ldexpf(st.o[n][d][i], st.shift - ROOM) + st.z[n]);
+      for (int i = 0; i < 4; ++i) st.o[n][d][i] = __builtin_fmaf(f2, st.o[n][d][i], z);
+#pragma unroll
+    for (int d = 0; d < 4 * ND; ++d) mine[(n * 4 * ND + d) * 64 + lane] = st.o[n][d];
   }
+  __syncthreads();
+  const int cols = t.cols - t.col0 < CT ? t.cols - t.col0 : CT;
+  for (int u = threadIdx.x; u < cols * (16 * ND); u += THREADS) {
+    const int in = u / (16 * ND), d4 = u % (16 * ND);  // column, four elements
+    const int at4 = ((in / 16) * 4 * ND + d4 / 4) * 64 + in % 16 + 16 * (d4 % 4);
+    floatx4 v = {0.f, 0.f, 0.f, 0.f};
+    float top = -__builtin_inff(), l = 0.f;
 #pragma unroll
-  for (int w = WAVES - 1; w > 0; --w) {
-    if (wave == w) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int d = 0; d < 4 * ND; ++d)
-          sums[n][d][lane] = w == WAVES - 1 ? st.o[n][d] : sums[n][d][lane] + st.o[n][d];
+    for (int w = 0; w < WAVES; ++w) {
+      v += reinterpret_cast<const floatx4*>(&ring[w][0][0])[at4];
+      top = fmaxf(top, tops[w][in]);
     }
-    __syncthreads();
-  }
-  if (wave != 0) return;
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int in = 16 * n + (lane & 15), col = t.col0 + in;
-    const bool valid = col < t.cols;
+    for (int w = 0; w < WAVES; ++w)
+      l += (tops[w][in] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(tops[w][in] - top)) * ls[w][in];
+    const bool none = top == -__builtin_inff();
     if (t.chunks > 1) {
       float* out = a.part + ((slot * c.heads + head) * a.chunks + chunk) * (int64_t)(CT * (DP + 2));
-#pragma unroll
-      for (int d = 0; d < 4 * ND; ++d) {
-        const floatx4 v = sums[n][d][lane] + st.o[n][d];
-        if (valid) *reinterpret_cast<floatx4*>(out + in * DP + 16 * d + 4 * g) = v;
-      }
-      if (valid && g == 0) {
-        out[CT * DP + in] = top[n];
-        out[CT * (DP + 1) + in] = l[n];
-      }
+      *reinterpret_cast<floatx4*>(out + in * DP + 4 * d4) = v;
+      if (d4 == 0) out[CT * DP + in] = top;
+      if (d4 == 1) out[CT * (DP + 1) + in] = l;
     } else {
+      const int col = t.col0 + in;
       const int64_t row = t.row + col / a.group;
       const int hq = head * a.group + col % a.group;
-      const float f = l[n] == 0.f ? 0.f : 1.f / l[n];
-      T* out = (T*)a.out + row * a.out_token + hq * a.out_head;
+      const float f = none ? 0.f : 1.f / l;
+      T* out = (T*)a.out + row * a.out_token + hq * a.out_head + 4 * d4;
 #pragma unroll
-      for (int d = 0; d < 4 * ND; ++d) {
-        const floatx4 v = sums[n][d][lane] + st.o[n][d];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const typename Elem<TYPE>::T x = from_f32<TYPE>(f == 0.f ? 0.f : v[i] * f);
-          if (valid && 16 * d + 4 * g + i < c.dim) out[16 * d + 4 * g + i] = x;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const T x = from_f32<TYPE>(none ? 0.f : v[i] * f);
+        if (4 * d4 + i < c.dim) out[i] = x;
       }
-      if (valid && a.lse && g == 0)
-        a.lse[row * (int64_t)(c.heads * a.group) + hq] = l[n] == 0.f ? -__builtin_inff() : (top[n] + __builtin_log2f(l[n])) * LN2;
+      if (d4 == 0 && a.lse)
+        a.lse[row * (int64_t)(c.heads * a.group) + hq] = none ? -__builtin_inff() : (top + __builtin_log2f(l)) * LN2;
     }
   }
 }
@@ -585,7 +619,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
     }
     if (wave == 0) affine = base[c.page * (16 * ND + (lane >> 5)) + at * 32 + (lane & 31)];
   };
-  auto put = [&](int kb, int buf) {
+  auto put = [&](int kb, int buf, const unsigned* page) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       const int ch = wave + PWAVES * i;
@@ -595,16 +629,18 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
       }
     }
     if (wave == 0) {  // lanes 0..31 the keys, 32..63 the values
-      unsigned w = kb * 32 + (lane & 31) < len ? affine : 0u;  // beyond the sequence: whatever the page holds
+      unsigned w = page && kb * 32 + (lane & 31) < len ? affine : 0u;  // beyond the sequence: whatever the page holds
       const float s = __uint_as_float(w << 16), z = __builtin_fmaf(8.f, s, __uint_as_float(w & 0xffff0000u));
-      int big = lane >= 32 && (w >> 7 & 255u) != 255u ? (int)(w >> 7 & 255u) - 126 : -126;
+      const int ex = lane >= 32 && (w >> 7 & 255u) != 255u ? (int)(w >> 7 & 255u) - 126 : -126;  // s < 2^ex
+      if (__builtin_amdgcn_ballot_w64(ex > held)) {
+        int big = ex;
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int x = __shfl_xor(big, d);
-        big = x > big ? x : big;
+        for (int d = 1; d < 64; d *= 2) {
+          const int x = __shfl_xor(big, d);
+          big = x > big ? x : big;
+        }
+        held = __builtin_amdgcn_readfirstlane(big) + 2;  // room for scales four times as large
       }
-      big = __builtin_amdgcn_readfirstlane(big);
-      if (big > held) held = big + 2;  // room for scales four times as large
       aff[buf][lane >> 5 << 1][lane & 31] = lane < 32 ? s * factor : __builtin_ldexpf(s, ROOM - held);
       aff[buf][(lane >> 5 << 1) + 1][lane & 31] = lane < 32 ? z * factor : z;
       if (lane == 0) shifts[buf] = held;
@@ -614,19 +650,20 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   const unsigned* base = begin < end ? kv_head(c, b, begin, head, hw, at) : nullptr;
   if (base) load(base, at);
   const unsigned* next = begin + 1 < end ? kv_head(c, b, begin + 1, head, hw, at2) : nullptr;
-  if (base) put(begin, 0);
+  if (begin < end) put(begin, 0, base);
   __syncthreads();
   for (int kb = begin; kb < end; ++kb) {
     const int buf = (kb - begin) & 1;
     if (next) load(next, at2);
     int at3 = 0;
     const unsigned* after = kb + 2 < end ? kv_head(c, b, kb + 2, head, hw, at3) : nullptr;
-    if (base) {
-      const int shift = __builtin_amdgcn_readfirstlane(shifts[buf]);
-      const bool mask = !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
-      prompt_block<ND, QP, PP>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], mask, kb * 32 + 4 * g, pos, a.window, shift);
-    }
-    if (next) put(kb + 1, 1 - buf);
+    const int shift = __builtin_amdgcn_readfirstlane(shifts[buf]);
+    const bool mask = !base || !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
+    int seen[PQ];
+#pragma unroll
+    for (int n = 0; n < PQ; ++n) seen[n] = base ? pos[n] : -1;  // without a page nobody sees its keys
+    prompt_block<ND, QP, PP>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], mask, kb * 32 + 4 * g, seen, a.window, shift);
+    if (kb + 1 < end) put(kb + 1, 1 - buf, next);
     __syncthreads();
     base = next, next = after, at2 = at3;
   }
@@ -634,7 +671,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   for (int n = 0; n < PQ; ++n) {
     const float l = quad_sum(st.l[n]), z = quad_sum(st.z[n]);
     const int in = 16 * (PQ * wave + n) + (lane & 15);
-    const bool none = st.fresh[n];
+    const bool none = st.fresh[n] && l == 0.f;  // scores that are no numbers stay such
     if (t.chunks > 1) {
       float* out = a.part + ((slot * c.heads + head) * a.chunks + part) * (int64_t)(CT * (DP + 2));
 #pragma unroll

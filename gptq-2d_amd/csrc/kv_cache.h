@@ -98,7 +98,9 @@ __device__ __forceinline__ unsigned* kv_head(const KvCache& c, int64_t b, int kb
   const int p = (int)__umulhi((unsigned)kb, c.mag);
   at = kb - p * c.blocks;
   if (c.blocks == 1) at = 0;
-  const int64_t id = c.table[b * c.table_stride + (c.blocks == 1 ? kb : p)];
+  // a uniform index: through the scalar data cache (no kernel writes the table), whose loads wait for no others
+  typedef const __attribute__((address_space(4))) int32_t* scalar;
+  const int64_t id = ((scalar)(c.table + b * c.table_stride))[__builtin_amdgcn_readfirstlane(c.blocks == 1 ? kb : p)];
   if (id < 0 || id >= c.page_count) return nullptr;
   return c.pages + id * c.page_words + (int64_t)h * head_words;
 }

@@ -10,25 +10,6 @@ namespace {
 
 constexpr int PREP = 512;
 
-// Eight consecutive elements as they lie, 0 past the row's end; loads only, so that several can be in flight.
-template <int TYPE>
-struct Raw8 {
-  typedef typename Elem<TYPE>::T T;
-  static constexpr int V = 16 / (int)sizeof(T);  // elements of a 16-byte load
-  typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
-  vec v[8 / V];
-  __device__ __forceinline__ void load(const T* __restrict__ row, int d, int n) {
-    if (d + 8 <= n) {
-#pragma unroll
-      for (int i = 0; i < 8 / V; ++i) v[i] = *reinterpret_cast<const vec*>(row + d + V * i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i / V][i % V] = d + i < n ? row[d + i] : (T)0;
-    }
-  }
-  __device__ __forceinline__ float operator[](int i) const { return to_f32<TYPE>(v[i / V][i % V]); }
-};
-
 template <int TYPE>
 __device__ __forceinline__ void prepare_token(const Linear& p, int pieces) {
   typedef typename Elem<TYPE>::T T;

@@ -271,6 +271,21 @@ def test_nan_and_infinity_where_nothing_looks(new):
                 assert bool(b[sees][:, 4:].isnan().all())
 
 
+@pytest.mark.parametrize("new", [1, 5, 80])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_queries_that_are_no_numbers(new, what):
+    """A NaN or an infinity in a query makes that query's head NaN, and no other."""
+    s = Sequences([300], 2, 80, torch.bfloat16, 32, seed=8)
+    q = torch.randn(new, 6, 80, generator=s.g).bfloat16()
+    clean, clean_lse = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), starts([new]), return_lse=True)
+    bad = torch.zeros(new, 6, dtype=torch.bool)
+    bad[new // 2, 4] = True
+    q[new // 2, 4, 77] = what
+    got, lse = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), starts([new]), return_lse=True)
+    assert bool(got.cpu()[bad].isnan().all()) and bool(lse.cpu()[bad].isnan().all())
+    assert torch.equal(got.cpu()[~bad], clean.cpu()[~bad]) and torch.equal(lse.cpu()[~bad], clean_lse.cpu()[~bad])
+
+
 def test_pages_that_are_none_and_lengths_past_the_table():
     """Entries outside the pool hold no token; lengths beyond the table's pages end there."""
     s = Sequences([96, 64], 1, 64, torch.float32, 32, seed=5)
