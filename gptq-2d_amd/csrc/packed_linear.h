@@ -223,62 +223,70 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int type, float x)
   else
     static_cast<_Float16*>(p)[i] = (_Float16)x;
 }
-__device__ __forceinline__ void load_any8(float (&x)[8], const void* p, int64_t row, int d, int dim, int type) {
-  if (type == TYPE_F32)
-    load_row<TYPE_F32, 8>(x, static_cast<const float*>(p) + row, d, dim);
-  else if (type == TYPE_BF16)
-    load_row<TYPE_BF16, 8>(x, static_cast<const uint16_t*>(p) + row, d, dim);
-  else
-    load_row<TYPE_F16, 8>(x, static_cast<const _Float16*>(p) + row, d, dim);
-}
-
 // The index of the adapter of token t, -1 for none.
 __device__ __forceinline__ int adapter_of(const Linear& p, int t) {
   const int a = t < p.tokens ? p.index[t] : -1;
   return a >= 0 && a < p.adapters ? a : -1;
 }
 
-// acc[j] += V B^T for the 16 tokens from t0 and the 16 rows of W from r0 + 16 j, one distinct adapter of the tokens after
-// the other, the others' rows of V zeros.  V (fp32) and B are taken in bf16 pieces: six products, 2^-23 of the result; of
-// bf16 adapters B is one piece, and two of V leave out 2^-17.  For long batches, where 16 tokens have one or two adapters.
-template <int MR>
-__device__ __forceinline__ void add_adapters(floatx4 (&acc)[MR], const Linear& p, int t0, int r0) {
-  const int lane = threadIdx.x & 63, g = lane >> 4, t = t0 + (lane & 15);
-  const int mine = adapter_of(p, t);
-  unsigned pending = (unsigned)__builtin_amdgcn_ballot_w64(mine >= 0) & 0xffffu;
+// tot[j][n] += V B^T for the 16 NT tokens from t0 and the rows r0 + 16 j of W, one distinct adapter of the tokens after the
+// other, the others' rows of V zeros; its B is read once for all of them.  V (fp32) and B (fp16 or bf16) are taken in bf16
+// pieces: six products, 2^-23 of the result; of bf16 adapters B is one piece, and two of V leave out 2^-17.  For long
+// batches, where a wave's tokens have few adapters.
+template <int MR, int NT>
+__device__ __forceinline__ void add_adapters(floatx4 (&tot)[MR][NT], const Linear& p, int t0, int r0) {
+  static_assert(16 * NT <= 64, "a lane a token");
+  const int lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+  const int mine = lane < 16 * NT ? adapter_of(p, t0 + lane) : -1;
+  uint64_t pending = __builtin_amdgcn_ballot_w64(mine >= 0);
   while (pending) {
-    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctz(pending));
-    pending &= ~(unsigned)__builtin_amdgcn_ballot_w64(mine == a);
+    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(pending));
+    const uint64_t same = __builtin_amdgcn_ballot_w64(mine == a);
+    pending &= ~same;
     const float c = p.scaling ? p.scaling[a] : 1.f;
     for (int j0 = 0; j0 < p.rank_pad; j0 += 32) {
-      float v[8] = {};
-      if (mine == a) {
-        const float* row = p.v + (int64_t)t * p.rank_pad + j0 + 8 * g;
-#pragma unroll 4
-        for (int k = 0; k < p.chunks; ++k) {
-          const float4 lo = *reinterpret_cast<const float4*>(row), hi = *reinterpret_cast<const float4*>(row + 4);
-          v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
-          v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
-          row += (int64_t)p.tokens * p.rank_pad;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= c;
-      }
-      bf16x8 vp[3];
-      split8(v, vp);
+      Raw8<TYPE_BF16> b[MR];  // the bits of either type
 #pragma unroll
       for (int j = 0; j < MR; ++j) {
-        const int r = r0 + 16 * j + (lane & 15);
-        float b[8];
-        load_any8(b, p.b, ((int64_t)a * p.m + (r < p.m ? r : p.m - 1)) * p.rank, j0 + 8 * g, p.rank, p.type);
-        bf16x8 bp[3];
-        split8(b, bp);
+        const int r = r0 + 16 * j + c16;
+        b[j].load(static_cast<const uint16_t*>(p.b) + ((int64_t)a * p.m + (r < p.m ? r : p.m - 1)) * p.rank, j0 + 8 * g, p.rank);
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const unsigned these = (unsigned)(same >> (16 * n)) & 0xffffu;
+        if (!these) continue;
+        float v[8] = {};
+        if (these >> c16 & 1u) {
+          const float* row = p.v + (int64_t)(t0 + 16 * n + c16) * p.rank_pad + j0 + 8 * g;
+#pragma unroll 2
+          for (int k = 0; k < p.chunks; ++k) {
+            const float4 lo = *reinterpret_cast<const float4*>(row), hi = *reinterpret_cast<const float4*>(row + 4);
+            v[0] += lo.x, v[1] += lo.y, v[2] += lo.z, v[3] += lo.w;
+            v[4] += hi.x, v[5] += hi.y, v[6] += hi.z, v[7] += hi.w;
+            row += (int64_t)p.tokens * p.rank_pad;
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= c;
+        }
+        bf16x8 vp[3];
+        split8(v, vp);
         if (p.type == TYPE_BF16) {
-          acc[j] = mma(vp[1], bp[0], acc[j]);
-          acc[j] = mma(vp[0], bp[0], acc[j]);
+#pragma unroll
+          for (int q = 1; q >= 0; --q)
+#pragma unroll
+            for (int j = 0; j < MR; ++j) tot[j][n] = mma(vp[q], __builtin_bit_cast(bf16x8, b[j].v[0]), tot[j][n]);
         } else {
 #pragma unroll
-          for (int q = 0; q < NPROD; ++q) acc[j] = mma(vp[prod_a[q]], bp[prod_b[q]], acc[j]);
+          for (int j = 0; j < MR; ++j) {
+            const half8 h = __builtin_bit_cast(half8, b[j].v[0]);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (float)h[e];
+            bf16x8 bp[3];
+            split8(x, bp);
+#pragma unroll
+            for (int q = 0; q < NPROD; ++q) tot[j][n] = mma(vp[prod_a[q]], bp[prod_b[q]], tot[j][n]);
+          }
         }
       }
     }

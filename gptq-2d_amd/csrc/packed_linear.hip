@@ -11,15 +11,16 @@ namespace {
 constexpr int PREP = 512;
 
 template <int TYPE>
-__device__ __forceinline__ void prepare_token(const Linear& p, int pieces) {
+__device__ __forceinline__ void prepare_token(const Linear& p, int t, int pieces) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int U = 2;  // loads in flight
+  constexpr int U = 4;  // loads in flight
   __shared__ float tops[PREP / 64];
-  const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const T* row = static_cast<const T*>(p.x) + (int64_t)t * p.x_token;
+  const bool held = p.n <= 8 * PREP * U;  // the row stays in registers
+  Raw8<TYPE> x[U];
   float top = 0.f;
   for (int d0 = 8 * tid; d0 < p.n; d0 += 8 * PREP * U) {
-    Raw8<TYPE> x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) x[u].load(row, d0 + 8 * PREP * u, p.n);
 #pragma unroll
@@ -41,11 +42,12 @@ __device__ __forceinline__ void prepare_token(const Linear& p, int pieces) {
   const bool by_lanes = p.corrected && p.group <= 512 && (p.group & (p.group - 1)) == 0;  // a group is 4 to 64 lanes' runs
   float all = 0.f;
   for (int d0 = 8 * tid; d0 - 8 * tid < 128 * p.blocks; d0 += 8 * PREP * U) {
-    Raw8<TYPE> x[U];
+    if (!held || d0 >= p.n)
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u].load(row, d0 + 8 * PREP * u, p.n);
+      for (int u = 0; u < U; ++u) x[u].load(row, d0 + 8 * PREP * u, p.n);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (d0 - 8 * tid + 8 * PREP * u >= 128 * p.blocks) break;
       const int d = d0 + 8 * PREP * u;
       half8 h, l;
       float sum = 0.f;
@@ -123,87 +125,92 @@ __device__ __forceinline__ floatx4 multiply(const Operand<TYPE>& a, const Operan
   return c;
 }
 
-// V[chunk, t, j] = sum over the chunk's columns of x[t, k] A[a, j, k], for the 16 tokens of a tile that have one adapter:
-// workgroup `slot` of the tile takes its slot-th distinct one.  The eight waves take every eighth step of 32 columns, two
-// or four steps' loads in flight; 64 ranks at a time.
+// V[chunk, t, j] = sum over the chunk's columns of x[t, k] A[a, j, k], for those of a tile's 16 tokens (bits `same`) that have
+// adapter a.  The eight waves take every eighth step of 32 columns, two or four steps' loads in flight; ranks
+// j0 .. j0 + 31 (64 take so many registers that a CU holds one workgroup, with nothing beside it).
 template <int TYPE>
-__device__ __forceinline__ void shrink(const Linear& p, int item) {
+__device__ __forceinline__ void shrink_one(const Linear& p, int tile, int chunk, int a, unsigned same, int j0, int k0, int k1,
+                                           floatx4 (*parts)[2][64]) {
   typedef typename Elem<TYPE>::T T;
   constexpr int W = PREP / 64, U = TYPE == TYPE_F32 ? 2 : 4;  // steps whose loads are in flight
-  __shared__ floatx4 parts[W - 1][4][64];
-  const int slot = item % p.slots, rest = item / p.slots, tiles = (p.tokens + 15) / 16, tile = rest % tiles, chunk = rest / tiles;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
-  const int t = 16 * tile + (lane & 15), mine = adapter_of(p, t);
-  unsigned pending = (unsigned)__builtin_amdgcn_ballot_w64(mine >= 0) & 0xffffu, same = 0;
-  int a = -1;
-  for (int s = 0; s <= slot; ++s) {
-    if (!pending) return;
-    a = __builtin_amdgcn_readlane(mine, __builtin_ctz(pending));
-    same = (unsigned)__builtin_amdgcn_ballot_w64(mine == a) & 0xffffu;
-    pending &= ~same;
+  const bool match = same >> (lane & 15) & 1u;
+  const T* row = static_cast<const T*>(p.x) + (int64_t)(match ? 16 * tile + (lane & 15) : 0) * p.x_token;
+  floatx4 acc[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) acc[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
+  const T* w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = j0 + 16 * j + (lane & 15);
+    w[j] = static_cast<const T*>(p.a) + ((int64_t)a * p.rank + (r < p.rank ? r : p.rank - 1)) * p.n;
   }
-  const bool match = mine == a;
-  const T* row = static_cast<const T*>(p.x) + (int64_t)(match ? t : 0) * p.x_token;
-  const int k0 = chunk * p.chunk, k1 = k0 + p.chunk < p.n ? k0 + p.chunk : p.n;
-  for (int j0 = 0; j0 < p.rank_pad; j0 += 64) {
-    floatx4 acc[4];
+  const int tiles16 = p.rank - j0 > 16 ? 2 : 1;
+  for (int k = k0 + 32 * wave; k < k1; k += 32 * W * U) {
+    Raw8<TYPE> x[U], b[U][2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = (floatx4){0.f, 0.f, 0.f, 0.f};
-    const T* w[4];
+    for (int u = 0; u < U; ++u) {  // past the chunk's end: nothing
+      const int d = k + 32 * W * u + 8 * g, n = k + 32 * W * u < k1 ? p.n : 0;
+      x[u].load(row, d, match ? n : 0);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 2; ++j)
+        if (j < tiles16) b[u][j].load(w[j], d, n);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Operand<TYPE> xo(x[u]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        if (j < tiles16) acc[j] = multiply<TYPE>(xo, Operand<TYPE>(b[u][j]), acc[j]);
+    }
+  }
+  if (wave) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) parts[wave - 1][j][lane] = acc[j];
+  }
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      floatx4 v = acc[j];
+#pragma unroll
+      for (int w = 0; w < W - 1; ++w) v += parts[w][j][lane];
       const int r = j0 + 16 * j + (lane & 15);
-      w[j] = static_cast<const T*>(p.a) + ((int64_t)a * p.rank + (r < p.rank ? r : p.rank - 1)) * p.n;
-    }
-    const int tiles16 = p.rank - j0 > 48 ? 4 : p.rank - j0 > 32 ? 3 : p.rank - j0 > 16 ? 2 : 1;
-    for (int k = k0 + 32 * wave; k < k1; k += 32 * W * U) {
-      Raw8<TYPE> x[U], b[U][4];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {  // past the chunk's end: nothing
-        const int d = k + 32 * W * u + 8 * g, n = k + 32 * W * u < k1 ? p.n : 0;
-        x[u].load(row, d, match ? n : 0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < tiles16) b[u][j].load(w[j], d, n);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const Operand<TYPE> xo(x[u]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (j < tiles16) acc[j] = multiply<TYPE>(xo, Operand<TYPE>(b[u][j]), acc[j]);
+      for (int i = 0; i < 4; ++i) {
+        const int in = 4 * g + i;
+        const float out = r < p.rank ? v[i] : 0.f;
+        if (r < p.rank_pad && same >> in & 1u) p.v[((int64_t)chunk * p.tokens + 16 * tile + in) * p.rank_pad + r] = out;
       }
     }
-    if (wave) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) parts[wave - 1][j][lane] = acc[j];
-    }
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        floatx4 v = acc[j];
-#pragma unroll
-        for (int w = 0; w < W - 1; ++w) v += parts[w][j][lane];
-        const int r = j0 + 16 * j + (lane & 15);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int in = 4 * g + i;
-          const float out = r < p.rank ? v[i] : 0.f;
-          if (r < p.rank_pad && same >> in & 1u) p.v[((int64_t)chunk * p.tokens + 16 * tile + in) * p.rank_pad + r] = out;
-        }
-      }
-    }
-    __syncthreads();
+  }
+  __syncthreads();
+}
+
+// Workgroup `slot` of a tile of 16 tokens, 32 ranks and a chunk of columns takes every slots-th of the tile's distinct adapters.
+template <int TYPE>
+__device__ __forceinline__ void shrink(const Linear& p, int item) {
+  __shared__ floatx4 parts[PREP / 64 - 1][2][64];
+  const int ranks = p.rank_pad / 32, tiles = (p.tokens + 15) / 16;
+  const int slot = item % p.slots, j0 = item / p.slots % ranks * 32, rest = item / p.slots / ranks;
+  const int tile = rest % tiles, chunk = rest / tiles;
+  const int mine = adapter_of(p, 16 * tile + (threadIdx.x & 15));
+  const int k0 = chunk * p.chunk, k1 = k0 + p.chunk < p.n ? k0 + p.chunk : p.n;
+  unsigned pending = (unsigned)__builtin_amdgcn_ballot_w64(mine >= 0) & 0xffffu;
+  for (int s = 0; pending; ++s) {
+    const int a = __builtin_amdgcn_readlane(mine, __builtin_ctz(pending));
+    const unsigned same = (unsigned)__builtin_amdgcn_ballot_w64(mine == a) & 0xffffu;
+    pending &= ~same;
+    if (s % p.slots == slot) shrink_one<TYPE>(p, tile, chunk, a, same, j0, k0, k1, parts);
   }
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(PREP) void prepare_kernel(Linear p, int pieces) {
-  if ((int)blockIdx.x < p.tokens)
-    prepare_token<TYPE>(p, pieces);
+__global__ __launch_bounds__(PREP, 4) void prepare_kernel(Linear p, int shrinks, int pieces) {
+  if ((int)blockIdx.x < shrinks)  // first: they take longer
+    shrink<TYPE>(p, blockIdx.x);
   else
-    shrink<TYPE>(p, blockIdx.x - p.tokens);
+    prepare_token<TYPE>(p, blockIdx.x - shrinks, pieces);
 }
 
 // y = the splits' parts added in their order, and the bias.
@@ -247,13 +254,16 @@ inline bool make_plan(Plan& q, int64_t tokens, int64_t m, int64_t n, int bits, i
   q.split_blocks = (int)cdiv(blocks, splits);
   q.splits = (int)cdiv(blocks, q.split_blocks);
   q.rank_pad = adapters ? (int)((rank + 31) / 32 * 32) : 0;
-  // the adapters' columns in chunks: about 512 workgroups, a chunk at least 1024 columns and at most 8 of them
-  q.slots = adapters < 16 ? (int)adapters : 16;
-  int64_t chunks = adapters ? cdiv(512, cdiv(tokens + !tokens, 16) * q.slots) : 1;
+  // the adapters' columns in chunks: a workgroup for each CU where 16 tokens share an adapter, a chunk at least 1024 columns
+  // and at most 8 of them; 16 tokens may have 16 adapters, which as many workgroups take as find room beside each other
+  const int64_t tiles = cdiv(tokens + !tokens, 16);
+  int64_t chunks = cdiv(256, tiles);
   chunks = chunks > 8 ? 8 : chunks;
   q.chunk = (int)(cdiv(cdiv(n, chunks), 128) * 128);
   if (q.chunk < 1024) q.chunk = 1024;
   q.chunks = (int)cdiv(n, q.chunk);
+  const int64_t slots = cdiv(512, tiles * q.chunks * (q.rank_pad / 32 + !q.rank_pad)), most = adapters < 16 ? adapters : 16;
+  q.slots = (int)(slots < most ? slots : most);
   q.sums_row = cdiv(tokens, 16) * 16 + 128;  // a tile's reads past the last token stay inside
   int64_t at = 0;
   q.xp = at, at += align4(q.pieces * tokens * blocks * 64);
@@ -288,6 +298,9 @@ int gptq2d_packed_linear(const void* x, int64_t x_token, int32_t type, int64_t t
   const bool shifted = zero || __builtin_fabs(offset) > 512.;
   if (!make_plan(q, tokens, m, n, bits, group, shifted, type, adapters, rank)) return GPTQ2D_EINVAL;
   if (row_words < cdiv(n * bits, 32)) return GPTQ2D_EINVAL;
+  const int64_t far = (m < 128 ? m : 128) - 1, limit = (int64_t)1 << 28;  // a workgroup's byte offsets have 31 bits
+  if (far * row_words > limit || far * scale_row + q.groups * scale_col > limit || far * zero_row + q.groups * zero_col > limit)
+    return GPTQ2D_EUNSUPPORTED;
   if (tokens == 0) return 0;
   if (!work || (uintptr_t)work % 16 || work_bytes < 4 * q.total) return GPTQ2D_ESCRATCH;
   if (group >= n) group = 0;
@@ -316,15 +329,15 @@ int gptq2d_packed_linear(const void* x, int64_t x_token, int32_t type, int64_t t
   p.y = y, p.y_token = y_token, p.bias = bias;
   p.splits = q.splits, p.split_blocks = q.split_blocks, p.part = w + q.part;
   const hipStream_t st = (hipStream_t)stream;
-  const int64_t prep = tokens + (index ? q.slots * cdiv(tokens, 16) * q.chunks : 0);
+  const int64_t shrinks = index ? q.slots * (q.rank_pad / 32) * cdiv(tokens, 16) * q.chunks : 0, prep = tokens + shrinks;
   if (prep > 0x7fffffff || (q.tile && cdiv(tokens, q.tile) > 65535)) return GPTQ2D_EUNSUPPORTED;
   const dim3 grid((unsigned)prep), block(PREP);
   if (type == TYPE_F32)
-    hipLaunchKernelGGL((prepare_kernel<TYPE_F32>), grid, block, 0, st, p, q.pieces);
+    hipLaunchKernelGGL((prepare_kernel<TYPE_F32>), grid, block, 0, st, p, (int)shrinks, q.pieces);
   else if (type == TYPE_BF16)
-    hipLaunchKernelGGL((prepare_kernel<TYPE_BF16>), grid, block, 0, st, p, q.pieces);
+    hipLaunchKernelGGL((prepare_kernel<TYPE_BF16>), grid, block, 0, st, p, (int)shrinks, q.pieces);
   else
-    hipLaunchKernelGGL((prepare_kernel<TYPE_F16>), grid, block, 0, st, p, q.pieces);
+    hipLaunchKernelGGL((prepare_kernel<TYPE_F16>), grid, block, 0, st, p, (int)shrinks, q.pieces);
   const int rc = bits == 2   ? packed_product_bits2(&p, &q, st)
                  : bits == 3 ? packed_product_bits3(&p, &q, st)
                  : bits == 4 ? packed_product_bits4(&p, &q, st)

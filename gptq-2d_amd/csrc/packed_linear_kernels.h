@@ -16,120 +16,123 @@ struct Affine {
 
 template <int MODE>
 __device__ __forceinline__ int group_of(const Linear& p, int kb, int i) {
-  if constexpr (MODE == ROWS) return 0;
   const int step = narrow(MODE) ? 4 * kb + i : kb;
   const int k = p.steps == 1 ? step : (int)__umulhi((unsigned)step, p.mag);
   return k < p.groups ? k : p.groups - 1;  // steps past the row's end
 }
 
-template <int MODE, int MR>
-__device__ __forceinline__ void load_affine(Affine<MODE, MR>& f, const Linear& p, const int (&row)[MR], int kb) {
+// Whole rows': read once.
+template <int MR>
+__device__ __forceinline__ void load_affine(Affine<ROWS, MR>& f, const Linear& p, const int (&row)[MR]) {
 #pragma unroll
-  for (int i = 0; i < Affine<MODE, MR>::N; ++i) {
-    const int k = group_of<MODE>(p, kb, i);
-#pragma unroll
-    for (int j = 0; j < MR; ++j) f.s[j][i] = p.scale[row[j] * p.scale_row + k * p.scale_col];
-    if ((MODE == ROWS || zeros(MODE)) && p.zero) {
-#pragma unroll
-      for (int j = 0; j < MR; ++j) f.z[j][i] = p.zero[row[j] * p.zero_row + k * p.zero_col];
-    } else {
-#pragma unroll
-      for (int j = 0; j < MR; ++j) f.z[j][i] = 0.f;
-    }
+  for (int j = 0; j < MR; ++j) {
+    f.s[j][0] = p.scale[row[j] * p.scale_row];
+    f.z[j][0] = p.zero ? p.zero[row[j] * p.zero_row] : 0.f;
   }
 }
 
-// tot += s acc, and where the group ends here s rest times the sums of its activations (tokens t0 + 16 n + 4 g .. + 3).
-template <int NT, bool Z>
-__device__ __forceinline__ void add_group(floatx4 (&tot)[NT], const floatx4 (&acc)[NT], const Linear& p, int t0, int k, float s,
-                                          float rest, bool ends) {
+// Where a group ends: tot -= s rest times the sums of its activations (tokens t0 + 16 n + 4 g .. + 3).
+template <int NT>
+__device__ __forceinline__ void add_rest(floatx4 (&tot)[NT], const Linear& p, int t0, int k, float s, float rest) {
+  if (!p.corrected || !__builtin_amdgcn_ballot_w64(rest != 0.f)) return;
+  const float f = -s * rest;
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n) {
+    const floatx4 x = *reinterpret_cast<const floatx4*>(p.sums + k * p.sums_row + t0 + 16 * n + 4 * (threadIdx.x >> 4 & 3));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tot[n][i] = __builtin_fmaf(acc[n][i], s, tot[n][i]);
-  if (Z && p.corrected && ends && __builtin_amdgcn_ballot_w64(rest != 0.f)) {
-    const float f = -s * rest;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const floatx4 x = *reinterpret_cast<const floatx4*>(p.sums + k * p.sums_row + t0 + 16 * n + 4 * (threadIdx.x >> 4 & 3));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) tot[n][i] = __builtin_fmaf(x[i], f, tot[n][i]);
-    }
+    for (int i = 0; i < 4; ++i) tot[n][i] = __builtin_fmaf(x[i], f, tot[n][i]);
   }
 }
 
-// A block's products into tot, or acc where its group goes on: c its codes of MR tiles of 16 rows, f their scales and zero
+// A block's products into tot, times their scales where there are groups: c its codes of MR tiles of 16 rows, f their scales and zero
 // points, x(n, i, q) the activations' operand of tokens 16 n, step i, piece q.
 template <int BITS, int MODE, int NT, int MR, int NP, class X>
-__device__ __forceinline__ void block_products(floatx4 (&tot)[MR][NT], floatx4 (&acc)[MR][NT], const Codes<BITS> (&c)[MR],
-                                               const Affine<MODE, MR>& f, X x, const Linear& p, int kb, int kb_last, int t0) {
+__device__ __forceinline__ void block_products(floatx4 (&tot)[MR][NT], const Codes<BITS> (&c)[MR],
+                                               const Affine<MODE, MR>& f, X x, const Linear& p, int kb, int t0) {
   Run<BITS> runs[MR][4];
 #pragma unroll
   for (int j = 0; j < MR; ++j) step_runs<BITS, !narrow(MODE)>(runs[j], c[j]);
   Middle<BITS> mid[MR];
   float rest[MR];
+  if constexpr (!narrow(MODE)) {  // all steps of a tile of tokens in turn: a group's sums live no longer than the block
+    half8 o[MR][4];
+#pragma unroll
+    for (int j = 0; j < MR; ++j) {
+      rest[j] = split_shift<BITS>(mid[j], f.z[j][0] + p.offset);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[j][i] = centred<BITS>(runs[j][i], mid[j]);
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      floatx4 part[MR];
+#pragma unroll
+      for (int j = 0; j < MR; ++j) part[j] = MODE == ROWS ? tot[j][n] : (floatx4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < NP; ++q) {
+          const half8 a = x(n, i, q);
+#pragma unroll
+          for (int j = 0; j < MR; ++j) part[j] = mma(a, o[j][i], part[j]);
+        }
+#pragma unroll
+      for (int j = 0; j < MR; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          tot[j][n][e] = MODE == ROWS ? part[j][e] : __builtin_fmaf(part[j][e], f.s[j][0], tot[j][n][e]);
+      if (MR > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (zeros(MODE)) {
+      const int k = group_of<MODE>(p, kb, 0);
+      if (kb + 1 == (int)((k + 1) * p.steps) || kb + 1 == p.blocks)
+#pragma unroll
+        for (int j = 0; j < MR; ++j) add_rest<NT>(tot[j], p, t0, k, f.s[j][0], rest[j]);
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    if ((narrow(MODE) && zeros(MODE)) || i == 0) {
+    if (zeros(MODE) || i == 0) {
 #pragma unroll
-      for (int j = 0; j < MR; ++j) rest[j] = split_shift<BITS>(mid[j], f.z[j][narrow(MODE) ? i : 0] + p.offset);
+      for (int j = 0; j < MR; ++j) rest[j] = split_shift<BITS>(mid[j], f.z[j][i] + p.offset);
     }
     half8 o[MR];
 #pragma unroll
     for (int j = 0; j < MR; ++j) o[j] = centred<BITS>(runs[j][i], mid[j]);
-    if constexpr (narrow(MODE)) {
-      floatx4 part[MR][NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+    for (int n = 0; n < NT; ++n) {
+      floatx4 part[MR];
 #pragma unroll
-        for (int q = 0; q < NP; ++q) {
-          const half8 a = x(n, i, q);
+      for (int q = 0; q < NP; ++q) {
+        const half8 a = x(n, i, q);
 #pragma unroll
-          for (int j = 0; j < MR; ++j) part[j][n] = mma(a, o[j], q ? part[j][n] : (floatx4){0.f, 0.f, 0.f, 0.f});
-        }
+        for (int j = 0; j < MR; ++j) part[j] = mma(a, o[j], q ? part[j] : (floatx4){0.f, 0.f, 0.f, 0.f});
       }
-      const int step = 4 * kb + i, k = group_of<MODE>(p, kb, i);
-      const bool ends = 32 * step < p.n && (step + 1 == (int)((k + 1) * p.steps) || 32 * (step + 1) >= p.n);
 #pragma unroll
-      for (int j = 0; j < MR; ++j) add_group<NT, zeros(MODE)>(tot[j], part[j], p, t0, k, f.s[j][i], rest[j], ends);
-    } else {
+      for (int j = 0; j < MR; ++j)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int q = 0; q < NP; ++q) {
-          const half8 a = x(n, i, q);
-#pragma unroll
-          for (int j = 0; j < MR; ++j) acc[j][n] = mma(a, o[j], acc[j][n]);
-        }
-      }
+        for (int e = 0; e < 4; ++e) tot[j][n][e] = __builtin_fmaf(part[j][e], f.s[j][i], tot[j][n][e]);
     }
-  }
-  if constexpr (wide(MODE)) {
-    const int k = group_of<MODE>(p, kb, 0);
-    const bool ends = kb + 1 == (int)((k + 1) * p.steps) || kb + 1 == p.blocks;
-    if (ends || kb == kb_last) {
+    if constexpr (zeros(MODE)) {
+      const int step = 4 * kb + i, k = group_of<MODE>(p, kb, i);
+      if (32 * step < p.n && (step + 1 == (int)((k + 1) * p.steps) || 32 * (step + 1) >= p.n))
 #pragma unroll
-      for (int j = 0; j < MR; ++j) {
-        add_group<NT, zeros(MODE)>(tot[j], acc[j], p, t0, k, f.s[j][0], rest[j], ends);
-#pragma unroll
-        for (int n = 0; n < NT; ++n) acc[j][n] = (floatx4){0.f, 0.f, 0.f, 0.f};
-      }
+        for (int j = 0; j < MR; ++j) add_rest<NT>(tot[j], p, t0, k, f.s[j][i], rest[j]);
     }
   }
 }
 
-// After the last block [.., kb_end): whole rows' sums.
+// After the last block [.., kb_end) of whole rows: their scales.
 template <int BITS, int MODE, int NT, int MR>
-__device__ __forceinline__ void end_rows(floatx4 (&tot)[MR][NT], const floatx4 (&acc)[MR][NT], const Affine<MODE, MR>& f,
-                                         const Linear& p, int kb_end, int t0) {
+__device__ __forceinline__ void end_rows(floatx4 (&tot)[MR][NT], const Affine<MODE, MR>& f, const Linear& p, int kb_end, int t0) {
   if constexpr (MODE == ROWS) {
 #pragma unroll
     for (int j = 0; j < MR; ++j) {
       Middle<BITS> mid;
       const float rest = split_shift<BITS>(mid, f.z[j][0] + p.offset);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) tot[j][n] = (floatx4){0.f, 0.f, 0.f, 0.f};
-      add_group<NT, true>(tot[j], acc[j], p, t0, 0, f.s[j][0], rest, kb_end == p.blocks);
+      for (int n = 0; n < NT; ++n) tot[j][n] *= f.s[j][0];
+      if (kb_end == p.blocks) add_rest<NT>(tot[j], p, t0, 0, f.s[j][0], rest);
     }
   }
 }
@@ -272,17 +275,17 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 2) void stream_kernel(Linea
       }
     }
   };
-  floatx4 tot[MR][NT], acc[MR][NT], low[MR][NT];
+  floatx4 tot[MR][NT], low[MR][NT];
 #pragma unroll
   for (int j = 0; j < MR; ++j)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) tot[j][n] = acc[j][n] = low[j][n] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NT; ++n) tot[j][n] = low[j][n] = (floatx4){0.f, 0.f, 0.f, 0.f};
   Affine<MODE, MR> f;
   if constexpr (MODE == ROWS) {
     int row[MR];
 #pragma unroll
     for (int j = 0; j < MR; ++j) row[j] = first + (16 * j + c16 < rows ? 16 * j + c16 : rows - 1);
-    load_affine<MODE, MR>(f, p, row, 0);
+    load_affine<MR>(f, p, row);
   }
 #pragma unroll
   for (int s = 0; s < S - 1; ++s)
@@ -329,16 +332,16 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 2) void stream_kernel(Linea
           }
       }
       block_products<BITS, MODE, NT, MR, NP>(
-          tot, acc, c, f,
+          tot, c, f,
           [&](int n, int i, int q) {
             const int token = (16 * n + c16) % (4 * TQ), piece = narrow(MODE) ? 4 * i + g : 4 * g + i;
             return *reinterpret_cast<const half8*>(at + q * (TQ * 1024) + token * 256 + (piece ^ (token & 15)) * 16);
           },
-          p, b0 + it, b0 + count - 1, t0);
+          p, b0 + it, t0);
     }
     buf = buf + 1 < S ? buf + 1 : 0;
   }
-  if (count) end_rows<BITS, MODE, NT, MR>(tot, acc, f, p, b0 + count, t0);
+  if (count) end_rows<BITS, MODE, NT, MR>(tot, f, p, b0 + count, t0);
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
     const floatx4 f4 = factors(p, t0 + 16 * n);
@@ -380,11 +383,11 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 2) void stream_kernel(Linea
 // the 16 tokens of an operand read lie in different banks.
 template <int BITS, int MODE, int NT, int MR, int WT, int NP>
 __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
-  constexpr int TOK = 16 * NT * WT;
+  constexpr int TOK = 16 * NT * WT, ROWS_OF = 16 * MR * (4 / WT), N = Affine<MODE, MR>::N;
   extern __shared__ float4 lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c16 = lane & 15;
   const int wt = wave % WT, wr = wave / WT;
-  const int tile_t = blockIdx.y * TOK, t0 = tile_t + 16 * NT * wt, r0 = blockIdx.x * (16 * MR * (4 / WT)) + 16 * MR * wr;
+  const int tile_t = blockIdx.y * TOK, t0 = tile_t + 16 * NT * wt, tile_r = blockIdx.x * ROWS_OF, r0 = tile_r + 16 * MR * wr;
   const int split = blockIdx.z;
   const int b0 = split * p.split_blocks, b1 = b0 + p.split_blocks < p.blocks ? b0 + p.split_blocks : p.blocks;
   const int pitch = 256 * p.blocks;  // bytes of a token
@@ -410,6 +413,28 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
         dma_load<4>(rsrc[q], reinterpret_cast<float*>(lds + (buf * NP + q) * (TOK * 16) + (wave * LOADS + i) * 64),
                     off[i] == OOB ? OOB : off[i] + 256 * kb);
   };
+  // scales, then zero points: of row i / N in step i % N, 64 of them a load.  (Loaded by the lanes that use them they are 4
+  // to 32 loads a wave and block, each of 16 lines, and their registers: 2048 tokens x 8192 x 8192, with zero points, groups
+  // of 128 482 us for 342, groups of 32 1500 us for 536.)
+  constexpr int AL = ROWS_OF * N / 64, ALL = zeros(MODE) ? 2 * AL : AL;
+  const int rows_w = p.m - tile_r < ROWS_OF ? p.m - tile_r : ROWS_OF;
+  float* const affine = reinterpret_cast<float*>(lds + 2 * NP * TOK * 16);
+  [[maybe_unused]] auto stage_affine = [&](int kb, int buf) {
+    const int k = narrow(MODE) ? group_of<MODE>(p, kb, lane & 3) : group_of<MODE>(p, kb, 0);
+#pragma unroll
+    for (int i = 0; i < ALL; i += 4) {
+      const int load = i + wave, part = load % AL;
+      if (load >= ALL) break;
+      const bool z = load >= AL;
+      const int r = (64 * part + lane) / N, at = r < rows_w ? r : rows_w - 1;
+      const int64_t first = tile_r * (z ? p.zero_row : p.scale_row);
+      const float* const from = z ? p.zero + (p.zero ? first : 0) : p.scale + first;
+      const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(from), (short)0,
+                                                                         from ? 0x7fffffff : 0, 0x00020000);
+      dma_load<1>(ar, affine + (buf * ALL + load) * 64,
+                  at * (int)(z ? p.zero_row : p.scale_row) * 4 + k * (int)(z ? p.zero_col : p.scale_col) * 4);
+    }
+  };
   int row[MR];
   const unsigned* words[MR];
 #pragma unroll
@@ -418,11 +443,11 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
     row[j] = r < p.m ? r : p.m - 1;
     words[j] = p.words + row[j] * p.row_words;
   }
-  floatx4 tot[MR][NT], acc[MR][NT];
+  floatx4 tot[MR][NT];
 #pragma unroll
   for (int j = 0; j < MR; ++j)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) tot[j][n] = acc[j][n] = (floatx4){0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NT; ++n) tot[j][n] = (floatx4){0.f, 0.f, 0.f, 0.f};
   Codes<BITS> c[MR];
   Affine<MODE, MR> f;
   auto load = [&](int kb) {
@@ -433,8 +458,9 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
 #pragma unroll
       for (int j = 0; j < MR; ++j) load_codes<BITS, true>(c[j], words[j], (4 * kb + g) * BITS, (int)p.row_words);
     }
-    if (MODE != ROWS || kb == b0) load_affine<MODE, MR>(f, p, row, kb);
+    if constexpr (MODE != ROWS) stage_affine(kb, (kb - b0) & 1);
   };
+  if constexpr (MODE == ROWS) load_affine<MR>(f, p, row);
   stage(b0, 0);
   load(b0);
   for (int kb = b0; kb < b1; ++kb) {
@@ -444,31 +470,44 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
     Codes<BITS> now[MR];
 #pragma unroll
     for (int j = 0; j < MR; ++j) now[j] = c[j];
-    const Affine<MODE, MR> nowf = f;
     if (kb + 1 < b1) {
       stage(kb + 1, 1 - buf);
       load(kb + 1);
     }
+    if constexpr (MODE != ROWS) {
+      const float* const at = affine + buf * (ALL * 64) + (16 * MR * wr + c16) * N;
+#pragma unroll
+      for (int j = 0; j < MR; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          f.s[j][i] = at[16 * N * j + i];
+          f.z[j][i] = zeros(MODE) ? at[AL * 64 + 16 * N * j + i] : 0.f;
+        }
+    }
     const float4* in = lds + buf * NP * (TOK * 16);
     block_products<BITS, MODE, NT, MR, NP>(
-        tot, acc, now, nowf,
+        tot, now, f,
         [&](int n, int i, int q) {
           const int token = 16 * (NT * wt + n) + c16, piece = narrow(MODE) ? 4 * i + g : 4 * g + i;
           return __builtin_bit_cast(half8, in[q * (TOK * 16) + token * 16 + (piece ^ c16)]);
         },
-        p, kb, b1 - 1, t0);
+        p, kb, t0);
   }
-  end_rows<BITS, MODE, NT, MR>(tot, acc, f, p, b1, t0);
+  end_rows<BITS, MODE, NT, MR>(tot, f, p, b1, t0);
+  if (t0 >= p.tokens) return;
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    if (t0 + 16 * n < p.tokens) {
-      const floatx4 f = factors(p, t0 + 16 * n);
-      floatx4 out[MR];
+    const floatx4 back = factors(p, t0 + 16 * n);
 #pragma unroll
-      for (int j = 0; j < MR; ++j) out[j] = tot[j][n] * f;
-      if (p.index && split == 0) add_adapters<MR>(out, p, t0 + 16 * n, r0);
-      store_tile<MR>(out, p, t0 + 16 * n, r0, split);
-    }
+    for (int j = 0; j < MR; ++j) tot[j][n] *= back;
+  }
+  if (p.index && split == 0) add_adapters<MR, NT>(tot, p, t0, r0);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    floatx4 out[MR];
+#pragma unroll
+    for (int j = 0; j < MR; ++j) out[j] = tot[j][n];
+    store_tile<MR>(out, p, t0 + 16 * n, r0, split);
   }
 }
 
@@ -505,10 +544,11 @@ int launch_product(const Linear& p, const Plan& q, hipStream_t st) {
   if (q.tile == 16) return launch_stream<BITS, MODE, 1, 4, 1, 4, 2, 1>(p, q, st);
   if (q.tile == 32) return launch_stream<BITS, MODE, 2, 8, 1, 8, 1, 1>(p, q, st);
   if (q.tile == 64) return launch_stream<BITS, MODE, 4, 16, 1, 8, 1, 1>(p, q, st);
+  constexpr int affine = MODE == ROWS ? 0 : 128 * (narrow(MODE) ? 4 : 1) * (zeros(MODE) ? 2 : 1);  // floats of a block
   const auto kernel = tile_kernel<BITS, MODE, 4, 4, 2, 1>;
   if (const int rc = allow_lds(kernel)) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(p.m, q.rows), (unsigned)cdiv(p.tokens, q.tile), (unsigned)q.splits), dim3(256),
-                     (size_t)q.tile * 512, st, p);
+                     (size_t)q.tile * 512 + 8 * affine, st, p);
   return (int)hipGetLastError();
 }
 

@@ -315,3 +315,30 @@ def test_refusals():
             call()
     with pytest.raises(_hip.GPTQ2DError):
         packed_linear(x.cpu(), words, scale, **ok)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_more_adapters_in_sixteen_tokens_than_workgroups(dtype):
+    """1300 tokens (82 tiles of 16, each shared out to fewer workgroups than it has adapters), 40 adapters in any order."""
+    layer = Layer(24, 160, -8, 7, 32, True, seed=9)
+    x = torch.randn(1300, layer.n, generator=layer.g).to(TYPES[dtype])
+    adapters, index = make_adapters(40, 35, layer, x.dtype, 1300, layer.g)
+    want, slack = reference(x, layer, None, adapters, index)
+    check(layer.call(x, adapters=Adapters(*(t.to(DEV) for t in adapters)), index=index.to(DEV)), want, slack)
+
+
+@pytest.mark.parametrize("n", [8000, 16384, 16512, 20001])
+def test_long_rows(n):
+    """Rows that stay in a workgroup's registers while they are brought to fp16, and rows that do not."""
+    for group, zero in ((0, True), (256, True), (32, True)):
+        layer = Layer(5, n, -8, 7, group, zero, seed=n + group)
+        x = torch.randn(3, n, generator=layer.g).bfloat16()
+        want, slack = reference(x, layer)
+        check(layer.call(x), want, slack * (n / 9000 if n > 9000 else 1))
+
+
+def test_rows_too_far_apart_are_refused():
+    """Byte offsets within a workgroup's rows have 31 bits: a stride beyond is an error, not a wrong result."""
+    words = torch.zeros((1 << 28) + 300, dtype=torch.int32, device=DEV).as_strided((2, 16), ((1 << 28) + 1, 1))
+    with pytest.raises(_hip.GPTQ2DError):
+        packed_linear(torch.ones(3, 128, device=DEV), words, torch.ones(2, 1, device=DEV), qmin=-8, qmax=7)
