@@ -375,12 +375,16 @@ __device__ __forceinline__ void read_block(Words<ND>& w, const char* from, int l
   }
 }
 
-// A workgroup takes 16 NQ columns and `chunk` blocks of 32 keys, its waves every fourth block each; the waves' results are
-// joined through LDS.
-template <int TYPE, int ND, int NQ>
-__global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(KvCache c, Attend a) {
+// Few columns.  A workgroup takes 16 of them and `chunk` blocks of 32 keys, its waves every fourth block each; the waves'
+// results are joined through LDS.  Bound by vector instructions for one token a sequence (some 250 a block and wave, most
+// of them on the 32 keys' scales and codes, whatever the columns) and by memory: 64 sequences of up to 8000 tokens, 8 kv
+// heads of 128, bf16: 116 us, 2.5 TB/s of the cache; 4 of up to 131072: 161 us, 3.5 TB/s.  Two tiles of 16 columns a wave,
+// which share a block's codes, need registers that leave half of the waves: 32 columns of 16 x 4000 tokens 95 us for 55 in
+// two workgroups.
+template <int TYPE, int ND>
+__global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int CT = 16 * NQ, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2;
+  constexpr int NQ = 1, CT = 16, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2;
   typedef Ring<ND> R;
   constexpr int S = R::S;
   static_assert(S * R::STAGE >= NQ * 4 * ND * 1024, "a wave's sums fit where its blocks were");
@@ -518,7 +522,10 @@ __global__ __launch_bounds__(THREADS, ND * NQ <= 2 ? 2 : 1) void attend_kernel(K
 // Many columns (a prompt's tokens times the heads that share a kv head).  A workgroup takes 32 columns a wave and `chunk` blocks of
 // 32 keys; the block's codes are brought to fp16 once, by all waves, into LDS, where they lie as operands (two blocks in
 // turn, one barrier a block; the next one's words are in flight meanwhile), and its scales and zeros in fp32 with what all
-// columns share already in them.
+// columns share already in them.  2048 new tokens of 8192, 32 heads on 8 of 128, bf16: 379 us, 635 TFLOP/s of 240 GFLOP.
+// Bound by the two waves a SIMD that its 210 registers allow: of 2030 cycles a block and wave 512 are matrix and about 1000
+// vector instructions', one after the other.  64 columns a wave spill (591 us); the next block's scores beside this one's
+// weights, which needs half as much LDS again, took 408.
 constexpr int PQ = 2, PWAVES = 4;  // columns of a wave: 16 PQ
 
 template <int ND, int QP, int PP>
@@ -754,7 +761,8 @@ __global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a, int 
 
 // How a call is split: columns of a workgroup and blocks of 32 keys of a chunk.
 struct Plan {
-  int nq, nd, ct, chunk, chunks;  // nq 0: prompt_kernel; ct: columns of a workgroup
+  bool prompt;
+  int nd, ct, chunk, chunks;  // ct: columns of a workgroup
   int64_t slots, part;  // part: floats of the partial results
 };
 
@@ -762,15 +770,20 @@ inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int di
   Plan p;
   p.nd = (dim + 63) / 64;
   const int64_t columns = tokens * group;
-  p.nq = columns >= 64 * seqs ? 0 : p.nd > 2 || columns <= 16 * seqs ? 1 : 2;
-  p.ct = p.nq ? 16 * p.nq : 16 * PQ * PWAVES;
+  // From 96 columns a sequence on, a workgroup that brings a block to fp16 once for 128 columns is ahead of workgroups that
+  // each do so for their 16 (16 sequences of 4000, 8 kv heads of 128: 64 columns 93 against 90 us, 96 101 against 120, 256
+  // 199 against 267).
+  p.prompt = columns >= 96 * seqs;
+  p.ct = p.prompt ? 16 * PQ * PWAVES : 16;
   p.slots = columns / p.ct + seqs;
   int64_t range = most;
   if (window && window + p.ct < range) range = window + p.ct;
   const int64_t blocks = range / 32 + 2;
+  // Chunks as large as leave 1024 workgroups, two rounds of two a CU: sequences of different lengths then end together
+  // (64 of up to 8000 tokens, one token each: 116 us, with 512 workgroups 135); at least a block a wave.
   const int64_t want = (blocks * p.slots * heads + 1023) / 1024;
-  if (p.nq)
-    p.chunk = (int)(want < 4 ? 4 : want > 64 ? 64 : want);
+  if (!p.prompt)
+    p.chunk = (int)(want < WAVES ? WAVES : want);
   else  // as many as fill the chip, no more: each writes its columns' sums
     p.chunk = (int)(p.slots * heads >= 256 ? blocks : want < 16 ? 16 : want);
   p.chunks = (int)((blocks + p.chunk - 1) / p.chunk);
@@ -782,15 +795,13 @@ inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int di
 template <int TYPE, int ND>
 int launch(const KvCache& c, const Attend& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)p.slots, (unsigned)c.heads, (unsigned)p.chunks), block(THREADS);
-  if (p.nq == 0) {  // heads first: the workgroups of one XCD (every eighth) then read few heads' keys and values
+  if (p.prompt) {  // heads first: the workgroups of one XCD (every eighth) then read few heads' keys and values
     const int64_t turns = cdiv(p.slots, 65535);
     hipLaunchKernelGGL((prompt_kernel<TYPE, ND>),
                        dim3((unsigned)c.heads, (unsigned)cdiv(p.slots, turns), (unsigned)(p.chunks * turns)),
                        dim3(64 * PWAVES), 0, st, c, a);
-  } else if (p.nq == 1) {
-    hipLaunchKernelGGL((attend_kernel<TYPE, ND, 1>), grid, block, 0, st, c, a);
   } else {
-    if constexpr (ND <= 2) hipLaunchKernelGGL((attend_kernel<TYPE, ND, 2>), grid, block, 0, st, c, a);
+    hipLaunchKernelGGL((attend_kernel<TYPE, ND>), grid, block, 0, st, c, a);
   }
   if (p.chunks > 1)
     hipLaunchKernelGGL((join_kernel<TYPE, ND>), dim3((unsigned)cdiv(c.tokens * c.heads * a.group, WAVES)), block, 0, st, c, a,
@@ -840,7 +851,7 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
     return GPTQ2D_EINVAL;
   if (tokens == 0 || seqs == 0) return 0;
   const Plan p = make_plan(tokens, seqs, heads, group, dim, width * page, window);
-  if (p.slots > 0x7fffffff || p.chunks * (p.nq ? 1 : cdiv(p.slots, 65535)) > 65535) return GPTQ2D_EUNSUPPORTED;
+  if (p.slots > 0x7fffffff || p.chunks * (p.prompt ? cdiv(p.slots, 65535) : 1) > 65535) return GPTQ2D_EUNSUPPORTED;
   if (work_bytes < 4 * p.part || (p.part && (!work || (uintptr_t)work % 16))) return GPTQ2D_ESCRATCH;
   Attend a;
   a.q = q, a.q_token = q_token, a.q_head = q_head;

@@ -354,7 +354,8 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
  * b [adapters, m, rank] of the same type.  words: the codes u of gptq2d_pack_int (m rows of row_words words, bits 2, 3, 4
  * or 8).  scale and zero (NULL: 0) are fp32, read at row *_row + group *_col elements; group: a multiple of 32 columns, 0
  * for whole rows.  index (int32, NULL or adapters 0: none): a token whose index is no adapter has none.  scaling NULL: 1.
- * n below 2^21.  work: 16-byte aligned, gptq2d_packed_linear_workspace bytes, of no use afterwards; GPTQ2D_ESCRATCH where it
+ * n below 2^21; 128 rows of words, scales or zeros (and all groups of a row) must span less than 2^28 elements
+ * (GPTQ2D_EUNSUPPORTED).  work: 16-byte aligned, gptq2d_packed_linear_workspace bytes, of no use afterwards; GPTQ2D_ESCRATCH where it
  * is smaller.  adapters and rank: 0 where index is NULL. */
 int64_t gptq2d_packed_linear_workspace(int64_t tokens, int64_t m, int64_t n, int32_t bits, int64_t group, int32_t type,
                                        int64_t adapters, int64_t rank); /* -1 for sizes it does not take */
