@@ -180,7 +180,7 @@ struct Linear {
   const float* scale;
   const float* zero;  // or none: `offset` everywhere
   int64_t scale_row, scale_col, zero_row, zero_col;
-  float qmin, offset;  // offset: -qmin - 2^(bits - 1)
+  float offset;    // -qmin - 2^(bits - 1)
   int group;       // columns of a group, a multiple of 32 (whole rows: 128 blocks)
   unsigned steps;  // group / 32 (not WIDE: steps of 32 columns of a group) or group / 128
   unsigned mag;    // of the division by `steps`
@@ -383,7 +383,7 @@ __host__ __device__ constexpr bool zeros(int mode) { return mode & ZEROS; }
 // How a call is computed: tile (tokens of a workgroup; up to 64 stream_kernel, 128 tile_kernel), rows of a workgroup, splits
 // of the columns, and where its workspace holds what (floats).
 struct Plan {
-  int pieces, tile, rows, splits, split_blocks, mode, bits, rank_pad, slots, chunks, chunk;
+  int pieces, tile, rows, splits, split_blocks, mode, rank_pad, slots, chunks, chunk;
   int64_t groups, sums_row, xp, factor, sums, v, part, total;  // offsets; total: floats
 };
 

@@ -4,6 +4,8 @@
 //                   others, beside them, multiply 16 tokens by one adapter's A over a chunk of columns;
 //   stream_kernel (up to 64 tokens) or tile_kernel (more): the product, with B and the bias in its epilogue;
 //   finish_kernel: adds the parts of a row that several workgroups summed.
+// Measured: prepare_kernel 5.4 us for one token (launch and two latencies), 2048 x 8192 bf16 22 us (67 MB, 3.1 TB/s), 42
+// with four adapters of rank 64 beside them (their loads' latency: two CU-fulls of workgroups); finish_kernel 4 to 5 us.
 #include "packed_linear.h"
 
 namespace {
@@ -234,21 +236,28 @@ inline bool make_plan(Plan& q, int64_t tokens, int64_t m, int64_t n, int bits, i
     return false;
   const int64_t blocks = cdiv(n, 128);
   if (group >= n) group = 0;
-  q.bits = bits;
   q.pieces = type == TYPE_F32 ? 2 : 1;
   q.mode = group == 0 ? ROWS : (group % 128 == 0 ? WIDE : NARROW) | (zero ? ZEROS : 0);
   q.groups = group ? cdiv(n, group) : 1;
-  int64_t wgs, least;  // workgroups without splits, blocks of a split at least
+  // Rows and tokens of a workgroup (fp32, whose activations are two pieces, stays with small tiles).  Measured, us, bf16:
+  //   up to 4 tokens 16 rows of W, else 64: 4096 x 4096, 1 token 18.5 against 21.0; 8192 x 28672, 4 tokens 37.8 against 39.3;
+  //   up to 64 tokens stream_kernel, more tile_kernel: 64 tokens, 14336 x 4096 33.9 against 38.1; 128 tokens, 8192 x 28672
+  //   101 against 92; and 65 to 128 tokens of a layer that tile_kernel makes fewer than 256 workgroups of: 128 tokens,
+  //   4096 x 4096 25.0 against 34.9.
+  int64_t wgs, least, enough;  // workgroups without splits, blocks of a split at least, workgroups that need no splits
+  const bool small = cdiv(m, 128) * cdiv(blocks, 8) < 256;
   if (tokens <= 4) {
-    q.tile = 16, q.rows = 16, least = 16;
-  } else if (tokens <= 64 || q.pieces == 2) {
+    q.tile = 16, q.rows = 16, least = 16, enough = 192;
+  } else if (tokens <= 64 || q.pieces == 2 || (tokens <= 128 && small)) {
     q.tile = tokens <= 16 ? 16 : tokens <= 32 || q.pieces == 2 ? 32 : 64;
-    q.rows = tokens <= 16 || q.pieces == 2 ? 64 : 128, least = 8;
+    q.rows = tokens <= 16 || q.pieces == 2 ? 64 : 128, least = 8, enough = 192;
   } else {
-    q.tile = 128, q.rows = 128, least = 8;
+    q.tile = 128, q.rows = 128, least = 8, enough = 384;
   }
   wgs = cdiv(m, q.rows) * cdiv(tokens + !tokens, q.tile);
-  int64_t splits = wgs >= 192 ? 1 : cdiv(512, wgs);
+  // Columns are split where the workgroups leave CUs idle, at the price of finish_kernel: 16 tokens, 8192 x 8192 (128
+  // workgroups) 22.5 us in four parts, 25.3 in one; 14336 x 4096 (224) 21.9 and 19.2.
+  int64_t splits = wgs >= enough ? 1 : cdiv(512, wgs);
   if (splits > cdiv(blocks, least)) splits = cdiv(blocks, least);
   if (splits > 64) splits = 64;
   q.split_blocks = (int)cdiv(blocks, splits);
@@ -309,7 +318,6 @@ int gptq2d_packed_linear(const void* x, int64_t x_token, int32_t type, int64_t t
   p.words = words, p.row_words = row_words;
   p.scale = scale, p.scale_row = scale_row, p.scale_col = scale_col;
   p.zero = zero, p.zero_row = zero_row, p.zero_col = zero_col;
-  p.qmin = (float)qmin;
   p.offset = (float)offset;
   p.group = group ? (int)group : 128 * p.blocks;
   p.steps = (unsigned)(narrow(q.mode) ? p.group / 32 : p.group / 128);

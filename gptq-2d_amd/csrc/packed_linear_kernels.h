@@ -181,6 +181,9 @@ __device__ __forceinline__ void wait_loads() {
 // register; every wave issues the same number of loads a block and waits for its own by count.  In LDS a token's 16 pieces
 // of 16 bytes lie at piece ^ token, so that the 16 tokens of an operand read lie in different banks; codes and scales lie
 // as the lanes read them.  TQ: quads of tokens that are staged.
+// Measured, INT4: 14336 x 4096 in groups of 128, 16 tokens 18.5 us (1.9 TB/s: seven blocks a wave, of which the ring's
+// first fill and the sums' joining take half); 8192 x 28672 in groups of 32, 32 tokens 50 us (3.0 TB/s; 64 fused multiply-adds and
+// 40 conversions a block for 16 products); 4096 x 4096, one token 7 us.
 template <int BITS, int MODE, int NT, int TQ, int MR, int WR, int WK, int NP>
 struct Ring {
   static constexpr int X = NP * TQ;                              // loads of 1 KB: activations
@@ -378,9 +381,13 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 2) void stream_kernel(Linea
 }
 
 // More tokens: 256 threads take 16 NT WT tokens and 16 MR (4 / WT) rows of W, each wave 16 NT tokens and 16 MR rows.  The
-// activations of a block of 128 columns go to LDS straight from memory, two blocks in turn; the codes and scales from memory
-// to the wave that multiplies by them, a block ahead.  In LDS a token's 16 pieces of 16 bytes lie at piece ^ token, so that
+// activations of a block of 128 columns, scales and zero points go to LDS straight from memory, two blocks in turn; the codes
+// from memory to the wave that multiplies by them, a block ahead.  In LDS a token's 16 pieces of 16 bytes lie at piece ^ token, so that
 // the 16 tokens of an operand read lie in different banks.
+// Measured, INT4, 2048 tokens x 8192 x 8192: rows 296 us, groups of 128 300 us (916 TFLOP/s; a library's fp16 product of that size
+// takes 221 us), with zero points 320, groups of 32 with zero points 505.
+// Bound by the two waves a SIMD that 255 registers leave: 1024 cycles of matrix and some 850 of vector instructions a block
+// and wave overlap only between them.
 template <int BITS, int MODE, int NT, int MR, int WT, int NP>
 __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
   constexpr int TOK = 16 * NT * WT, ROWS_OF = 16 * MR * (4 / WT), N = Affine<MODE, MR>::N;
