@@ -376,11 +376,11 @@ __device__ __forceinline__ void read_block(Words<ND>& w, const char* from, int l
 }
 
 // Few columns.  A workgroup takes 16 of them and `chunk` blocks of 32 keys, its waves every fourth block each; the waves'
-// results are joined through LDS.  Bound by vector instructions for one token a sequence (some 250 a block and wave, most
-// of them on the 32 keys' scales and codes, whatever the columns) and by memory: 64 sequences of up to 8000 tokens, 8 kv
-// heads of 128, bf16: 116 us, 2.5 TB/s of the cache; 4 of up to 131072: 161 us, 3.5 TB/s.  Two tiles of 16 columns a wave,
-// which share a block's codes, need registers that leave half of the waves: 32 columns of 16 x 4000 tokens 95 us for 55 in
-// two workgroups.
+// results are joined through LDS.  Bound by memory for long sequences: 4 of up to 131072 tokens, 8 kv heads of 128, bf16,
+// one token each: 159 us, 3.6 TB/s of the cache (a read-only sum: 4.0); by the unequal lengths otherwise: 64 of 300 to 8000
+// tokens 120 us, 2.4 TB/s.  Some 300 vector instructions a block and wave, most of them on the 32 keys' scales and codes,
+// whatever the columns.  Two tiles of 16 columns a wave, which share them, need registers that leave half of the waves:
+// 32 columns of 16 x 4000 tokens 95 us for 55 in two workgroups.
 template <int TYPE, int ND>
 __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
@@ -710,7 +710,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   }
 }
 
-// Joins the chunks' results: a wave a (token, query head), whose chunks are added in their order.
+// Joins the chunks' results: a wave a (token, query head), whose chunks are added in their order.  Bound by latency (4 to 7 us).
 template <int TYPE, int ND>
 __global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a, int CT) {
   typedef typename Elem<TYPE>::T T;
@@ -741,15 +741,34 @@ __global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a, int 
   float sum[ND], l = 0.f;
 #pragma unroll
   for (int d = 0; d < ND; ++d) sum[d] = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < t.chunks; ++i) {
-    const float* p = part + (int64_t)i * (CT * (DP + 2));
-    const float x = p[CT * DP + in];
-    const float f = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - top);
-    l += f * p[CT * (DP + 1) + in];
+  for (int i0 = 0; i0 < t.chunks; i0 += 64) {  // a lane a chunk's weight, then the chunks' sums, U loads in flight
+    constexpr int U = 16 / ND;
+    const int n = t.chunks - i0 < 64 ? t.chunks - i0 : 64;
+    const float* p = part + (int64_t)i0 * (CT * (DP + 2));
+    float f = 0.f;
+    if (lane < n) {
+      const float* mine = p + (int64_t)lane * (CT * (DP + 2)) + CT * DP + in;
+      const float x = mine[0];
+      f = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - top);
+      l += f * mine[CT];
+    }
+    for (int i = 0; i < n; i += U) {
+      float v[U][ND];
 #pragma unroll
-    for (int d = 0; d < ND; ++d) sum[d] += f * p[in * DP + 64 * d + lane];
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+          v[u][d] = p[(int64_t)(i + u < n ? i + u : n - 1) * (CT * (DP + 2)) + in * DP + 64 * d + lane];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = __shfl(f, i + u < n ? i + u : 0);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) sum[d] += i + u < n ? w * v[u][d] : 0.f;
+      }
+    }
   }
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) l += __shfl_xor(l, s);
   const float f = l == 0.f ? 0.f : 1.f / l;
   T* out = (T*)a.out + row * a.out_token + hq * a.out_head;
 #pragma unroll
@@ -779,11 +798,14 @@ inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int di
   int64_t range = most;
   if (window && window + p.ct < range) range = window + p.ct;
   const int64_t blocks = range / 32 + 2;
-  // Chunks as large as leave 1024 workgroups, two rounds of two a CU: sequences of different lengths then end together
-  // (64 of up to 8000 tokens, one token each: 116 us, with 512 workgroups 135); at least a block a wave.
-  const int64_t want = (blocks * p.slots * heads + 1023) / 1024;
+  // Chunks as large as leave 768 workgroups, one and a half rounds of two a CU, so that sequences of different lengths end
+  // together (one token each, us for 512, 768 and 1024: 64 sequences of up to 8000 tokens 135, 121, 119; 4 of 131072 179,
+  // 159, 154; 64 of 4000 94, 86, 91; one of 100000 41, 49, 53); at least two blocks a wave, whose start takes longer than
+  // that (one of 16000: 19 us, with one block a wave 29).
+  const int64_t tiles = cdiv(columns, p.ct) > seqs ? cdiv(columns, p.ct) : seqs;  // that hold columns, about
+  const int64_t want = cdiv(blocks * tiles * heads, 768);
   if (!p.prompt)
-    p.chunk = (int)(want < WAVES ? WAVES : want);
+    p.chunk = (int)(want < 2 * WAVES ? 2 * WAVES : want);
   else  // as many as fill the chip, no more: each writes its columns' sums
     p.chunk = (int)(p.slots * heads >= 256 ? blocks : want < 16 ? 16 : want);
   p.chunks = (int)((blocks + p.chunk - 1) / p.chunk);
