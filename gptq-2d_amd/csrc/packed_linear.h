@@ -27,10 +27,11 @@ struct Codes {
   unsigned w[BITS];
 };
 
-// Words at .. at + BITS - 1 of a row (vector loads need only a word's own alignment); GUARD: zeros past the row's end, where
-// the activations are zeros.
+// Words at .. at + BITS - 1 of a row (vector loads need only a word's own alignment); GUARD: zeros from word `end` on, the
+// end of those that hold codes (the next row may begin anywhere after it, the last one has nothing behind it), where the
+// activations are zeros.
 template <int BITS, bool GUARD>
-__device__ __forceinline__ void load_codes(Codes<BITS>& c, const unsigned* row, int at, int row_words) {
+__device__ __forceinline__ void load_codes(Codes<BITS>& c, const unsigned* row, int at, int end) {
   typedef unsigned vec4 __attribute__((ext_vector_type(4), aligned(4)));
   typedef unsigned vec3 __attribute__((ext_vector_type(3), aligned(4)));
   typedef unsigned vec2 __attribute__((ext_vector_type(2), aligned(4)));
@@ -38,7 +39,7 @@ __device__ __forceinline__ void load_codes(Codes<BITS>& c, const unsigned* row, 
 #pragma unroll
     for (int i = 0; i < BITS; ++i) {
       c.w[i] = 0;
-      if (at + i < row_words) c.w[i] = row[at + i];
+      if (at + i < end) c.w[i] = row[at + i];
     }
   } else if constexpr (BITS == 2) {
     const vec2 v = *reinterpret_cast<const vec2*>(row + at);

@@ -460,10 +460,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
   auto load = [&](int kb) {
     if (kb < p.whole) {
 #pragma unroll
-      for (int j = 0; j < MR; ++j) load_codes<BITS, false>(c[j], words[j], (4 * kb + g) * BITS, (int)p.row_words);
+      for (int j = 0; j < MR; ++j) load_codes<BITS, false>(c[j], words[j], (4 * kb + g) * BITS, (int)p.need_words);
     } else {
 #pragma unroll
-      for (int j = 0; j < MR; ++j) load_codes<BITS, true>(c[j], words[j], (4 * kb + g) * BITS, (int)p.row_words);
+      for (int j = 0; j < MR; ++j) load_codes<BITS, true>(c[j], words[j], (4 * kb + g) * BITS, (int)p.need_words);
     }
     if constexpr (MODE != ROWS) stage_affine(kb, (kb - b0) & 1);
   };

@@ -342,3 +342,21 @@ def test_rows_too_far_apart_are_refused():
     words = torch.zeros((1 << 28) + 300, dtype=torch.int32, device=DEV).as_strided((2, 16), ((1 << 28) + 1, 1))
     with pytest.raises(_hip.GPTQ2DError):
         packed_linear(torch.ones(3, 128, device=DEV), words, torch.ones(2, 1, device=DEV), qmin=-8, qmax=7)
+
+
+@pytest.mark.parametrize("bits", [2, 3, 4, 8])
+@pytest.mark.parametrize("tokens", [3, 30, 140])
+def test_words_that_end_where_their_storage_does(tokens, bits):
+    """Words as the last columns of a wider array, few tokens and many: nothing behind the last row's codes is read, and what
+    lies between the rows' codes is of no matter."""
+    half = 1 << (bits - 1)
+    layer = Layer(40, 200, -half, half - 1, 0, False, seed=bits)
+    x = torch.randn(tokens, 200, generator=layer.g).bfloat16().to(DEV)
+    words = layer.words()
+    wide = torch.full((40, words.size(1) + 15), -1, dtype=torch.int32, device=DEV)
+    wide[:, 15:] = words
+    kw = dict(qmin=-half, qmax=half - 1)
+    got = packed_linear(x, wide[:, 15:], layer.scale.to(DEV), **kw)
+    assert torch.equal(got, packed_linear(x, words, layer.scale.to(DEV), **kw))
+    want, slack = reference(x.cpu(), layer)
+    check(got, want, slack)
