@@ -1,9 +1,8 @@
 // The product's kernels for one width of the codes (each width is a source file of its own: packed_linear_bits*.hip).
 #pragma once
 
+#include "lds_limit.h"
 #include "packed_linear.h"
-
-#include <atomic>
 
 namespace {
 
@@ -518,24 +517,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
   }
 }
 
-// A kernel that may use all of a CU's LDS: said once for each device (the attribute is per device).
-template <class K>
-int allow_lds(K kernel) {
-  static std::atomic<uint64_t> told{0};
-  int dev = 0;
-  const int rc = (int)hipGetDevice(&dev);
-  if (rc) return rc;
-  if (dev < 64 && told.load(std::memory_order_relaxed) >> dev & 1) return 0;
-  const int set = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                           163840);
-  if (!set && dev < 64) told.fetch_or((uint64_t)1 << dev, std::memory_order_relaxed);
-  return set;
-}
-
 template <int BITS, int MODE, int NT, int TQ, int MR, int WR, int WK, int NP>
 int launch_stream(const Linear& p, const Plan& q, hipStream_t st) {
-  const auto kernel = stream_kernel<BITS, MODE, NT, TQ, MR, WR, WK, NP>;
-  if (const int rc = allow_lds(kernel)) return rc;
+  constexpr auto kernel = stream_kernel<BITS, MODE, NT, TQ, MR, WR, WK, NP>;
+  if (const int rc = allow_lds<kernel>()) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(p.m, 16 * MR * WR), (unsigned)cdiv(p.tokens, q.tile), (unsigned)q.splits),
                      dim3(64 * WR * WK), (Ring<BITS, MODE, NT, TQ, MR, WR, WK, NP>::BYTES), st, p);
   return (int)hipGetLastError();
@@ -552,8 +537,8 @@ int launch_product(const Linear& p, const Plan& q, hipStream_t st) {
   if (q.tile == 32) return launch_stream<BITS, MODE, 2, 8, 1, 8, 1, 1>(p, q, st);
   if (q.tile == 64) return launch_stream<BITS, MODE, 4, 16, 1, 8, 1, 1>(p, q, st);
   constexpr int affine = MODE == ROWS ? 0 : 128 * (narrow(MODE) ? 4 : 1) * (zeros(MODE) ? 2 : 1);  // floats of a block
-  const auto kernel = tile_kernel<BITS, MODE, 4, 4, 2, 1>;
-  if (const int rc = allow_lds(kernel)) return rc;
+  constexpr auto kernel = tile_kernel<BITS, MODE, 4, 4, 2, 1>;
+  if (const int rc = allow_lds<kernel>()) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(p.m, q.rows), (unsigned)cdiv(p.tokens, q.tile), (unsigned)q.splits), dim3(256),
                      (size_t)q.tile * 512 + 8 * affine, st, p);
   return (int)hipGetLastError();

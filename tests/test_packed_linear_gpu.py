@@ -360,3 +360,22 @@ def test_words_that_end_where_their_storage_does(tokens, bits):
     assert torch.equal(got, packed_linear(x, words, layer.scale.to(DEV), **kw))
     want, slack = reference(x.cpu(), layer)
     check(got, want, slack)
+
+
+@pytest.mark.parametrize("tokens", [2, 24, 140])
+def test_first_call_of_a_kernel_in_a_graph(tokens):
+    """A kernel that the process has not launched yet may be captured: 2-bit codes in groups of 160, which no other test has."""
+    layer = Layer(50, 800, -2, 1, 160, tokens > 30, seed=tokens)
+    x = torch.randn(tokens, 800, generator=layer.g).half().to(DEV)
+    words, scale = layer.words(), layer.scale.to(DEV)
+    zero = None if layer.zero is None else layer.zero.to(DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = packed_linear(x, words, scale, zero, qmin=-2, qmax=1, group=160)
+    for turn in range(3):
+        x.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        want, slack = reference(x.cpu(), layer)
+        check(out, want, slack)
