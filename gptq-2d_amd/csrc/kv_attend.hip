@@ -37,7 +37,7 @@ struct Tile {
   int col0, cols;  // first column, columns of the sequence
   int pos0;        // position of the sequence's first query
   int kb0, kb1;
-  int pos_lo, pos_hi;  // least and largest position of a column
+  int pos_lo, pos_hi;  // least and largest position of a column; they may lie past the tokens held
   int len;             // tokens that the sequence holds
   int chunks;          // workgroups that share the blocks
 };
@@ -50,14 +50,16 @@ __device__ __forceinline__ Tile make_tile(const KvCache& c, const Attend& a, int
   const int n = t1 > t0 ? (int)(t1 - t0) : 0;
   t.cols = n * a.group;
   t.col0 = col0;
+  const int length = c.lengths[b];  // the table may have no room for all of it: that bounds the keys, not the positions
   t.len = kv_length(c, b);
-  t.pos0 = t.len - n;
+  t.pos0 = (length < 0 ? 0 : length) - n;
   const int last = t.cols - 1 < col0 + CT - 1 ? t.cols - 1 : col0 + CT - 1;
   t.pos_lo = t.pos0 + col0 / a.group;
   t.pos_hi = t.pos0 + (last < 0 ? 0 : last) / a.group;
   const int first = a.window && t.pos_lo - a.window + 1 > 0 ? t.pos_lo - a.window + 1 : 0;
   t.kb0 = first / 32;
-  t.kb1 = t.pos_hi < 0 ? t.kb0 : t.pos_hi / 32 + 1;
+  const int end = t.pos_hi < t.len ? t.pos_hi + 1 : t.len;  // of the keys that a column sees
+  t.kb1 = end > 0 ? (end - 1) / 32 + 1 : t.kb0;
   if (t.kb1 < t.kb0) t.kb1 = t.kb0;
   t.chunks = t.kb1 - t.kb0 > a.chunk ? (t.kb1 - t.kb0 + a.chunk - 1) / a.chunk : 1;
   return t;
@@ -162,11 +164,12 @@ __device__ __forceinline__ void clear(State<ND, NQ>& st) {
 
 // Exponents e of a block's scores off the reference, and the sums so far brought to the values' new `shift` and, where a
 // column's reference moves, to it -- in one place, so that the sums stay in their registers.  key0: this lane's first key
-// (keys key0 + 16 (i / 4) + i % 4); ks, kz: scales and zeros with what all columns share in them.
+// (keys key0 + 16 (i / 4) + i % 4); len: tokens that the block's page can have (0 without a page); ks, kz: scales and
+// zeros with what all columns share in them.
 template <int ND, int NQ>
 __device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], const floatx4 (&s)[NQ][2], const float (&ks)[8],
                                           const float (&kz)[8], const float (&qsum)[NQ], bool mask, int key0,
-                                          const int (&pos)[NQ], int window, int shift) {
+                                          const int (&pos)[NQ], int window, int len, int shift) {
   float most[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n)
@@ -177,11 +180,11 @@ __device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], 
     asm volatile("");  // a branch, not sixteen selects for every block
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int from = window ? pos[n] - window : -1;
+      const int from = window ? pos[n] - window : -1, to = pos[n] < len ? pos[n] : len - 1;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int key = key0 + 16 * (i / 4) + i % 4;
-        e[n][i] = key > pos[n] || key <= from ? -__builtin_inff() : e[n][i];
+        e[n][i] = key > to || key <= from ? -__builtin_inff() : e[n][i];
       }
     }
   }
@@ -316,7 +319,7 @@ __device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)
     ks[i] *= factor, kz[i] *= factor;
   }
   const int shift = admit(st.shift, bits, vs);
-  exponents<ND, NQ>(st, e, s, ks, kz, qsum, mask, key0, pos, window, shift);
+  exponents<ND, NQ>(st, e, s, ks, kz, qsum, mask, key0, pos, window, len, shift);
 #pragma unroll
   for (int i = 0; i < 8; ++i) vs[i] = __builtin_ldexpf(vs[i], ROOM - shift);
   half8 p[NQ][PP];
@@ -401,7 +404,9 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
 
   const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + chunk * a.chunk);
   const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
-  const int pos_lo = __builtin_amdgcn_readfirstlane(t.pos_lo), pos_hi = __builtin_amdgcn_readfirstlane(t.pos_hi);
+  // all columns see the keys in [all_from, all_to]
+  const int all_to = __builtin_amdgcn_readfirstlane(t.pos_lo < t.len ? t.pos_lo : t.len - 1);
+  const int all_from = __builtin_amdgcn_readfirstlane(a.window ? t.pos_hi - a.window + 1 : 0);
   const int hw = (int)kv_head_words(ND, c.page);
   const int64_t b = t.b;
   const int first = begin + wave, count = end > first ? (end - first + WAVES - 1) / WAVES : 0;
@@ -447,11 +452,8 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
     read_block<ND>(w, ring[wave][buf], lane);
     const int kb = first + WAVES * i;
     const bool page = there >> buf & 1u;
-    const bool mask = !page || !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
-    int seen[NQ];
-#pragma unroll
-    for (int n = 0; n < NQ; ++n) seen[n] = page ? pos[n] : -1;  // without a page nobody sees its keys
-    attend_block<ND, NQ, QP, PP>(st, q, qsum, w, factor, mask, kb * 32 + 4 * g, page ? t.len : 0, seen, a.window);
+    const bool mask = !page || kb * 32 + 31 > all_to || kb * 32 < all_from;
+    attend_block<ND, NQ, QP, PP>(st, q, qsum, w, factor, mask, kb * 32 + 4 * g, page ? t.len : 0, pos, a.window);
     buf = buf + 1 < S ? buf + 1 : 0;
   }
   // the waves' results, brought to one reference, in the place of their own blocks; then every thread adds four elements
@@ -531,7 +533,7 @@ constexpr int PQ = 2, PWAVES = 4;  // columns of a wave: 16 PQ
 template <int ND, int QP, int PP>
 __device__ __forceinline__ void prompt_block(State<ND, PQ>& st, const half8 (&q)[PQ][2 * ND][QP], const float (&qsum)[PQ],
                                              const half8 (*kop)[64], const half8 (*vop)[64], const float (*aff)[32], bool mask,
-                                             int key0, const int (&pos)[PQ], int window, int shift) {
+                                             int key0, const int (&pos)[PQ], int window, int len, int shift) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
   floatx4 s[PQ][2];
 #pragma unroll
@@ -558,7 +560,7 @@ __device__ __forceinline__ void prompt_block(State<ND, PQ>& st, const half8 (&q)
   };
   read(a0, 0);
   read(a1, 1);
-  exponents<ND, PQ>(st, e, s, a0, a1, qsum, mask, key0, pos, window, shift);
+  exponents<ND, PQ>(st, e, s, a0, a1, qsum, mask, key0, pos, window, len, shift);
   half8 p[PQ][PP];
   read(a0, 2);
   read(a1, 3);
@@ -610,7 +612,9 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   clear(st);
   const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + part * a.chunk);
   const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
-  const int pos_lo = __builtin_amdgcn_readfirstlane(t.pos_lo), pos_hi = __builtin_amdgcn_readfirstlane(t.pos_hi);
+  // all columns see the keys in [all_from, all_to]
+  const int all_to = __builtin_amdgcn_readfirstlane(t.pos_lo < t.len ? t.pos_lo : t.len - 1);
+  const int all_from = __builtin_amdgcn_readfirstlane(a.window ? t.pos_hi - a.window + 1 : 0);
   const int hw = (int)kv_head_words(ND, c.page), len = t.len;
   const int64_t b = t.b;
   uint4v words[CH];
@@ -665,11 +669,9 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
     int at3 = 0;
     const unsigned* after = kb + 2 < end ? kv_head(c, b, kb + 2, head, hw, at3) : nullptr;
     const int shift = __builtin_amdgcn_readfirstlane(shifts[buf]);
-    const bool mask = !base || !(kb * 32 + 31 <= pos_lo && (!a.window || kb * 32 > pos_hi - a.window));
-    int seen[PQ];
-#pragma unroll
-    for (int n = 0; n < PQ; ++n) seen[n] = base ? pos[n] : -1;  // without a page nobody sees its keys
-    prompt_block<ND, QP, PP>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], mask, kb * 32 + 4 * g, seen, a.window, shift);
+    const bool mask = !base || kb * 32 + 31 > all_to || kb * 32 < all_from;
+    prompt_block<ND, QP, PP>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], mask, kb * 32 + 4 * g, pos, a.window,
+                             base ? len : 0, shift);
     if (kb + 1 < end) put(kb + 1, 1 - buf, next);
     __syncthreads();
     base = next, next = after, at2 = at3;

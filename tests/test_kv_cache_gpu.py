@@ -409,3 +409,34 @@ def test_refusals():
     for call in bad:
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("window", [None, 3, 40])
+@pytest.mark.parametrize("new", [1, 8, 90])
+@pytest.mark.parametrize("length", [97, 100, 135, 500])
+def test_positions_past_the_table(length, new, window):
+    """Queries stand at length - T + i also where the table has no room for all tokens: those past it are seen by nobody, and
+    the others by the queries that they are before.  (As `append` places them: 4 more tokens after 96 end at position 99.)"""
+    s = Sequences([96, 33], 2, 80, torch.float32, 32, seed=length + new)
+    q = torch.randn(new + 1, 6, 80, generator=s.g)
+    lengths = torch.tensor([length, 33], dtype=torch.int32, device=DEV)
+    got, lse = s.cache.attend(q.to(DEV), s.dev_table, lengths, starts([new, 1]), window=window, return_lse=True)
+    kv, vv = held_values(s.k), held_values(s.v)
+    want, want_lse = torch.zeros(q.shape, dtype=torch.float64), torch.full(q.shape[:2], -math.inf, dtype=torch.float64)
+    for r in range(new + 1):
+        first, last = 0, min(length - new + r, 95)
+        at = length - new + r
+        if r == new:
+            last = at = 32
+        if window:
+            first = max(0, at - window + 1)
+        if first <= last:
+            rows = torch.arange(first, last + 1) + (96 if r == new else 0)
+            z = torch.einsum("hd,nhd->hn", q[r].double(), kv[rows].repeat_interleave(3, 1)) * 80 ** -0.5
+            want_lse[r] = torch.logsumexp(z, -1)
+            want[r] = torch.einsum("hn,nhd->hd", torch.softmax(z, -1), vv[rows].repeat_interleave(3, 1))
+    check(got, want, float(vv.abs().max()), torch.float32)
+    empty = want_lse == -math.inf
+    assert torch.equal(lse.cpu() == -math.inf, empty) and not got.cpu()[empty].any()
+    off = (lse.cpu().double() - want_lse)[~empty].abs()
+    assert off.numel() == 0 or float(off.max()) < 1e-4
