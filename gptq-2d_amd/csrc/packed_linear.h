@@ -231,7 +231,8 @@ __device__ __forceinline__ int adapter_of(const Linear& p, int t) {
 }
 
 // tot[j][n] += V B^T for the 16 NT tokens from t0 and the rows r0 + 16 j of W, one distinct adapter of the tokens after the
-// other, the others' rows of V zeros; its B is read once for all of them.  V (fp32) and B (fp16 or bf16) are taken in bf16
+// other; its B is read once for all of them.  The other tokens' rows of V are zeros, and what they make of B is dropped: an
+// infinity or NaN in one request's adapter stays in its own tokens.  V (fp32) and B (fp16 or bf16) are taken in bf16
 // pieces: six products, 2^-23 of the result; of bf16 adapters B is one piece, and two of V leave out 2^-17.  For long
 // batches, where a wave's tokens have few adapters.
 template <int MR, int NT>
@@ -271,6 +272,9 @@ __device__ __forceinline__ void add_adapters(floatx4 (&tot)[MR][NT], const Linea
         }
         bf16x8 vp[3];
         split8(v, vp);
+        floatx4 before[MR];
+#pragma unroll
+        for (int j = 0; j < MR; ++j) before[j] = tot[j][n];
         if (p.type == TYPE_BF16) {
 #pragma unroll
           for (int q = 1; q >= 0; --q)
@@ -288,6 +292,12 @@ __device__ __forceinline__ void add_adapters(floatx4 (&tot)[MR][NT], const Linea
 #pragma unroll
             for (int q = 0; q < NPROD; ++q) tot[j][n] = mma(vp[prod_a[q]], bp[prod_b[q]], tot[j][n]);
           }
+        }
+        if (these != 0xffffu) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < MR; ++j) tot[j][n][i] = these >> (4 * g + i) & 1u ? tot[j][n][i] : before[j][i];
         }
       }
     }

@@ -379,3 +379,23 @@ def test_first_call_of_a_kernel_in_a_graph(tokens):
         torch.cuda.synchronize()
         want, slack = reference(x.cpu(), layer)
         check(out, want, slack)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("what", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("tokens", [7, 60, 150, 400])
+def test_adapters_that_are_no_numbers(tokens, what, dtype):
+    """An infinity or NaN in one adapter (its A, its B or its scaling) changes the tokens that have it and no others, in short
+    batches and in long ones, where 16 tokens share the matrix cores' tiles."""
+    layer = Layer(70, 200, -8, 7, 0, False, seed=tokens)
+    x = torch.randn(tokens, layer.n, generator=layer.g).to(TYPES[dtype])
+    adapters, index = make_adapters(4, 20, layer, x.dtype, tokens, layer.g)
+    index[tokens // 2] = 2
+    run = lambda ad: layer.call(x, adapters=Adapters(*(t.to(DEV) for t in ad)), index=index.to(DEV)).cpu()
+    clean, own = run(adapters), index == 2
+    for part in range(3):
+        dirty = [t.clone() for t in adapters]
+        dirty[part].view(4, -1)[2] = what
+        got = run(dirty)
+        assert torch.equal(got[~own], clean[~own])
+        assert not bool(got[own].isfinite().any())
