@@ -30,7 +30,8 @@ __device__ __forceinline__ void load_affine(Affine<ROWS, MR>& f, const Linear& p
   }
 }
 
-// Where a group ends: tot -= s rest times the sums of its activations (tokens t0 + 16 n + 4 g .. + 3).
+// Where a group ends: tot -= s rest times the sums of its activations (tokens t0 + 16 n + 4 g .. + 3), in the rows with a
+// rest: the sums may be infinite or NaN, which times 0 would be NaN in rows that only share the wave with such a row.
 template <int NT>
 __device__ __forceinline__ void add_rest(floatx4 (&tot)[NT], const Linear& p, int t0, int k, float s, float rest) {
   if (!p.corrected || !__builtin_amdgcn_ballot_w64(rest != 0.f)) return;
@@ -39,7 +40,7 @@ __device__ __forceinline__ void add_rest(floatx4 (&tot)[NT], const Linear& p, in
   for (int n = 0; n < NT; ++n) {
     const floatx4 x = *reinterpret_cast<const floatx4*>(p.sums + k * p.sums_row + t0 + 16 * n + 4 * (threadIdx.x >> 4 & 3));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tot[n][i] = __builtin_fmaf(x[i], f, tot[n][i]);
+    for (int i = 0; i < 4; ++i) tot[n][i] = rest != 0.f ? __builtin_fmaf(x[i], f, tot[n][i]) : tot[n][i];
   }
 }
 

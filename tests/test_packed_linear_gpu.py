@@ -399,3 +399,23 @@ def test_adapters_that_are_no_numbers(tokens, what, dtype):
         got = run(dirty)
         assert torch.equal(got[~own], clean[~own])
         assert not bool(got[own].isfinite().any())
+
+
+@pytest.mark.parametrize("group", [0, 32, 128])
+@pytest.mark.parametrize("tokens", [2, 20, 140])
+def test_infinities_beside_rows_of_other_zero_points(tokens, group):
+    """A row with whole zero points gives what it gives alone, whatever its neighbours' zero points are: infinities of the
+    weight's sign where an activation is infinite."""
+    layer = Layer(64, 300, 0, 15, group, True, seed=tokens + group)
+    layer.zero = layer.zero - 0.5 + 8.
+    x = torch.randn(tokens, 300, generator=layer.g).bfloat16()
+    x[1, 40] = math.inf
+    whole = layer.call(x).cpu()
+    sign = layer.weights()[:, 40].sign()
+    assert torch.equal(whole[1].double()[sign != 0], sign[sign != 0] * math.inf)
+    layer.zero[1::2] += 0.25
+    mixed = layer.call(x).cpu()
+    assert torch.equal(mixed[:, ::2].nan_to_num(7.), whole[:, ::2].nan_to_num(7.))
+    finite = torch.arange(tokens) != 1
+    want, slack = reference(x[finite], layer)
+    check(mixed[finite], want, slack)
