@@ -4,9 +4,10 @@
 // u the code in the layer's bit field (pack.hip).  The matrix cores multiply fp16 activations by u - 2^(bits - 1), which
 // fp16 holds exactly, less the nearest whole number to what w differs from that; a group's products are summed in fp32 and
 // then multiplied by its scale, and the rest of w (0 for whole zero points) is taken off through the sum of the group's
-// activations.  Activations are scaled by a power of two per token
-// (the largest element to 2^14..2^15): bf16 and fp16 elements down to 2^-30 of the largest stay as they are, fp32 ones
-// are two pieces of together 22 bits.  So no weight is rounded, whatever its scale, and a whole zero point costs nothing.
+// activations.  Activations are scaled by a power of two per token, the largest finite element to 2^14..2^15, where fp16 has
+// steps of 2^-24 at the least: an element is held to 22 bits (fp32, in two pieces; those of bf16 and fp16 are all held), or to
+// 2^-39 of the token's largest where that is coarser -- below an fp32 sum's rounding, unless the largest element's weight is 0.
+// So no weight is rounded, whatever its scale, and a whole zero point costs nothing.
 #pragma once
 
 #include "elements.h"

@@ -39,7 +39,9 @@ __device__ __forceinline__ void prepare_token(const Linear& p, int t, int pieces
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < PREP / 64; ++w) top = fmaxf(top, tops[w]);
-  const int ex = exponent_of(top) - 14;
+  // At least -126, so that the factor back is a normal number; the smallest fp32 numbers are then multiples of 2^-23, which
+  // fp16 holds.
+  const int ex = exponent_of(top) - 14 > -126 ? exponent_of(top) - 14 : -126;
   _Float16* out = p.xp + (int64_t)t * (128 * p.blocks);
   const bool by_lanes = p.corrected && p.group <= 512 && (p.group & (p.group - 1)) == 0;  // a group is 4 to 64 lanes' runs
   float all = 0.f;

@@ -7,8 +7,9 @@ layer straight from them:
     y = x W^T + bias,   W[i, k] = (u[i, k] + qmin - zero_point[i, k / group]) * scale[i, k / group]
 
 and, for requests that each bring an adapter (A, B) of their own to the shared layer, adds to every token the product with
-its own: scaling (x A^T) B^T.  Codes and 16-bit activations enter the products exactly and are summed in 32 bits; results
-are rounded once, to the activations' type.
+its own: scaling (x A^T) B^T.  Codes enter the products exactly; an activation to 22 bits (all that bf16 and fp16 have), or
+to 2^-39 of its token's largest finite element where that is coarser: what lies below is dropped, which a sum in 32 bits
+shows only where that element's weight is 0.  Sums are in 32 bits; results are rounded once, to the activations' type.
 """
 
 from __future__ import annotations

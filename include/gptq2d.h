@@ -354,6 +354,7 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
  * b [adapters, m, rank] of the same type.  words: the codes u of gptq2d_pack_int (m rows of row_words words, bits 2, 3, 4
  * or 8).  scale and zero (NULL: 0) are fp32, read at row *_row + group *_col elements; group: a multiple of 32 columns, 0
  * for whole rows.  index (int32, NULL or adapters 0: none): a token whose index is no adapter has none.  scaling NULL: 1.
+ * x is taken to 22 bits (all of bf16's and fp16's), or to 2^-39 of the token's largest finite element where that is coarser.
  * n below 2^21; 128 rows of words, scales or zeros (and all groups of a row) must span less than 2^28 elements
  * (GPTQ2D_EUNSUPPORTED).  work: 16-byte aligned, gptq2d_packed_linear_workspace bytes, of no use afterwards; GPTQ2D_ESCRATCH where it
  * is smaller.  adapters and rank: 0 where index is NULL. */

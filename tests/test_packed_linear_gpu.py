@@ -419,3 +419,37 @@ def test_infinities_beside_rows_of_other_zero_points(tokens, group):
     finite = torch.arange(tokens) != 1
     want, slack = reference(x[finite], layer)
     check(mixed[finite], want, slack)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tokens", [3, 30, 150])
+def test_tokens_of_subnormal_numbers(tokens, dtype):
+    """Tokens whose largest element is anything down to the type's least positive number, against weights near 1e35."""
+    layer = Layer(40, 300, -8, 7, 64, True, seed=tokens)
+    layer.scale *= 1e36
+    x = torch.randn(tokens, 300, generator=layer.g) * torch.logspace(-38, -44, tokens).view(-1, 1)
+    least = 2.0 ** -149 if dtype == "f32" else 2.0 ** -133
+    x[0], x[0, 5], x[1] = 0., least, 0.
+    x = x.to(TYPES[dtype])
+    want, slack = reference(x, layer)
+    check(layer.call(x), want, slack)
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("tokens", [2, 30, 150])
+def test_a_large_element_whose_weight_is_zero(tokens, dtype):
+    """What is held of the others beside it: 22 bits, or 2^-39 of the largest."""
+    layer = Layer(40, 300, -8, 7, 0, False, seed=tokens)
+    layer.codes[:, 7] = 0
+    for up in (10, 20, 30, 36):
+        x = torch.randn(tokens, 300, generator=layer.g)
+        x[:, 7] = 0.
+        x = x.double()
+        x *= 2.0 ** (-20 if dtype == "f16" else 0)
+        x[:, 7] = 2.0 ** (up - (20 if dtype == "f16" else 0)) * 0.99
+        x = x.to(TYPES[dtype])
+        if not bool(x.isfinite().all()):
+            continue
+        want, slack = reference(torch.where(torch.arange(300) == 7, 0., x), layer)
+        held = 2.0 ** -39 * x.double().abs().amax(1, keepdim=True) * layer.size().sum(1)
+        check(layer.call(x), want, slack + held)
