@@ -5,9 +5,9 @@
 // none gives zeros.  With k = (c - 8) s + (z + 8 s) (kv_cache.h) a score is s (q . (c - 8)) + (z + 8 s) sum q: the matrix
 // cores multiply q by whole numbers and a key's two numbers are applied once to the sum.  Likewise
 //   o = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (z_j + 8 s_j).
-// Operands are fp16 and exact: codes by nature; a query is scaled by a power of two (its largest element to 2^14..2^15),
-// which leaves every bf16 or fp16 element within 2^-38 of the largest as it is, and fp32 ones in two pieces of together 22
-// bits.  p_j s_j is brought to fp16's range by a power of two above the largest s seen, and rounded to 11 bits for
+// Operands are fp16.  Codes are exact; a query is scaled by a power of two, its largest finite element to 2^14..2^15, where fp16
+// has steps of 2^-24 at the least: an element is held to 22 bits (fp32, in two pieces; those of bf16 and fp16 are all held),
+// or to 2^-39 of the query's largest where that is coarser, far below the rounding of the score's fp32 sum.  p_j s_j is brought to fp16's range by a power of two above the largest s seen, and rounded to 11 bits for
 // bf16 results (which have 8), in two pieces otherwise.  Sums, maxima and rescaling are fp32.
 #include "kv_cache.h"
 #include "lds_dma.h"
@@ -80,38 +80,33 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// The queries of NQ x 16 columns as B operands, QP pieces, scaled by one power of two for all columns of the workgroup (its
-// largest element to 2^14..2^15, found by the first pass over them; `tops`: LDS for WV waves); `sum` is the sum of what a
-// column's operands hold.  Returns the exponent that takes the products back.
-template <int TYPE, int ND, int NQ, int QP, int WV>
-__device__ __forceinline__ int load_queries(half8 (&q)[NQ][2 * ND][QP], float (&sum)[NQ],
-                                            const typename Elem<TYPE>::T* const (&row)[NQ], const bool (&valid)[NQ], int dim,
-                                            float* tops) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
-  Raw8<TYPE> x[NQ][2 * ND];
-  float top = 0.f;
+// The queries of NQ x 16 columns as they lie, and each column's largest finite element (0 if it has none).
+template <int TYPE, int ND, int NQ>
+__device__ __forceinline__ void read_queries(Raw8<TYPE> (&x)[NQ][2 * ND], float (&top)[NQ],
+                                             const typename Elem<TYPE>::T* const (&row)[NQ], const bool (&valid)[NQ], int dim) {
+  const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
   for (int n = 0; n < NQ; ++n)
 #pragma unroll
     for (int s = 0; s < 2 * ND; ++s) x[n][s].load(row[n], 32 * s + 8 * g, valid[n] ? dim : 0);
 #pragma unroll
-  for (int n = 0; n < NQ; ++n)
+  for (int n = 0; n < NQ; ++n) {
+    top[n] = 0.f;
 #pragma unroll
     for (int s = 0; s < 2 * ND; ++s)
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float v = __builtin_fabsf(x[n][s][e]);
-        top = v < __builtin_inff() && v > top ? v : top;  // infinities and NaN stay what they are in fp16
+        top[n] = v < __builtin_inff() && v > top[n] ? v : top[n];  // infinities and NaN stay what they are in fp16
       }
-#pragma unroll
-  for (int s = 1; s < 64; s *= 2) top = fmaxf(top, __shfl_xor(top, s));
-  if (WV > 1) {
-    if (lane == 0) tops[wave] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WV; ++w) top = fmaxf(top, tops[w]);
+    top[n] = quad_max(top[n]);
   }
-  const int ex = __builtin_amdgcn_readfirstlane(exponent_of(top) - 14);
+}
+
+// Queries as B operands, QP pieces, column n times 2^-ex[n]; `sum` is the sum of what a column's operands hold.
+template <int TYPE, int ND, int NQ, int QP>
+__device__ __forceinline__ void query_operands(half8 (&q)[NQ][2 * ND][QP], float (&sum)[NQ], const Raw8<TYPE> (&x)[NQ][2 * ND],
+                                               const int (&ex)[NQ]) {
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     float total = 0.f;
@@ -119,7 +114,7 @@ __device__ __forceinline__ int load_queries(half8 (&q)[NQ][2 * ND][QP], float (&
     for (int s = 0; s < 2 * ND; ++s) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float v = __builtin_ldexpf(x[n][s][e], -ex);
+        const float v = __builtin_ldexpf(x[n][s][e], -ex[n]);
         const _Float16 h = (_Float16)v;
         q[n][s][0][e] = h;
         total += (float)h;
@@ -132,7 +127,6 @@ __device__ __forceinline__ int load_queries(half8 (&q)[NQ][2 * ND][QP], float (&
     }
     sum[n] = quad_sum(total);
   }
-  return ex;
 }
 
 // Softmax over a wave's columns, a block of 32 keys at a time.  Bound by vector instructions, so a score takes few: its
@@ -433,7 +427,12 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
     pos[n] = valid[n] ? t.pos0 + token : t.pos_hi;
     rows[n] = (const T*)a.q + (t.row + (valid[n] ? token : 0)) * a.q_token + hq * a.q_head;
   }
-  const float factor = __builtin_ldexpf(a.scale, load_queries<TYPE, ND, NQ, QP, 1>(q, qsum, rows, valid, c.dim, nullptr));
+  Raw8<TYPE> x[NQ][2 * ND];
+  float top[NQ];
+  read_queries<TYPE, ND, NQ>(x, top, rows, valid, c.dim);
+  const int ex[NQ] = {exponent_of(top[0]) - 14};
+  query_operands<TYPE, ND, NQ, QP>(q, qsum, x, ex);
+  const float factor = __builtin_ldexpf(a.scale, ex[0]);  // of the lane's column
   State<ND, NQ> st;
   clear(st);
   int buf = 0;
@@ -529,11 +528,13 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
 // vector instructions', one after the other.  64 columns a wave spill (591 us); the next block's scores beside this one's
 // weights, which needs half as much LDS again, took 408.
 constexpr int PQ = 2, PWAVES = 4;  // columns of a wave: 16 PQ
+constexpr int EVEN = 8;            // leaves an element 2^-31 of its own query's largest
 
 template <int ND, int QP, int PP>
 __device__ __forceinline__ void prompt_block(State<ND, PQ>& st, const half8 (&q)[PQ][2 * ND][QP], const float (&qsum)[PQ],
                                              const half8 (*kop)[64], const half8 (*vop)[64], const float (*aff)[32], bool mask,
-                                             int key0, const int (&pos)[PQ], int window, int len, int shift) {
+                                             int key0, const int (&pos)[PQ], int window, int len, int shift, bool uneven,
+                                             int downs) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
   floatx4 s[PQ][2];
 #pragma unroll
@@ -560,6 +561,13 @@ __device__ __forceinline__ void prompt_block(State<ND, PQ>& st, const half8 (&q)
   };
   read(a0, 0);
   read(a1, 1);
+  if (uneven) {
+    asm volatile("" : "+v"(downs));  // a branch, and both exponents in one register outside it
+#pragma unroll
+    for (int n = 0; n < PQ; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s[n][i / 4][i % 4] = __builtin_ldexpf(s[n][i / 4][i % 4], (int16_t)(downs >> 16 * n));
+  }
   exponents<ND, PQ>(st, e, s, a0, a1, qsum, mask, key0, pos, window, len, shift);
   half8 p[PQ][PP];
   read(a0, 2);
@@ -607,7 +615,40 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
     row_of[n] = token, head_of[n] = head * a.group + col % a.group;
     rows[n] = (const T*)a.q + (t.row + (valid[n] ? token : 0)) * a.q_token + head_of[n] * a.q_head;
   }
-  const float factor = __builtin_ldexpf(a.scale, load_queries<TYPE, ND, PQ, QP, PWAVES>(q, qsum, rows, valid, c.dim, tops));
+  // One exponent for all columns of the workgroup, which the keys' scales in LDS then hold; a wave with a column whose largest
+  // element is 2^EVEN below the largest of all gives each its own, and takes its scores to the common one.
+  Raw8<TYPE> x[PQ][2 * ND];
+  float top[PQ];
+  int ex[PQ], down[PQ];
+  read_queries<TYPE, ND, PQ>(x, top, rows, valid, c.dim);
+  float most = top[0];
+#pragma unroll
+  for (int n = 1; n < PQ; ++n) most = fmaxf(most, top[n]);
+#pragma unroll
+  for (int s = 1; s < 16; s *= 2) most = fmaxf(most, __shfl_xor(most, s));
+  if (lane == 0) tops[wave] = most;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < PWAVES; ++w) most = fmaxf(most, tops[w]);
+  const int common = __builtin_amdgcn_readfirstlane(exponent_of(most) - 14);
+  bool low = false;
+#pragma unroll
+  for (int n = 0; n < PQ; ++n) {
+    down[n] = top[n] > 0.f ? exponent_of(top[n]) - 14 - common : 0;
+    low |= down[n] < -EVEN;
+  }
+  const bool uneven = __builtin_amdgcn_ballot_w64(low);
+#pragma unroll
+  for (int n = 0; n < PQ; ++n) {
+    down[n] = uneven ? down[n] : 0;
+    ex[n] = common + down[n];
+  }
+  query_operands<TYPE, ND, PQ, QP>(q, qsum, x, ex);
+#pragma unroll
+  for (int n = 0; n < PQ; ++n) qsum[n] = __builtin_ldexpf(qsum[n], down[n]);
+  static_assert(PQ == 2, "two columns' exponents in one register");
+  const int downs = (down[0] & 0xffff) | down[1] << 16;
+  const float factor = __builtin_ldexpf(a.scale, common);
   State<ND, PQ> st;
   clear(st);
   const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + part * a.chunk);
@@ -671,7 +712,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
     const int shift = __builtin_amdgcn_readfirstlane(shifts[buf]);
     const bool mask = !base || kb * 32 + 31 > all_to || kb * 32 < all_from;
     prompt_block<ND, QP, PP>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], mask, kb * 32 + 4 * g, pos, a.window,
-                             base ? len : 0, shift);
+                             base ? len : 0, shift, uneven, downs);
     if (kb + 1 < end) put(kb + 1, 1 - buf, next);
     __syncthreads();
     base = next, next = after, at2 = at3;

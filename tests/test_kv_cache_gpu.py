@@ -440,3 +440,28 @@ def test_positions_past_the_table(length, new, window):
     assert torch.equal(lse.cpu() == -math.inf, empty) and not got.cpu()[empty].any()
     off = (lse.cpu().double() - want_lse)[~empty].abs()
     assert off.numel() == 0 or float(off.max()) < 1e-4
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("new", [1, 5, 80])
+@pytest.mark.parametrize("dim", [64, 128, 200])
+def test_queries_of_very_different_size(dim, new, dtype):
+    """Heads and tokens whose queries differ by up to 2^42 (2^20 in fp16), in one workgroup's columns: the ordinary ones are as exact
+    as they are alone, the large ones give the value of the key that wins where it wins by more than fp32 sums are off."""
+    g = torch.Generator().manual_seed(dim + new)
+    f16 = dtype == "f16"
+    k = torch.randn(300, 2, dim, generator=g) * (256. if f16 else 1.)
+    s = Sequences([300], 2, dim, TYPES[dtype], 32, k=k, seed=new)
+    size = torch.tensor([0., 0., 0., 12., 20.] if f16 else [0., 0., 0., 20., 28., 34., 42.])
+    size = size[torch.randint(0, len(size), (new, 8), generator=g)]
+    q = (torch.randn(new, 8, dim, generator=g).clamp(-3.9, 3.9) * 2. ** (size - (8 if f16 else 0))[:, :, None]).to(TYPES[dtype])
+    scale = dim ** -0.5
+    want, _ = s.reference(q, [new], scale, None)
+    got = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), starts([new])).cpu()
+    most = float(held_values(s.v).abs().max())
+    check(got[size == 0], want[size == 0], most, TYPES[dtype])
+    keys = held_values(s.k).repeat_interleave(4, 1)
+    for i, h in (size > 0).nonzero().tolist():
+        z = keys[:300 - new + i + 1, h] @ q[i, h].double() * scale
+        if z.numel() > 1 and float(z.topk(2).values.diff().neg()) > max(40., 1e-4 * float(z.abs().max())):
+            check(got[i, h], want[i, h], most, TYPES[dtype])
