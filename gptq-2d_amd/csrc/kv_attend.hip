@@ -5,9 +5,9 @@
 // none gives zeros.  With k = (c - 8) s + (z + 8 s) (kv_cache.h) a score is s (q . (c - 8)) + (z + 8 s) sum q: the matrix
 // cores multiply q by whole numbers and a key's two numbers are applied once to the sum.  Likewise
 //   o = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (z_j + 8 s_j).
-// Operands are fp16.  Codes are exact; a query is scaled by a power of two, its largest finite element to 2^14..2^15, where fp16
+// Operands are fp16.  Codes are exact; a query is scaled by a power of two, its largest finite element to 2^6..2^15, where fp16
 // has steps of 2^-24 at the least: an element is held to 22 bits (fp32, in two pieces; those of bf16 and fp16 are all held),
-// or to 2^-39 of the query's largest where that is coarser, far below the rounding of the score's fp32 sum.  p_j s_j is brought to fp16's range by a power of two above the largest s seen, and rounded to 11 bits for
+// or to 2^-31 of the query's largest where that is coarser, below the rounding of the score's fp32 sum.  p_j s_j is brought to fp16's range by a power of two above the largest s seen, and rounded to 11 bits for
 // bf16 results (which have 8), in two pieces otherwise.  Sums, maxima and rescaling are fp32.
 #include "kv_cache.h"
 #include "lds_dma.h"

@@ -336,9 +336,9 @@ int gptq2d_kv_read(const void* pages, int64_t page_count, int32_t heads, int32_t
  *   out = sum_j softmax_j(scale q . k_j) v_j over the tokens j <= its position and, with window > 0, j > position - window.
  * q, out: [tokens, heads group, dim], query head h on kv head h / group.  lse (optional, [tokens, heads group]): the
  * natural logarithm of sum_j exp(scale q . k_j).  A query that sees no token gives zeros and -inf.  A query's elements are
- * taken to 22 bits (all of bf16's and fp16's), or to 2^-39 of its largest finite one where that is coarser.  work: 16-byte aligned,
- * gptq2d_kv_attend_workspace bytes (`most`: width page), its contents of no use afterwards; GPTQ2D_ESCRATCH where it is
- * smaller. */
+ * taken to 22 bits (all of bf16's and fp16's), or to 2^-31 of its largest finite one where that is coarser.  work:
+ * 16-byte aligned, gptq2d_kv_attend_workspace bytes (`most`: width page), its contents of no use afterwards;
+ * GPTQ2D_ESCRATCH where it is smaller. */
 int64_t gptq2d_kv_attend_workspace(int64_t tokens, int64_t seqs, int32_t heads, int32_t group, int32_t dim, int64_t most,
                                    int64_t window);
 int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, const void* q,
