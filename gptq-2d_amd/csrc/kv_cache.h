@@ -3,7 +3,8 @@
 // Values.  A token's key (or value) vector x of one head is held as codes c in 0..15 with a scale s and a zero z of 16
 // bits each: s = bf16((max x - min x) / 15), 1 where that is 0; z = bf16(min x); c = clamp(rint((x - z) / s), 0, 15), every
 // step in fp32.  It stands for c s + z, which the kernels take as (c - 8) s + (z + 8 s): c - 8 is exact in fp16 and
-// centred, so products with it keep no offset that a later subtraction would have to cancel.
+// centred, so products with it keep no offset that a later subtraction would have to cancel.  Where s is 1 in the place of 0
+// and all c are 0, s is held as 0: the same value, without an offset of 8.
 //
 // Layout.  The head size is padded to DP = 64 ND with codes that no query meets (its elements there are 0) and no
 // output shows.  A page holds `page` tokens (a multiple of 32) of every head, head by head; one head's part is

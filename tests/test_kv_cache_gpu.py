@@ -465,3 +465,35 @@ def test_queries_of_very_different_size(dim, new, dtype):
         z = keys[:300 - new + i + 1, h] @ q[i, h].double() * scale
         if z.numel() > 1 and float(z.topk(2).values.diff().neg()) > max(40., 1e-4 * float(z.abs().max())):
             check(got[i, h], want[i, h], most, TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("new", [1, 6, 90])
+@pytest.mark.parametrize("what", ["zeros", "some zeros", "constants", "constant keys"])
+def test_vectors_without_a_spread(what, new, dtype):
+    """A vector whose elements are all alike stands for that number and has no scale: values of 0 (a head that is pruned, a
+    token that is masked) add nothing, however small the other values are, and equal keys give equal weights."""
+    dt = TYPES[dtype]
+    g = torch.Generator().manual_seed(new)
+    k, v = torch.randn(333, 2, 96, generator=g), torch.randn(333, 2, 96, generator=g)
+    if what == "zeros":
+        v[:, 1] = 0.
+    elif what == "some zeros":
+        v *= 2. ** -10
+        v[::2] = 0.
+    elif what == "constants":
+        v = (torch.randn(333, 2, 1, generator=g) * 2. ** -10).expand(333, 2, 96).contiguous()
+    else:
+        k = (torch.randn(333, 2, 1, generator=g) * 2. ** -4).expand(333, 2, 96).contiguous()
+    s = Sequences([333], 2, 96, dt, 32, k=k, v=v)
+    for x in (s.k, s.v):  # as the definition holds them
+        assert bool(((held_values(x) - x.double()).abs().amax(-1) <= (x.double().amax(-1) - x.double().amin(-1)) / 15 + 2. ** -7 * x.double().abs().amax(-1)).all())
+    read = s.cache.read(s.dev_table, s.lengths(), starts([333]), tokens=333)
+    assert torch.equal(read[0].cpu().double(), held_values(s.k)) and torch.equal(read[1].cpu().double(), held_values(s.v))
+    q = torch.randn(new, 6, 96, generator=g).to(dt)
+    want, _ = s.reference(q, [new], 96 ** -0.5, None)
+    got = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), starts([new])).cpu()
+    for head in range(2):  # each against its own largest value
+        check(got[:, 3 * head:3 * head + 3], want[:, 3 * head:3 * head + 3], float(held_values(s.v)[:, head].abs().max()), dt)
+    if what == "zeros":
+        assert not got[:, 3:].any()
