@@ -96,10 +96,11 @@ __global__ __launch_bounds__(THREADS) void append_kernel(KvCache c, Rows r) {
     const float step = round_to_bf16((hi - lo) / 15.f), s = step == 0.f ? 1.f : step;
     const float z = round_to_bf16(lo);
     // Without a spread and with codes of 0 (as the largest element's) the vector stands for its zero, and is held with a scale of
-    // 0: the scale of 1 would not be its size, and (c - 8) s and z + 8 s would have to cancel (attention holds the first to
+    // -0: the scale of 1 would not be its size, and (c - 8) s and z + 8 s would have to cancel (attention holds the first to
     // 11 bits).
-    const float held = step == 0.f && round_even(hi - z) <= 0.f ? 0.f : s;
-    if (part == 0) affine[token] = __float_as_uint(held) >> 16 | (__float_as_uint(z) & 0xffff0000u);
+    const bool flat = step == 0.f && round_even(hi - z) <= 0.f;
+    if (part == 0)
+      affine[token] = (flat ? FLAT : __float_as_uint(s) >> 16 & 0x7fffu) | (__float_as_uint(z) & 0xffff0000u);
     // The quotient (x - z) / s as IEEE rounds it, from the correctly rounded 1 / s and one correction with the exact
     // remainder (Markstein's method), where s is in a range in which nothing on the way leaves the normal numbers (the
     // differences are below 2^5 s, and below 2^-24 of s they round to code 0 whatever the remainder); a division otherwise.

@@ -7,8 +7,9 @@
 //   o = sum_j (p_j s_j) (c_j - 8) + sum_j p_j (z_j + 8 s_j).
 // Operands are fp16.  Codes are exact; a query is scaled by a power of two, its largest finite element to 2^6..2^15, where fp16
 // has steps of 2^-24 at the least: an element is held to 22 bits (fp32, in two pieces; those of bf16 and fp16 are all held),
-// or to 2^-31 of the query's largest where that is coarser, below the rounding of the score's fp32 sum.  p_j s_j is brought to fp16's range by a power of two above the largest s seen, and rounded to 11 bits for
-// bf16 results (which have 8), in two pieces otherwise.  Sums, maxima and rescaling are fp32.
+// or to 2^-31 of the query's largest where that is coarser, below the rounding of the score's fp32 sum.  p_j s_j is brought to
+// fp16's range by a power of two above the largest s seen (or, where the scales are far apart, p s: SPREAD), and rounded to 11
+// bits for bf16 results (which have 8), in two pieces otherwise.  Sums, maxima and rescaling are fp32.
 #include "kv_cache.h"
 #include "lds_dma.h"
 
@@ -135,20 +136,28 @@ __device__ __forceinline__ void query_operands(half8 (&q)[NQ][2 * ND][QP], float
 // its product with the value's scale and the two sums, and half of one each for the comparison and the conversion.
 constexpr int AHEAD = 8;  // log2 of how far weights may exceed 1
 constexpr int ROOM = 7;   // weights times scales are held as p s 2^(ROOM - shift) <= 2^(ROOM + AHEAD) in fp16: s < 2^shift
+// The shift is that of the largest scale seen, common to all columns, whatever little weight its key has.  What p s loses
+// below fp16's steps, 2^(shift - 32), is 2^(spread - 32) of what the key of the largest weight adds at least, where no scale
+// seen is below 2^(shift - spread).  Where one is, the columns part: each has the shift of the largest p s that it has seen
+// (its sums are rescaled every block then: 2048 of 8192 tokens, every 50th value 2^16 times the others, 737 us instead of
+// 384; 64 x up to 8000 143 us instead of 114).
+template <int PP>
+constexpr int SPREAD = PP == 1 ? 14 : 11;
 
 template <int ND, int NQ>
 struct State {
-  floatx4 o[NQ][4 * ND];        // elements 16 t + 4 g .. + 3 of column l % 16, times 2^(ROOM - shift)
+  floatx4 o[NQ][4 * ND];        // elements 16 t + 4 g .. + 3 of column l % 16, times 2^(ROOM - shift[n])
   float top[NQ], l[NQ], z[NQ];  // reference; this lane's sums of p and of p (z + 8 s)
   bool fresh[NQ];               // the column has not seen a key: its reference is still to be taken, however low
-  int shift;
+  int common, shift[NQ];
 };
 
 template <int ND, int NQ>
 __device__ __forceinline__ void clear(State<ND, NQ>& st) {
-  st.shift = -1000;
+  st.common = -1000;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
+    st.shift[n] = -1000;
     st.top[n] = st.l[n] = st.z[n] = 0.f;
     st.fresh[n] = true;
 #pragma unroll
@@ -156,21 +165,22 @@ __device__ __forceinline__ void clear(State<ND, NQ>& st) {
   }
 }
 
-// Exponents e of a block's scores off the reference, and the sums so far brought to the values' new `shift` and, where a
-// column's reference moves, to it -- in one place, so that the sums stay in their registers.  key0: this lane's first key
+// Exponents e of a block's scores off the reference, and the sums so far brought to the values' new `shift` (apart: to the
+// columns' own; vex(i) is the exponent of value i's scale) and, where a column's reference moves, to it -- in one place, so
+// that the sums stay in their registers.  key0: this lane's first key
 // (keys key0 + 16 (i / 4) + i % 4); len: tokens that the block's page can have (0 without a page); ks, kz: scales and
 // zeros with what all columns share in them.
-template <int ND, int NQ>
+template <int ND, int NQ, class X>
 __device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], const floatx4 (&s)[NQ][2], const float (&ks)[8],
                                           const float (&kz)[8], const float (&qsum)[NQ], bool mask, int key0,
-                                          const int (&pos)[NQ], int window, int len, int shift) {
+                                          const int (&pos)[NQ], int window, int len, int shift, bool apart, X vex) {
   float most[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n)
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       e[n][i] = __builtin_fmaf(ks[i], s[n][i / 4][i % 4], __builtin_fmaf(kz[i], qsum[n], -st.top[n]));
-  if (mask) {
+  if (__builtin_expect(mask, 0)) {
     asm volatile("");  // a branch, not sixteen selects for every block
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -182,7 +192,7 @@ __device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], 
       }
     }
   }
-  bool move = shift != st.shift;
+  bool move = apart || shift != st.common;
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     most[n] = e[n][0];
@@ -190,17 +200,27 @@ __device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], 
     for (int i = 1; i < 8; ++i) most[n] = fmaxf(most[n], e[n][i]);
     move |= most[n] > (st.fresh[n] ? -__builtin_inff() : (float)AHEAD);
   }
-  if (__builtin_amdgcn_ballot_w64(move)) {
-    const int less = st.shift - shift;
-    st.shift = shift;
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(move) != 0, 0)) {
+    st.common = shift;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const float m = quad_max(most[n]);
       const float up = st.fresh[n] ? (m == -__builtin_inff() ? 0.f : m) : m > (float)AHEAD ? m : 0.f;
       const float f = st.fresh[n] ? 1.f : __builtin_amdgcn_exp2f(-up);  // sums of 0 stay, however far down it goes
-      st.fresh[n] = st.fresh[n] && m == -__builtin_inff();
 #pragma unroll
       for (int i = 0; i < 8; ++i) e[n][i] -= up;
+      int to = shift;
+      if (apart) {
+        float ps = -1000.f;  // at least the exponent of the largest p s; the sums' own goes down with the reference
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ps = fmaxf(ps, e[n][i] + (float)vex(i));
+        to = (int)__builtin_ceilf(fminf(quad_max(ps), 1000.f)) + ROOM - 15;
+        const int was = st.shift[n] - (int)fminf(__builtin_floorf(up), 1000.f);
+        to = was > to && !st.fresh[n] ? was : to;
+      }
+      const int less = st.fresh[n] ? 0 : st.shift[n] - to;  // sums of 0 need no factor, which may be infinite
+      st.shift[n] = to;
+      st.fresh[n] = st.fresh[n] && m == -__builtin_inff();
       st.top[n] += up;
       st.l[n] *= f;
       st.z[n] *= f;
@@ -211,12 +231,13 @@ __device__ __forceinline__ void exponents(State<ND, NQ>& st, float (&e)[NQ][8], 
   }
 }
 
-// The block's weights: p s as B operands in PP pieces, and the sums of p and p (z + 8 s).
+// The block's weights: p s as B operands in PP pieces, and the sums of p and p (z + 8 s).  shift: what the scales vs are held
+// with, where that may not be the columns' (apart).
 template <int ND, int NQ, int PP>
 __device__ __forceinline__ void weights(State<ND, NQ>& st, half8 (&p)[NQ][PP], const float (&e)[NQ][8], const float (&vs)[8],
-                                        const float (&vz)[8], bool mask) {
+                                        const float (&vz)[8], bool mask, bool apart, int shift) {
   float ps[NQ][8];
-  if (mask) {  // a scale or zero that is no number must not reach columns that do not see its key
+  if (__builtin_expect(mask || apart, 0)) {  // a scale or zero that is no number must not reach columns that do not see its key
     asm volatile("");
 #pragma unroll
     for (int n = 0; n < NQ; ++n)
@@ -224,7 +245,7 @@ __device__ __forceinline__ void weights(State<ND, NQ>& st, half8 (&p)[NQ][PP], c
       for (int i = 0; i < 8; ++i) {
         const bool hidden = e[n][i] == -__builtin_inff();
         const float w = __builtin_amdgcn_exp2f(e[n][i]), z = w * vz[i];
-        ps[n][i] = hidden ? 0.f : w * vs[i];
+        ps[n][i] = hidden ? 0.f : __builtin_ldexpf(w * vs[i], apart ? shift - st.shift[n] : 0);
         st.l[n] += w;
         st.z[n] += hidden ? 0.f : z;
       }
@@ -250,9 +271,9 @@ __device__ __forceinline__ void weights(State<ND, NQ>& st, half8 (&p)[NQ][PP], c
 }
 
 // The shift that admits the scales whose largest bits (of 32) this lane found to be `bits`: the present one where it does.
-__device__ __forceinline__ int admit(int shift, unsigned bits, const float (&s)[8]) {
+__device__ __forceinline__ int admit(int shift, int bits, const float (&s)[8]) {
   const int limit = shift < -126 ? 0 : (shift + 127) << 23;  // bits of 2^shift
-  if (!__builtin_amdgcn_ballot_w64((int)bits >= limit)) return shift;
+  if (!__builtin_amdgcn_ballot_w64(bits >= limit)) return shift;
   int big = -126;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {  // infinities and NaN apart
@@ -281,10 +302,11 @@ __device__ __forceinline__ void unpack_affine(float (&s)[8], float (&z)[8], cons
   }
 }
 
-template <int ND, int NQ, int QP, int PP>
+template <int ND, int NQ, int QP, int PP>  // low: bits of the least scale that this lane has seen
 __device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)[NQ][2 * ND][QP], const float (&qsum)[NQ],
                                              Words<ND>& w, float factor, bool mask, int key0, int len,
-                                             const int (&pos)[NQ], int window) {
+                                             const int (&pos)[NQ], int window, unsigned& low) {
+  static_assert(NQ == 1, "the values' scales are brought to the shift of the lane's column");
   floatx4 s[NQ][2];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = (floatx4){0.f, 0.f, 0.f, 0.f};
@@ -301,23 +323,26 @@ __device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)
   if (mask) {  // beyond the sequence: whatever the page holds
     asm volatile("");
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w.va[i / 4][i % 4] = key0 + 16 * (i / 4) + i % 4 < len ? w.va[i / 4][i % 4] : 0u;
+    for (int i = 0; i < 8; ++i) w.va[i / 4][i % 4] = key0 + 16 * (i / 4) + i % 4 < len ? w.va[i / 4][i % 4] : FLAT;
   }
   unpack_affine(ks, kz, w.ka);
   unpack_affine(vs, vz, w.va);
-  unsigned bits = 0;
+  int bits = 0;  // the largest scale's (a NaN's is larger than any); and the least, whose bit of the sign no scale but FLAT's has
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const unsigned u = __float_as_uint(vs[i]) & 0x7fffffffu;  // a NaN may have any sign
-    bits = u > bits ? u : bits;
+    const unsigned u = __float_as_uint(vs[i]);
+    bits = (int)u > bits ? (int)u : bits;
+    low = u < low ? u : low;
     ks[i] *= factor, kz[i] *= factor;
   }
-  const int shift = admit(st.shift, bits, vs);
-  exponents<ND, NQ>(st, e, s, ks, kz, qsum, mask, key0, pos, window, len, shift);
+  const int shift = admit(st.common, bits, vs), least = shift - SPREAD<PP>;
+  const bool apart = __builtin_amdgcn_ballot_w64(low < (least < -126 ? 0u : (unsigned)(least + 127) << 23));
+  exponents<ND, NQ>(st, e, s, ks, kz, qsum, mask, key0, pos, window, len, shift, apart,
+                    [&](int i) { return (int)(__float_as_uint(vs[i]) >> 23 & 255u) - 126; });
 #pragma unroll
-  for (int i = 0; i < 8; ++i) vs[i] = __builtin_ldexpf(vs[i], ROOM - shift);
+  for (int i = 0; i < 8; ++i) vs[i] = __builtin_ldexpf(vs[i], ROOM - st.shift[0]);  // a lane has one column
   half8 p[NQ][PP];
-  weights<ND, NQ, PP>(st, p, e, vs, vz, mask);
+  weights<ND, NQ, PP>(st, p, e, vs, vz, mask, false, 0);
 #pragma unroll
   for (int W = 0; W < 4 * ND; ++W) {
     const half8 v = centred_codes(w.vw[W / 4][W % 4]);
@@ -435,6 +460,7 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
   const float factor = __builtin_ldexpf(a.scale, ex[0]);  // of the lane's column
   State<ND, NQ> st;
   clear(st);
+  unsigned low = 0xffffffffu;
   int buf = 0;
   for (int i = 0; i < count; ++i) {
     if (i + S - 1 <= count)
@@ -452,7 +478,7 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
     const int kb = first + WAVES * i;
     const bool page = there >> buf & 1u;
     const bool mask = !page || kb * 32 + 31 > all_to || kb * 32 < all_from;
-    attend_block<ND, NQ, QP, PP>(st, q, qsum, w, factor, mask, kb * 32 + 4 * g, page ? t.len : 0, pos, a.window);
+    attend_block<ND, NQ, QP, PP>(st, q, qsum, w, factor, mask, kb * 32 + 4 * g, page ? t.len : 0, pos, a.window, low);
     buf = buf + 1 < S ? buf + 1 : 0;
   }
   // the waves' results, brought to one reference, in the place of their own blocks; then every thread adds four elements
@@ -474,7 +500,7 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) m = fmaxf(m, tops[w][16 * n + (lane & 15)]);
     const float f = st.top[n] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.top[n] - m);
-    const float f2 = __builtin_ldexpf(f, st.shift - ROOM), z = f * st.z[n];
+    const float f2 = __builtin_ldexpf(f, st.shift[n] - ROOM), z = f * st.z[n];
 #pragma unroll
     for (int d = 0; d < 4 * ND; ++d)
 #pragma unroll
@@ -533,8 +559,8 @@ constexpr int EVEN = 8;            // leaves an element 2^-31 of its own query's
 template <int ND, int QP, int PP>
 __device__ __forceinline__ void prompt_block(State<ND, PQ>& st, const half8 (&q)[PQ][2 * ND][QP], const float (&qsum)[PQ],
                                              const half8 (*kop)[64], const half8 (*vop)[64], const float (*aff)[32], bool mask,
-                                             int key0, const int (&pos)[PQ], int window, int len, int shift, bool uneven,
-                                             int downs) {
+                                             int key0, const int (&pos)[PQ], int window, int len, int shift, bool apart,
+                                             bool uneven, int downs) {
   const int lane = threadIdx.x & 63, g = lane >> 4;
   floatx4 s[PQ][2];
 #pragma unroll
@@ -561,18 +587,21 @@ __device__ __forceinline__ void prompt_block(State<ND, PQ>& st, const half8 (&q)
   };
   read(a0, 0);
   read(a1, 1);
-  if (uneven) {
+  if (__builtin_expect(uneven, 0)) {
     asm volatile("" : "+v"(downs));  // a branch, and both exponents in one register outside it
 #pragma unroll
     for (int n = 0; n < PQ; ++n)
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[n][i / 4][i % 4] = __builtin_ldexpf(s[n][i / 4][i % 4], (int16_t)(downs >> 16 * n));
   }
-  exponents<ND, PQ>(st, e, s, a0, a1, qsum, mask, key0, pos, window, len, shift);
+  exponents<ND, PQ>(st, e, s, a0, a1, qsum, mask, key0, pos, window, len, shift, apart, [&](int i) {
+    const float x = aff[2][16 * (i / 4) + 4 * g + i % 4];  // s 2^(ROOM - shift)
+    return x > 0.f ? exponent_of(x) + 1 - ROOM + shift : -1000;
+  });
   half8 p[PQ][PP];
   read(a0, 2);
   read(a1, 3);
-  weights<ND, PQ, PP>(st, p, e, a0, a1, mask);
+  weights<ND, PQ, PP>(st, p, e, a0, a1, mask, apart, shift);
 #pragma unroll
   for (int W = 0; W < 4 * ND; ++W) {
     const half8 v = vop[W][lane];
@@ -590,7 +619,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   constexpr int CH = (2 * ND + PWAVES - 1) / PWAVES;  // chunks of 1 KB of words of a block that a wave brings
   __shared__ half8 ops[2][8 * ND][64];                // K's operands, then V's
   __shared__ float aff[2][4][32];                     // scale and zero of keys (times what scores share), of values
-  __shared__ int shifts[2];
+  __shared__ int shifts[2];  // and whether columns part in the lowest bit
   __shared__ float tops[PWAVES];
   const int head = blockIdx.x, chunk = blockIdx.z;
   const int64_t slot = blockIdx.y + (int64_t)gridDim.y * (blockIdx.z / a.chunks);
@@ -660,7 +689,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   const int64_t b = t.b;
   uint4v words[CH];
   unsigned affine = 0;
-  int held = -1000;  // the shift that values are staged with
+  int held = -1000, least = -1000;  // the shift that values are staged with; no scale seen is below 2^least
   auto load = [&](const unsigned* base, int at) {
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
@@ -681,21 +710,28 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
       }
     }
     if (wave == 0) {  // lanes 0..31 the keys, 32..63 the values
-      unsigned w = page && kb * 32 + (lane & 31) < len ? affine : 0u;  // beyond the sequence: whatever the page holds
+      unsigned w = page && kb * 32 + (lane & 31) < len ? affine : FLAT;  // beyond the sequence: whatever the page holds
       const float s = __uint_as_float(w << 16), z = __builtin_fmaf(8.f, s, __uint_as_float(w & 0xffff0000u));
-      const int ex = lane >= 32 && (w >> 7 & 255u) != 255u ? (int)(w >> 7 & 255u) - 126 : -126;  // s < 2^ex
-      if (__builtin_amdgcn_ballot_w64(ex > held)) {
-        int big = ex;
+      const unsigned bits = (w >> 7 & 255u) - 1;  // zeros, subnormal numbers, infinities and NaN are of no matter
+      const bool real = lane >= 32 && bits < 254u;
+      const int ex = real ? (int)bits - 125 : held;  // s in [2^(ex - 1), 2^ex)
+      if (__builtin_amdgcn_ballot_w64((unsigned)(held - ex) >= (unsigned)(held - least))) {
+        int big = real ? ex : -1000, low = real ? ex : 1000;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
-          const int x = __shfl_xor(big, d);
+          const int x = __shfl_xor(big, d), y = __shfl_xor(low, d);
           big = x > big ? x : big;
+          low = y < low ? y : low;
         }
-        held = __builtin_amdgcn_readfirstlane(big) + 2;  // room for scales four times as large
+        big = __builtin_amdgcn_readfirstlane(big), low = __builtin_amdgcn_readfirstlane(low);
+        if (big > -1000) {
+          least = held == -1000 || low <= least ? low - 2 : least;  // room for half the least scale
+          held = big > held ? big + 2 : held;                       // and for four times the largest
+        }
       }
       aff[buf][lane >> 5 << 1][lane & 31] = lane < 32 ? s * factor : __builtin_ldexpf(s, ROOM - held);
       aff[buf][(lane >> 5 << 1) + 1][lane & 31] = lane < 32 ? z * factor : z;
-      if (lane == 0) shifts[buf] = held;
+      if (lane == 0) shifts[buf] = 2 * held + (least < held - SPREAD<PP>);
     }
   };
   int at = 0, at2 = 0;
@@ -709,10 +745,11 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
     if (next) load(next, at2);
     int at3 = 0;
     const unsigned* after = kb + 2 < end ? kv_head(c, b, kb + 2, head, hw, at3) : nullptr;
-    const int shift = __builtin_amdgcn_readfirstlane(shifts[buf]);
+    const int staged = __builtin_amdgcn_readfirstlane(shifts[buf]), shift = staged >> 1;
+    const bool apart = staged & 1;
     const bool mask = !base || kb * 32 + 31 > all_to || kb * 32 < all_from;
     prompt_block<ND, QP, PP>(st, q, qsum, ops[buf], ops[buf] + 4 * ND, aff[buf], mask, kb * 32 + 4 * g, pos, a.window,
-                             base ? len : 0, shift, uneven, downs);
+                             base ? len : 0, shift, apart, uneven, downs);
     if (kb + 1 < end) put(kb + 1, 1 - buf, next);
     __syncthreads();
     base = next, next = after, at2 = at3;
@@ -728,7 +765,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
       for (int d = 0; d < 4 * ND; ++d) {
         floatx4 v;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(st.o[n][d][i], st.shift - ROOM) + z;
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_ldexpf(st.o[n][d][i], st.shift[n] - ROOM) + z;
         if (valid[n]) *reinterpret_cast<floatx4*>(out + in * DP + 16 * d + 4 * g) = v;
       }
       if (valid[n] && g == 0) {
@@ -743,7 +780,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
       for (int d = 0; d < 4 * ND; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float v = (__builtin_ldexpf(st.o[n][d][i], st.shift - ROOM) + z) * f;
+          const float v = (__builtin_ldexpf(st.o[n][d][i], st.shift[n] - ROOM) + z) * f;
           const T x = from_f32<TYPE>(none ? 0.f : v);
           if (valid[n] && 16 * d + 4 * g + i < c.dim) out[16 * d + 4 * g + i] = x;
         }

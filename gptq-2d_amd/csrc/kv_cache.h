@@ -4,7 +4,7 @@
 // bits each: s = bf16((max x - min x) / 15), 1 where that is 0; z = bf16(min x); c = clamp(rint((x - z) / s), 0, 15), every
 // step in fp32.  It stands for c s + z, which the kernels take as (c - 8) s + (z + 8 s): c - 8 is exact in fp16 and
 // centred, so products with it keep no offset that a later subtraction would have to cancel.  Where s is 1 in the place of 0
-// and all c are 0, s is held as 0: the same value, without an offset of 8.
+// and all c are 0, s is held as -0: the same value, without an offset of 8.  No other scale has a sign, not a NaN's either.
 //
 // Layout.  The head size is padded to DP = 64 ND with codes that no query meets (its elements there are 0) and no
 // output shows.  A page holds `page` tokens (a multiple of 32) of every head, head by head; one head's part is
@@ -39,6 +39,8 @@ __device__ __forceinline__ half8 centred_codes(unsigned w) {
   r.h[3] = __builtin_elementwise_fma(codes_at(x, 0x00f000f0u), both(0.0625f), both(-72.f));
   return r.v;
 }
+
+constexpr unsigned FLAT = 0x8000u;  // scale -0, zero 0
 
 struct KvCache {
   unsigned* pages;

@@ -497,3 +497,50 @@ def test_vectors_without_a_spread(what, new, dtype):
         check(got[:, 3 * head:3 * head + 3], want[:, 3 * head:3 * head + 3], float(held_values(s.v)[:, head].abs().max()), dt)
     if what == "zeros":
         assert not got[:, 3:].any()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 6, 90])
+@pytest.mark.parametrize("what", ["unlikely", "hidden", "falling", "rising"])
+def test_values_of_very_different_size(what, new, dim, dtype):
+    """Values 2^30 times larger than the others (2^20 in fp16), in keys of next to no weight, in keys that a window hides from most
+    queries, before the others and after them: every query against what its own weights make of the values' sizes."""
+    dt = TYPES[dtype]
+    g = torch.Generator().manual_seed(new + dim)
+    up, base = (2. ** 20, 2. ** -8) if dtype == "f16" else (2. ** 30, 1.)
+    k, v = torch.randn(400, 2, dim, generator=g), torch.randn(400, 2, dim, generator=g) * base
+    q = torch.randn(new, 4, dim, generator=g)
+    window = None
+    if what == "unlikely":  # a score 100 below the others' middle
+        far = torch.arange(400) % 37 == 5
+        q[:, :, 0] = dim ** 0.5
+        k[far, :, 0] = -100.
+        v[far] *= up
+    elif what == "hidden":
+        window = 30
+        v[400 - new // 2 - 40:400 - new // 2 - 37] *= up
+        v[400 - new // 3 - 1] *= up
+    else:
+        size = torch.linspace(0, 1, 400) if what == "rising" else torch.linspace(1, 0, 400)
+        v *= (up ** size).view(-1, 1, 1)
+        k[:, :, 0] = -(up ** size).log().view(-1, 1) * 1.2  # large values get small weights
+        q[:, :, 0] = dim ** 0.5
+    s = Sequences([400], 2, dim, dt, 32, k=k, v=v)
+    q = q.to(dt)
+    want, _ = s.reference(q, [new], dim ** -0.5, window)
+    got = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), starts([new]), window=window).cpu()
+    s.v = held_values(s.v).abs().amax(-1, keepdim=True).expand(-1, -1, dim).contiguous()
+    kv = held_values(s.k)
+    for i in range(new):
+        last = 400 - new + i
+        first = max(0, last - window + 1) if window else 0
+        z = torch.einsum("hd,nhd->hn", q[i].double(), kv[first:last + 1].repeat_interleave(2, 1)) * dim ** -0.5
+        size = (torch.softmax(z, -1) * s.v[first:last + 1, :, 0].repeat_interleave(2, 1).t()).sum(-1)  # [heads]
+        # a weight is off by its score's rounding, up to 100 here in fp32 sums: 100 x 2^-24 x sqrt(dim) x 2 <= 2e-4 of it
+        of = max(OF_VALUES[dt], 2e-4)
+        allowed = want[i].abs() * OWN[dt] * 1.01 + torch.finfo(dt).tiny + of * size[:, None]
+        if dt is torch.float16:
+            allowed = allowed + 2. ** -25  # its subnormal numbers' half step
+        off = ((got[i].double() - want[i]).abs() / allowed).max()
+        assert bool(off <= 1), f"query {i}: {float(off):.3g} of what is allowed"
