@@ -35,13 +35,13 @@ __device__ __forceinline__ BlockIds block_ids(const KvCache& c, int64_t slot, bo
   id.b = c.offsets ? kv_find(c, slot, 1, 32, 2) : slot;
   const int64_t t0 = kv_offset(c, id.b), t1 = kv_offset(c, id.b + 1);
   const int64_t most = (int64_t)c.width * c.page, n = t1 > t0 ? t1 - t0 : 0;
-  const int64_t held = c.lengths[id.b];
+  const int64_t held = c.seqs ? c.lengths[id.b] : 0;
   const int64_t start = back ? held - n : held;  // position of the first token
   const int64_t begin = start < 0 ? 0 : start;
   const int64_t end = start + n < most ? start + n : most;
-  const int64_t rel = c.offsets ? slot - kv_first_slot(c, id.b, 1, 32, 2) : 0;
+  const int64_t rel = c.offsets ? slot - kv_first_slot(c, id.b, 1, 32, 2) : 0;  // below 0 before the first sequence
   const int64_t kb = begin / 32 + rel;
-  id.any = end > begin && kb * 32 < end;
+  id.any = rel >= 0 && end > begin && kb * 32 < end;
   id.kb = (int)kb;
   id.first = (int)(begin > kb * 32 ? begin - kb * 32 : 0);
   id.last = (int)(end < kb * 32 + 32 ? end - kb * 32 : 32);
@@ -184,6 +184,17 @@ __global__ __launch_bounds__(THREADS) void read_kernel(KvCache c, Rows r) {
       if (row < id.none0 || row >= id.none1)
         for (int d = threadIdx.x; d < c.dim; d += THREADS) out[row * stride + d] = from_f32<TYPE>(0.f);
   }
+  // rows that no sequence has: 32 of them a slot before the first one's, and as the last one's that would follow its own
+  if (__builtin_expect(c.offsets && ((id.b == 0 && id.t0 > 0) || (id.b + 1 >= c.seqs && id.t1 < c.tokens)), 0)) {
+    const int64_t slot = blockIdx.x, rel = slot - kv_first_slot(c, id.b, 1, 32, 2);
+    const auto clear = [&](int64_t from, int64_t to, int64_t least, int64_t most) {
+      from = from > least ? from : least, to = to < most ? to : most;
+      for (int64_t row = from; row < to; ++row)
+        for (int d = threadIdx.x; d < c.dim; d += THREADS) out[row * stride + d] = from_f32<TYPE>(0.f);
+    };
+    if (id.b == 0) clear(32 * slot, 32 * slot + 32, 0, id.t0);
+    if (id.b + 1 >= c.seqs && rel >= 0) clear(id.t0 + 32 * rel, id.t0 + 32 * rel + 32, id.t1, c.tokens);
+  }
   if (!id.any) return;
   const int hw = (int)kv_head_words(ND, c.page);
   int at;
@@ -241,7 +252,7 @@ __global__ __launch_bounds__(THREADS) void read_kernel(KvCache c, Rows r) {
 
 template <int TYPE>
 int launch(bool back, const KvCache& c, const Rows& r, int nd, hipStream_t st) {
-  const int64_t slots = c.offsets ? c.tokens / 32 + 2 * c.seqs : c.seqs;
+  const int64_t slots = c.offsets ? c.tokens / 32 + 2 * (c.seqs + !c.seqs) : c.seqs;
   if (slots > 0x7fffffff) return GPTQ2D_EUNSUPPORTED;
   const dim3 grid((unsigned)slots, (unsigned)c.heads, 2);
 #define GPTQ2D_KV_CASE(ND)                                                             \
@@ -302,7 +313,7 @@ int gptq2d_kv_read(const void* pages, int64_t page_count, int32_t heads, int32_t
   KvCache c;
   if (!make_cache(c, pages, page_count, heads, dim, page, table, seqs, width, table_stride, lengths, offsets, tokens))
     return GPTQ2D_EINVAL;
-  if (tokens == 0 || seqs == 0) return 0;
+  if (tokens == 0) return 0;
   const Rows r = {k, v, k_token, k_head, v_token, v_head};
   return run(true, type, c, r, (hipStream_t)stream);
 }

@@ -51,9 +51,9 @@ __device__ __forceinline__ Tile make_tile(const KvCache& c, const Attend& a, int
   const int n = t1 > t0 ? (int)(t1 - t0) : 0;
   t.cols = n * a.group;
   t.col0 = col0;
-  const int length = c.lengths[b];  // the table may have no room for all of it: that bounds the keys, not the positions
-  t.len = kv_length(c, b);
-  t.pos0 = (length < 0 ? 0 : length) - n;
+  const int length = c.seqs && c.lengths[b] > 0 ? c.lengths[b] : 0, most = c.width * c.page;
+  t.len = length < most ? length : most;  // the table may have no room for all: that bounds the keys, not the positions
+  t.pos0 = length - n;
   const int last = t.cols - 1 < col0 + CT - 1 ? t.cols - 1 : col0 + CT - 1;
   t.pos_lo = t.pos0 + col0 / a.group;
   t.pos_hi = t.pos0 + (last < 0 ? 0 : last) / a.group;
@@ -64,6 +64,33 @@ __device__ __forceinline__ Tile make_tile(const KvCache& c, const Attend& a, int
   if (t.kb1 < t.kb0) t.kb1 = t.kb0;
   t.chunks = t.kb1 - t.kb0 > a.chunk ? (t.kb1 - t.kb0 + a.chunk - 1) / a.chunk : 1;
   return t;
+}
+
+// Zeros (and an lse of -inf) in the rows that no sequence has: those of this slot before the first sequence, and those after
+// the last one, as the columns (token, query head of the group) that would follow its own.
+template <class T>
+__device__ __forceinline__ void clear_rows(const KvCache& c, const Attend& a, int head, int64_t from, int64_t to) {
+  for (int64_t u = from * c.dim + threadIdx.x; u < to * c.dim; u += blockDim.x) {
+    const int64_t col = u / c.dim, row = col / a.group;
+    const int d = (int)(u - col * c.dim), hq = head * a.group + (int)(col - row * a.group);
+    ((T*)a.out)[row * a.out_token + hq * a.out_head + d] = (T)0;
+    if (a.lse && d == 0) a.lse[row * (int64_t)(c.heads * a.group) + hq] = -__builtin_inff();
+  }
+}
+template <class T>
+__device__ __forceinline__ void clear_others(const KvCache& c, const Attend& a, int head, int64_t seq, int64_t slot, int64_t first,
+                                             int CT) {
+  if (!c.offsets || (seq > 0 && seq + 1 < c.seqs)) return;
+  const int64_t before = kv_offset(c, 0) * a.group, after = kv_offset(c, c.seqs) * a.group, end = c.tokens * a.group;
+  if (__builtin_expect(before == 0 && after == end, 1)) return;
+  if (seq == 0) {
+    const int64_t begin = slot * CT;
+    clear_rows<T>(c, a, head, begin, begin + CT < before ? begin + CT : before);
+  }
+  if (seq + 1 >= c.seqs && slot >= first) {
+    const int64_t begin = kv_offset(c, seq) * a.group + (slot - first) * CT;
+    clear_rows<T>(c, a, head, begin > after ? begin : after, begin + CT < end ? begin + CT : end);
+  }
 }
 
 // Partial results of (slot, head, chunk): CT columns of DP sums, then CT maxima, then CT sums of weights.
@@ -415,8 +442,9 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
   const int64_t slot = blockIdx.x;
   const int head = blockIdx.y, chunk = blockIdx.z;
   const int64_t seq = kv_find(c, slot, a.group, CT, 1);
-  const int64_t col0 = (slot - kv_first_slot(c, seq, a.group, CT, 1)) * CT;
-  if (col0 > 0x7fffff00) return;
+  const int64_t first_slot = kv_first_slot(c, seq, a.group, CT, 1), col0 = (slot - first_slot) * CT;
+  if (chunk == 0) clear_others<T>(c, a, head, seq, slot, first_slot, CT);
+  if (col0 < 0 || col0 > 0x7fffff00) return;
   const Tile t = make_tile(c, a, seq, (int)col0, CT);
   if (t.col0 >= t.cols || chunk >= t.chunks) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
@@ -626,6 +654,7 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
   const int part = chunk % a.chunks;
   const int64_t seq = kv_find(c, slot, a.group, CT, 1);
   const int64_t first = kv_first_slot(c, seq, a.group, CT, 1);
+  if (part == 0) clear_others<T>(c, a, head, seq, slot, first, CT);
   if (slot < first || (slot - first) * CT > 0x7fffff00) return;
   const Tile t = make_tile(c, a, seq, (int)((slot - first) * CT), CT);
   if (t.col0 >= t.cols || part >= t.chunks) return;
@@ -802,6 +831,7 @@ __global__ __launch_bounds__(THREADS) void join_kernel(KvCache c, Attend a, int 
   const int64_t row = item / heads;
   const int hq = (int)(item - row * heads), head = hq / a.group;
   const int64_t seq = kv_find(c, row, 1, 1, 0);
+  if (row < kv_offset(c, seq) || row >= kv_offset(c, seq + 1)) return;  // no sequence's
   const int col = (int)(row - kv_offset(c, seq)) * a.group + hq % a.group;
   const Tile t = make_tile(c, a, seq, col / CT * CT, CT);
   if (t.chunks <= 1) return;
@@ -867,6 +897,7 @@ struct Plan {
 
 inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int dim, int64_t most, int64_t window) {
   Plan p;
+  seqs += !seqs;
   p.nd = (dim + 63) / 64;
   const int64_t columns = tokens * group;
   // From 96 columns a sequence on, a workgroup that brings a block to fp16 once for 128 columns is ahead of workgroups that
@@ -951,7 +982,7 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
   if (!make_cache(c, pages, page_count, heads, dim, page, table, seqs, width, table_stride, lengths, offsets, tokens) ||
       !attend_ok(tokens, seqs, heads, group, dim, width * page, window))
     return GPTQ2D_EINVAL;
-  if (tokens == 0 || seqs == 0) return 0;
+  if (tokens == 0) return 0;
   const Plan p = make_plan(tokens, seqs, heads, group, dim, width * page, window);
   if (p.slots > 0x7fffffff || p.chunks * (p.prompt ? cdiv(p.slots, 65535) : 1) > 65535) return GPTQ2D_EUNSUPPORTED;
   if (work_bytes < 4 * p.part || (p.part && (!work || (uintptr_t)work % 16))) return GPTQ2D_ESCRATCH;

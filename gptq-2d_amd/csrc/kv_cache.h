@@ -62,15 +62,16 @@ __host__ __device__ __forceinline__ int64_t kv_head_words(int nd, int page) { re
 // First token of sequence b among the packed ones, kept within them whatever the array holds.
 __device__ __forceinline__ int64_t kv_offset(const KvCache& c, int64_t b) {
   if (!c.offsets) return b < c.tokens ? b : c.tokens;
-  if (b <= 0) return 0;
-  const int64_t o = c.offsets[b];
+  const int64_t o = c.offsets[b < c.seqs ? b : c.seqs];
   return o < 0 ? 0 : o > c.tokens ? c.tokens : o;
 }
 
 // Sequence b's tokens (times `mul`) are dealt to groups of `per` in slots first(b) .. first(b + 1) - 1 with
 // first(b) = mul offset(b) / per + extra b: with extra = 1 a sequence has slots for all of its groups, with extra = 2 also
 // where its first group begins inside another.  No sequence's slots depend on more than its offset, so a workgroup finds
-// its own with one wave-wide search of 64 candidates a step.
+// its own with one wave-wide search of 64 candidates a step.  Slots before the first sequence's are found as its: they, and
+// the last sequence's past its groups, are where the rows that no sequence has are dealt with.  (No sequences: slots of one
+// without tokens.)
 __device__ __forceinline__ int64_t kv_first_slot(const KvCache& c, int64_t b, int mul, int per, int extra) {
   return (int64_t)((uint64_t)(kv_offset(c, b) * mul) / (unsigned)per) + extra * b;
 }
@@ -87,12 +88,6 @@ __device__ __forceinline__ int64_t kv_find(const KvCache& c, int64_t slot, int m
     n = n - skip < step ? n - skip : step;
   }
   return lo;
-}
-
-// Tokens that sequence b holds, kept within its row of the table.
-__device__ __forceinline__ int kv_length(const KvCache& c, int64_t b) {
-  const int64_t most = (int64_t)c.width * c.page, n = c.lengths[b];
-  return (int)(n < 0 ? 0 : n > most ? most : n);
 }
 
 // Block kb (of 32 tokens) of sequence b, head h: its first K code, or none where the table's entry is no page.

@@ -33,9 +33,11 @@ class KVCache4:
     elements.
 
     The methods take ``table`` [B, W] (int32: the pages of each sequence, in order; an entry outside the pool holds no
-    token), ``lengths`` [B] (int32) and ``offsets`` [B + 1] (int32: sequence b's rows among the packed tokens of the call;
-    None: one token a sequence), all on the cache's device.  A page that tokens are appended to belongs to one sequence;
-    full pages may be shared between sequences."""
+    token), ``lengths`` [B] (int32) and ``offsets`` [B + 1] (int32: sequence b's rows among the packed tokens of the call are
+    ``offsets[b]`` to ``offsets[b + 1] - 1``; None: one token a sequence), all on the cache's device.  Rows before
+    ``offsets[0]`` and from ``offsets[B]`` on, as a padded batch has them, are no sequence's: they are not appended, and
+    are zeros where they are read or attended.  A page that tokens are appended to belongs to one sequence; full pages may
+    be shared between sequences."""
 
     def __init__(self, pages: int, kv_heads: int, head_dim: int, *, page_size: int = 64,
                  device: torch.device | str = "cuda"):
@@ -108,7 +110,8 @@ class KVCache4:
              tokens: int | None = None, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """The values [tokens, kv_heads, head_dim] that the last tokens of each sequence are held as, keys and values:
         sequence b's rows are its positions up to ``lengths[b] - 1``.  ``tokens``: rows in all (``offsets[B]``, which is
-        not read on the host; without offsets one a sequence).  Rows without a token in the cache are zeros."""
+        not read on the host; without offsets one a sequence).  Rows without a token in the cache are zeros, as are rows that no
+        sequence has."""
         if tokens is None:
             if offsets is not None:
                 raise ValueError("read needs the number of tokens where offsets are given")
@@ -128,7 +131,7 @@ class KVCache4:
         """Causal attention of q [tokens, heads, head_dim] (fp32, bf16 or fp16; heads a multiple of kv_heads, consecutive
         ones sharing a kv head) over the cache.  The queries of a sequence are its last tokens: of its T, number i is at
         position ``lengths[b] - T + i`` and sees the positions up to its own, with ``window`` only the last `window` of
-        them.  ``scale`` defaults to head_dim^-1/2.  A query that sees nothing gives zeros.  Each head's query counts to 22
+        them.  ``scale`` defaults to head_dim^-1/2.  A query that sees nothing, or is no sequence's, gives zeros.  Each head's query counts to 22
         bits an element (all that bf16 and fp16 have), or to 2^-31 of its largest where that is coarser.  ``return_lse``: the
         logarithm of the softmax's denominator [tokens, heads] too (-inf where a query sees nothing)."""
         if q.dim() != 3 or q.size(1) % self.kv_heads or q.size(1) == 0:

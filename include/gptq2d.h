@@ -315,7 +315,8 @@ GPTQ2D_DECLARE(double, f64)
  * no token (nothing is written there, read as zeros, attended to by nobody).  The page that a call appends to belongs
  * to one sequence; full pages may be shared.  lengths[seqs]: tokens of each sequence, at most width page of which are
  * there.  offsets[seqs + 1]: sequence b's tokens of the call are the packed rows offsets[b] .. offsets[b + 1] - 1 of
- * `tokens`; NULL: one each (tokens == seqs).  Arrays are in device memory.  *_token and *_head: strides in elements of
+ * `tokens` (rows before offsets[0] and from offsets[seqs] on are no sequence's: not appended, read and attended as zeros);
+ * NULL: one each (tokens == seqs).  Arrays are in device memory.  *_token and *_head: strides in elements of
  * a packed [tokens, heads, dim] operand whose last axis is contiguous.  type 0: fp32, 1: bf16, 2: fp16. */
 int64_t gptq2d_kv_page_words(int32_t heads, int32_t dim, int32_t page); /* -1 for sizes it does not take */
 

@@ -544,3 +544,67 @@ def test_values_of_very_different_size(what, new, dim, dtype):
             allowed = allowed + 2. ** -25  # its subnormal numbers' half step
         off = ((got[i].double() - want[i]).abs() / allowed).max()
         assert bool(off <= 1), f"query {i}: {float(off):.3g} of what is allowed"
+
+
+def poison(*shapes):
+    """Memory that the next tensors of these shapes are likely to be given holds NaN."""
+    gone = [torch.full(shape, math.nan, dtype=dtype, device=DEV) for shape, dtype in shapes]
+    torch.cuda.synchronize()
+    del gone
+
+
+@pytest.mark.parametrize("before,after", [(0, 1), (0, 200), (7, 0), (70, 45), (300, 33)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [1, 0, 5], [40, 90, 2], [0, 0, 0], []])
+def test_rows_that_no_sequence_has(new, before, after):
+    """Rows before the first sequence's and after the last one's: not appended, zeros where they are read or attended (an lse of
+    -inf), and the sequences' own as their definition says."""
+    held = [100, 3000, 40][:len(new)]
+    s = Sequences(held or [40], 2, 80, torch.bfloat16, 32, seed=before + after)
+    table, lengths = s.dev_table[:len(new)], s.lengths()[:len(new)]
+    tokens = before + sum(new) + after
+    plain, offsets = starts(new), starts(new) + before
+    own = torch.zeros(tokens, dtype=torch.bool)
+    own[before:before + sum(new)] = True
+    q = torch.randn(tokens, 6, 80, generator=s.g).bfloat16().to(DEV)
+    poison((q.shape, q.dtype), (q.shape[:2], torch.float32))
+    got, lse = s.cache.attend(q, table, lengths, offsets, return_lse=True)
+    assert not got[~own.to(DEV)].any() and bool((lse[~own.to(DEV)] == -math.inf).all())
+    poison(((tokens, 2, 80), torch.float32), ((tokens, 2, 80), torch.float32))
+    k, v = s.cache.read(table, lengths, offsets, tokens=tokens)
+    assert not k[~own.to(DEV)].any() and not v[~own.to(DEV)].any()
+    if sum(new):
+        want, want_lse = s.reference(q.cpu()[own], new, 80 ** -0.5, None)
+        check(got.cpu()[own], want, float(held_values(s.v).abs().max()), torch.bfloat16)
+        assert float((lse.cpu()[own].double() - want_lse).abs().max()) < 1e-4
+        for a, b in zip((k, v), s.cache.read(table, lengths, plain, tokens=sum(new))):
+            assert torch.equal(a[own.to(DEV)], b)
+        pages = s.cache.pages.clone()
+        fresh = torch.randn(tokens, 2, 80, generator=s.g).bfloat16().to(DEV)
+        back = lengths - (plain[1:] - plain[:-1])
+        s.cache.append(fresh[own.to(DEV)], fresh[own.to(DEV)], table, back, plain)
+        want = s.cache.pages.clone()
+        s.cache.pages.copy_(pages)
+        s.cache.append(fresh, fresh, table, back, offsets)
+        assert torch.equal(s.cache.pages, want)
+
+
+def test_padded_batches_in_a_graph():
+    """A captured call of 200 rows, replayed with other sequences among them: rows that were a sequence's before are zeros."""
+    s = Sequences([90, 300, 65], 2, 64, torch.float16, 32, seed=3)
+    q = torch.randn(200, 4, 64, generator=s.g).half().to(DEV)
+    lengths, offsets = s.lengths(), starts([30, 100, 60])
+    run = lambda: s.cache.attend(q, s.dev_table, lengths, offsets)
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for new in ([30, 100, 60], [1, 1, 1], [0, 150, 0], [60, 0, 65], [0, 0, 0]):
+        offsets.copy_(starts(new))
+        q.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not out[sum(new):].any()
+        if sum(new):
+            want, _ = s.reference(q[:sum(new)].cpu(), new, 0.125, None)
+            check(out[:sum(new)], want, float(held_values(s.v).abs().max()), torch.float16)
