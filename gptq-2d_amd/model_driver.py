@@ -137,6 +137,8 @@ class LayerResult:
     words: torch.Tensor | None = None   # packed INT codes [m, ceil(n bits / 32)] (int32 bit patterns)
     scale: torch.Tensor | None = None   # the scale the codes were packed with (e.g. per row, [m, 1])
     zero_point: torch.Tensor | None = None
+    qmin: float | None = None           # the code range they were packed with
+    qmax: float | None = None
 
 
 def _objective(r: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> float:
@@ -181,6 +183,7 @@ def quantize_model(model: torch.nn.Module, collector: HessianCollector, *,
         if pack and spec.pack_scale is not None:
             res.words = packing.pack_int(z, spec.pack_scale, spec.pack_zero, qmin=spec.qmin, qmax=spec.qmax)
             res.scale, res.zero_point = spec.pack_scale, spec.pack_zero
+            res.qmin, res.qmax = spec.qmin, spec.qmax
         lin.weight.copy_(z.to(w.dtype))
         results.append(res)
     return results

@@ -25,6 +25,16 @@ from kv_cache import KVCache4
 from packed_linear import Adapters, packed_linear
 
 
+def _by_group(t, m, n, group, what) -> torch.Tensor:
+    """t, broadcastable to the weight [m, n], as one number a row and group: float32 [m, groups]."""
+    full = torch.as_tensor(t, dtype=torch.float32).expand(m, n)
+    size = group or n
+    each = full[:, ::size]
+    if not torch.equal(full, each.repeat_interleave(size, 1)[:, :n]):
+        raise ValueError(f"{what} is not one number a row" + (f" and {group} columns" if group else "; say the group"))
+    return each.contiguous()
+
+
 @dataclass
 class PackedLayer:
     """A linear layer as `packing.pack_int` packed it: the arguments of `packed_linear`."""
@@ -37,11 +47,22 @@ class PackedLayer:
     bias: torch.Tensor | None = None
 
     @classmethod
-    def from_result(cls, result, *, qmin: float = -8, qmax: float = 7, bias: torch.Tensor | None = None) -> PackedLayer:
-        """Of a `model_driver.LayerResult` with packed codes; the bounds are those of its quantizer."""
+    def from_result(cls, result, *, qmin: float | None = None, qmax: float | None = None, group: int | None = None,
+                    bias: torch.Tensor | None = None) -> PackedLayer:
+        """Of a `model_driver.LayerResult` with packed codes, whose range it has.  ``group``: columns that share a scale and zero
+        point, where the quantizer's are not one a row (its scale then is a map of every entry, [m, n]).  ``qmin`` and
+        ``qmax`` only for a result that was made without a range; where it has one they must be that."""
         if result.words is None:
             raise ValueError(f"layer {result.name} has no packed codes")
-        return cls(result.words, result.scale, result.zero_point, qmin, qmax, None, bias)
+        own = (getattr(result, "qmin", None), getattr(result, "qmax", None))
+        bounds = tuple(o if v is None else v for v, o in zip((qmin, qmax), own))
+        if None in bounds or any(o is not None and o != v for v, o in zip(bounds, own)):
+            raise ValueError(f"layer {result.name} was packed with the code range {own}, asked for {(qmin, qmax)}")
+        m, n = result.shape
+        scale = _by_group(result.scale, m, n, group, f"layer {result.name}: scale")
+        zero = None if result.zero_point is None else \
+            _by_group(result.zero_point, m, n, group, f"layer {result.name}: zero point").to(scale.device)
+        return cls(result.words, scale, zero, *bounds, group, bias)
 
     def __call__(self, x: torch.Tensor, adapters: Adapters | None = None, index: torch.Tensor | None = None) -> torch.Tensor:
         return packed_linear(x, self.words, self.scale, self.zero_point, qmin=self.qmin, qmax=self.qmax, group=self.group,

@@ -6,16 +6,19 @@ most that times |k| and the scale, a weight by exp of twice that, attention by t
 the cache holds, read back; they are compared with the quantizer's formula of the projections, where a code may differ by
 one step."""
 
+import functools
 import math
 
 import pytest
 import torch
 
+import model_driver as MD
 import packed_serving
 from kv_cache import KVCache4
 from packed_linear import Adapters
 from packed_serving import PackedAttention, PackedLayer
 import packing
+import quantizer_int as QI
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -165,3 +168,50 @@ def test_example(capsys):
     packed_serving.main()
     said = capsys.readouterr().out
     assert float(said.split("within ")[1].split("%")[0]) < 20.
+
+
+def affine_spec(weight, qmin, qmax, group=None, zero=False):
+    """An affine quantizer with a scale (and zero point) a row or group, its maps of every entry where there are groups."""
+    m, n = weight.shape
+    size = group or n
+    columns = torch.arange(n, device=weight.device) // size
+    parts = [weight[:, k:k + size] for k in range(0, n, size)]
+    if zero:
+        lo = torch.stack([p.amin(1) for p in parts], 1)
+        scale = ((torch.stack([p.amax(1) for p in parts], 1) - lo) / (qmax - qmin)).to(torch.bfloat16).to(weight.dtype)
+        zp = (qmin - lo / scale).round()
+    else:
+        scale = (torch.stack([p.abs().amax(1) for p in parts], 1) / ((qmax - qmin) / 2)).to(torch.bfloat16).to(weight.dtype)
+        zp = torch.zeros_like(scale)
+    s, z = scale[:, columns].contiguous(), zp[:, columns].contiguous()
+    return MD.QuantSpec(functools.partial(QI.affine_quantizer_hip, qmin=qmin, qmax=qmax), (s, z),
+                        pack_scale=s if group else scale, pack_zero=(z if group else zp) if zero else None, qmin=qmin, qmax=qmax)
+
+
+@pytest.mark.parametrize("bounds,group,zero", [((-7, 7), None, False), ((0, 15), None, True), ((-128, 127), None, False),
+                                               ((-2, 1), None, False), ((0, 15), 32, True), ((-8, 7), 64, False)])
+def test_layers_of_other_ranges_and_groups(bounds, group, zero):
+    """A layer that quantize_model packs comes through from_result with the range it was packed with, rows or groups."""
+    g = torch.Generator().manual_seed(1)
+    lin = torch.nn.Linear(160, 96, bias=False).to(DEV)
+    x = torch.randn(70, 160, generator=g).to(DEV)
+    model = torch.nn.Sequential(lin)
+    with MD.HessianCollector(model, output_side=False) as col, torch.no_grad():
+        model(x)
+    res, = MD.quantize_model(model, col, make_quantizer=lambda w: affine_spec(w, *bounds, group, zero))
+    assert (res.qmin, res.qmax) == bounds
+    layer = PackedLayer.from_result(res, group=group)
+    want, slack = x.double().cpu() @ lin.weight.detach().double().cpu().t(), 0.
+    # 2^-20 of the terms, whose codes and zero points are up to a range's width each
+    slack = 2.0 ** -20 * 3 * (x.double().abs().cpu() @ (res.scale.double().cpu().expand(96, 160) * (bounds[1] - bounds[0])).t())
+    assert bool(((layer(x).double().cpu() - want).abs() <= slack + 2.0 ** -23 * want.abs()).all())
+    PackedLayer.from_result(res, qmin=bounds[0], qmax=bounds[1], group=group)
+    with pytest.raises(ValueError):  # another range than the codes'
+        PackedLayer.from_result(res, qmin=bounds[0] - 1, qmax=bounds[1], group=group)
+    if group:
+        with pytest.raises(ValueError):  # scales that differ within a row
+            PackedLayer.from_result(res)
+    res.qmin = res.qmax = None
+    with pytest.raises(ValueError):  # no range at all
+        PackedLayer.from_result(res, group=group)
+    assert PackedLayer.from_result(res, qmin=bounds[0], qmax=bounds[1], group=group).qmax == bounds[1]
