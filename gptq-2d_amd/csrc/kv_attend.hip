@@ -329,24 +329,20 @@ __device__ __forceinline__ void unpack_affine(float (&s)[8], float (&z)[8], cons
   }
 }
 
-template <int ND, int NQ, int QP, int PP>  // low: bits of the least scale that this lane has seen
-__device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)[NQ][2 * ND][QP], const float (&qsum)[NQ],
+template <int ND, int QP, int PP>  // low: bits of the least scale that this lane has seen
+__device__ __forceinline__ void attend_block(State<ND, 1>& st, const half8 (&q)[1][2 * ND][QP], const float (&qsum)[1],
                                              Words<ND>& w, float factor, bool mask, int key0, int len,
-                                             const int (&pos)[NQ], int window, unsigned& low) {
-  static_assert(NQ == 1, "the values' scales are brought to the shift of the lane's column");
-  floatx4 s[NQ][2];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = (floatx4){0.f, 0.f, 0.f, 0.f};
+                                             const int (&pos)[1], int window, unsigned& low) {
+  floatx4 s[1][2];
+  s[0][0] = s[0][1] = (floatx4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 4 * ND; ++i) {
     const int W = i / 2 + i % 2 * (2 * ND);  // the two tiles of keys in turn
     const half8 k = centred_codes(w.kw[W / 4][W % 4]);
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int p = 0; p < QP; ++p) s[n][i % 2] = mfma(k, q[n][i / 2][p], s[n][i % 2]);
+    for (int p = 0; p < QP; ++p) s[0][i % 2] = mfma(k, q[0][i / 2][p], s[0][i % 2]);
   }
-  float ks[8], kz[8], vs[8], vz[8], e[NQ][8];
+  float ks[8], kz[8], vs[8], vz[8], e[1][8];
   if (mask) {  // beyond the sequence: whatever the page holds
     asm volatile("");
 #pragma unroll
@@ -364,19 +360,17 @@ __device__ __forceinline__ void attend_block(State<ND, NQ>& st, const half8 (&q)
   }
   const int shift = admit(st.common, bits, vs), least = shift - SPREAD<PP>;
   const bool apart = __builtin_amdgcn_ballot_w64(low < (least < -126 ? 0u : (unsigned)(least + 127) << 23));
-  exponents<ND, NQ>(st, e, s, ks, kz, qsum, mask, key0, pos, window, len, shift, apart,
+  exponents<ND, 1>(st, e, s, ks, kz, qsum, mask, key0, pos, window, len, shift, apart,
                     [&](int i) { return (int)(__float_as_uint(vs[i]) >> 23 & 255u) - 126; });
 #pragma unroll
   for (int i = 0; i < 8; ++i) vs[i] = __builtin_ldexpf(vs[i], ROOM - st.shift[0]);  // a lane has one column
-  half8 p[NQ][PP];
-  weights<ND, NQ, PP>(st, p, e, vs, vz, mask, false, 0);
+  half8 p[1][PP];
+  weights<ND, 1, PP>(st, p, e, vs, vz, mask, false, 0);
 #pragma unroll
   for (int W = 0; W < 4 * ND; ++W) {
     const half8 v = centred_codes(w.vw[W / 4][W % 4]);
 #pragma unroll
-    for (int n = 0; n < NQ; ++n)
-#pragma unroll
-      for (int r = 0; r < PP; ++r) st.o[n][W] = mfma(v, p[n][r], st.o[n][W]);
+    for (int r = 0; r < PP; ++r) st.o[0][W] = mfma(v, p[0][r], st.o[0][W]);
   }
 }
 
@@ -433,10 +427,10 @@ __device__ __forceinline__ void read_block(Words<ND>& w, const char* from, int l
 template <int TYPE, int ND>
 __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int NQ = 1, CT = 16, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2;
+  constexpr int CT = 16, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2;
   typedef Ring<ND> R;
   constexpr int S = R::S;
-  static_assert(S * R::STAGE >= NQ * 4 * ND * 1024, "a wave's sums fit where its blocks were");
+  static_assert(S * R::STAGE >= 4 * ND * 1024, "a wave's sums fit where its blocks were");
   alignas(16) __shared__ char ring[WAVES][S][R::STAGE];
   __shared__ float tops[WAVES][CT], ls[WAVES][CT];
   const int64_t slot = blockIdx.x;
@@ -468,25 +462,18 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
       stage_block<ND>(ring[wave][i], base, at, c.page, lane);
     }
   base = S - 1 < count ? kv_head(c, b, first + WAVES * (S - 1), head, hw, at) : nullptr;
-  half8 q[NQ][2 * ND][QP];
-  float qsum[NQ];
-  int pos[NQ];
-  bool valid[NQ];
-  const T* rows[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int col = t.col0 + 16 * n + (lane & 15), token = col / a.group, hq = head * a.group + col % a.group;
-    valid[n] = col < t.cols;
-    pos[n] = valid[n] ? t.pos0 + token : t.pos_hi;
-    rows[n] = (const T*)a.q + (t.row + (valid[n] ? token : 0)) * a.q_token + hq * a.q_head;
-  }
-  Raw8<TYPE> x[NQ][2 * ND];
-  float top[NQ];
-  read_queries<TYPE, ND, NQ>(x, top, rows, valid, c.dim);
-  const int ex[NQ] = {exponent_of(top[0]) - 14};
-  query_operands<TYPE, ND, NQ, QP>(q, qsum, x, ex);
+  half8 q[1][2 * ND][QP];
+  const int col = t.col0 + (lane & 15), token = col / a.group, hq = head * a.group + col % a.group;
+  const bool valid[1] = {col < t.cols};
+  const int pos[1] = {valid[0] ? t.pos0 + token : t.pos_hi};
+  const T* const rows[1] = {(const T*)a.q + (t.row + (valid[0] ? token : 0)) * a.q_token + hq * a.q_head};
+  Raw8<TYPE> x[1][2 * ND];
+  float top[1], qsum[1];
+  read_queries<TYPE, ND, 1>(x, top, rows, valid, c.dim);
+  const int ex[1] = {exponent_of(top[0]) - 14};
+  query_operands<TYPE, ND, 1, QP>(q, qsum, x, ex);
   const float factor = __builtin_ldexpf(a.scale, ex[0]);  // of the lane's column
-  State<ND, NQ> st;
+  State<ND, 1> st;
   clear(st);
   unsigned low = 0xffffffffu;
   int buf = 0;
@@ -506,41 +493,35 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
     const int kb = first + WAVES * i;
     const bool page = there >> buf & 1u;
     const bool mask = !page || kb * 32 + 31 > all_to || kb * 32 < all_from;
-    attend_block<ND, NQ, QP, PP>(st, q, qsum, w, factor, mask, kb * 32 + 4 * g, page ? t.len : 0, pos, a.window, low);
+    attend_block<ND, QP, PP>(st, q, qsum, w, factor, mask, kb * 32 + 4 * g, page ? t.len : 0, pos, a.window, low);
     buf = buf + 1 < S ? buf + 1 : 0;
   }
   // the waves' results, brought to one reference, in the place of their own blocks; then every thread adds four elements
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    st.l[n] = quad_sum(st.l[n]);
-    st.z[n] = quad_sum(st.z[n]);
-    if (st.fresh[n] && st.l[n] == 0.f) st.top[n] = -__builtin_inff();  // saw no key; scores that are no numbers stay such
-    if (g == 0) {
-      tops[wave][16 * n + lane] = st.top[n];
-      ls[wave][16 * n + lane] = st.l[n];
-    }
+  st.l[0] = quad_sum(st.l[0]);
+  st.z[0] = quad_sum(st.z[0]);
+  if (st.fresh[0] && st.l[0] == 0.f) st.top[0] = -__builtin_inff();  // saw no key; scores that are no numbers stay such
+  if (g == 0) {
+    tops[wave][lane] = st.top[0];
+    ls[wave][lane] = st.l[0];
   }
   __syncthreads();
   floatx4* const mine = reinterpret_cast<floatx4*>(&ring[wave][0][0]);
+  float m = -__builtin_inff();
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    float m = -__builtin_inff();
+  for (int w = 0; w < WAVES; ++w) m = fmaxf(m, tops[w][lane & 15]);
+  const float f = st.top[0] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.top[0] - m);
+  const float f2 = __builtin_ldexpf(f, st.shift[0] - ROOM), z = f * st.z[0];
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) m = fmaxf(m, tops[w][16 * n + (lane & 15)]);
-    const float f = st.top[n] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(st.top[n] - m);
-    const float f2 = __builtin_ldexpf(f, st.shift[n] - ROOM), z = f * st.z[n];
+  for (int d = 0; d < 4 * ND; ++d) {
 #pragma unroll
-    for (int d = 0; d < 4 * ND; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st.o[n][d][i] = __builtin_fmaf(f2, st.o[n][d][i], z);
-#pragma unroll
-    for (int d = 0; d < 4 * ND; ++d) mine[(n * 4 * ND + d) * 64 + lane] = st.o[n][d];
+    for (int i = 0; i < 4; ++i) st.o[0][d][i] = __builtin_fmaf(f2, st.o[0][d][i], z);
+    mine[d * 64 + lane] = st.o[0][d];
   }
   __syncthreads();
   const int cols = t.cols - t.col0 < CT ? t.cols - t.col0 : CT;
   for (int u = threadIdx.x; u < cols * (16 * ND); u += THREADS) {
     const int in = u / (16 * ND), d4 = u % (16 * ND);  // column, four elements
-    const int at4 = ((in / 16) * 4 * ND + d4 / 4) * 64 + in % 16 + 16 * (d4 % 4);
+    const int at4 = d4 / 4 * 64 + in + 16 * (d4 % 4);
     floatx4 v = {0.f, 0.f, 0.f, 0.f};
     float top = -__builtin_inff(), l = 0.f;
 #pragma unroll

@@ -354,10 +354,8 @@ int gptq2d_packed_linear(const void* x, int64_t x_token, int32_t type, int64_t t
                  : bits == 4 ? packed_product_bits4(&p, &q, st)
                              : packed_product_bits8(&p, &q, st);
   if (rc) return rc;
-  if (q.splits > 1) {
-    if (tokens > 65535) return GPTQ2D_EUNSUPPORTED;
+  if (q.splits > 1)  // of fewer than 384 workgroups of up to 128 tokens: few enough for the grid's second axis
     hipLaunchKernelGGL(finish_kernel, dim3((unsigned)cdiv(m, 256), (unsigned)tokens), dim3(256), 0, st, p);
-  }
   return (int)hipGetLastError();
 }
 

@@ -388,7 +388,7 @@ __global__ __launch_bounds__(64 * WR * WK, WR * WK / 2) void stream_kernel(Linea
 // takes 221 us), with zero points 320, groups of 32 with zero points 505.
 // Bound by the two waves a SIMD that 255 registers leave: 1024 cycles of matrix and some 850 of vector instructions a block
 // and wave overlap only between them.
-template <int BITS, int MODE, int NT, int MR, int WT, int NP>
+template <int BITS, int MODE, int NT, int MR, int WT>
 __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
   constexpr int TOK = 16 * NT * WT, ROWS_OF = 16 * MR * (4 / WT), N = Affine<MODE, MR>::N;
   extern __shared__ float4 lds[];
@@ -399,13 +399,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
   const int b0 = split * p.split_blocks, b1 = b0 + p.split_blocks < p.blocks ? b0 + p.split_blocks : p.blocks;
   const int pitch = 256 * p.blocks;  // bytes of a token
   const int rows = p.tokens - tile_t < TOK ? p.tokens - tile_t : TOK;
-  __amdgpu_buffer_rsrc_t rsrc[NP];
-#pragma unroll
-  for (int q = 0; q < NP; ++q)
-    rsrc[q] = __builtin_amdgcn_make_buffer_rsrc(p.xp + q * p.piece + (int64_t)tile_t * (128 * p.blocks), (short)0,
-                                                rows * pitch, 0x00020000);
+  const __amdgpu_buffer_rsrc_t rsrc =
+      __builtin_amdgcn_make_buffer_rsrc(p.xp + (int64_t)tile_t * (128 * p.blocks), (short)0, rows * pitch, 0x00020000);
   // 1 KB = four tokens a load: lane l brings piece (l % 16) ^ token of token l / 16 of the four
-  constexpr int LOADS = TOK / 4 / 4;  // of a wave, a piece
+  constexpr int LOADS = TOK / 4 / 4;  // of a wave
   int off[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
@@ -414,18 +411,16 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
   }
   auto stage = [&](int kb, int buf) {
 #pragma unroll
-    for (int q = 0; q < NP; ++q)
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-        dma_load<4>(rsrc[q], reinterpret_cast<float*>(lds + (buf * NP + q) * (TOK * 16) + (wave * LOADS + i) * 64),
-                    off[i] == OOB ? OOB : off[i] + 256 * kb);
+    for (int i = 0; i < LOADS; ++i)
+      dma_load<4>(rsrc, reinterpret_cast<float*>(lds + buf * (TOK * 16) + (wave * LOADS + i) * 64),
+                  off[i] == OOB ? OOB : off[i] + 256 * kb);
   };
   // scales, then zero points: of row i / N in step i % N, 64 of them a load.  (Loaded by the lanes that use them they are 4
   // to 32 loads a wave and block, each of 16 lines, and their registers: 2048 tokens x 8192 x 8192, with zero points, groups
   // of 128 482 us for 342, groups of 32 1500 us for 536.)
   constexpr int AL = ROWS_OF * N / 64, ALL = zeros(MODE) ? 2 * AL : AL;
   const int rows_w = p.m - tile_r < ROWS_OF ? p.m - tile_r : ROWS_OF;
-  float* const affine = reinterpret_cast<float*>(lds + 2 * NP * TOK * 16);
+  float* const affine = reinterpret_cast<float*>(lds + 2 * TOK * 16);
   [[maybe_unused]] auto stage_affine = [&](int kb, int buf) {
     const int k = narrow(MODE) ? group_of<MODE>(p, kb, lane & 3) : group_of<MODE>(p, kb, 0);
 #pragma unroll
@@ -491,12 +486,12 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(Linear p) {
           f.z[j][i] = zeros(MODE) ? at[AL * 64 + 16 * N * j + i] : 0.f;
         }
     }
-    const float4* in = lds + buf * NP * (TOK * 16);
-    block_products<BITS, MODE, NT, MR, NP>(
+    const float4* in = lds + buf * (TOK * 16);
+    block_products<BITS, MODE, NT, MR, 1>(
         tot, now, f,
-        [&](int n, int i, int q) {
+        [&](int n, int i, int) {
           const int token = 16 * (NT * wt + n) + c16, piece = narrow(MODE) ? 4 * i + g : 4 * g + i;
-          return __builtin_bit_cast(half8, in[q * (TOK * 16) + token * 16 + (piece ^ c16)]);
+          return __builtin_bit_cast(half8, in[token * 16 + (piece ^ c16)]);
         },
         p, kb, t0);
   }
@@ -538,7 +533,7 @@ int launch_product(const Linear& p, const Plan& q, hipStream_t st) {
   if (q.tile == 32) return launch_stream<BITS, MODE, 2, 8, 1, 8, 1, 1>(p, q, st);
   if (q.tile == 64) return launch_stream<BITS, MODE, 4, 16, 1, 8, 1, 1>(p, q, st);
   constexpr int affine = MODE == ROWS ? 0 : 128 * (narrow(MODE) ? 4 : 1) * (zeros(MODE) ? 2 : 1);  // floats of a block
-  constexpr auto kernel = tile_kernel<BITS, MODE, 4, 4, 2, 1>;
+  constexpr auto kernel = tile_kernel<BITS, MODE, 4, 4, 2>;
   if (const int rc = allow_lds<kernel>()) return rc;
   hipLaunchKernelGGL(kernel, dim3((unsigned)cdiv(p.m, q.rows), (unsigned)cdiv(p.tokens, q.tile), (unsigned)q.splits), dim3(256),
                      (size_t)q.tile * 512 + 8 * affine, st, p);
