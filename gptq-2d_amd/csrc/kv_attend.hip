@@ -383,10 +383,12 @@ struct Ring {
   static constexpr int S = 20480 / STAGE < 8 ? 20480 / STAGE : 8;
 };
 
+// Waits until at most N of this wave's loads are on their way, and until its LDS reads have returned: the stage that they read
+// is loaded next, and nothing else orders the two.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   static_assert(N >= 0 && N < 64, "vmcnt has six bits");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 // Block `at` of the head's part of a page at `base`; without a page zeros.

@@ -167,11 +167,12 @@ __device__ __forceinline__ void store_tile(const floatx4 (&tot)[MR], const Linea
   }
 }
 
-// Waits until at most N of this wave's loads are on their way (they return in order).
+// Waits until at most N of this wave's loads are on their way (they return in order), and until its LDS reads have returned:
+// the stage that they read is loaded next, and a wave alone with its stages has no barrier between the two.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
   static_assert(N >= 0 && N < 64, "vmcnt has six bits");
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 // Up to 64 tokens, where the codes' bytes are the bound.  A workgroup takes 16 NT tokens and 16 MR WR rows of W: WR waves beside
