@@ -45,6 +45,7 @@ class PackedLayer:
     qmax: float = 7
     group: int | None = None
     bias: torch.Tensor | None = None
+    columns: int | None = None  # of the weight; None: whatever is multiplied by it
 
     @classmethod
     def from_result(cls, result, *, qmin: float | None = None, qmax: float | None = None, group: int | None = None,
@@ -62,9 +63,11 @@ class PackedLayer:
         scale = _by_group(result.scale, m, n, group, f"layer {result.name}: scale")
         zero = None if result.zero_point is None else \
             _by_group(result.zero_point, m, n, group, f"layer {result.name}: zero point").to(scale.device)
-        return cls(result.words, scale, zero, *bounds, group, bias)
+        return cls(result.words, scale, zero, *bounds, group, bias, n)
 
     def __call__(self, x: torch.Tensor, adapters: Adapters | None = None, index: torch.Tensor | None = None) -> torch.Tensor:
+        if self.columns is not None and x.size(-1) != self.columns:
+            raise ValueError(f"the layer has {self.columns} columns, x {x.size(-1)}")
         return packed_linear(x, self.words, self.scale, self.zero_point, qmin=self.qmin, qmax=self.qmax, group=self.group,
                              bias=self.bias, adapters=adapters, index=None if adapters is None else index)
 
@@ -80,6 +83,8 @@ class PackedAttention:
         for name, layer, rows in (("q", q, heads * dim), ("k", k, kv * dim), ("v", v, kv * dim)):
             if layer.words.size(0) != rows:
                 raise ValueError(f"{name} has {layer.words.size(0)} rows, its heads take {rows}")
+        if out.columns not in (None, heads * dim):
+            raise ValueError(f"out has {out.columns} columns, the heads give {heads * dim}")
         self.q, self.k, self.v, self.out, self.cache, self.heads, self.window = q, k, v, out, cache, heads, window
 
     def __call__(self, x: torch.Tensor, table: torch.Tensor, held: torch.Tensor, offsets: torch.Tensor | None = None, *,

@@ -215,3 +215,19 @@ def test_layers_of_other_ranges_and_groups(bounds, group, zero):
     with pytest.raises(ValueError):  # no range at all
         PackedLayer.from_result(res, group=group)
     assert PackedLayer.from_result(res, qmin=bounds[0], qmax=bounds[1], group=group).qmax == bounds[1]
+
+
+def test_inputs_of_another_width_are_refused():
+    """Rows of words may be longer than the codes that a product takes: a layer of a quantized model knows its width."""
+    lin = torch.nn.Linear(160, 96, bias=False).to(DEV)
+    with MD.HessianCollector(torch.nn.Sequential(lin), output_side=False) as col, torch.no_grad():
+        lin(torch.randn(40, 160, device=DEV))
+    layer = PackedLayer.from_result(MD.quantize_model(None, col)[0])
+    assert layer(torch.ones(3, 160, device=DEV)).shape == (3, 96)
+    for n in (96, 159, 161):
+        with pytest.raises(ValueError):
+            layer(torch.ones(3, n, device=DEV))
+    s = Block()
+    b = s.block
+    with pytest.raises(ValueError):
+        PackedAttention(b.q, b.k, b.v, layer, s.cache, heads=6)
