@@ -74,7 +74,8 @@ def packed_linear(x: torch.Tensor, words: torch.Tensor, scale: torch.Tensor, zer
         raise _hip.GPTQ2DError("packed_linear needs GPU tensors")
     n = x.size(-1)
     bits = _bits(qmin, qmax)
-    if words.dtype is not torch.int32 or words.dim() != 2 or words.device != device or words.stride(1) != 1:
+    if words.dtype is not torch.int32 or words.dim() != 2 or words.device != device or \
+            (words.stride(1) != 1 and words.size(1) > 1):
         raise ValueError("words must be int32 [m, row_words] on x's device, with contiguous rows")
     m, row_words = words.shape
     if n == 0 or m == 0 or row_words * 32 < n * bits:
@@ -126,9 +127,10 @@ def packed_linear(x: torch.Tensor, words: torch.Tensor, scale: torch.Tensor, zer
         raise ValueError(f"packed_linear of {tokens} tokens, a [{m}, {n}] layer and {count} adapters of rank {rank} is "
                          "too large")
     work = torch.empty(size, dtype=torch.uint8, device=device)
-    args = (rows.data_ptr(), rows.stride(0), kind, tokens, words.data_ptr(), m, n, words.stride(0), bits, s, s_row, s_col,
-            z, z_row, z_col, qmin, group or 0, None if bias is None else bias.data_ptr(), a_ptr, b_ptr, scaling_ptr,
-            index_ptr, count, rank, y.data_ptr(), m, work.data_ptr(), size)
+    args = (rows.data_ptr(), rows.stride(0), kind, tokens, words.data_ptr(), m, n,
+            words.stride(0) if m > 1 else row_words, bits, s, s_row, s_col, z, z_row, z_col, qmin, group or 0,
+            None if bias is None else bias.data_ptr(), a_ptr, b_ptr, scaling_ptr, index_ptr, count, rank, y.data_ptr(), m,
+            work.data_ptr(), size)
     if torch.cuda.current_device() == device.index:
         rc = lib.gptq2d_packed_linear(*args, torch.cuda.current_stream(device).cuda_stream)
     else:

@@ -453,3 +453,20 @@ def test_a_large_element_whose_weight_is_zero(tokens, dtype):
         want, slack = reference(torch.where(torch.arange(300) == 7, 0., x), layer)
         held = 2.0 ** -39 * x.double().abs().amax(1, keepdim=True) * layer.size().sum(1)
         check(layer.call(x), want, slack + held)
+
+
+@pytest.mark.parametrize("tokens", [2, 140])
+def test_strides_of_axes_of_one(tokens):
+    """One row, one word a row, one column: the stride of an axis with one entry is of no matter."""
+    for m, n in ((1, 100), (70, 7), (1, 1)):
+        layer = Layer(m, n, -8, 7, 0, False, seed=m + n)
+        x = torch.randn(tokens, n, generator=layer.g).to(DEV)
+        want, words = layer.call(x), layer.words()
+        strides = (words.size(1) if m > 1 else 1, 1 if words.size(1) > 1 else m + 3)
+        odd = torch.zeros(4096, dtype=torch.int32, device=DEV).as_strided(words.shape, strides)
+        odd.copy_(words)
+        assert torch.equal(packed_linear(x, odd, layer.scale.to(DEV), qmin=-8, qmax=7), want)
+        if n == 1:
+            wide = torch.zeros(tokens, 5, device=DEV)
+            wide[:, :1] = x
+            assert torch.equal(layer.call(wide.as_strided((tokens, 1), (5, 9))), want)
