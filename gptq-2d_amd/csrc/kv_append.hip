@@ -6,8 +6,8 @@
 // into the words' order, so that whole blocks are written 16 bytes a thread in order.  In a block that is not all new
 // the words of K (one token each) and the scales of the new tokens are written alone, and in the words of V the new
 // tokens' nibbles replace the old.
-// Measured, 8000 tokens, 8 heads of 128, fp16, keys and values: append 24 us (42 MB: one round of workgroups, each a chain
-// of load, maximum, division, LDS and store), read into fp32 18.5 us (74 MB, 4.0 TB/s).  One token of 64 sequences: 6 us
+// Measured, 8000 tokens, 8 heads of 128, fp16, keys and values: append 25 us (42 MB: one round of workgroups, each a chain
+// of load, maximum, division, LDS and store), read into fp32 19.4 us (74 MB, 3.8 TB/s).  One token of 64 sequences: 6 us
 // and 4.
 #include "kv_cache.h"
 

@@ -422,8 +422,8 @@ __device__ __forceinline__ void read_block(Words<ND>& w, const char* from, int l
 
 // Few columns.  A workgroup takes 16 of them and `chunk` blocks of 32 keys, its waves every fourth block each; the waves'
 // results are joined through LDS.  Bound by memory for long sequences: 4 of up to 131072 tokens, 8 kv heads of 128, bf16,
-// one token each: 159 us, 3.6 TB/s of the cache (a read-only sum: 4.0); by the unequal lengths otherwise: 64 of 300 to 8000
-// tokens 120 us, 2.4 TB/s.  Some 300 vector instructions a block and wave, most of them on the 32 keys' scales and codes,
+// one token each: 156 us, 3.6 TB/s of the cache (a read-only sum: 4.0); by the unequal lengths otherwise: 64 of 300 to 8000
+// tokens 115 us, 2.5 TB/s.  Some 300 vector instructions a block and wave, most of them on the 32 keys' scales and codes,
 // whatever the columns.  Two tiles of 16 columns a wave, which share them, need registers that leave half of the waves:
 // 32 columns of 16 x 4000 tokens 95 us for 55 in two workgroups.
 template <int TYPE, int ND>
@@ -560,8 +560,8 @@ __global__ __launch_bounds__(THREADS, ND <= 2 ? 2 : 1) void attend_kernel(KvCach
 // Many columns (a prompt's tokens times the heads that share a kv head).  A workgroup takes 32 columns a wave and `chunk` blocks of
 // 32 keys; the block's codes are brought to fp16 once, by all waves, into LDS, where they lie as operands (two blocks in
 // turn, one barrier a block; the next one's words are in flight meanwhile), and its scales and zeros in fp32 with what all
-// columns share already in them.  2048 new tokens of 8192, 32 heads on 8 of 128, bf16: 379 us, 635 TFLOP/s of 240 GFLOP.
-// Bound by the two waves a SIMD that its 210 registers allow: of 2030 cycles a block and wave 512 are matrix and about 1000
+// columns share already in them.  2048 new tokens of 8192, 32 heads on 8 of 128, bf16: 384 us, 627 TFLOP/s of 240 GFLOP.
+// Bound by the two waves a SIMD that its 222 registers allow: of 2050 cycles a block and wave 512 are matrix and about 1000
 // vector instructions', one after the other.  64 columns a wave spill (591 us); the next block's scores beside this one's
 // weights, which needs half as much LDS again, took 408.
 constexpr int PQ = 2, PWAVES = 4;  // columns of a wave: 16 PQ
