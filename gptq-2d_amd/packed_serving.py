@@ -26,8 +26,11 @@ from packed_linear import Adapters, packed_linear
 
 
 def _by_group(t, m, n, group, what) -> torch.Tensor:
-    """t, broadcastable to the weight [m, n], as one number a row and group: float32 [m, groups]."""
-    full = torch.as_tensor(t, dtype=torch.float32).expand(m, n)
+    """t, broadcastable to the weight [m, n], as one number a row and group: float32 [m, groups], or [m, 1]."""
+    t = torch.as_tensor(t, dtype=torch.float32)
+    if t.dim() == 0 or t.size(-1) == 1:
+        return t.expand(m, 1).contiguous()
+    full = t.expand(m, n)
     size = group or n
     each = full[:, ::size]
     if not torch.equal(full, each.repeat_interleave(size, 1)[:, :n]):
@@ -60,9 +63,8 @@ class PackedLayer:
         if None in bounds or any(o is not None and o != v for v, o in zip(bounds, own)):
             raise ValueError(f"layer {result.name} was packed with the code range {own}, asked for {(qmin, qmax)}")
         m, n = result.shape
-        scale = _by_group(result.scale, m, n, group, f"layer {result.name}: scale")
-        zero = None if result.zero_point is None else \
-            _by_group(result.zero_point, m, n, group, f"layer {result.name}: zero point").to(scale.device)
+        scale, zero = (None if t is None else _by_group(t, m, n, group, f"layer {result.name}: {what}").to(result.words.device)
+                       for t, what in ((result.scale, "scale"), (result.zero_point, "zero point")))
         return cls(result.words, scale, zero, *bounds, group, bias, n)
 
     def __call__(self, x: torch.Tensor, adapters: Adapters | None = None, index: torch.Tensor | None = None) -> torch.Tensor:
