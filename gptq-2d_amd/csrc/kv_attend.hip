@@ -895,9 +895,9 @@ inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int di
   // Chunks as large as leave 768 workgroups, one and a half rounds of two a CU, so that sequences of different lengths end
   // together (one token each, us for 512, 768 and 1024: 64 sequences of up to 8000 tokens 135, 121, 119; 4 of 131072 179,
   // 159, 154; 64 of 4000 94, 86, 91; one of 100000 41, 49, 53); at least two blocks a wave, whose start takes longer than
-  // that (one of 16000: 19 us, with one block a wave 29) -- one where that leaves fewer than 256 workgroups, all on the chip at once,
-  // and the chunks are joined anyway (both kernels, 8 kv heads of 128, two and one: one of 300 13.1 and 12.2 us, of 1000
-  // 13.7 and 12.2, of 2000 13.4 and 12.6, of 4000, 256 workgroups, 13.4 and 13.8; 4 of 200, unjoined, 11.9 and 13.0).
+  // that (one of 16000: 19 us, with one block a wave 29) -- one where that leaves fewer than 256 workgroups, all on the chip
+  // at once, and the chunks are joined anyway (both kernels, 8 kv heads of 128, two and one: one of 300 13.1 and 12.2 us, of
+  // 1000 13.7 and 12.2, of 2000 13.4 and 12.6, of 4000, 256 workgroups, 13.4 and 13.8; 4 of 200, unjoined, 11.9 and 13.0).
   const int64_t tiles = cdiv(columns, p.ct) > seqs ? cdiv(columns, p.ct) : seqs;  // that hold columns, about
   const int64_t want = cdiv(blocks * tiles * heads, 768);
   const bool few = range > 64 * WAVES && cdiv(blocks, WAVES) * tiles * heads < 256;

@@ -129,11 +129,12 @@ class KVCache4:
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None, *,
                scale: float | None = None, window: int | None = None, return_lse: bool = False):
         """Causal attention of q [tokens, heads, head_dim] (fp32, bf16 or fp16; heads a multiple of kv_heads, consecutive
-        ones sharing a kv head) over the cache.  The queries of a sequence are its last tokens: of its T, number i is at
+        ones sharing a kv head) over the cache. The queries of a sequence are its last tokens: of its T, number i is at
         position ``lengths[b] - T + i`` and sees the positions up to its own, with ``window`` only the last `window` of
-        them.  ``scale`` defaults to head_dim^-1/2.  A query that sees nothing, or is no sequence's, gives zeros.  Each head's query counts to 22
-        bits an element (all that bf16 and fp16 have), or to 2^-31 of its largest where that is coarser.  ``return_lse``: the
-        logarithm of the softmax's denominator [tokens, heads] too (-inf where a query sees nothing)."""
+        them. ``scale`` defaults to head_dim^-1/2. A query that sees nothing, or is no sequence's, gives zeros. Each
+        head's query counts to 22 bits an element (all that bf16 and fp16 have), or to 2^-31 of its largest where that is
+        coarser. ``return_lse``: the logarithm of the softmax's denominator [tokens, heads] too (-inf where a query sees
+        nothing)."""
         if q.dim() != 3 or q.size(1) % self.kv_heads or q.size(1) == 0:
             raise ValueError(f"q must be [tokens, heads, {self.head_dim}], heads a multiple of {self.kv_heads}")
         tokens, heads, dim = q.shape

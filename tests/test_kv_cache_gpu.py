@@ -608,3 +608,27 @@ def test_padded_batches_in_a_graph():
         if sum(new):
             want, _ = s.reference(q[:sum(new)].cpu(), new, 0.125, None)
             check(out[:sum(new)], want, float(held_values(s.v).abs().max()), torch.float16)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 60])
+def test_values_of_very_different_size_in_chunks(new, dtype):
+    """As above over keys that several workgroups share, the large values in some of the chunks only."""
+    dt, dim, held = TYPES[dtype], 64, 6000
+    g = torch.Generator().manual_seed(new)
+    k, v = torch.randn(held, 1, dim, generator=g), torch.randn(held, 1, dim, generator=g)
+    q = torch.randn(new, 2, dim, generator=g)
+    far = (torch.arange(held) % 91 == 5) & (torch.arange(held) > 2500) & (torch.arange(held) < 4100)
+    q[:, :, 0] = dim ** 0.5
+    k[far, :, 0] = -100.  # of next to no weight
+    v[far] *= 2. ** 30
+    s = Sequences([held], 1, dim, dt, 128, k=k, v=v)
+    q = q.to(dt)
+    want, _ = s.reference(q, [new], dim ** -0.5, None)
+    got = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), starts([new])).cpu()
+    kv, most = held_values(s.k)[:, 0], held_values(s.v).abs().amax(-1)[:, 0]
+    for i in range(new):
+        z = kv[:held - new + i + 1] @ q[i].double().t() * dim ** -0.5
+        size = (torch.softmax(z, 0) * most[:held - new + i + 1, None]).sum(0)
+        allowed = want[i].abs() * OWN[dt] * 1.01 + max(OF_VALUES[dt], 2e-4) * size[:, None]
+        assert bool(((got[i].double() - want[i]).abs() <= allowed).all())
