@@ -1,0 +1,236 @@
+// Rotation of queries and keys by their positions, one launch for both; the gradient is the rotation back.
+//
+// Of a head's first r elements pair i, (x[i], x[i + r/2]) or interleaved (x[2 i], x[2 i + 1]), is turned by the angle t = p f_i:
+//   y1 = a (x1 cos t - x2 sin t),  y2 = a (x2 cos t + x1 sin t);  its transpose turns by -t.
+// The elements from r on are passed on.
+//
+// Frequencies are held as turns a position, in fp64: the product with a position of up to 2^31 leaves the fraction of a turn
+// good to 2^-53 of the turns made, where fp32 would leave nothing of far positions.  The fraction is brought to an eighth of
+// a turn around the nearest quarter, exactly, and only then rounded to fp32, for which the Taylor series of sine (to x^9) and
+// cosine (to x^10) are good to 2^-28.  So an angle costs some 40 instructions and no memory (a table of 131072 positions and
+// 64 pairs is 64 MB, and as many reads a head's worth each token), and a thread uses it for several heads.
+//
+// Bound by memory.  A thread takes V pairs (two loads of 16 bytes) of one token and walks over `span` heads, BATCH of them in
+// flight; neighbours take the next pairs, then the next tokens, so that a wave's load covers whole lines of each row.  16384
+// tokens, 40 heads of 128, bf16: 73 us, 4.6 TB/s (a large copy: 5.0); 4096 tokens 18.4 us; 64 tokens 4.1 us, all launch.
+#include "elements.h"
+
+namespace {
+
+constexpr int THREADS = 256, BATCH = 4, PARTS = 2;
+
+struct Part {
+  const void* x;
+  void* y;
+  int heads;
+  int64_t x_outer, x_token, x_head, y_outer, y_token, y_head;
+};
+
+struct Rotate {
+  Part part[PARTS];
+  int heads;  // of all parts
+  int64_t outer, inner;
+  int dim, rotated, turned, units;  // units of V pairs that turn, units of a row
+  int span;
+  const double* turns;
+  float amplitude;
+  const void* positions;
+  int64_t pos_outer, pos_inner;
+  bool wide, back;
+};
+
+// cos and sin of `part` turns, any of them: |part| below 2^52.
+__device__ __forceinline__ void cos_sin(double part, float& c, float& s) {
+  const double r = part - __builtin_rint(part), q = __builtin_rint(4. * r);
+  const float x = (float)(6.283185307179586 * __builtin_fma(-0.25, q, r)), x2 = x * x;  // [-pi/4, pi/4]
+  float a = __builtin_fmaf(x2, 2.7557319e-6f, -1.9841270e-4f);
+  a = __builtin_fmaf(x2, a, 8.3333333e-3f);
+  a = __builtin_fmaf(x2, a, -1.6666667e-1f);
+  a = __builtin_fmaf(x * x2, a, x);
+  float b = __builtin_fmaf(x2, -2.7557319e-7f, 2.4801587e-5f);
+  b = __builtin_fmaf(x2, b, -1.3888889e-3f);
+  b = __builtin_fmaf(x2, b, 4.1666667e-2f);
+  b = __builtin_fmaf(x2, b, -0.5f);
+  b = __builtin_fmaf(x2, b, 1.f);
+  const int quarter = (int)q;  // -2 .. 2
+  const float cc = quarter & 1 ? a : b, ss = quarter & 1 ? b : a;
+  c = (quarter + 1) & 2 ? -cc : cc;
+  s = quarter & 2 ? -ss : ss;
+}
+
+template <int TYPE, int V>
+struct Row {
+  typedef typename Elem<TYPE>::T T;
+  typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+
+template <int TYPE>
+__device__ __forceinline__ void round_all(typename Elem<TYPE>::T (&to)[16 / sizeof(typename Elem<TYPE>::T)],
+                                          const float (&x)[16 / sizeof(typename Elem<TYPE>::T)]) {
+  constexpr int V = 16 / sizeof(typename Elem<TYPE>::T);
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    if constexpr (TYPE == TYPE_BF16)
+      to[i] = __builtin_bit_cast(uint16_t, (__bf16)x[i]);  // to nearest even, one instruction a pair
+    else
+      to[i] = (typename Elem<TYPE>::T)x[i];
+  }
+}
+
+template <int TYPE, bool INTERLEAVED>
+__global__ __launch_bounds__(THREADS) void rotary_kernel(Rotate a) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr int V = 16 / (int)sizeof(T);
+  typedef typename Row<TYPE, V>::vec vec;
+  const uint32_t item = blockIdx.x * THREADS + threadIdx.x, units = (uint32_t)a.units, tokens = (uint32_t)(a.outer * a.inner);
+  const uint32_t token = item / units;
+  const int unit = (int)(item - token * units);
+  if (token >= tokens) return;
+  const int64_t o = a.outer > 1 ? token / (uint32_t)a.inner : 0, t = token - o * a.inner;
+  const int h0 = blockIdx.y * a.span, h1 = h0 + a.span < a.heads ? h0 + a.span : a.heads;
+  const bool turned = unit < a.turned;
+  // this unit's two runs of V elements, and how many of each there are
+  int d0, d1, n0, n1;
+  float c[V], s[V];
+  if (turned) {
+    const int half = a.rotated / 2, i0 = unit * V;
+    const double p = a.wide ? (double)((const int64_t*)a.positions)[o * a.pos_outer + t * a.pos_inner]
+                            : (double)((const int32_t*)a.positions)[o * a.pos_outer + t * a.pos_inner];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      cos_sin(p * a.turns[i0 + i < half ? i0 + i : half - 1], c[i], s[i]);
+      c[i] *= a.amplitude;
+      s[i] *= a.back ? -a.amplitude : a.amplitude;
+    }
+    const int n = half - i0 < V ? half - i0 : V;
+    if (INTERLEAVED) {
+      d0 = 2 * i0, d1 = d0 + V;
+      n0 = 2 * n < V ? 2 * n : V, n1 = 2 * n - n0;
+    } else {
+      d0 = i0, d1 = half + i0;
+      n0 = n1 = n;
+    }
+  } else {
+    d0 = a.rotated + (unit - a.turned) * 2 * V, d1 = d0 + V;
+    n0 = a.dim - d0 < V ? a.dim - d0 : V;
+    n1 = a.dim - d1 < 0 ? 0 : a.dim - d1 < V ? a.dim - d1 : V;
+  }
+  const bool whole = n0 == V && n1 == V;
+  for (int h = h0; h < h1; h += BATCH) {
+    vec u[BATCH], w[BATCH];
+    T* to[BATCH];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int g = h + b < h1 ? h + b : h1 - 1, second = g >= a.part[0].heads;
+      const Part& part = a.part[second];
+      const int head = second ? g - a.part[0].heads : g;
+      const T* from = (const T*)part.x + o * part.x_outer + t * part.x_token + head * part.x_head;
+      to[b] = (T*)part.y + o * part.y_outer + t * part.y_token + head * part.y_head;
+      if (whole) {
+        u[b] = *reinterpret_cast<const vec*>(from + d0);
+        w[b] = *reinterpret_cast<const vec*>(from + d1);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          u[b][i] = i < n0 ? from[d0 + i] : (T)0;
+          w[b][i] = i < n1 ? from[d1 + i] : (T)0;
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      if (h + b >= h1) break;
+      if (turned) {
+        float y0[V], y1[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          // pair i of the unit: elements of the two runs, or neighbours in the 2 V of both
+          if (INTERLEAVED) {
+            const int j = 2 * i;
+            const float x1 = to_f32<TYPE>(j < V ? u[b][j % V] : w[b][j % V]);
+            const float x2 = to_f32<TYPE>(j < V ? u[b][(j + 1) % V] : w[b][(j + 1) % V]);
+            const float r1 = __builtin_fmaf(x1, c[i], -x2 * s[i]), r2 = __builtin_fmaf(x2, c[i], x1 * s[i]);
+            (j < V ? y0 : y1)[j % V] = r1;
+            (j < V ? y0 : y1)[(j + 1) % V] = r2;
+          } else {
+            const float x1 = to_f32<TYPE>(u[b][i]), x2 = to_f32<TYPE>(w[b][i]);
+            y0[i] = __builtin_fmaf(x1, c[i], -x2 * s[i]);
+            y1[i] = __builtin_fmaf(x2, c[i], x1 * s[i]);
+          }
+        }
+        T r0[V], r1[V];
+        round_all<TYPE>(r0, y0);
+        round_all<TYPE>(r1, y1);
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[b][i] = r0[i], w[b][i] = r1[i];
+      }
+      if (whole) {
+        *reinterpret_cast<vec*>(to[b] + d0) = u[b];
+        *reinterpret_cast<vec*>(to[b] + d1) = w[b];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if (i < n0) to[b][d0 + i] = u[b][i];
+          if (i < n1) to[b][d1 + i] = w[b][i];
+        }
+      }
+    }
+  }
+}
+
+template <int TYPE>
+int launch(Rotate& a, bool interleaved, hipStream_t st) {
+  constexpr int V = 16 / (int)sizeof(typename Elem<TYPE>::T);
+  a.turned = (a.rotated / 2 + V - 1) / V;
+  a.units = a.turned + (a.dim - a.rotated + 2 * V - 1) / (2 * V);
+  const int64_t items = a.outer * a.inner * a.units;
+  if (items >= ((int64_t)1 << 32) - THREADS) return GPTQ2D_EUNSUPPORTED;
+  // A head a thread while that fills the chip's 2^17 lanes twice at most, when latency is the bound; then as many as are in
+  // flight (us for 1, 4 and 8 heads a thread, 40 heads of 128, bf16: 64 tokens 4.1, 4.8, 6.5; 512 tokens 5.7, 5.3, 6.9; 4096
+  // 24.3, 18.4, 17.9; 16384 100, 73, 74; 15 heads of 80, fp32, 1001 tokens 6.2, 7.3, 10.9).
+  a.span = items * a.heads <= 1 << 18 ? 1 : BATCH;
+  const dim3 grid((unsigned)((items + THREADS - 1) / THREADS), (unsigned)((a.heads + a.span - 1) / a.span));
+  if (grid.y > 65535 || (int64_t)grid.x * THREADS >= (int64_t)1 << 32) return GPTQ2D_EUNSUPPORTED;
+  if (interleaved)
+    hipLaunchKernelGGL((rotary_kernel<TYPE, true>), grid, dim3(THREADS), 0, st, a);
+  else
+    hipLaunchKernelGGL((rotary_kernel<TYPE, false>), grid, dim3(THREADS), 0, st, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" int gptq2d_rotary(int32_t count, const void* const* x, void* const* y, const int64_t* heads, const int64_t* strides,
+                             int32_t type, int64_t outer, int64_t inner, int32_t dim, int32_t rotated, int32_t interleaved,
+                             const double* turns, double amplitude, const void* positions, int32_t wide, int64_t pos_outer,
+                             int64_t pos_inner, int32_t back, void* stream) {
+  if (count < 1 || count > PARTS || outer < 0 || inner < 0 || dim < 2 || dim > 1 << 20 || rotated < 2 || rotated > dim ||
+      rotated % 2)
+    return GPTQ2D_EINVAL;
+  if (outer > 0x7fffffff || inner > 0x7fffffff) return GPTQ2D_EUNSUPPORTED;
+  Rotate a = {};
+  int64_t all = 0;
+  for (int i = 0; i < count; ++i) {
+    const int64_t* s = strides + 6 * i;
+    if (heads[i] < 0 || heads[i] > 1 << 20) return GPTQ2D_EINVAL;
+    a.part[i] = {x[i], y[i], (int)heads[i], s[0], s[1], s[2], s[3], s[4], s[5]};
+    all += heads[i];
+  }
+  if (outer * inner == 0 || all == 0) return 0;
+  if (outer * inner >= (int64_t)1 << 32) return GPTQ2D_EUNSUPPORTED;
+  a.heads = (int)all;
+  a.outer = outer, a.inner = inner, a.dim = dim, a.rotated = rotated;
+  a.turns = turns, a.amplitude = (float)amplitude;
+  a.positions = positions, a.wide = wide != 0, a.pos_outer = pos_outer, a.pos_inner = pos_inner;
+  a.back = back != 0;
+  const hipStream_t st = (hipStream_t)stream;
+  switch (type) {
+    case TYPE_F32:
+      return launch<TYPE_F32>(a, interleaved != 0, st);
+    case TYPE_BF16:
+      return launch<TYPE_BF16>(a, interleaved != 0, st);
+    case TYPE_F16:
+      return launch<TYPE_F16>(a, interleaved != 0, st);
+  }
+  return GPTQ2D_EINVAL;
+}

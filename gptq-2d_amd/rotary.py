@@ -1,0 +1,182 @@
+"""Rotary positions on the GPU (csrc/rotary.hip; no reference counterpart: the reference quantizes weights only).
+
+Pair i of a head's first ``rotated`` elements, (x[i], x[i + rotated/2]) or with ``interleaved`` (x[2 i], x[2 i + 1]), is
+turned by position times f_i:
+
+    y1 = a (x1 cos t - x2 sin t),   y2 = a (x2 cos t + x1 sin t),   t = position f_i,   f_i = base^(-2 i / rotated)
+
+and the elements behind them are passed on.  Frequencies may be scaled for contexts longer than a model was trained on
+(`Linear`, `Ntk`, `Bands`, `Yarn`; a is 1 but for the last).  Angles are formed in 64 bits, so that far positions are as good
+as near ones; sums are in 32 bits and rounded once.
+
+    rotary = Rotary(128, base=500000., scaling=Bands(8., context=8192))
+    q, k = rotary(q, k, positions=positions)        # one launch; differentiable in q and k
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple, Sequence
+
+import torch
+
+import _hip
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class Linear(NamedTuple):
+    """Positions divided by ``factor``: f_i / factor."""
+    factor: float
+
+
+class Ntk(NamedTuple):
+    """A larger base: base factor^(r / (r - 2)), so that the lowest frequency is divided by ``factor`` and the highest stays."""
+    factor: float
+
+
+class Bands(NamedTuple):
+    """By the turns that a pair makes in ``context`` tokens: fewer than ``low`` f_i / factor, more than ``high`` f_i, in between
+    in proportion."""
+    factor: float
+    context: int
+    low: float = 1.
+    high: float = 4.
+
+
+class Yarn(NamedTuple):
+    """By the pair's number: f_i where the pair makes ``fast`` turns or more in ``context`` tokens, f_i / factor where it makes
+    ``slow`` or fewer, a ramp over the numbers in between (from the whole one below to the whole one above).  The rotated part
+    is multiplied by ``amplitude`` (None: 0.1 ln factor + 1, or 1 for a factor of at most 1)."""
+    factor: float
+    context: int
+    fast: float = 32.
+    slow: float = 1.
+    amplitude: float | None = None
+
+
+def rotary_frequencies(rotated: int, base: float = 10000., scaling: Linear | Ntk | Bands | Yarn | None = None) -> tuple[list, float]:
+    """Radians a position of each of the rotated / 2 pairs, and the factor on what is rotated."""
+    if isinstance(scaling, Ntk) and rotated > 2:
+        base = base * scaling.factor ** (rotated / (rotated - 2))
+    f = [base ** (-2 * i / rotated) for i in range(rotated // 2)]
+    if scaling is None or isinstance(scaling, Ntk):
+        return f, 1.
+    if isinstance(scaling, Linear):
+        return [x / scaling.factor for x in f], 1.
+    if isinstance(scaling, Bands):
+        out = []
+        for x in f:
+            part = (scaling.context * x / (2 * math.pi) - scaling.low) / (scaling.high - scaling.low)
+            part = min(max(part, 0.), 1.)
+            out.append((1 - part) * x / scaling.factor + part * x)
+        return out, 1.
+    if isinstance(scaling, Yarn):
+        def number(turns):  # of the pair that makes that many in the context
+            return rotated * math.log(scaling.context / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = max(math.floor(number(scaling.fast)), 0), min(math.ceil(number(scaling.slow)), rotated - 1)
+        out = []
+        for i, x in enumerate(f):
+            part = min(max((i - low) / max(high - low, 0.001), 0.), 1.)
+            out.append(part * x / scaling.factor + (1 - part) * x)
+        amplitude = scaling.amplitude
+        if amplitude is None:
+            amplitude = 0.1 * math.log(scaling.factor) + 1. if scaling.factor > 1 else 1.
+        return out, amplitude
+    raise ValueError(f"scaling must be Linear, Ntk, Bands, Yarn or None, got {scaling!r}")
+
+
+class Rotary:
+    """Rotation of heads of ``dim`` elements, of which the first ``rotated`` (even; None: all) turn.  ``frequencies``: radians
+    a position of each pair, in the place of those that ``base`` and ``scaling`` give."""
+
+    def __init__(self, dim: int, *, base: float = 10000., rotated: int | None = None, interleaved: bool = False,
+                 scaling: Linear | Ntk | Bands | Yarn | None = None, frequencies: Sequence[float] | None = None,
+                 device: torch.device | str = "cuda"):
+        rotated = dim if rotated is None else rotated
+        if not 2 <= rotated <= dim <= 1 << 20 or rotated % 2:
+            raise ValueError(f"an even number of a head's {dim} elements turns, at least 2, not {rotated}")
+        if frequencies is None:
+            if base <= 1 or (scaling is not None and scaling.factor <= 0):
+                raise ValueError("the base must be above 1 and a scaling's factor above 0")
+            if isinstance(scaling, Bands) and not scaling.high > scaling.low:
+                raise ValueError("high must be above low")
+            if isinstance(scaling, (Bands, Yarn)) and scaling.context < 1:
+                raise ValueError("the context must be at least one token")
+            frequencies, amplitude = rotary_frequencies(rotated, base, scaling)
+        elif scaling is not None or len(frequencies) != rotated // 2:
+            raise ValueError(f"frequencies must be {rotated // 2} numbers, without a scaling")
+        else:
+            amplitude = 1.
+        self.dim, self.rotated, self.interleaved, self.amplitude = dim, rotated, bool(interleaved), float(amplitude)
+        self.turns = torch.tensor([float(f) / (2 * math.pi) for f in frequencies], dtype=torch.float64, device=device)
+        _hip.require_device(self.turns)
+        self.device = self.turns.device
+
+    def __call__(self, *xs: torch.Tensor, positions: torch.Tensor):
+        """One or two tensors (queries, keys) [..., heads, dim] of one type (fp32, bf16 or fp16) rotated, each with its own
+        number of heads, any strides.  ``positions`` (int32 or int64) broadcasts to their leading axes, of which there are one
+        or two ([tokens], [batch, tokens]); a position may be negative and counts to 2^53."""
+        if not 1 <= len(xs) <= 2:
+            raise ValueError("one or two tensors are rotated in a call")
+        lead = xs[0].shape[:-2]
+        for x in xs:
+            if x.dim() not in (3, 4) or x.size(-1) != self.dim or x.shape[:-2] != lead:
+                raise ValueError(f"tensors must be [tokens, heads, {self.dim}] or [batch, tokens, heads, {self.dim}], alike but "
+                                 f"for the heads; got {[tuple(x.shape) for x in xs]}")
+            if x.dtype not in _TYPES or x.dtype is not xs[0].dtype:
+                raise ValueError("tensors must be all float32, bfloat16 or float16")
+            if x.device != self.device:
+                raise ValueError("tensors must be on the rotation's device")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != self.device:
+            raise ValueError("positions must be int32 or int64 on the rotation's device")
+        if positions.dim() > len(lead) or any(a != b and a != 1 for a, b in zip(positions.shape[::-1], lead[::-1])):
+            raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to {tuple(lead)}")
+        if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+            out = _Rotation.apply(self, False, positions, *xs)
+        else:
+            out = self._rotate(xs, positions, False)
+        return out[0] if len(xs) == 1 else out
+
+    def _rotate(self, xs, positions, back):
+        lead = xs[0].shape[:-2]
+        outer, inner = (1, *lead) if len(lead) == 1 else lead
+        p = positions.expand(lead)
+        p_strides = (0, *p.stride()) if len(lead) == 1 else p.stride()
+        xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
+        out = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
+        strides = []
+        for t in (t for pair in zip(xs, out) for t in pair):
+            strides += (0, *t.stride()[:2]) if len(lead) == 1 else t.stride()[:3]
+        count = len(xs)
+        args = (count, (_hip._P * count)(*(x.data_ptr() for x in xs)), (_hip._P * count)(*(y.data_ptr() for y in out)),
+                _hip.i64_array([x.size(-2) for x in xs]), _hip.i64_array(strides), _TYPES[xs[0].dtype], outer, inner, self.dim,
+                self.rotated, self.interleaved, self.turns.data_ptr(), self.amplitude, p.data_ptr(),
+                p.dtype is torch.int64, *p_strides, back)
+        fn = _hip.lib().gptq2d_rotary
+        if torch.cuda.current_device() == self.device.index:
+            rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
+        else:
+            with torch.cuda.device(self.device):
+                rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
+        if rc:
+            raise _hip.GPTQ2DError(f"gptq2d_rotary failed with code {rc}")
+        return out
+
+
+class _Rotation(torch.autograd.Function):
+    """The rotation (or, `back`, its transpose), whose gradient is the other one."""
+
+    @staticmethod
+    def forward(ctx, rotary, back, positions, *xs):
+        ctx.set_materialize_grads(False)
+        ctx.rotary, ctx.back = rotary, back
+        ctx.save_for_backward(positions)
+        return rotary._rotate(xs, positions, back)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        grads = [g if wanted else None for g, wanted in zip(grads, ctx.needs_input_grad[3:])]
+        there = [g for g in grads if g is not None]
+        turned = iter(_Rotation.apply(ctx.rotary, not ctx.back, ctx.saved_tensors[0], *there) if there else ())
+        return (None, None, None, *(None if g is None else next(turned) for g in grads))
