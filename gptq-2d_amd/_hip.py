@@ -120,6 +120,13 @@ def lib() -> ctypes.CDLL:
         handle.gptq2d_rotary.argtypes = [_I32, _P, _P, _AP, _AP, _I32, _I64, _I64, _I32, _I32, _I32, _P, _F64, _P, _I32, _I64,
                                          _I64, _I32, _P]
         handle.gptq2d_rotary.restype = ctypes.c_int
+        handle.gptq2d_page_pool.argtypes = [_P, _I64, _I64, _I64, _I32, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _P, _P, _P,
+                                            _P, _P, _I64, _P]
+        handle.gptq2d_page_pool.restype = ctypes.c_int
+        handle.gptq2d_page_pool_workspace.argtypes = [_I64]
+        handle.gptq2d_page_pool_workspace.restype = ctypes.c_int64
+        handle.gptq2d_row_positions.argtypes = [_P, _P, _I64, _I64, _P, _P]
+        handle.gptq2d_row_positions.restype = ctypes.c_int
         handle.gptq2d_profile_start.argtypes = [_I64, ctypes.c_uint32]
         handle.gptq2d_profile_start.restype = ctypes.c_int
         handle.gptq2d_profile_read.argtypes = [_I32, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double),

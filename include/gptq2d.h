@@ -381,6 +381,26 @@ int gptq2d_rotary(int32_t count, const void* const* x, void* const* y, const int
                   const double* turns, double amplitude, const void* positions, int32_t wide, int64_t pos_outer,
                   int64_t pos_inner, int32_t back, void* stream);
 
+/* The pages of a cache dealt to sequences (no reference counterpart).  State, all int32: table[seqs][width] (rows table_stride
+ * apart, -1: no page), owned[seqs] (the first entries of a row are the sequence's pages), lengths[seqs] (tokens), missing[seqs]
+ * (pages that the call had none left for), free[pages] with left[1] (the stack of the other pages, and its height).
+ * request[seqs]: the sequences' lengths, or with extend != 0 what they grow by (below 0: 0; a length is at most 2^30).  Sequence
+ * b is to have min(ceil(length / page), width) pages: the entries past that of all sequences in order go back on the stack, the
+ * last one first; then the missing ones, in order, are taken from its top while there are pages.
+ * With extend, the call's tokens (optional, NULL: not given): offsets[seqs + 1] (sums of request, at most `tokens`), held[seqs] (lengths
+ * before), positions[tokens] and slots[tokens] (page number times page plus the place in it; -1 without a page) of the packed
+ * rows; rows that no sequence has: 0 and -1.  work: 4-byte aligned, gptq2d_page_pool_workspace bytes (-1 for seqs it does
+ * not take), of no use afterwards.  seqs width and tokens are below 2^31, seqs at most 2^24. */
+int64_t gptq2d_page_pool_workspace(int64_t seqs);
+int gptq2d_page_pool(int32_t* table, int64_t seqs, int64_t width, int64_t table_stride, int32_t page, int64_t pages,
+                     int32_t* owned, int32_t* lengths, int32_t* missing, int32_t* free, int32_t* left, const int32_t* request,
+                     int32_t extend, int64_t tokens, int32_t* offsets, int32_t* held, int32_t* positions, int64_t* slots,
+                     void* work, int64_t work_bytes, void* stream);
+
+/* positions[r] = held[b] + r - offsets[b] of the packed rows r of sequence b, 0 for rows that no sequence has. */
+int gptq2d_row_positions(const int32_t* held, const int32_t* offsets, int64_t seqs, int64_t tokens, int32_t* positions,
+                         void* stream);
+
 /* Launch profiler (no reference counterpart; the reference times with host clocks, demo.ipynb:109-118).
  * While on, every launch of a profiled kernel class is bracketed with HIP events on its stream.
  * Process-global, not thread-safe, not for use under stream capture.
