@@ -115,6 +115,17 @@ def lib() -> ctypes.CDLL:
         handle.gptq2d_kv_attend.restype = ctypes.c_int
         handle.gptq2d_kv_attend_workspace.argtypes = [_I64, _I64, _I32, _I32, _I32, _I64, _I64]
         handle.gptq2d_kv_attend_workspace.restype = ctypes.c_int64
+        handle.gptq2d_kv_attend_tree.argtypes = [*cache, _P, _I64, _I64, _I32, _I32, *tokens, _P, _P, _I64, _F64, _I64, _P, _I64,
+                                                 _I64, _P, _P, _I64, _P]
+        handle.gptq2d_kv_attend_tree.restype = ctypes.c_int
+        handle.gptq2d_kv_attend_tree_workspace.argtypes = [_I64, _I64, _I32, _I32, _I32, _I64, _I64, _I64]
+        handle.gptq2d_kv_attend_tree_workspace.restype = ctypes.c_int64
+        handle.gptq2d_kv_keep.argtypes = [*cache, *tokens, _P, _I64, _I64, _P, _P]
+        handle.gptq2d_kv_keep.restype = ctypes.c_int
+        handle.gptq2d_draft_tree.argtypes = [_P, _P, _P, _I64, _I64, _I64, _P, _P, _P]
+        handle.gptq2d_draft_tree.restype = ctypes.c_int
+        handle.gptq2d_draft_accept.argtypes = [_P, _P, _I64, _I64, _I64, _P, _P, _I32, _P, _P, _P, _P]
+        handle.gptq2d_draft_accept.restype = ctypes.c_int
         handle.gptq2d_kv_page_words.argtypes = [_I32, _I32, _I32]
         handle.gptq2d_kv_page_words.restype = ctypes.c_int64
         handle.gptq2d_rotary.argtypes = [_I32, _P, _P, _AP, _AP, _I32, _I64, _I64, _I32, _I32, _I32, _P, _F64, _P, _I32, _I64,
@@ -142,6 +153,19 @@ def call_untyped(name: str, *args) -> None:
     """Call ``gptq2d_<name>`` (an entry point with no element type) and raise on a non-zero return code."""
     rc = getattr(lib(), f"gptq2d_{name}")(*args)
     if rc != 0:
+        raise GPTQ2DError(f"gptq2d_{name} failed with code {rc}")
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call ``gptq2d_<name>`` with ``device`` current and its current stream as the last argument, and raise on a non-zero
+    return code."""
+    fn = getattr(lib(), f"gptq2d_{name}")
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if rc:
         raise GPTQ2DError(f"gptq2d_{name} failed with code {rc}")
 
 

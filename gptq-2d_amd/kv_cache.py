@@ -24,6 +24,7 @@ import math
 import torch
 
 import _hip
+from drafts import DraftTree
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -50,8 +51,9 @@ class KVCache4:
         _hip.require_device(self.pages)
         self.device = self.pages.device
         lib = _hip.lib()
-        self._append, self._read, self._attend = lib.gptq2d_kv_append, lib.gptq2d_kv_read, lib.gptq2d_kv_attend
-        self._workspace = lib.gptq2d_kv_attend_workspace
+        self._append, self._read, self._keep = lib.gptq2d_kv_append, lib.gptq2d_kv_read, lib.gptq2d_kv_keep
+        self._attend = {"attend": lib.gptq2d_kv_attend, "attend_tree": lib.gptq2d_kv_attend_tree}
+        self._workspace = {"attend": lib.gptq2d_kv_attend_workspace, "attend_tree": lib.gptq2d_kv_attend_tree_workspace}
         self._cache = (self.pages.data_ptr(), pages, kv_heads, head_dim, page_size)
 
     # Arguments of the sequences, as the C entries take them.
@@ -127,14 +129,18 @@ class KVCache4:
 
     @torch.no_grad()
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None, *,
-               scale: float | None = None, window: int | None = None, return_lse: bool = False):
+               scale: float | None = None, window: int | None = None, return_lse: bool = False, tree: DraftTree | None = None):
         """Causal attention of q [tokens, heads, head_dim] (fp32, bf16 or fp16; heads a multiple of kv_heads, consecutive
         ones sharing a kv head) over the cache. The queries of a sequence are its last tokens: of its T, number i is at
         position ``lengths[b] - T + i`` and sees the positions up to its own, with ``window`` only the last `window` of
         them. ``scale`` defaults to head_dim^-1/2. A query that sees nothing, or is no sequence's, gives zeros. Each
         head's query counts to 22 bits an element (all that bf16 and fp16 have), or to 2^-31 of its largest where that is
         coarser. ``return_lse``: the logarithm of the softmax's denominator [tokens, heads] too (-inf where a query sees
-        nothing)."""
+        nothing).
+
+        ``tree``: the sequences' last tokens are the nodes of a `drafts.DraftTree` of the same ``offsets``, made with ``held`` =
+        ``lengths[b]`` less the nodes. Each sees the tokens before the nodes -- with ``window``, which holds the tree's
+        `nodes` at least, the last `window` up to its own position -- and the nodes that it comes from."""
         if q.dim() != 3 or q.size(1) % self.kv_heads or q.size(1) == 0:
             raise ValueError(f"q must be [tokens, heads, {self.head_dim}], heads a multiple of {self.kv_heads}")
         tokens, heads, dim = q.shape
@@ -146,13 +152,40 @@ class KVCache4:
             raise ValueError("a window holds at least one token, and fewer than 2^30")
         where = self._sequences(table, lengths, offsets, tokens)
         group, window = heads // self.kv_heads, window or 0
+        name, nodes, of_tree = "attend", (), ()
+        if tree is not None:
+            if offsets is None or tree.seqs != where[1] or tree.tokens != tokens or tree.device != self.device:
+                raise ValueError(f"the tree is one of {tree.tokens} tokens of {tree.seqs} sequences on {tree.device}, and takes "
+                                 f"their offsets")
+            if window and window < tree.nodes:
+                raise ValueError(f"a window holds the tree's {tree.nodes} nodes at least")
+            name, nodes = "attend_tree", (tree.nodes,)
+            of_tree = (tree.ancestors.data_ptr(), tree.positions.data_ptr(), tree.nodes)
         out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=self.device)
         lse = torch.empty(tokens, heads, dtype=torch.float32, device=self.device) if return_lse else None
-        size = self._workspace(tokens, where[1], self.kv_heads, group, dim, where[2] * self.page_size, window)
+        size = self._workspace[name](tokens, where[1], self.kv_heads, group, dim, where[2] * self.page_size, window, *nodes)
         if size < 0:
             raise ValueError(f"attention of {tokens} tokens over {where[1]} sequences is too large")
         work = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
-        self._call(self._attend, "attend", *self._cache, q.data_ptr(), q.stride(0), q.stride(1), group, kind, *where,
+        self._call(self._attend[name], name, *self._cache, q.data_ptr(), q.stride(0), q.stride(1), group, kind, *where, *of_tree,
                    math.pow(dim, -0.5) if scale is None else scale, window, out.data_ptr(), out.stride(0), out.stride(1),
                    None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), size)
         return (out, lse) if return_lse else out
+
+    @torch.no_grad()
+    def keep(self, table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor, path: torch.Tensor,
+             counts: torch.Tensor) -> None:
+        """Of each sequence's last tokens, the nodes of a tree, put those that were accepted where the nodes begin: node
+        ``path[b, i]`` for i < ``counts[b]`` (int32 [B, P] and [B], `DraftTree.accept`'s) comes to position ``lengths[b]`` less
+        the nodes plus i; other places stay as they are. A path ends where it does not ascend among the sequence's nodes."""
+        seqs = table.size(0)
+        if offsets is None:
+            raise ValueError("keep needs the nodes' offsets")
+        where = self._sequences(table, lengths, offsets, 0x7fffffff)
+        if path.dtype is not torch.int32 or path.dim() != 2 or path.size(0) != seqs or path.device != self.device or \
+                (path.size(1) > 1 and path.stride(1) != 1):
+            raise ValueError(f"path must be int32 [{seqs}, P] with contiguous rows, on the cache's device")
+        if counts.dtype is not torch.int32 or counts.shape != (seqs,) or counts.device != self.device or \
+                not counts.is_contiguous():
+            raise ValueError(f"counts must be a contiguous int32 [{seqs}] on the cache's device")
+        self._call(self._keep, "keep", *self._cache, *where, path.data_ptr(), path.stride(0), path.size(1), counts.data_ptr())

@@ -36,17 +36,6 @@ class Rows(NamedTuple):
     slots: torch.Tensor
 
 
-def _call(device, name, *args):
-    fn = getattr(_hip.lib(), f"gptq2d_{name}")
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    if rc:
-        raise _hip.GPTQ2DError(f"gptq2d_{name} failed with code {rc}")
-
-
 class PagePool:
     """``pages`` pages of ``page_size`` tokens for ``seqs`` sequences of at most ``width`` pages.
 
@@ -81,7 +70,7 @@ class PagePool:
     @torch.no_grad()
     def resize(self, lengths: torch.Tensor) -> None:
         """Pages for ``lengths[b]`` tokens of sequence b (int32; below 0 counts as 0, at most 2^30), no more and no fewer."""
-        _call(self.device, "page_pool", *self._state, self._request(lengths, "lengths"), False, 0, None, None, None, None,
+        _hip.launch("page_pool", self.device, *self._state, self._request(lengths, "lengths"), False, 0, None, None, None, None,
               *self._scratch)
 
     @torch.no_grad()
@@ -94,7 +83,7 @@ class PagePool:
         seqs = self.lengths.numel()
         rows = Rows(torch.empty(seqs + 1, **whole), torch.empty(seqs, **whole), torch.empty(tokens, **whole),
                     torch.empty(tokens, dtype=torch.int64, device=self.device))
-        _call(self.device, "page_pool", *self._state, self._request(new, "new"), True, tokens, *(t.data_ptr() for t in rows),
+        _hip.launch("page_pool", self.device, *self._state, self._request(new, "new"), True, tokens, *(t.data_ptr() for t in rows),
               *self._scratch)
         return rows
 
@@ -112,5 +101,5 @@ def row_positions(held: torch.Tensor, offsets: torch.Tensor, tokens: int) -> tor
     if not 0 <= tokens < 1 << 31:
         raise ValueError("tokens must be a number of rows below 2^31")
     positions = torch.empty(tokens, dtype=torch.int32, device=held.device)
-    _call(held.device, "row_positions", held.data_ptr(), offsets.data_ptr(), held.numel(), tokens, positions.data_ptr())
+    _hip.launch("row_positions", held.device, held.data_ptr(), offsets.data_ptr(), held.numel(), tokens, positions.data_ptr())
     return positions

@@ -149,18 +149,10 @@ class Rotary:
         for t in (t for pair in zip(xs, out) for t in pair):
             strides += (0, *t.stride()[:2]) if len(lead) == 1 else t.stride()[:3]
         count = len(xs)
-        args = (count, (_hip._P * count)(*(x.data_ptr() for x in xs)), (_hip._P * count)(*(y.data_ptr() for y in out)),
+        _hip.launch("rotary", self.device, count, (_hip._P * count)(*(x.data_ptr() for x in xs)), (_hip._P * count)(*(y.data_ptr() for y in out)),
                 _hip.i64_array([x.size(-2) for x in xs]), _hip.i64_array(strides), _TYPES[xs[0].dtype], outer, inner, self.dim,
                 self.rotated, self.interleaved, self.turns.data_ptr(), self.amplitude, p.data_ptr(),
-                p.dtype is torch.int64, *p_strides, back)
-        fn = _hip.lib().gptq2d_rotary
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
-        else:
-            with torch.cuda.device(self.device):
-                rc = fn(*args, torch.cuda.current_stream(self.device).cuda_stream)
-        if rc:
-            raise _hip.GPTQ2DError(f"gptq2d_rotary failed with code {rc}")
+                    p.dtype is torch.int64, *p_strides, back)
         return out
 
 

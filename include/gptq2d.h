@@ -348,6 +348,40 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
                      double scale, int64_t window, void* out, int64_t out_token, int64_t out_head, float* lse, void* work,
                      int64_t work_bytes, void* stream);
 
+/* Trees of drafted tokens (no reference counterpart).  Sequence b's T_b packed rows are the nodes of a tree, node i's parent the
+ * earlier node parents[row] (any other number: none), at most `nodes` (up to 512) of them.
+ *
+ * ancestors[tokens][(nodes + 31) / 32]: bit j of a row is set for the nodes j that it comes from and for itself; positions[tokens]:
+ * held[b] and as many as there are nodes before it.  Rows that no sequence has: 0; nodes past `nodes`: no bits, held[b]. */
+int gptq2d_draft_tree(const int32_t* parents, const int32_t* offsets, const int32_t* held, int64_t seqs, int64_t tokens,
+                      int64_t nodes, uint32_t* ancestors, int32_t* positions, void* stream);
+
+/* The accepted nodes path[b][0 .. counts[b] - 1] (rows of `nodes`, -1 behind them): node 0, then each time the first child whose
+ * drafted token is the one chosen after its parent; last[b] is the token chosen after the last of them (-1 where T_b is 0).
+ * drafted, chosen [tokens] and last: int32, or int64 with wide != 0. */
+int gptq2d_draft_accept(const int32_t* parents, const int32_t* offsets, int64_t seqs, int64_t tokens, int64_t nodes,
+                        const void* drafted, const void* chosen, int32_t wide, int32_t* path, int32_t* counts, void* last,
+                        void* stream);
+
+/* gptq2d_kv_attend of the nodes, that the cache holds as the last tokens (node i at length - T_b + i): each sees the tokens held
+ * before them (with window > 0 those of positions > positions[row] - window), the nodes of its `ancestors` and no others.
+ * window: 0, or at least `nodes`. */
+int64_t gptq2d_kv_attend_tree_workspace(int64_t tokens, int64_t seqs, int32_t heads, int32_t group, int32_t dim, int64_t most,
+                                        int64_t window, int64_t nodes);
+int gptq2d_kv_attend_tree(const void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, const void* q,
+                          int64_t q_token, int64_t q_head, int32_t group, int32_t type, const int32_t* table, int64_t seqs,
+                          int64_t width, int64_t table_stride, const int32_t* lengths, const int32_t* offsets, int64_t tokens,
+                          const uint32_t* ancestors, const int32_t* positions, int64_t nodes, double scale, int64_t window,
+                          void* out, int64_t out_token, int64_t out_head, float* lse, void* work, int64_t work_bytes,
+                          void* stream);
+
+/* Entries of the nodes path[b][0] < path[b][1] < ... (rows path_stride apart; counts[b] of them, at most `most`) to the places
+ * of the sequence's nodes 0, 1, ..., length - T_b and up; other places stay.  What does not ascend below T_b ends the path;
+ * a place or an entry without a page is left. */
+int gptq2d_kv_keep(void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, const int32_t* table, int64_t seqs,
+                   int64_t width, int64_t table_stride, const int32_t* lengths, const int32_t* offsets, int64_t tokens,
+                   const int32_t* path, int64_t path_stride, int64_t most, const int32_t* counts, void* stream);
+
 /* Product with a packed INT layer, beside it the low-rank adapters of many requests (no reference counterpart: the
  * reference returns dequantized weights):
  *   y[t, i] = sum_k x[t, k] (u[i, k] + qmin - zero[i, k / group]) scale[i, k / group] + bias[i]
