@@ -17,8 +17,22 @@ int gptq2d_kv_attend(const void* pages, int64_t page_count, int32_t heads, int32
   KvCache c;
   if (!make_cache(c, pages, page_count, heads, dim, page, table, seqs, width, table_stride, lengths, offsets, tokens))
     return GPTQ2D_EINVAL;
-  return attend<false>(c, Attend{}, q, q_token, q_head, group, type, scale, window, out, out_token, out_head, lse, work,
-                       work_bytes, stream);
+  const int64_t most = width * page;
+  if (!attend_ok(tokens, seqs, heads, group, dim, most, window)) return GPTQ2D_EINVAL;
+  if (tokens == 0) return 0;
+  Attend a = {};
+  const Plan p = make_plan(tokens, seqs, heads, group, dim, most, window);
+  const int rc = set_call(a, p, !p.prompt, q, q_token, q_head, group, scale, window, out, out_token, out_head, lse, work, work_bytes);
+  if (rc) return rc;
+  switch (type) {
+    case TYPE_F32:
+      return launch_type<false, TYPE_F32>(c, a, p, (hipStream_t)stream);
+    case TYPE_BF16:
+      return launch_type<false, TYPE_BF16>(c, a, p, (hipStream_t)stream);
+    case TYPE_F16:
+      return launch_type<false, TYPE_F16>(c, a, p, (hipStream_t)stream);
+  }
+  return GPTQ2D_EINVAL;
 }
 
 }  // extern "C"

@@ -932,6 +932,15 @@ struct Plan {
   bool prompt;
   int nd, ct, chunk, chunks;  // ct: columns of a workgroup
   int64_t slots, part;  // part: floats of the partial results
+  int64_t blocks;       // of the longest possible range
+  int64_t turns;        // of 65532 slots, where they are not the grid's first axis
+
+  void set_chunks(int heads) {
+    chunks = (int)((blocks + chunk - 1) / chunk);
+    if (chunks <= 1) chunks = 1;
+    part = chunks > 1 ? slots * heads * chunks * (int64_t)(ct * (64 * nd + 2)) : 0;
+    turns = (slots + 65531) / 65532;
+  }
 };
 
 inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int dim, int64_t most, int64_t window, int64_t nodes = 0) {
@@ -948,7 +957,7 @@ inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int di
   int64_t range = most;
   const int64_t span = nodes ? nodes : p.ct;  // positions of a workgroup's columns
   if (window && window + span < range) range = window + span;
-  const int64_t blocks = range / 32 + 2;
+  const int64_t blocks = p.blocks = range / 32 + 2;
   // Chunks as large as leave 768 workgroups, one and a half rounds of two a CU, so that sequences of different lengths end
   // together (one token each, us for 512, 768 and 1024: 64 sequences of up to 8000 tokens 135, 121, 119; 4 of 131072 179,
   // 159, 154; 64 of 4000 94, 86, 91; one of 100000 41, 49, 53); at least two blocks a wave, whose start takes longer than
@@ -963,9 +972,7 @@ inline Plan make_plan(int64_t tokens, int64_t seqs, int heads, int group, int di
     p.chunk = (int)(want < least ? least : want);
   else  // as many as fill the chip, no more: each writes its columns' sums
     p.chunk = (int)(p.slots * heads >= 256 ? blocks : want < 16 ? 16 : want);
-  p.chunks = (int)((blocks + p.chunk - 1) / p.chunk);
-  if (p.chunks <= 1) p.chunks = 1;
-  p.part = p.chunks > 1 ? p.slots * heads * p.chunks * (int64_t)(p.ct * (64 * p.nd + 2)) : 0;
+  p.set_chunks(heads);
   return p;
 }
 
@@ -973,9 +980,8 @@ template <bool TREE, int TYPE, int ND>
 int launch(const KvCache& c, const Attend& a, const Plan& p, hipStream_t st) {
   const dim3 grid((unsigned)p.slots, (unsigned)c.heads, (unsigned)p.chunks), block(THREADS);
   if (p.prompt) {  // heads first: the workgroups of one XCD (every eighth) then read few heads' keys and values
-    const int64_t turns = cdiv(p.slots, 65535);
     hipLaunchKernelGGL((prompt_kernel<TREE, TYPE, ND>),
-                       dim3((unsigned)c.heads, (unsigned)cdiv(p.slots, turns), (unsigned)(p.chunks * turns)),
+                       dim3((unsigned)c.heads, (unsigned)cdiv(p.slots, p.turns), (unsigned)(p.chunks * p.turns)),
                        dim3(64 * PWAVES), 0, st, c, a);
   } else {
     hipLaunchKernelGGL((attend_kernel<TREE, TYPE, ND>), grid, block, 0, st, c, a);
@@ -1007,16 +1013,10 @@ bool attend_ok(int64_t tokens, int64_t seqs, int32_t heads, int32_t group, int32
          group <= 65535 && tokens * group < ((int64_t)1 << 31) && window <= 0x3fffffff;
 }
 
-// A call's arguments checked, and its launches: those of the C entries.
-template <bool TREE>
-int attend(const KvCache& c, Attend a, const void* q, int64_t q_token, int64_t q_head, int32_t group, int32_t type, double scale,
-           int64_t window, void* out, int64_t out_token, int64_t out_head, float* lse, void* work, int64_t work_bytes,
-           void* stream) {
-  const int64_t most = (int64_t)c.width * c.page;
-  if (!attend_ok(c.tokens, c.seqs, c.heads, group, c.dim, most, window)) return GPTQ2D_EINVAL;
-  if (c.tokens == 0) return 0;
-  const Plan p = make_plan(c.tokens, c.seqs, c.heads, group, c.dim, most, window, 32 * (int64_t)a.words);
-  if (p.slots > 0x7fffffff || p.chunks * (p.prompt ? cdiv(p.slots, 65535) : 1) > 65535) return GPTQ2D_EUNSUPPORTED;
+// The call's plan and operands in `a`; an error code where they do not do.  first_axis: the slots are the grid's.
+inline int set_call(Attend& a, const Plan& p, bool first_axis, const void* q, int64_t q_token, int64_t q_head, int32_t group, double scale,
+                    int64_t window, void* out, int64_t out_token, int64_t out_head, float* lse, void* work, int64_t work_bytes) {
+  if (p.slots > 0x7fffffff || p.chunks * (first_axis ? 1 : p.turns) > 65535) return GPTQ2D_EUNSUPPORTED;
   if (work_bytes < 4 * p.part || (p.part && (!work || (uintptr_t)work % 16))) return GPTQ2D_ESCRATCH;
   a.q = q, a.q_token = q_token, a.q_head = q_head;
   a.out = out, a.out_token = out_token, a.out_head = out_head;
@@ -1026,16 +1026,7 @@ int attend(const KvCache& c, Attend a, const void* q, int64_t q_token, int64_t q
   a.group = group;
   a.window = (int)window;
   a.chunk = p.chunk, a.chunks = p.chunks;
-  const hipStream_t st = (hipStream_t)stream;
-  switch (type) {
-    case TYPE_F32:
-      return launch_type<TREE, TYPE_F32>(c, a, p, st);
-    case TYPE_BF16:
-      return launch_type<TREE, TYPE_BF16>(c, a, p, st);
-    case TYPE_F16:
-      return launch_type<TREE, TYPE_F16>(c, a, p, st);
-  }
-  return GPTQ2D_EINVAL;
+  return 0;
 }
 
 }  // namespace
