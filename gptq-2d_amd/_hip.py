@@ -128,8 +128,9 @@ def lib() -> ctypes.CDLL:
         handle.gptq2d_draft_accept.restype = ctypes.c_int
         handle.gptq2d_kv_page_words.argtypes = [_I32, _I32, _I32]
         handle.gptq2d_kv_page_words.restype = ctypes.c_int64
-        handle.gptq2d_rotary.argtypes = [_I32, _P, _P, _AP, _AP, _I32, _I64, _I64, _I32, _I32, _I32, _P, _F64, _P, _I32, _I64,
-                                         _I64, _I32, _P]
+        part = [_P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I32]  # x and its strides, y and its strides, heads
+        handle.gptq2d_rotary.argtypes = [*part, *part, _I32, _I64, _I64, _I32, _I32, _I32, _P, _F64, _P, _I32, _I64, _I64, _I32,
+                                         _P]
         handle.gptq2d_rotary.restype = ctypes.c_int
         handle.gptq2d_page_pool.argtypes = [_P, _I64, _I64, _I64, _I32, _I64, _P, _P, _P, _P, _P, _P, _I32, _I64, _P, _P, _P,
                                             _P, _P, _I64, _P]
@@ -159,14 +160,24 @@ def call_untyped(name: str, *args) -> None:
 def launch(name: str, device: torch.device, *args) -> None:
     """Call ``gptq2d_<name>`` with ``device`` current and its current stream as the last argument, and raise on a non-zero
     return code."""
-    fn = getattr(lib(), f"gptq2d_{name}")
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    fn = getattr(lib(), "gptq2d_" + name)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, raw_stream(index))
     if rc:
         raise GPTQ2DError(f"gptq2d_{name} failed with code {rc}")
+
+
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The handle of a device's current stream.  torch.cuda.current_stream makes an object of it, 2 us a call; the function that the
+# code torch.compile writes calls gives the handle alone.
+raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
 def function(name: str, dtype: torch.dtype):

@@ -200,25 +200,22 @@ int launch(Rotate& a, bool interleaved, hipStream_t st) {
 
 }  // namespace
 
-extern "C" int gptq2d_rotary(int32_t count, const void* const* x, void* const* y, const int64_t* heads, const int64_t* strides,
-                             int32_t type, int64_t outer, int64_t inner, int32_t dim, int32_t rotated, int32_t interleaved,
-                             const double* turns, double amplitude, const void* positions, int32_t wide, int64_t pos_outer,
-                             int64_t pos_inner, int32_t back, void* stream) {
-  if (count < 1 || count > PARTS || outer < 0 || inner < 0 || dim < 2 || dim > 1 << 20 || rotated < 2 || rotated > dim ||
+extern "C" int gptq2d_rotary(const void* x0, int64_t x0_outer, int64_t x0_token, int64_t x0_head, void* y0, int64_t y0_outer,
+                             int64_t y0_token, int64_t y0_head, int32_t heads0, const void* x1, int64_t x1_outer,
+                             int64_t x1_token, int64_t x1_head, void* y1, int64_t y1_outer, int64_t y1_token, int64_t y1_head,
+                             int32_t heads1, int32_t type, int64_t outer, int64_t inner, int32_t dim, int32_t rotated,
+                             int32_t interleaved, const double* turns, double amplitude, const void* positions, int32_t wide,
+                             int64_t pos_outer, int64_t pos_inner, int32_t back, void* stream) {
+  if (heads0 < 0 || heads0 > 1 << 20 || heads1 < 0 || heads1 > 1 << 20 || outer < 0 || inner < 0 || dim < 2 || dim > 1 << 20 || rotated < 2 || rotated > dim ||
       rotated % 2)
     return GPTQ2D_EINVAL;
   if (outer > 0x7fffffff || inner > 0x7fffffff) return GPTQ2D_EUNSUPPORTED;
   Rotate a = {};
-  int64_t all = 0;
-  for (int i = 0; i < count; ++i) {
-    const int64_t* s = strides + 6 * i;
-    if (heads[i] < 0 || heads[i] > 1 << 20) return GPTQ2D_EINVAL;
-    a.part[i] = {x[i], y[i], (int)heads[i], s[0], s[1], s[2], s[3], s[4], s[5]};
-    all += heads[i];
-  }
-  if (outer * inner == 0 || all == 0) return 0;
+  a.part[0] = {x0, y0, heads0, x0_outer, x0_token, x0_head, y0_outer, y0_token, y0_head};
+  a.part[1] = {x1, y1, heads1, x1_outer, x1_token, x1_head, y1_outer, y1_token, y1_head};
+  if (outer * inner == 0 || heads0 + heads1 == 0) return 0;
   if (outer * inner >= (int64_t)1 << 32) return GPTQ2D_EUNSUPPORTED;
-  a.heads = (int)all;
+  a.heads = heads0 + heads1;
   a.outer = outer, a.inner = inner, a.dim = dim, a.rotated = rotated;
   a.turns = turns, a.amplitude = (float)amplitude;
   a.positions = positions, a.wide = wide != 0, a.pos_outer = pos_outer, a.pos_inner = pos_inner;

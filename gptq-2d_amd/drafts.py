@@ -58,7 +58,6 @@ class DraftTree:
         _hip.launch("draft_tree", self.device, parents.data_ptr(), offsets.data_ptr(), held.data_ptr(), seqs, self.tokens, nodes,
                     self.ancestors.data_ptr(), self.positions.data_ptr())
 
-    @torch.no_grad()
     def accept(self, drafted: torch.Tensor, chosen: torch.Tensor) -> Accepted:
         """From node 0 of each sequence, each time to the first child whose ``drafted`` token is the one ``chosen`` after its
         parent (both [tokens], int32 or int64)."""

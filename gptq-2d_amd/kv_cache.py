@@ -85,16 +85,15 @@ class KVCache4:
         return x if x.stride(2) == 1 or self.head_dim == 1 else x.contiguous()
 
     def _call(self, fn, name, *args):
-        device = self.device
-        if torch.cuda.current_device() == device.index:
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+        index = self.device.index
+        if torch.cuda.current_device() == index:
+            rc = fn(*args, _hip.raw_stream(index))
         else:
-            with torch.cuda.device(device):
-                rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            with torch.cuda.device(index):
+                rc = fn(*args, _hip.raw_stream(index))
         if rc:
             raise _hip.GPTQ2DError(f"gptq2d_kv_{name} failed with code {rc}")
 
-    @torch.no_grad()
     def append(self, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
                offsets: torch.Tensor | None = None) -> None:
         """Put keys and values [tokens, kv_heads, head_dim] (fp32, bf16 or fp16) into the cache: sequence b's at positions
@@ -107,7 +106,6 @@ class KVCache4:
         self._call(self._append, "append", *self._cache, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
                    v.stride(0), v.stride(1), kind, *self._sequences(table, lengths, offsets, k.size(0)))
 
-    @torch.no_grad()
     def read(self, table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None, *,
              tokens: int | None = None, dtype: torch.dtype = torch.float32) -> tuple[torch.Tensor, torch.Tensor]:
         """The values [tokens, kv_heads, head_dim] that the last tokens of each sequence are held as, keys and values:
@@ -127,7 +125,6 @@ class KVCache4:
                    v.stride(1), kind, *self._sequences(table, lengths, offsets, tokens))
         return k, v
 
-    @torch.no_grad()
     def attend(self, q: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor | None = None, *,
                scale: float | None = None, window: int | None = None, return_lse: bool = False, tree: DraftTree | None = None):
         """Causal attention of q [tokens, heads, head_dim] (fp32, bf16 or fp16; heads a multiple of kv_heads, consecutive
@@ -172,7 +169,6 @@ class KVCache4:
                    None if lse is None else lse.data_ptr(), None if work is None else work.data_ptr(), size)
         return (out, lse) if return_lse else out
 
-    @torch.no_grad()
     def keep(self, table: torch.Tensor, lengths: torch.Tensor, offsets: torch.Tensor, path: torch.Tensor,
              counts: torch.Tensor) -> None:
         """Of each sequence's last tokens, the nodes of a tree, put those that were accepted where the nodes begin: node

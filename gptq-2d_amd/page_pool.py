@@ -67,28 +67,24 @@ class PagePool:
             raise ValueError(f"{name} must be a contiguous int32 [{self.lengths.numel()}] on the pool's device")
         return t.data_ptr()
 
-    @torch.no_grad()
     def resize(self, lengths: torch.Tensor) -> None:
         """Pages for ``lengths[b]`` tokens of sequence b (int32; below 0 counts as 0, at most 2^30), no more and no fewer."""
         _hip.launch("page_pool", self.device, *self._state, self._request(lengths, "lengths"), False, 0, None, None, None, None,
               *self._scratch)
 
-    @torch.no_grad()
     def extend(self, new: torch.Tensor, *, tokens: int) -> Rows:
         """Pages for ``new[b]`` more tokens of sequence b (int32; below 0 counts as 0), and their rows.  ``tokens``: rows in all,
         at least the sum of ``new`` (which is not read on the host); more where a batch is padded."""
         if not 0 <= tokens < 1 << 31:
             raise ValueError("tokens must be a number of rows below 2^31")
-        whole = dict(dtype=torch.int32, device=self.device)
-        seqs = self.lengths.numel()
-        rows = Rows(torch.empty(seqs + 1, **whole), torch.empty(seqs, **whole), torch.empty(tokens, **whole),
-                    torch.empty(tokens, dtype=torch.int64, device=self.device))
+        device, seqs = self.device, self.lengths.size(0)
+        rows = Rows(torch.empty(seqs + 1, dtype=torch.int32, device=device), torch.empty(seqs, dtype=torch.int32, device=device),
+                    torch.empty(tokens, dtype=torch.int32, device=device), torch.empty(tokens, dtype=torch.int64, device=device))
         _hip.launch("page_pool", self.device, *self._state, self._request(new, "new"), True, tokens, *(t.data_ptr() for t in rows),
               *self._scratch)
         return rows
 
 
-@torch.no_grad()
 def row_positions(held: torch.Tensor, offsets: torch.Tensor, tokens: int) -> torch.Tensor:
     """Positions [tokens] (int32) of packed rows whose sequence b, rows ``offsets[b]`` to ``offsets[b + 1] - 1`` (int32 [B + 1]),
     follows ``held[b]`` tokens (int32 [B]); 0 for rows that no sequence has."""

@@ -23,6 +23,7 @@ import torch
 import _hip
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_NO_PART = (None, 0, 0, 0, None, 0, 0, 0, 0)
 
 
 class Linear(NamedTuple):
@@ -111,7 +112,7 @@ class Rotary:
         self.dim, self.rotated, self.interleaved, self.amplitude = dim, rotated, bool(interleaved), float(amplitude)
         self.turns = torch.tensor([float(f) / (2 * math.pi) for f in frequencies], dtype=torch.float64, device=device)
         _hip.require_device(self.turns)
-        self.device = self.turns.device
+        self.device, self._turns = self.turns.device, self.turns.data_ptr()
 
     def __call__(self, *xs: torch.Tensor, positions: torch.Tensor):
         """One or two tensors (queries, keys) [..., heads, dim] of one type (fp32, bf16 or fp16) rotated, each with its own
@@ -119,18 +120,20 @@ class Rotary:
         or two ([tokens], [batch, tokens]); a position may be negative and counts to 2^53."""
         if not 1 <= len(xs) <= 2:
             raise ValueError("one or two tensors are rotated in a call")
-        lead = xs[0].shape[:-2]
+        first = xs[0]
+        lead, kind = first.shape[:-2], first.dtype
         for x in xs:
             if x.dim() not in (3, 4) or x.size(-1) != self.dim or x.shape[:-2] != lead:
                 raise ValueError(f"tensors must be [tokens, heads, {self.dim}] or [batch, tokens, heads, {self.dim}], alike but "
                                  f"for the heads; got {[tuple(x.shape) for x in xs]}")
-            if x.dtype not in _TYPES or x.dtype is not xs[0].dtype:
+            if x.dtype is not kind or kind not in _TYPES:
                 raise ValueError("tensors must be all float32, bfloat16 or float16")
             if x.device != self.device:
                 raise ValueError("tensors must be on the rotation's device")
         if positions.dtype not in (torch.int32, torch.int64) or positions.device != self.device:
             raise ValueError("positions must be int32 or int64 on the rotation's device")
-        if positions.dim() > len(lead) or any(a != b and a != 1 for a, b in zip(positions.shape[::-1], lead[::-1])):
+        if positions.shape != lead and (positions.dim() > len(lead) or
+                                        any(a != b and a != 1 for a, b in zip(positions.shape[::-1], lead[::-1]))):
             raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to {tuple(lead)}")
         if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
             out = _Rotation.apply(self, False, positions, *xs)
@@ -140,20 +143,25 @@ class Rotary:
 
     def _rotate(self, xs, positions, back):
         lead = xs[0].shape[:-2]
-        outer, inner = (1, *lead) if len(lead) == 1 else lead
-        p = positions.expand(lead)
-        p_strides = (0, *p.stride()) if len(lead) == 1 else p.stride()
-        xs = [x if x.stride(-1) == 1 else x.contiguous() for x in xs]
-        out = tuple(torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs)
-        strides = []
-        for t in (t for pair in zip(xs, out) for t in pair):
-            strides += (0, *t.stride()[:2]) if len(lead) == 1 else t.stride()[:3]
-        count = len(xs)
-        _hip.launch("rotary", self.device, count, (_hip._P * count)(*(x.data_ptr() for x in xs)), (_hip._P * count)(*(y.data_ptr() for y in out)),
-                _hip.i64_array([x.size(-2) for x in xs]), _hip.i64_array(strides), _TYPES[xs[0].dtype], outer, inner, self.dim,
-                self.rotated, self.interleaved, self.turns.data_ptr(), self.amplitude, p.data_ptr(),
-                    p.dtype is torch.int64, *p_strides, back)
-        return out
+        p = positions if positions.shape == lead else positions.expand(lead)
+        outer, inner = (1, lead[0]) if len(lead) == 1 else lead
+        p_outer, p_inner = (0, p.stride(0)) if len(lead) == 1 else p.stride()
+        out, parts, kept = [], [], []
+        for x in xs:
+            if x.stride(-1) != 1:
+                x = x.contiguous()
+                kept.append(x)
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
+            out.append(y)
+            if len(lead) == 1:
+                parts += (x.data_ptr(), 0, x.stride(0), x.stride(1), y.data_ptr(), 0, y.stride(0), y.stride(1), x.size(1))
+            else:
+                parts += (x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3], x.size(2))
+        if len(xs) == 1:
+            parts += _NO_PART
+        _hip.launch("rotary", self.device, *parts, _TYPES[xs[0].dtype], outer, inner, self.dim, self.rotated, self.interleaved,
+                    self._turns, self.amplitude, p.data_ptr(), p.dtype is torch.int64, p_outer, p_inner, back)
+        return tuple(out)
 
 
 class _Rotation(torch.autograd.Function):

@@ -406,14 +406,15 @@ int gptq2d_packed_linear(const void* x, int64_t x_token, int32_t type, int64_t t
 /* Rotary positions (no reference counterpart).  Of the first `rotated` (even) of a head's dim elements, pair i, (x[i], x[i +
  * rotated / 2]) or with interleaved (x[2 i], x[2 i + 1]), is turned by t = position turns[i] whole turns (fp64, [rotated / 2]):
  *   y1 = amplitude (x1 cos t - x2 sin t),  y2 = amplitude (x2 cos t + x1 sin t),
- * with back != 0 by -t (the transpose, for gradients); the other elements are copied.  count: 1 or 2 tensors x[i] [outer,
- * inner, heads[i], dim] of `type` (0: fp32, 1: bf16, 2: fp16) and their results y[i] (which may be x[i], strides and all);
- * strides[6 i ..]: of x[i] (outer, inner, head), of y[i] likewise, in elements, last axes contiguous.  x, y, heads and strides
- * are host arrays.  positions: int32, or int64 with wide != 0, at outer pos_outer + inner pos_inner. */
-int gptq2d_rotary(int32_t count, const void* const* x, void* const* y, const int64_t* heads, const int64_t* strides,
-                  int32_t type, int64_t outer, int64_t inner, int32_t dim, int32_t rotated, int32_t interleaved,
-                  const double* turns, double amplitude, const void* positions, int32_t wide, int64_t pos_outer,
-                  int64_t pos_inner, int32_t back, void* stream);
+ * with back != 0 by -t (the transpose, for gradients); the other elements are copied.  One or two tensors x [outer, inner,
+ * heads, dim] of `type` (0: fp32, 1: bf16, 2: fp16) with their results y (which may be x, strides and all): strides in elements,
+ * last axes contiguous; heads 0: none.  positions: int32, or int64 with wide != 0, at outer pos_outer + inner pos_inner. */
+int gptq2d_rotary(const void* x0, int64_t x0_outer, int64_t x0_token, int64_t x0_head, void* y0, int64_t y0_outer,
+                  int64_t y0_token, int64_t y0_head, int32_t heads0, const void* x1, int64_t x1_outer, int64_t x1_token,
+                  int64_t x1_head, void* y1, int64_t y1_outer, int64_t y1_token, int64_t y1_head, int32_t heads1, int32_t type,
+                  int64_t outer, int64_t inner, int32_t dim, int32_t rotated, int32_t interleaved, const double* turns,
+                  double amplitude, const void* positions, int32_t wide, int64_t pos_outer, int64_t pos_inner, int32_t back,
+                  void* stream);
 
 /* The pages of a cache dealt to sequences (no reference counterpart).  State, all int32: table[seqs][width] (rows table_stride
  * apart, -1: no page), owned[seqs] (the first entries of a row are the sequence's pages), lengths[seqs] (tokens), missing[seqs]
