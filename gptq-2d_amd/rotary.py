@@ -88,15 +88,15 @@ def rotary_frequencies(rotated: int, base: float = 10000., scaling: Linear | Ntk
 
 
 class Rotary:
-    """Rotation of heads of ``dim`` elements, of which the first ``rotated`` (even; None: all) turn.  ``frequencies``: radians
+    """Rotation of heads of ``dim`` elements (2 to 1024), of which the first ``rotated`` (even; None: all) turn.  ``frequencies``: radians
     a position of each pair, in the place of those that ``base`` and ``scaling`` give."""
 
     def __init__(self, dim: int, *, base: float = 10000., rotated: int | None = None, interleaved: bool = False,
                  scaling: Linear | Ntk | Bands | Yarn | None = None, frequencies: Sequence[float] | None = None,
                  device: torch.device | str = "cuda"):
         rotated = dim if rotated is None else rotated
-        if not 2 <= rotated <= dim <= 1 << 20 or rotated % 2:
-            raise ValueError(f"an even number of a head's {dim} elements turns, at least 2, not {rotated}")
+        if not 2 <= rotated <= dim <= 1024 or rotated % 2:
+            raise ValueError(f"an even number of a head's {dim} elements turns, at least 2 (of at most 1024), not {rotated}")
         if frequencies is None:
             if base <= 1 or (scaling is not None and scaling.factor <= 0):
                 raise ValueError("the base must be above 1 and a scaling's factor above 0")
@@ -130,6 +130,8 @@ class Rotary:
                 raise ValueError("tensors must be all float32, bfloat16 or float16")
             if x.device != self.device:
                 raise ValueError("tensors must be on the rotation's device")
+            if x.size(-2) > 0x7fff:
+                raise ValueError("a tensor has at most 32767 heads")
         if positions.dtype not in (torch.int32, torch.int64) or positions.device != self.device:
             raise ValueError("positions must be int32 or int64 on the rotation's device")
         if positions.shape != lead and (positions.dim() > len(lead) or

@@ -403,12 +403,12 @@ int gptq2d_packed_linear(const void* x, int64_t x_token, int32_t type, int64_t t
                          const int32_t* index, int64_t adapters, int64_t rank, void* y, int64_t y_token, void* work,
                          int64_t work_bytes, void* stream);
 
-/* Rotary positions (no reference counterpart).  Of the first `rotated` (even) of a head's dim elements, pair i, (x[i], x[i +
+/* Rotary positions (no reference counterpart).  Of the first `rotated` (even) of a head's dim (at most 1024) elements, pair i, (x[i], x[i +
  * rotated / 2]) or with interleaved (x[2 i], x[2 i + 1]), is turned by t = position turns[i] whole turns (fp64, [rotated / 2]):
  *   y1 = amplitude (x1 cos t - x2 sin t),  y2 = amplitude (x2 cos t + x1 sin t),
  * with back != 0 by -t (the transpose, for gradients); the other elements are copied.  One or two tensors x [outer, inner,
  * heads, dim] of `type` (0: fp32, 1: bf16, 2: fp16) with their results y (which may be x, strides and all): strides in elements,
- * last axes contiguous; heads 0: none.  positions: int32, or int64 with wide != 0, at outer pos_outer + inner pos_inner. */
+ * last axes contiguous; heads (at most 32767) 0: none.  positions: int32, or int64 with wide != 0, at outer pos_outer + inner pos_inner. */
 int gptq2d_rotary(const void* x0, int64_t x0_outer, int64_t x0_token, int64_t x0_head, void* y0, int64_t y0_outer,
                   int64_t y0_token, int64_t y0_head, int32_t heads0, const void* x1, int64_t x1_outer, int64_t x1_token,
                   int64_t x1_head, void* y1, int64_t y1_outer, int64_t y1_token, int64_t y1_head, int32_t heads1, int32_t type,

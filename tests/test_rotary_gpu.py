@@ -46,7 +46,7 @@ def check(got, want, dtype):
 
 
 SHAPES = [(128, 128, False), (128, 128, True), (80, 44, True), (80, 44, False), (64, 2, False), (2, 2, True), (3, 2, False),
-          (250, 250, False), (256, 192, True), (37, 36, False), (37, 20, True)]
+          (250, 250, False), (256, 192, True), (37, 36, False), (37, 20, True), (1024, 1024, False), (1024, 6, True)]
 
 
 @pytest.mark.gpu
@@ -57,7 +57,7 @@ def test_rotation(dtype, dim, rotated, interleaved):
     g = torch.Generator().manual_seed(dim)
     rot = R.Rotary(dim, rotated=rotated, interleaved=interleaved)
     f, a = R.rotary_frequencies(rotated)
-    for tokens, hq, hkv in ((1, 1, 1), (7, 5, 1), (300, 12, 3), (0, 4, 4), (33, 64, 8)):
+    for tokens, hq, hkv in ((1, 1, 1), (7, 5, 1), (300, 12, 3), (0, 4, 4), (33, 64, 8), (1500, 1, 1)):
         x = torch.randn(tokens, hq + 2 * hkv, dim, generator=g).to(DEV, TYPES[dtype])
         q, k = x[:, :hq], x[:, hq:hq + hkv]  # strided parts of one projection's result
         positions = torch.randint(0, 200000, (tokens,), generator=g).to(DEV, torch.int32)
@@ -193,6 +193,8 @@ def test_captured_and_on_another_stream():
 def test_refusals():
     x = torch.zeros(4, 2, 8, device=DEV)
     p = torch.zeros(4, dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError):
+        R.Rotary(1026)
     for kw in (dict(rotated=3), dict(rotated=0), dict(rotated=10), dict(base=1.), dict(scaling=R.Linear(0.)), dict(frequencies=[1.]),
                dict(scaling=R.Bands(2., 100, 4., 4.)), dict(scaling=R.Yarn(2., 0)), dict(scaling=R.Linear(2.), frequencies=[1.] * 4)):
         with pytest.raises(ValueError):
