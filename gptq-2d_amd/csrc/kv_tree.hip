@@ -132,6 +132,13 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
   }
 }
 
+// The slot of a workgroup of grid (heads, a multiple of 4, ...).  Slots without columns come in patterns (every second one where a
+// sequence's columns fill theirs), and neighbours are dealt to the XCD's parts in turn: a quarter of the slots each, or some parts
+// would have nothing to do (64 sequences of 32 columns: 185 us, so 145).
+__device__ __forceinline__ int64_t slot_of(int turn) {
+  return (blockIdx.y & 3) * (gridDim.y >> 2) + (blockIdx.y >> 2) + (int64_t)gridDim.y * turn;
+}
+
 template <int TYPE, int ND>
 __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <= 2 ? 3 : 2) void shared_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
@@ -143,11 +150,9 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
   __shared__ int shifts[RINGS][2];        // and whether columns part in the lowest bit
   __shared__ float tops[SWAVES][16], ls[COLS][16];
   static_assert(S * R::STAGE >= COLS * 4 * ND * 1024, "a ring's sums fit where its blocks were");
-  // Heads first: the workgroups of one XCD (every eighth) read few heads' keys and values.  Slots without columns come in
-  // patterns (every second one where a sequence's columns fill theirs), and neighbours are dealt to the XCD's parts in turn: a
-  // quarter of the slots each, or some parts would have nothing to do (64 sequences of 32 columns: 185 us, so 145).
+  // heads first: the workgroups of one XCD (every eighth) read few heads' keys and values
   const int head = blockIdx.x, part = blockIdx.z % a.chunks;
-  const int64_t slot = (blockIdx.y & 3) * (gridDim.y >> 2) + (blockIdx.y >> 2) + (int64_t)gridDim.y * (blockIdx.z / a.chunks);
+  const int64_t slot = slot_of(blockIdx.z / a.chunks);
   const int64_t seq = kv_find(c, slot, a.group, CT, 1);
   const int64_t first_slot = kv_first_slot(c, seq, a.group, CT, 1);
   if (part == 0) clear_others<T>(c, a, head, seq, slot, first_slot, CT);
@@ -330,6 +335,78 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
   }
 }
 
+// Joins the chunks' results of shared_kernel: a workgroup a slot and head, its 32 columns at once, so that what is looked up (the
+// sequence, its chunks, their maxima) is looked up once.  64 sequences of 8 nodes, 32 heads of 128, up to 6 chunks: 9 us (a wave
+// a column, as join_kernel, 19).
+template <int TYPE, int ND>
+__global__ __launch_bounds__(THREADS) void join_tile_kernel(KvCache c, Attend a) {
+  typedef typename Elem<TYPE>::T T;
+  constexpr int CT = SCT, DP = 64 * ND, SIZE = CT * (DP + 2), PER = THREADS / CT, ITEMS = CT * 16 * ND / THREADS, PIECE = 32;
+  __shared__ float factors[PIECE][CT], tops[CT], sums[CT];
+  const int head = blockIdx.x;
+  const int64_t slot = slot_of(blockIdx.z);
+  const int64_t seq = kv_find(c, slot, a.group, CT, 1), first_slot = kv_first_slot(c, seq, a.group, CT, 1);
+  if (slot < first_slot || (slot - first_slot) * CT > 0x7fffff00) return;
+  const Tile t = make_tile<true>(c, a, seq, (int)((slot - first_slot) * CT), CT);
+  if (t.col0 >= t.cols || t.chunks <= 1) return;
+  const float* part = a.part + (slot * c.heads + head) * (int64_t)a.chunks * SIZE;
+  const int cols = t.cols - t.col0 < CT ? t.cols - t.col0 : CT;
+  // the largest of each column's references, by PER threads
+  const int col = threadIdx.x / PER, j = threadIdx.x % PER;
+  const float* mine = part + CT * DP + (col < cols ? col : 0);
+  float top = -__builtin_inff(), l = 0.f;
+  for (int i = j; i < t.chunks; i += PER) {
+    const float x = mine[(int64_t)i * SIZE];
+    top = x > top || x != x ? x : top;
+  }
+#pragma unroll
+  for (int s = 1; s < PER; s *= 2) {
+    const float x = __shfl_xor(top, s);
+    top = x > top || x != x ? x : top;
+  }
+  floatx4 sum[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) sum[k] = (floatx4){0.f, 0.f, 0.f, 0.f};
+  for (int i0 = 0; i0 < t.chunks; i0 += PIECE) {
+    const int n = t.chunks - i0 < PIECE ? t.chunks - i0 : PIECE;
+    for (int i = j; i < n; i += PER) {
+      const float* at = mine + (int64_t)(i0 + i) * SIZE;
+      const float x = at[0], f = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - top);
+      l += f * at[CT];
+      factors[i][col] = f;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const floatx4* from = reinterpret_cast<const floatx4*>(part + (int64_t)(i0 + i) * SIZE);
+#pragma unroll
+      for (int k = 0; k < ITEMS; ++k) {  // columns past the sequence's are not written: the first one's in their place
+        const int u = threadIdx.x + THREADS * k, in = u / (16 * ND);
+        sum[k] += factors[i][in] * from[in < cols ? u : u % (16 * ND)];
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int s = 1; s < PER; s *= 2) l += __shfl_xor(l, s);
+  if (j == 0) tops[col] = top, sums[col] = l;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    const int u = threadIdx.x + THREADS * k, in = u / (16 * ND), d = 4 * (u % (16 * ND));
+    if (in >= cols) continue;
+    const int at = t.col0 + in, hq = head * a.group + at % a.group;
+    const int64_t row = t.row + at / a.group;
+    const float total = sums[in], f = total == 0.f ? 0.f : 1.f / total;
+    T* out = (T*)a.out + row * a.out_token + hq * a.out_head + d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < c.dim) out[i] = from_f32<TYPE>(f == 0.f ? 0.f : sum[k][i] * f);
+    if (a.lse && d == 0)
+      a.lse[row * (int64_t)(c.heads * a.group) + hq] = total == 0.f ? -__builtin_inff() : (tops[in] + __builtin_log2f(total)) * LN2;
+  }
+}
+
 // How a call is split: by attend_kernel or prompt_kernel as gptq2d_kv_attend's, or by shared_kernel.
 struct TreePlan : Plan {
   bool shared;
@@ -366,8 +443,8 @@ int launch_shared(const KvCache& c, const Attend& a, const TreePlan& p, hipStrea
   const dim3 grid((unsigned)c.heads, (unsigned)(4 * cdiv(p.slots, 4 * p.turns)), (unsigned)(p.chunks * p.turns));
   hipLaunchKernelGGL((shared_kernel<TYPE, ND>), grid, dim3(64 * SWAVES), 0, st, c, a);
   if (p.chunks > 1)
-    hipLaunchKernelGGL((join_kernel<true, TYPE, ND>), dim3((unsigned)cdiv(c.tokens * c.heads * a.group, WAVES)), dim3(THREADS), 0,
-                       st, c, a, p.ct);
+    hipLaunchKernelGGL((join_tile_kernel<TYPE, ND>), dim3(grid.x, grid.y, (unsigned)p.turns),
+                       dim3(THREADS), 0, st, c, a);
   return (int)hipGetLastError();
 }
 
