@@ -179,6 +179,9 @@ class _Rotation(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         grads = [g if wanted else None for g, wanted in zip(grads, ctx.needs_input_grad[3:])]
-        there = [g for g in grads if g is not None]
-        turned = iter(_Rotation.apply(ctx.rotary, not ctx.back, ctx.saved_tensors[0], *there) if there else ())
+        there, positions = [g for g in grads if g is not None], ctx.saved_tensors[0]
+        if torch.is_grad_enabled():  # of the gradient too
+            turned = iter(_Rotation.apply(ctx.rotary, not ctx.back, positions, *there) if there else ())
+        else:
+            turned = iter(ctx.rotary._rotate(there, positions, not ctx.back) if there else ())
         return (None, None, None, *(None if g is None else next(turned) for g in grads))

@@ -190,6 +190,36 @@ def test_captured_and_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_captured_training_step():
+    """Forward and backward in one graph, replayed with other inputs."""
+    g = torch.Generator().manual_seed(10)
+    rot = R.Rotary(32, interleaved=True)
+    f, a = R.rotary_frequencies(32)
+    q, k, gq, gk = (torch.randn(9, h, 32, generator=g).to(DEV) for h in (4, 2, 4, 2))
+    q.requires_grad_(), k.requires_grad_()
+    positions = torch.randint(0, 5000, (9,), generator=g).to(DEV)
+
+    def step():
+        return torch.autograd.grad(rot(q, k, positions=positions), (q, k), (gq, gk))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dq, dk = step()
+    for _ in range(3):
+        gq.copy_(torch.randn(9, 4, 32, generator=g))
+        positions.add_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(dq, formula(gq, positions, f, a, 32, True, back=True), torch.float32)
+        check(dk, formula(gk, positions, f, a, 32, True, back=True), torch.float32)
+
+
+@pytest.mark.gpu
 def test_refusals():
     x = torch.zeros(4, 2, 8, device=DEV)
     p = torch.zeros(4, dtype=torch.int32, device=DEV)
