@@ -13,7 +13,8 @@ namespace {
 //     of the values' scales where e & 2), 2^24 out of the sums.  A key is then (q . c) s + z sum q and a value c s + z.  A query's
 //     element is so held to 2^-27 of the largest where that is coarser, and the values' scales may lie 2^4 less apart.  The
 //     matrix cores align products by the exponents that operands are written with, so such sums are good to some 17 bits (fp32
-//     results measured 8e-6 off that way, 2e-7 with centred codes): eight bits finer than bf16, not enough for fp16 and fp32.
+//     results measured 1e-5 off that way, 2e-5 with scores of 30; 1e-7 and 2e-6 with centred codes): eight bits finer than bf16,
+//     not enough for fp16 and fp32.
 // One barrier a block: after it, the stage that was read in the turn before is loaded again.  A workgroup has two rings, with
 // every second block each, whose results are joined at the end; four workgroups a CU.
 constexpr int COLS = 2, RINGS = 2, SWAVES = COLS * RINGS, SCT = 16 * COLS;  // waves of a ring, rings, columns of a workgroup
