@@ -120,24 +120,24 @@ class Rotary:
         or two ([tokens], [batch, tokens]); a position may be negative and counts to 2^53."""
         if not 1 <= len(xs) <= 2:
             raise ValueError("one or two tensors are rotated in a call")
-        first = xs[0]
-        lead, kind = first.shape[:-2], first.dtype
+        lead, kind, device, grad = xs[0].shape[:-2], xs[0].dtype, self.device, False
+        if len(lead) not in (1, 2) or kind not in _TYPES:
+            raise ValueError(f"tensors must be [tokens, heads, {self.dim}] or [batch, tokens, heads, {self.dim}], float32, bfloat16 or "
+                             f"float16; got {tuple(xs[0].shape)} of {kind}")
         for x in xs:
-            if x.dim() not in (3, 4) or x.size(-1) != self.dim or x.shape[:-2] != lead:
-                raise ValueError(f"tensors must be [tokens, heads, {self.dim}] or [batch, tokens, heads, {self.dim}], alike but "
-                                 f"for the heads; got {[tuple(x.shape) for x in xs]}")
-            if x.dtype is not kind or kind not in _TYPES:
-                raise ValueError("tensors must be all float32, bfloat16 or float16")
-            if x.device != self.device:
-                raise ValueError("tensors must be on the rotation's device")
-            if x.size(-2) > 0x7fff:
-                raise ValueError("a tensor has at most 32767 heads")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != self.device:
+            shape = x.shape
+            if shape[-1] != self.dim or shape[:-2] != lead or shape[-2] > 0x7fff:
+                raise ValueError(f"tensors must have heads of {self.dim} elements, at most 32767 of them, and the same axes before "
+                                 f"these; got {[tuple(x.shape) for x in xs]}")
+            if x.dtype is not kind or x.device != device:
+                raise ValueError("tensors must be of one type, on the rotation's device")
+            grad = grad or x.requires_grad
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != device:
             raise ValueError("positions must be int32 or int64 on the rotation's device")
         if positions.shape != lead and (positions.dim() > len(lead) or
                                         any(a != b and a != 1 for a, b in zip(positions.shape[::-1], lead[::-1]))):
             raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to {tuple(lead)}")
-        if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+        if grad and torch.is_grad_enabled():
             out = _Rotation.apply(self, False, positions, *xs)
         else:
             out = self._rotate(xs, positions, False)
@@ -146,19 +146,24 @@ class Rotary:
     def _rotate(self, xs, positions, back):
         lead = xs[0].shape[:-2]
         p = positions if positions.shape == lead else positions.expand(lead)
-        outer, inner = (1, lead[0]) if len(lead) == 1 else lead
-        p_outer, p_inner = (0, p.stride(0)) if len(lead) == 1 else p.stride()
-        out, parts, kept = [], [], []
+        batched = len(lead) == 2
+        outer, inner = lead if batched else (1, lead[0])
+        p_outer, p_inner = p.stride() if batched else (0, p.stride(0))
+        out, parts, kept = [], [], []  # kept: copies, until the launch
         for x in xs:
-            if x.stride(-1) != 1:
+            strides = x.stride()
+            if strides[-1] != 1:
                 x = x.contiguous()
+                strides = x.stride()
                 kept.append(x)
+            heads = x.size(-2)
             y = torch.empty_like(x, memory_format=torch.contiguous_format)
             out.append(y)
-            if len(lead) == 1:
-                parts += (x.data_ptr(), 0, x.stride(0), x.stride(1), y.data_ptr(), 0, y.stride(0), y.stride(1), x.size(1))
+            row = heads * self.dim  # of y, which is contiguous
+            if batched:
+                parts += (x.data_ptr(), *strides[:3], y.data_ptr(), inner * row, row, self.dim, heads)
             else:
-                parts += (x.data_ptr(), *x.stride()[:3], y.data_ptr(), *y.stride()[:3], x.size(2))
+                parts += (x.data_ptr(), 0, strides[0], strides[1], y.data_ptr(), 0, row, self.dim, heads)
         if len(xs) == 1:
             parts += _NO_PART
         _hip.launch("rotary", self.device, *parts, _TYPES[xs[0].dtype], outer, inner, self.dim, self.rotated, self.interleaved,
