@@ -35,6 +35,8 @@ struct Attend {
   const unsigned* seen;  // trees: bits of the nodes that each token sees, `words` of 32 a token
   const int32_t* at;     // and the token's position
   int words;
+  int4* list;            // and of many sequences the pieces of the work,
+  int pieces, parts;     // those of a head, and of its partial results, at most
 };
 
 // What a workgroup's columns (token, query head of the group) are, and the blocks of 32 keys that they see.

@@ -133,11 +133,169 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
   }
 }
 
-// The slot of a workgroup of grid (heads, a multiple of 4, ...).  Slots without columns come in patterns (every second one where a
-// sequence's columns fill theirs), and neighbours are dealt to the XCD's parts in turn: a quarter of the slots each, or some parts
-// would have nothing to do (64 sequences of 32 columns: 185 us, so 145).
-__device__ __forceinline__ int64_t slot_of(int turn) {
-  return (blockIdx.y & 3) * (gridDim.y >> 2) + (blockIdx.y >> 2) + (int64_t)gridDim.y * turn;
+// How a call's work is dealt.  A sequence has a tile for every 32 of its columns, and its keys are cut into as many chunks as the
+// lengths that there are make right, whatever the table has room for (64 sequences of up to 8000 tokens: 120 us; chunks made for
+// the table, of 32768, 178); a piece is a chunk of a tile.  Pieces lie side by side, a chunk's tiles next to each other, and the
+// workgroups without one behind them: neighbours are dealt to an XCD's shader engines in turn, and engines without work are
+// what pieces that may or may not be there lead to (every second one of no columns: 185 us; 64 empty sequences at the end: 163, so
+// 129).  Up to 64 sequences every workgroup looks at all of them, a lane each, and finds its own; more are looked at by one
+// workgroup beforehand, that lists the pieces (4 us; done by every workgroup, 256 sequences 192 us for 143, 4096 8.6 ms for
+// 0.6).
+struct Work {
+  bool any;
+  int tile, tiles, chunk, chunks;  // of the sequence: the tile, how many; the chunk, how many
+  int first;                       // the sequence's first partial result, where it has some (chunks)
+  int idle;                        // none: how many of these are before this one
+  Tile t;
+};
+
+// Three rounds of four workgroups a CU.  Of less work than makes chunks of 32 blocks so, whose starts and joining take longer than
+// uneven ends, half a round, of still less chunks of 8 or a quarter of a round; two blocks a ring at least (a round: 32 sequences
+// of 300 tokens, 7 nodes, 32 heads of 128, 25 us, so 20, 32 of 1000 34 and 31).  `total`: blocks of all tiles and heads.
+__device__ __forceinline__ int chunk_size(float total) {
+  const int thirds = 1 + (int)(total * (1.0001f / 3072.f)), half = (int)(total * (1.f / 512.f));
+  const int few = half < 2 ? 4 : half < 4 ? 2 * half : 8, least = half < few ? few : half < 32 ? half : 32;
+  return thirds > least ? thirds : least;
+}
+// A head's blocks are so this many chunks at most, its pieces as many and the tiles, and those of tiles of two chunks or more
+// (of 3/4 of the size at least) 4/3 of it.
+inline int64_t most_chunks(int heads) { return 3072 / heads + 1; }
+
+// The sum of the lanes up to this one.
+template <class N>
+__device__ __forceinline__ N lanes_before(N x) {
+#define STEP(dpp, rows)                                                                                              \
+  {                                                                                                                  \
+    union { N n; int i; } u, v;                                                                                      \
+    u.n = x;                                                                                                         \
+    v.i = __builtin_amdgcn_update_dpp(0, u.i, dpp, rows, 0xf, false);                                                \
+    x += v.n;                                                                                                        \
+  }
+  STEP(0x111, 0xf)  // from 1, 2, 4, 8 lanes before in a row of 16
+  STEP(0x112, 0xf)
+  STEP(0x114, 0xf)
+  STEP(0x118, 0xf)
+  STEP(0x142, 0xa)  // a row's last lane to the next row
+  STEP(0x143, 0xc)  // the first half's to the second
+#undef STEP
+  return x;
+}
+
+struct Shape {
+  Tile t;
+  int tiles, blocks, chunks;
+  __device__ __forceinline__ Shape(const KvCache& c, const Attend& a, int64_t b) {
+    const bool valid = b < c.seqs;
+    t = make_tile<true>(c, a, valid ? b : 0, 0, SCT);
+    tiles = valid ? (int)(((int64_t)t.cols + SCT - 1) / SCT) : 0;
+    blocks = valid ? t.kb1 - t.kb0 : 0;
+  }
+  __device__ __forceinline__ float work() const { return (float)tiles * (float)blocks; }
+  // some `size` blocks a chunk: up to half as many again where it is one
+  __device__ __forceinline__ void cut(int size) { chunks = 2 * blocks >= 3 * size ? (2 * blocks + size) / (2 * size) : 1; }
+  __device__ __forceinline__ int pieces() const { return tiles * chunks; }
+  __device__ __forceinline__ int parts() const { return chunks > 1 ? tiles * chunks : 0; }
+};
+
+// The list: int4 {blocks of a chunk, pieces, tiles}, then {sequence, tile, chunk, the sequence's first partial result} for
+// a.pieces pieces, then the same for the tiles.
+constexpr int LISTING = 1024;
+__global__ __launch_bounds__(LISTING) void list_kernel(KvCache c, Attend a, int most_tiles) {
+  constexpr int WAVES = LISTING / 64;
+  __shared__ float works[WAVES];
+  __shared__ int sums[3][WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float work = 0.f;
+  for (int64_t b = threadIdx.x; b < c.seqs; b += LISTING) work += Shape(c, a, b).work();
+  work = lanes_before(work);
+  if (lane == 63) works[wave] = work;
+  __syncthreads();
+  float total = 0.f;
+  for (int w = 0; w < WAVES; ++w) total += works[w];
+  const int size = chunk_size(total * (float)c.heads);
+  int4 *const piece_at = a.list + 1, *const tile_at = piece_at + a.pieces;
+  int before[3] = {0, 0, 0};  // pieces, tiles, partial results of the sequences before these
+  for (int64_t b0 = 0; b0 < c.seqs; b0 += LISTING) {
+    Shape s(c, a, b0 + threadIdx.x);
+    s.cut(size);
+    const int count[3] = {s.pieces(), s.tiles, s.parts()};
+    int first[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      first[i] = lanes_before(count[i]);
+      if (lane == 63) sums[i][wave] = first[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      first[i] += before[i] - count[i];
+      for (int w = 0; w < WAVES; ++w) {
+        const int n = sums[i][w];
+        first[i] += w < wave ? n : 0;
+        before[i] += n;
+      }
+    }
+    const int seq = (int)(b0 + threadIdx.x);
+    // none past the list's ends, where offsets that do not ascend would lead
+    for (int i = 0; i < s.tiles && (unsigned)(first[1] + i) < (unsigned)most_tiles; ++i)
+      tile_at[first[1] + i] = make_int4(seq, i, 0, first[2]);
+    for (int k = 0, at = first[0]; k < s.chunks; ++k)
+      for (int i = 0; i < s.tiles && (unsigned)at < (unsigned)a.pieces; ++i, ++at) piece_at[at] = make_int4(seq, i, k, first[2]);
+    __syncthreads();
+  }
+  if (threadIdx.x == 0)
+    *a.list = make_int4(size, before[0] < a.pieces ? before[0] : a.pieces, before[1] < most_tiles ? before[1] : most_tiles, 0);
+}
+
+// Piece number `at`, or (of_tiles) tile number `at`.
+template <bool of_tiles>
+__device__ __forceinline__ Work find_work(const KvCache& c, const Attend& a, int at) {
+  Work w;
+  if (a.list) {
+    const int4 head = *a.list;
+    w.idle = at - head.y;
+    w.any = at < (of_tiles ? head.z : head.y);
+    if (!w.any) return w;
+    const int4 mine = a.list[1 + at + (of_tiles ? a.pieces : 0)];
+    Shape s(c, a, mine.x);
+    s.cut(head.x);
+    w.t = s.t, w.t.col0 = SCT * mine.y;
+    w.tile = mine.y, w.chunk = mine.z, w.first = mine.w, w.tiles = s.tiles, w.chunks = s.chunks;
+    return w;
+  }
+  Shape s(c, a, threadIdx.x & 63);
+  const int size = chunk_size(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(lanes_before(s.work())), 63)) * (float)c.heads);
+  s.cut(size);
+  const int count = of_tiles ? s.tiles : s.pieces(), to = lanes_before(count), from = to - count;
+  const int first = lanes_before(s.parts()) - s.parts();
+  const uint64_t here = __builtin_amdgcn_ballot_w64(from <= at && at < to);
+  w.any = here != 0;
+  w.idle = at - __builtin_amdgcn_readlane(to, 63);
+  if (!w.any) return w;
+  const int l = __builtin_ctzll(here);
+  const auto of = [&](int x) { return __builtin_amdgcn_readlane(x, l); };
+  w.tiles = of(s.tiles), w.chunks = of(s.chunks), w.first = of(first);
+  const int in = at - of(from);
+  w.chunk = of_tiles ? 0 : in / w.tiles;
+  w.tile = of_tiles ? in : in - w.chunk * w.tiles;
+  w.t.b = l;
+  w.t.row = (int64_t)((uint64_t)(unsigned)of((int)(s.t.row >> 32)) << 32 | (unsigned)of((int)s.t.row));
+  w.t.col0 = SCT * w.tile, w.t.cols = of(s.t.cols), w.t.pos0 = of(s.t.pos0);
+  w.t.kb0 = of(s.t.kb0), w.t.kb1 = of(s.t.kb1), w.t.pos_lo = of(s.t.pos_lo), w.t.pos_hi = of(s.t.pos_hi), w.t.len = of(s.t.len);
+  return w;
+}
+
+// Zeros (and an lse of -inf) in the rows that no sequence has, of one head, by the workgroups without a piece.
+template <class T>
+__device__ __forceinline__ void clear_idle(const KvCache& c, const Attend& a, int head, int idle, int idles) {
+  const int64_t before = kv_offset(c, 0), after = c.seqs ? kv_offset(c, c.seqs) : before;
+  if (__builtin_expect(before == 0 && after == c.tokens && c.seqs, 1)) return;
+  const int64_t from = c.seqs ? after : 0, end = c.seqs ? before : 0;  // [0, end) and [from, tokens)
+  const int64_t rows = end + c.tokens - from, per = (rows + idles - 1) / idles;
+  for (int64_t u = idle * per; u < (idle + 1) * per && u < rows; ++u) {
+    const int64_t row = u < end ? u : from + u - end;
+    clear_rows<T>(c, a, head, row * a.group, (row + 1) * a.group);
+  }
 }
 
 template <int TYPE, int ND>
@@ -152,18 +310,18 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
   __shared__ float tops[SWAVES][16], ls[COLS][16];
   static_assert(S * R::STAGE >= COLS * 4 * ND * 1024, "a ring's sums fit where its blocks were");
   // heads first: the workgroups of one XCD (every eighth) read few heads' keys and values
-  const int head = blockIdx.x, part = blockIdx.z % a.chunks;
-  const int64_t slot = slot_of(blockIdx.z / a.chunks);
-  const int64_t seq = kv_find(c, slot, a.group, CT, 1);
-  const int64_t first_slot = kv_first_slot(c, seq, a.group, CT, 1);
-  if (part == 0) clear_others<T>(c, a, head, seq, slot, first_slot, CT);
-  if (slot < first_slot || (slot - first_slot) * CT > 0x7fffff00) return;
-  const Tile t = make_tile<true>(c, a, seq, (int)((slot - first_slot) * CT), CT);
-  if (t.col0 >= t.cols || part >= t.chunks) return;
+  const int head = blockIdx.x, piece = (int)(blockIdx.y + gridDim.y * blockIdx.z);
+  const Work work = find_work<false>(c, a, piece);
+  if (!work.any) {
+    clear_idle<T>(c, a, head, work.idle, (int)(gridDim.y * gridDim.z) - (piece - work.idle));
+    return;
+  }
+  const Tile& t = work.t;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4;
   const int mine = wave / COLS, ct = wave % COLS;  // the wave's ring, and its tile of columns
-  const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + part * a.chunk);
-  const int end = __builtin_amdgcn_readfirstlane(begin + a.chunk < t.kb1 ? begin + a.chunk : t.kb1);
+  const int blocks = t.kb1 - t.kb0, size = blocks / work.chunks, more = blocks - size * work.chunks;  // one more in some
+  const int begin = __builtin_amdgcn_readfirstlane(t.kb0 + work.chunk * size + (work.chunk < more ? work.chunk : more));
+  const int end = __builtin_amdgcn_readfirstlane(begin + size + (work.chunk < more));
   // all columns see the keys in [all_from, all_to]
   const int all_to = __builtin_amdgcn_readfirstlane((t.pos_lo < t.len ? t.pos_lo : t.len) - 1);
   const int all_from = __builtin_amdgcn_readfirstlane(a.window ? t.pos_hi - a.window + 1 : 0);
@@ -312,8 +470,10 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
   }
   const bool none = m == -__builtin_inff();
   const int in = 16 * ct + (lane & 15);
-  if (t.chunks > 1) {
-    float* out = a.part + ((slot * c.heads + head) * a.chunks + part) * (int64_t)(CT * (DP + 2));
+  if (work.chunks > 1) {
+    const int at = work.first + work.chunk * work.tiles + work.tile;
+    if ((unsigned)at >= (unsigned)a.parts) return;  // offsets that do not ascend
+    float* out = a.part + ((int64_t)at * c.heads + head) * (int64_t)(CT * (DP + 2));
 #pragma unroll
     for (int d = 0; d < 4 * ND; ++d) *reinterpret_cast<floatx4*>(out + in * DP + 16 * d + 4 * g) = st.o[0][d];
     if (g == 0) {
@@ -336,28 +496,33 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
   }
 }
 
-// Joins the chunks' results of shared_kernel: a workgroup a slot and head, its 32 columns at once, so that what is looked up (the
-// sequence, its chunks, their maxima) is looked up once.  64 sequences of 8 nodes, 32 heads of 128, up to 6 chunks: 9 us (a wave
-// a column, as join_kernel, 19).
+// Joins the chunks' results of shared_kernel: a workgroup 8 columns of a tile and head, a wave's loads of 16 chunks on their way at
+// once: of few tiles, that many chunks share, it is the joining that is waited for.  One sequence of 8000 tokens, 7 nodes, 32 heads
+// of 128: both kernels 24 us (a workgroup all 32 columns, 4 loads at once: 34), of 32 nodes and 64 heads 37 (42), 4 of 131000 274
+// (294), 64 of up to 8000 111 (110).
+constexpr int CJ = 8;
 template <int TYPE, int ND>
 __global__ __launch_bounds__(THREADS) void join_tile_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int CT = SCT, DP = 64 * ND, SIZE = CT * (DP + 2), PER = THREADS / CT, ITEMS = CT * 16 * ND / THREADS, PIECE = 32;
-  __shared__ float factors[PIECE][CT], tops[CT], sums[CT];
-  const int head = blockIdx.x;
-  const int64_t slot = slot_of(blockIdx.z);
-  const int64_t seq = kv_find(c, slot, a.group, CT, 1), first_slot = kv_first_slot(c, seq, a.group, CT, 1);
-  if (slot < first_slot || (slot - first_slot) * CT > 0x7fffff00) return;
-  const Tile t = make_tile<true>(c, a, seq, (int)((slot - first_slot) * CT), CT);
-  if (t.col0 >= t.cols || t.chunks <= 1) return;
-  const float* part = a.part + (slot * c.heads + head) * (int64_t)a.chunks * SIZE;
-  const int cols = t.cols - t.col0 < CT ? t.cols - t.col0 : CT;
+  constexpr int CT = SCT, DP = 64 * ND, SIZE = CT * (DP + 2), PER = THREADS / CJ, PIECE = 32;
+  constexpr int VECTORS = CJ * 16 * ND, ITEMS = (VECTORS + THREADS - 1) / THREADS, UNROLL = ITEMS < 4 ? 16 / ITEMS : 4;
+  __shared__ float factors[PIECE][CJ], tops[CJ], sums[CJ];
+  const int head = blockIdx.x % c.heads, col0 = blockIdx.x / c.heads * CJ;
+  const Work work = find_work<true>(c, a, (int)(blockIdx.y + gridDim.y * blockIdx.z));
+  if (!work.any || work.chunks <= 1) return;
+  const int last = work.first + (work.chunks - 1) * work.tiles + work.tile;
+  if (work.first < 0 || (unsigned)last >= (unsigned)a.parts) return;  // offsets that do not ascend
+  const Tile& t = work.t;
+  const float* part = a.part + ((int64_t)(work.first + work.tile) * c.heads + head) * SIZE;
+  const int64_t stride = (int64_t)work.tiles * c.heads * SIZE;  // from chunk to chunk
+  const int cols = (t.cols - t.col0 < CT ? t.cols - t.col0 : CT) - col0;  // of these that there are
+  if (cols <= 0) return;
   // the largest of each column's references, by PER threads
   const int col = threadIdx.x / PER, j = threadIdx.x % PER;
-  const float* mine = part + CT * DP + (col < cols ? col : 0);
+  const float* mine = part + CT * DP + col0 + (col < cols ? col : 0);
   float top = -__builtin_inff(), l = 0.f;
-  for (int i = j; i < t.chunks; i += PER) {
-    const float x = mine[(int64_t)i * SIZE];
+  for (int i = j; i < work.chunks; i += PER) {
+    const float x = mine[i * stride];
     top = x > top || x != x ? x : top;
   }
 #pragma unroll
@@ -368,22 +533,22 @@ __global__ __launch_bounds__(THREADS) void join_tile_kernel(KvCache c, Attend a)
   floatx4 sum[ITEMS];
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) sum[k] = (floatx4){0.f, 0.f, 0.f, 0.f};
-  for (int i0 = 0; i0 < t.chunks; i0 += PIECE) {
-    const int n = t.chunks - i0 < PIECE ? t.chunks - i0 : PIECE;
+  for (int i0 = 0; i0 < work.chunks; i0 += PIECE) {
+    const int n = work.chunks - i0 < PIECE ? work.chunks - i0 : PIECE;
     for (int i = j; i < n; i += PER) {
-      const float* at = mine + (int64_t)(i0 + i) * SIZE;
+      const float* at = mine + (i0 + i) * stride;
       const float x = at[0], f = x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(x - top);
       l += f * at[CT];
       factors[i][col] = f;
     }
     __syncthreads();
-#pragma unroll 4
+#pragma unroll UNROLL
     for (int i = 0; i < n; ++i) {
-      const floatx4* from = reinterpret_cast<const floatx4*>(part + (int64_t)(i0 + i) * SIZE);
+      const floatx4* from = reinterpret_cast<const floatx4*>(part + (i0 + i) * stride + col0 * DP);
 #pragma unroll
       for (int k = 0; k < ITEMS; ++k) {  // columns past the sequence's are not written: the first one's in their place
-        const int u = threadIdx.x + THREADS * k, in = u / (16 * ND);
-        sum[k] += factors[i][in] * from[in < cols ? u : u % (16 * ND)];
+        const int u = threadIdx.x + THREADS * k, in = u / (16 * ND) % CJ;
+        sum[k] += factors[i][in] * from[in < cols ? u % VECTORS : u % (16 * ND)];
       }
     }
     __syncthreads();
@@ -395,8 +560,8 @@ __global__ __launch_bounds__(THREADS) void join_tile_kernel(KvCache c, Attend a)
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int u = threadIdx.x + THREADS * k, in = u / (16 * ND), d = 4 * (u % (16 * ND));
-    if (in >= cols) continue;
-    const int at = t.col0 + in, hq = head * a.group + at % a.group;
+    if (in >= cols || u >= VECTORS) continue;
+    const int at = t.col0 + col0 + in, hq = head * a.group + at % a.group;
     const int64_t row = t.row + at / a.group;
     const float total = sums[in], f = total == 0.f ? 0.f : 1.f / total;
     T* out = (T*)a.out + row * a.out_token + hq * a.out_head + d;
@@ -411,6 +576,8 @@ __global__ __launch_bounds__(THREADS) void join_tile_kernel(KvCache c, Attend a)
 // How a call is split: by attend_kernel or prompt_kernel as gptq2d_kv_attend's, or by shared_kernel.
 struct TreePlan : Plan {
   bool shared;
+  int64_t pieces, parts;  // of shared_kernel's work and of its partial results, for a head, at most
+  int64_t list;           // floats of the list of pieces, before the partial results
 };
 
 inline TreePlan make_tree_plan(int64_t tokens, int64_t seqs, int heads, int group, int dim, int64_t most, int64_t window,
@@ -420,32 +587,37 @@ inline TreePlan make_tree_plan(int64_t tokens, int64_t seqs, int heads, int grou
   seqs += !seqs;
   const int64_t columns = tokens * group, tiles = cdiv(columns, SCT) > seqs ? cdiv(columns, SCT) : seqs;
   const int64_t total = p.blocks * tiles * heads;
-  // Fewer blocks than workgroups of shared_kernel fit at once: the call is its start, which attend_kernel's waves, each alone,
-  // do sooner (8 kv heads of 128, 4 heads each, us of both kernels and the join, attend and shared: 7 nodes of one sequence of
-  // 100 tokens 10 and 15, of 1000 14 and 15, of 4000 16 and 22; of 4 of 1000 19 and 18, of 32 of 300 36 and 29, of 16 of 4000 55
-  // and 45).  From 384 columns a sequence on prompt_kernel, which brings codes to fp16 once for 128 columns (prompt and shared:
-  // 16 x 4000, 512 columns 209 and 313; one of 8000, 512 columns 53 and 67; 4 x 30000, 256 columns 252 and 256; 64 of up to 8000,
-  // 256 columns 635 and 569, 128 columns 567 and 344).
-  p.shared = total >= 1024 && columns < 384 * seqs;
+  // Few columns, and fewer blocks than workgroups of shared_kernel fit at once: the call is its start, which attend_kernel's waves,
+  // each alone, do sooner (8 kv heads of 128, 4 heads each, us of both kernels and the join, attend and shared: 7 nodes of one
+  // sequence of 100 tokens 11 and 15, of 1000 14 and 16, of 8000 21 and 21; of 4 of 1000 19 and 17, of 32 of 300 36 and 20, of
+  // 16 of 4000 55 and 39).  Many columns and more blocks than fit at a time: prompt_kernel, which brings codes to fp16 once for 128
+  // columns (prompt and shared: 24 nodes of 100 tokens 21 and 14; 128 of 1000 36 and 23, of 4000 48 and 39, of 8 of 300 46 and 39, of
+  // 16 of 300 50 and 68; 96 of 16 of 2000 122 and 151; 32 of 64 of up to 8000 573 and 332, 64 of those 638 and 587).
+  p.shared = p.prompt ? columns < 384 * seqs || total < 16384 : total >= 1024;
   if (!p.shared) return p;
   p.prompt = false;
   p.ct = SCT;
-  p.slots = columns / SCT + seqs;
-  // Three rounds of four workgroups a CU, or chunks of 24 blocks, whose starts and joining take longer than uneven ends, or one
-  // round; two blocks a ring at least.
-  const int64_t thirds = cdiv(total, 3072), once = cdiv(total, 1024), least = once < 24 ? once : 24;
-  p.chunk = (int)(thirds > least ? thirds : least < 4 ? 4 : least);
-  p.set_chunks(heads);
+  p.slots = columns / SCT + seqs;  // tiles at most
+  p.pieces = p.slots + most_chunks(heads);
+  p.parts = p.blocks > 5 ? (4 * most_chunks(heads) + 2) / 3 : 0;
+  p.turns = cdiv(p.pieces + 1, 65535);  // one more, for the rows that no sequence has
+  p.chunks = 1;
+  p.list = seqs > 64 ? 4 * (1 + p.pieces + p.slots) : 0;
+  p.part = p.list + p.parts * heads * (int64_t)(SCT * (64 * p.nd + 2));
   return p;
 }
 
 template <int TYPE, int ND>
-int launch_shared(const KvCache& c, const Attend& a, const TreePlan& p, hipStream_t st) {
-  const dim3 grid((unsigned)c.heads, (unsigned)(4 * cdiv(p.slots, 4 * p.turns)), (unsigned)(p.chunks * p.turns));
-  hipLaunchKernelGGL((shared_kernel<TYPE, ND>), grid, dim3(64 * SWAVES), 0, st, c, a);
-  if (p.chunks > 1)
-    hipLaunchKernelGGL((join_tile_kernel<TYPE, ND>), dim3(grid.x, grid.y, (unsigned)p.turns),
-                       dim3(THREADS), 0, st, c, a);
+int launch_shared(const KvCache& c, Attend a, const TreePlan& p, hipStream_t st) {
+  a.pieces = (int)p.pieces, a.parts = (int)p.parts;
+  if (p.list) {
+    a.list = reinterpret_cast<int4*>(a.part);
+    a.part += p.list;
+    hipLaunchKernelGGL(list_kernel, dim3(1), dim3(LISTING), 0, st, c, a, (int)p.slots);
+  }
+  const auto grid = [&](int64_t x, int64_t y) { return dim3((unsigned)x, (unsigned)cdiv(y, p.turns), (unsigned)p.turns); };
+  hipLaunchKernelGGL((shared_kernel<TYPE, ND>), grid(c.heads, p.pieces + 1), dim3(64 * SWAVES), 0, st, c, a);
+  if (p.parts) hipLaunchKernelGGL((join_tile_kernel<TYPE, ND>), grid(SCT / CJ * c.heads, p.slots), dim3(THREADS), 0, st, c, a);
   return (int)hipGetLastError();
 }
 

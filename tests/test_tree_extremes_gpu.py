@@ -272,3 +272,94 @@ def test_strided_queries_and_outputs_of_two_streams():
             got += [s.cache.attend(q, s.dev_table, lengths, s.offsets, tree=s.tree) for _ in range(3)]
     torch.cuda.synchronize()
     assert all(torch.equal(g, want) for g in got)
+
+
+def uneven(seqs, long=(0, 0.4, 1)):
+    """Lengths of sequences of which few are long, and their nodes: mostly few, none for some."""
+    rng = random.Random(seqs)
+    before, counts = [rng.randint(0, 40) for _ in range(seqs)], [rng.randint(0, 3) for _ in range(seqs)]
+    for i, part in enumerate(long):
+        b = round(part * (seqs - 1))
+        before[b], counts[b] = 2000 - 300 * i, (40, 5, 1)[i]
+    return before, counts
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("seqs", [63, 64, 65, 130, 1030])
+def test_few_long_ones_among_many(seqs, dtype):
+    """As many sequences as a workgroup looks at, one more, and more than are listed at once; the long ones are cut."""
+    print(f"many sequences {seqs} {dtype}", flush=True)
+    s = Trees(*uneven(seqs), 2, 64, TYPES[dtype], 32, seed=seqs)
+    s.check(8)
+    s.check(8, window=64)
+    s.dev_table = widened(s)
+    s.check(2)
+
+
+@pytest.mark.parametrize("before,after", [(0, 1), (70, 45)])
+@pytest.mark.parametrize("seqs", [64, 65, 200])
+def test_rows_that_none_of_many_sequences_has(seqs, before, after):
+    was, counts = uneven(seqs)
+    s = Trees(was, counts, 2, 64, torch.bfloat16, 32, seed=seqs)
+    tokens = before + sum(counts) + after
+    flat = [0] * before + [p for t in s.parents for p in t] + [0] * after
+    offsets = starts(counts) + before
+    q = torch.randn(tokens, 8, 64, generator=s.g).bfloat16()
+    own = torch.zeros(tokens, dtype=torch.bool)
+    own[before:before + sum(counts)] = True
+    poison((q.shape, q.dtype), (q.shape[:2], torch.float32))
+    got, lse = s.cache.attend(q.to(DEV), s.dev_table, s.lengths(), offsets, return_lse=True,
+                              tree=DraftTree(int32(flat), offsets, int32(was), nodes=40))
+    got, lse = got.cpu(), lse.cpu()
+    assert not got[~own].any() and bool((lse[~own] == -math.inf).all())
+    want, want_lse = s.reference(q[own], 64 ** -0.5)
+    check(got[own], want, float(held_values(s.v).abs().max()), torch.bfloat16)
+    assert float((lse[own].double() - want_lse).abs().max()) < 1e-3
+
+
+@pytest.mark.parametrize("seqs", [64, 65])
+def test_many_sequences_in_a_graph(seqs):
+    """Lengths, trees and the sequences that are there change between replays; what is left of a replay is not used by the next."""
+    was, counts = uneven(seqs)
+    s = Trees(was, counts, 2, 64, torch.float32, 32, seed=seqs)
+    tokens = sum(counts)
+    q = torch.randn(tokens, 4, 64, generator=s.g).to(DEV)
+    lengths, offsets, held, parents = s.lengths(), s.offsets.clone(), int32(was), int32([p for t in s.parents for p in t])
+
+    def run():
+        return s.cache.attend(q, s.dev_table, lengths, offsets, tree=DraftTree(parents, offsets, held, nodes=40))
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    rng = random.Random(7)
+    for keep in (1., 0.5, 0.02, 0., 1.):
+        new = [n if rng.random() < keep else 0 for n in counts]
+        now = [h if n else 0 for h, n in zip(was, new)]
+        trees = [random_tree(n, rng, "near") for n in new]
+        flat = [p for t in trees for p in t]
+        parents.copy_(int32(flat + [0] * (tokens - len(flat))))
+        offsets.copy_(starts(new))
+        held.copy_(int32(now))
+        lengths.copy_(int32([h + n for h, n in zip(now, new)]))
+        q.normal_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert not out[sum(new):].any()
+        assert torch.equal(out, run())
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("dim,hkv,group,page", [(128, 2, 4, 64), (64, 1, 8, 32), (80, 3, 4, 96), (256, 1, 4, 32), (33, 2, 5, 32)])
+def test_many_columns_of_much_work(dtype, dim, hkv, group, page):
+    """From 384 columns a sequence and 16384 blocks of all tiles on: prompt_kernel's, with trees; and windows, rows that no sequence
+    has, a sequence without a node."""
+    print(f"many columns {dtype} dim {dim} heads {hkv} x {group} page {page}", flush=True)
+    for before, counts, shape in (([90, 40], [150, 117], "random"), ([300, 10, 1], [230, 65, 200], "near"),
+                                  ([1, 40, 33, 0], [512, 200, 0, 200], "chain")):
+        s = Trees(before, counts, hkv, dim, TYPES[dtype], page, seed=dim + len(counts), shape=shape)
+        s.dev_table = widened(s, 2208)
+        s.check(hkv * group)
+        s.check(hkv * group, window=max(64, s.tree.nodes))
