@@ -58,9 +58,18 @@ class PagePool:
         self.left = torch.full((1,), pages, **whole)
         size = int(_hip.lib().gptq2d_page_pool_workspace(seqs))
         self._work = torch.empty(size, dtype=torch.uint8, device=device)
-        self._state = (self.table.data_ptr(), seqs, width, width, page_size, pages, self.owned.data_ptr(),
+        self._bind()
+
+    def _bind(self):
+        """The state as the C entry takes it."""
+        (seqs, width), pages = self.table.shape, self.free.numel()
+        self._state = (self.table.data_ptr(), seqs, width, width, self.page_size, pages, self.owned.data_ptr(),
                        self.lengths.data_ptr(), self.missing.data_ptr(), self.free.data_ptr(), self.left.data_ptr())
-        self._scratch = (self._work.data_ptr(), size)
+        self._scratch = (self._work.data_ptr(), self._work.numel())
+
+    def __setstate__(self, state):  # a copy has tensors of its own
+        self.__dict__.update(state)
+        self._bind()
 
     def _request(self, t, name):
         if t.dtype is not torch.int32 or t.shape != self.lengths.shape or t.device != self.device or not t.is_contiguous():

@@ -112,7 +112,7 @@ class Rotary:
         self.dim, self.rotated, self.interleaved, self.amplitude = dim, rotated, bool(interleaved), float(amplitude)
         self.turns = torch.tensor([float(f) / (2 * math.pi) for f in frequencies], dtype=torch.float64, device=device)
         _hip.require_device(self.turns)
-        self.device, self._turns = self.turns.device, self.turns.data_ptr()
+        self.device = self.turns.device
 
     def __call__(self, *xs: torch.Tensor, positions: torch.Tensor):
         """One or two tensors (queries, keys) [..., heads, dim] of one type (fp32, bf16 or fp16) rotated, each with its own
@@ -167,7 +167,7 @@ class Rotary:
         if len(xs) == 1:
             parts += _NO_PART
         _hip.launch("rotary", self.device, *parts, _TYPES[xs[0].dtype], outer, inner, self.dim, self.rotated, self.interleaved,
-                    self._turns, self.amplitude, p.data_ptr(), p.dtype is torch.int64, p_outer, p_inner, back)
+                    self.turns.data_ptr(), self.amplitude, p.data_ptr(), p.dtype is torch.int64, p_outer, p_inner, back)
         return tuple(out)
 
 

@@ -1,6 +1,7 @@
 """GPU tests of the pages dealt to sequences (page_pool.py over csrc/page_pool.hip) against lists on the CPU: whole numbers,
 so everything is equal."""
 
+import copy
 import random
 
 import pytest
@@ -184,3 +185,18 @@ def test_refusals():
     for held, offsets in ((int32([1, 2]), int32([0, 1])), (int32([1]).long(), int32([0, 1])), (int32([1]), int32([0, 1]).long())):
         with pytest.raises(ValueError):
             row_positions(held, offsets, 1)
+
+
+def test_copies_have_pages_of_their_own():
+    """A deep copy goes on from the same state without touching its original, also once that is gone."""
+    pool, other = PagePool(9, 3, 4, page_size=32), Lists(9, 3, 4, 32)
+    for p in (pool, other):
+        p.extend(int32([40, 0, 65]) if p is pool else [40, 0, 65], tokens=105)
+    twin = copy.deepcopy(pool)
+    was = [t.clone() for t in (pool.table, pool.lengths, pool.owned, pool.free, pool.left)]
+    for lengths in ([10, 90, 0], [128, 0, 128]):
+        twin.resize(int32(lengths))
+        other.resize(lengths)
+        assert [[p for p in row if p >= 0] for row in twin.table.tolist()] == other.table
+        assert twin.lengths.tolist() == other.lengths and twin.missing.tolist() == other.missing
+        assert all(torch.equal(a, b) for a, b in zip(was, (pool.table, pool.lengths, pool.owned, pool.free, pool.left)))

@@ -5,6 +5,7 @@ the subnormal numbers for fp16); cosine and sine, amplitude in them, are off by 
 evaluation 2^-23 at most, the product with a 2^-24), the product that the fused sum takes rounded by 2^-24: together 2^-21.5 a (|x1| +
 |x2|); and angles of far positions, whose turns carry two roundings in 64 bits and the reference's own one: 2^-51 |t|."""
 
+import copy
 import math
 
 import pytest
@@ -261,3 +262,13 @@ def test_frequencies():
         if turns < 0.5:
             assert math.isclose(y, f / 4)
     assert R.rotary_frequencies(2, 10000., R.Ntk(4.))[0] == [1.]
+
+
+@pytest.mark.gpu
+def test_copies_have_frequencies_of_their_own():
+    rotary = R.Rotary(64)
+    x, positions = torch.randn(5, 2, 64, device=DEV), torch.arange(5, device=DEV)
+    want, twin = rotary(x, positions=positions), copy.deepcopy(rotary)
+    rotary.turns.zero_()
+    assert torch.equal(rotary(x, positions=positions), x)
+    assert torch.equal(twin(x, positions=positions), want)
