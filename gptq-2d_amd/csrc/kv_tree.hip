@@ -149,17 +149,18 @@ struct Work {
   Tile t;
 };
 
-// Three rounds of four workgroups a CU.  Of less work than makes chunks of 32 blocks so, whose starts and joining take longer than
-// uneven ends, half a round, of still less chunks of 8 or a quarter of a round; two blocks a ring at least (a round: 32 sequences
-// of 300 tokens, 7 nodes, 32 heads of 128, 25 us, so 20, 32 of 1000 34 and 31).  `total`: blocks of all tiles and heads.
+// Three rounds of the workgroups that fit at once.  Of less work than makes chunks of 32 blocks so, whose starts and joining take
+// longer than uneven ends, half a round, of still less chunks of 8 or a quarter of a round; two blocks a ring at least (a round:
+// 32 sequences of 300 tokens, 7 nodes, 32 heads of 128, 25 us, so 20, 32 of 1000 34 and 31).  `total`: blocks of all tiles and heads.
+constexpr int ROUND = 1024;  // four a CU
 __device__ __forceinline__ int chunk_size(float total) {
-  const int thirds = 1 + (int)(total * (1.0001f / 3072.f)), half = (int)(total * (1.f / 512.f));
+  const int thirds = 1 + (int)(total * (1.0001f / (3 * ROUND))), half = (int)(total * (2.f / ROUND));
   const int few = half < 2 ? 4 : half < 4 ? 2 * half : 8, least = half < few ? few : half < 32 ? half : 32;
   return thirds > least ? thirds : least;
 }
 // A head's blocks are so this many chunks at most, its pieces as many and the tiles, and those of tiles of two chunks or more
 // (of 3/4 of the size at least) 4/3 of it.
-inline int64_t most_chunks(int heads) { return 3072 / heads + 1; }
+inline int64_t most_chunks(int heads) { return 3 * ROUND / heads + 1; }
 
 // The sum of the lanes up to this one.
 template <class N>
