@@ -17,7 +17,9 @@ namespace {
 //     not enough for fp16 and fp32.
 // One barrier a block: after it, the stage that was read in the turn before is loaded again.  A workgroup has two rings, with
 // every second block each, whose results are joined at the end; four workgroups a CU.
-constexpr int COLS = 2, RINGS = 2, SWAVES = COLS * RINGS, SCT = 16 * COLS;  // waves of a ring, rings, columns of a workgroup
+// Of up to 16 columns a sequence a ring has one wave (COLS): 64 sequences of 2 nodes and up to 8000 tokens 90 us (with two, one of
+// them without columns, 100), 100 of 4 nodes and 1000 46 (54).
+constexpr int RINGS = 2;
 
 template <bool PLAIN>
 __device__ __forceinline__ half8 codes_of(unsigned w) {
@@ -39,17 +41,17 @@ constexpr int CODE = PLAIN ? -24 : 0;
 template <bool PLAIN>
 constexpr int FOLD = PLAIN ? 4 : 0;
 
-template <int ND>
+template <int ND, int COLS>
 struct Shared {
   static constexpr int STAGE = 2048 * ND + 256, S = ND == 1 ? 6 : 4;  // stages of a ring: 35 KB a workgroup for heads of up to 128
-  static constexpr int LOADS[COLS] = {ND + 1, ND};                    // of a stage, by each wave
+  static constexpr int LOADS[2] = {COLS == 2 ? ND + 1 : 2 * ND + 1, ND};  // of a stage, by each wave
 };
 
 // Until wave `ct`'s loads of the oldest stage on its way have landed, and wave 0's first one, of scales, of the next stage.
-template <int ND>
+template <int ND, int COLS>
 __device__ __forceinline__ void wait_turn(int ct) {
-  typedef Shared<ND> R;
-  if (ct == 0)
+  typedef Shared<ND, COLS> R;
+  if (COLS == 1 || ct == 0)
     wait_loads<(R::S - 2) * R::LOADS[0] - 1>();
   else
     wait_loads<(R::S - 2) * R::LOADS[1]>();
@@ -133,7 +135,7 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
   }
 }
 
-// How a call's work is dealt.  A sequence has a tile for every 32 of its columns, and its keys are cut into as many chunks as the
+// How a call's work is dealt.  A sequence has a tile for every CT (32 or 16) of its columns, and its keys are cut into as many chunks as the
 // lengths that there are make right, whatever the table has room for (64 sequences of up to 8000 tokens: 120 us; chunks made for
 // the table, of 32768, 178); a piece is a chunk of a tile.  Pieces lie side by side, a chunk's tiles next to each other, and the
 // workgroups without one behind them: neighbours are dealt to an XCD's shader engines in turn, and engines without work are
@@ -185,10 +187,10 @@ __device__ __forceinline__ N lanes_before(N x) {
 struct Shape {
   Tile t;
   int tiles, blocks, chunks;
-  __device__ __forceinline__ Shape(const KvCache& c, const Attend& a, int64_t b) {
+  __device__ __forceinline__ Shape(const KvCache& c, const Attend& a, int64_t b, int CT) {
     const bool valid = b < c.seqs;
-    t = make_tile<true>(c, a, valid ? b : 0, 0, SCT);
-    tiles = valid ? (int)(((int64_t)t.cols + SCT - 1) / SCT) : 0;
+    t = make_tile<true>(c, a, valid ? b : 0, 0, CT);
+    tiles = valid ? (int)(((int64_t)t.cols + CT - 1) / CT) : 0;
     blocks = valid ? t.kb1 - t.kb0 : 0;
   }
   __device__ __forceinline__ float work() const { return (float)tiles * (float)blocks; }
@@ -201,13 +203,13 @@ struct Shape {
 // The list: int4 {blocks of a chunk, pieces, tiles}, then {sequence, tile, chunk, the sequence's first partial result} for
 // a.pieces pieces, then the same for the tiles.
 constexpr int LISTING = 1024;
-__global__ __launch_bounds__(LISTING) void list_kernel(KvCache c, Attend a, int most_tiles) {
+__global__ __launch_bounds__(LISTING) void list_kernel(KvCache c, Attend a, int most_tiles, int CT) {
   constexpr int WAVES = LISTING / 64;
   __shared__ float works[WAVES];
   __shared__ int sums[3][WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   float work = 0.f;
-  for (int64_t b = threadIdx.x; b < c.seqs; b += LISTING) work += Shape(c, a, b).work();
+  for (int64_t b = threadIdx.x; b < c.seqs; b += LISTING) work += Shape(c, a, b, CT).work();
   work = lanes_before(work);
   if (lane == 63) works[wave] = work;
   __syncthreads();
@@ -217,7 +219,7 @@ __global__ __launch_bounds__(LISTING) void list_kernel(KvCache c, Attend a, int 
   int4 *const piece_at = a.list + 1, *const tile_at = piece_at + a.pieces;
   int before[3] = {0, 0, 0};  // pieces, tiles, partial results of the sequences before these
   for (int64_t b0 = 0; b0 < c.seqs; b0 += LISTING) {
-    Shape s(c, a, b0 + threadIdx.x);
+    Shape s(c, a, b0 + threadIdx.x, CT);
     s.cut(size);
     const int count[3] = {s.pieces(), s.tiles, s.parts()};
     int first[3];
@@ -249,7 +251,7 @@ __global__ __launch_bounds__(LISTING) void list_kernel(KvCache c, Attend a, int 
 }
 
 // Piece number `at`, or (of_tiles) tile number `at`.
-template <bool of_tiles>
+template <bool of_tiles, int CT>
 __device__ __forceinline__ Work find_work(const KvCache& c, const Attend& a, int at) {
   Work w;
   if (a.list) {
@@ -258,13 +260,13 @@ __device__ __forceinline__ Work find_work(const KvCache& c, const Attend& a, int
     w.any = at < (of_tiles ? head.z : head.y);
     if (!w.any) return w;
     const int4 mine = a.list[1 + at + (of_tiles ? a.pieces : 0)];
-    Shape s(c, a, mine.x);
+    Shape s(c, a, mine.x, CT);
     s.cut(head.x);
-    w.t = s.t, w.t.col0 = SCT * mine.y;
+    w.t = s.t, w.t.col0 = CT * mine.y;
     w.tile = mine.y, w.chunk = mine.z, w.first = mine.w, w.tiles = s.tiles, w.chunks = s.chunks;
     return w;
   }
-  Shape s(c, a, threadIdx.x & 63);
+  Shape s(c, a, threadIdx.x & 63, CT);
   const int size = chunk_size(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(lanes_before(s.work())), 63)) * (float)c.heads);
   s.cut(size);
   const int count = of_tiles ? s.tiles : s.pieces(), to = lanes_before(count), from = to - count;
@@ -281,7 +283,7 @@ __device__ __forceinline__ Work find_work(const KvCache& c, const Attend& a, int
   w.tile = of_tiles ? in : in - w.chunk * w.tiles;
   w.t.b = l;
   w.t.row = (int64_t)((uint64_t)(unsigned)of((int)(s.t.row >> 32)) << 32 | (unsigned)of((int)s.t.row));
-  w.t.col0 = SCT * w.tile, w.t.cols = of(s.t.cols), w.t.pos0 = of(s.t.pos0);
+  w.t.col0 = CT * w.tile, w.t.cols = of(s.t.cols), w.t.pos0 = of(s.t.pos0);
   w.t.kb0 = of(s.t.kb0), w.t.kb1 = of(s.t.kb1), w.t.pos_lo = of(s.t.pos_lo), w.t.pos_hi = of(s.t.pos_hi), w.t.len = of(s.t.len);
   return w;
 }
@@ -299,11 +301,14 @@ __device__ __forceinline__ void clear_idle(const KvCache& c, const Attend& a, in
   }
 }
 
-template <int TYPE, int ND>
-__global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <= 2 ? 3 : 2) void shared_kernel(KvCache c, Attend a) {
+// (Workgroups a CU as registers are dealt: with one column tile four, as there is LDS for, made the compiler move sums to and fro,
+// 93 us for 89 with 64 sequences of 2 nodes.)
+template <int TYPE, int ND, int COLS>
+__global__ __launch_bounds__(64 * COLS * RINGS, COLS == 1 ? 2 : ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <= 2 ? 3 : 2) void
+shared_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
-  typedef Shared<ND> R;
-  constexpr int CT = SCT, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2, S = R::S;
+  typedef Shared<ND, COLS> R;
+  constexpr int SWAVES = COLS * RINGS, CT = 16 * COLS, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2, S = R::S;
   constexpr bool PLAIN = TYPE == TYPE_BF16;
   alignas(16) __shared__ char ring[RINGS][S][R::STAGE];
   __shared__ float aff[RINGS][2][4][32];  // scale and zero of keys (times what scores share), of values
@@ -312,7 +317,7 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
   static_assert(S * R::STAGE >= COLS * 4 * ND * 1024, "a ring's sums fit where its blocks were");
   // heads first: the workgroups of one XCD (every eighth) read few heads' keys and values
   const int head = blockIdx.x, piece = (int)(blockIdx.y + gridDim.y * blockIdx.z);
-  const Work work = find_work<false>(c, a, piece);
+  const Work work = find_work<false, CT>(c, a, piece);
   if (!work.any) {
     clear_idle<T>(c, a, head, work.idle, (int)(gridDim.y * gridDim.z) - (piece - work.idle));
     return;
@@ -422,7 +427,7 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
   int buf = 0;
   for (int i = 0; i < turns; ++i) {
     if (i + S - 1 <= count)
-      wait_turn<ND>(ct);
+      wait_turn<ND, COLS>(ct);
     else
       wait_loads<0>();
     __builtin_amdgcn_s_barrier();
@@ -502,14 +507,14 @@ __global__ __launch_bounds__(64 * SWAVES, ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <
 // of 128: both kernels 24 us (a workgroup all 32 columns, 4 loads at once: 34), of 32 nodes and 64 heads 37 (42), 4 of 131000 274
 // (294), 64 of up to 8000 111 (110).
 constexpr int CJ = 8;
-template <int TYPE, int ND>
+template <int TYPE, int ND, int CT>
 __global__ __launch_bounds__(THREADS) void join_tile_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
-  constexpr int CT = SCT, DP = 64 * ND, SIZE = CT * (DP + 2), PER = THREADS / CJ, PIECE = 32;
+  constexpr int DP = 64 * ND, SIZE = CT * (DP + 2), PER = THREADS / CJ, PIECE = 32;
   constexpr int VECTORS = CJ * 16 * ND, ITEMS = (VECTORS + THREADS - 1) / THREADS, UNROLL = ITEMS < 4 ? 16 / ITEMS : 4;
   __shared__ float factors[PIECE][CJ], tops[CJ], sums[CJ];
   const int head = blockIdx.x % c.heads, col0 = blockIdx.x / c.heads * CJ;
-  const Work work = find_work<true>(c, a, (int)(blockIdx.y + gridDim.y * blockIdx.z));
+  const Work work = find_work<true, CT>(c, a, (int)(blockIdx.y + gridDim.y * blockIdx.z));
   if (!work.any || work.chunks <= 1) return;
   const int last = work.first + (work.chunks - 1) * work.tiles + work.tile;
   if (work.first < 0 || (unsigned)last >= (unsigned)a.parts) return;  // offsets that do not ascend
@@ -586,26 +591,34 @@ inline TreePlan make_tree_plan(int64_t tokens, int64_t seqs, int heads, int grou
   TreePlan p;
   static_cast<Plan&>(p) = make_plan(tokens, seqs, heads, group, dim, most, window, nodes);
   seqs += !seqs;
-  const int64_t columns = tokens * group, tiles = cdiv(columns, SCT) > seqs ? cdiv(columns, SCT) : seqs;
+  const int64_t columns = tokens * group, tiles = cdiv(columns, 32) > seqs ? cdiv(columns, 32) : seqs;
   const int64_t total = p.blocks * tiles * heads;
   // Few columns, and fewer blocks than workgroups of shared_kernel fit at once: the call is its start, which attend_kernel's waves,
   // each alone, do sooner (8 kv heads of 128, 4 heads each, us of both kernels and the join, attend and shared: 7 nodes of one
   // sequence of 100 tokens 11 and 15, of 1000 14 and 16, of 8000 21 and 21; of 4 of 1000 19 and 17, of 32 of 300 36 and 20, of
-  // 16 of 4000 55 and 39).  Many columns and more blocks than fit at a time: prompt_kernel, which brings codes to fp16 once for 128
+  // 16 of 4000 55 and 39; where pieces are listed, 2 of 65 of 100 18 and 21, of 100 of 100 21 and 21, 4 of 100 of 300 42 and 29).  Many columns and more blocks than fit at a time: prompt_kernel, which brings codes to fp16 once for 128
   // columns (prompt and shared: 24 nodes of 100 tokens 21 and 14; 128 of 1000 36 and 23, of 4000 48 and 39, of 8 of 300 46 and 39, of
   // 16 of 300 50 and 68; 96 of 16 of 2000 122 and 151; 32 of 64 of up to 8000 573 and 332, 64 of those 638 and 587).
-  p.shared = p.prompt ? columns < 384 * seqs || total < 16384 : total >= 1024;
+  p.shared = p.prompt ? columns < 384 * seqs || total < 16384 : total >= (seqs > 64 ? 4096 : 1024);
   if (!p.shared) return p;
   p.prompt = false;
-  p.ct = SCT;
-  p.slots = columns / SCT + seqs;  // tiles at most
+  p.ct = columns <= 16 * seqs ? 16 : 32;
+  p.slots = columns / p.ct + seqs;  // tiles at most
   p.pieces = p.slots + most_chunks(heads);
   p.parts = p.blocks > 5 ? (4 * most_chunks(heads) + 2) / 3 : 0;
   p.turns = cdiv(p.pieces + 1, 65535);  // one more, for the rows that no sequence has
   p.chunks = 1;
   p.list = seqs > 64 ? 4 * (1 + p.pieces + p.slots) : 0;
-  p.part = p.list + p.parts * heads * (int64_t)(SCT * (64 * p.nd + 2));
+  p.part = p.list + p.parts * heads * (int64_t)(p.ct * (64 * p.nd + 2));
   return p;
+}
+
+template <int TYPE, int ND, int COLS>
+void launch_cols(const KvCache& c, const Attend& a, const TreePlan& p, hipStream_t st) {
+  const auto grid = [&](int64_t x, int64_t y) { return dim3((unsigned)x, (unsigned)cdiv(y, p.turns), (unsigned)p.turns); };
+  hipLaunchKernelGGL((shared_kernel<TYPE, ND, COLS>), grid(c.heads, p.pieces + 1), dim3(64 * COLS * RINGS), 0, st, c, a);
+  if (p.parts)
+    hipLaunchKernelGGL((join_tile_kernel<TYPE, ND, 16 * COLS>), grid(16 * COLS / CJ * c.heads, p.slots), dim3(THREADS), 0, st, c, a);
 }
 
 template <int TYPE, int ND>
@@ -614,11 +627,12 @@ int launch_shared(const KvCache& c, Attend a, const TreePlan& p, hipStream_t st)
   if (p.list) {
     a.list = reinterpret_cast<int4*>(a.part);
     a.part += p.list;
-    hipLaunchKernelGGL(list_kernel, dim3(1), dim3(LISTING), 0, st, c, a, (int)p.slots);
+    hipLaunchKernelGGL(list_kernel, dim3(1), dim3(LISTING), 0, st, c, a, (int)p.slots, p.ct);
   }
-  const auto grid = [&](int64_t x, int64_t y) { return dim3((unsigned)x, (unsigned)cdiv(y, p.turns), (unsigned)p.turns); };
-  hipLaunchKernelGGL((shared_kernel<TYPE, ND>), grid(c.heads, p.pieces + 1), dim3(64 * SWAVES), 0, st, c, a);
-  if (p.parts) hipLaunchKernelGGL((join_tile_kernel<TYPE, ND>), grid(SCT / CJ * c.heads, p.slots), dim3(THREADS), 0, st, c, a);
+  if (p.ct == 16)
+    launch_cols<TYPE, ND, 1>(c, a, p, st);
+  else
+    launch_cols<TYPE, ND, 2>(c, a, p, st);
   return (int)hipGetLastError();
 }
 

@@ -292,6 +292,7 @@ def test_few_long_ones_among_many(seqs, dtype):
     s = Trees(*uneven(seqs), 2, 64, TYPES[dtype], 32, seed=seqs)
     s.check(8)
     s.check(8, window=64)
+    s.check(34)
     s.dev_table = widened(s)
     s.check(2)
 
