@@ -135,14 +135,14 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
   }
 }
 
-// How a call's work is dealt.  A sequence has a tile for every CT (32 or 16) of its columns, and its keys are cut into as many chunks as the
-// lengths that there are make right, whatever the table has room for (64 sequences of up to 8000 tokens: 120 us; chunks made for
-// the table, of 32768, 178); a piece is a chunk of a tile.  Pieces lie side by side, a chunk's tiles next to each other, and the
-// workgroups without one behind them: neighbours are dealt to an XCD's shader engines in turn, and engines without work are
-// what pieces that may or may not be there lead to (every second one of no columns: 185 us; 64 empty sequences at the end: 163, so
-// 129).  Up to 64 sequences every workgroup looks at all of them, a lane each, and finds its own; more are looked at by one
-// workgroup beforehand, that lists the pieces (4 us; done by every workgroup, 256 sequences 192 us for 143, 4096 8.6 ms for
-// 0.6).
+// How a call's work is dealt.  A sequence has a tile for every CT (32 or 16) of its columns, and its keys are cut into as many
+// chunks as the lengths that there are make right, whatever the table has room for (64 sequences of 8 nodes, up to 8000 tokens,
+// 115 us; chunks made for a table of room for 32768 178); a piece is a chunk of a tile.  Pieces lie side by side, a chunk's tiles
+// next to each other, and the workgroups without one behind them: neighbours are dealt to an XCD's shader engines in turn, and
+// engines without work are what pieces that may or may not be there lead to (every second one of no columns 185 us; 64 empty
+// sequences at the end 163, so 119).  Up to 64 sequences every workgroup looks at all of them, a lane each, and finds its own
+// piece; more are looked at by one workgroup beforehand, which lists the pieces (some 5 us a call; done by every workgroup, 256
+// sequences 192 us for 141, 4096 8.6 ms for 0.65).
 struct Work {
   bool any;
   int tile, tiles, chunk, chunks;  // of the sequence: the tile, how many; the chunk, how many
@@ -596,9 +596,10 @@ inline TreePlan make_tree_plan(int64_t tokens, int64_t seqs, int heads, int grou
   // Few columns, and fewer blocks than workgroups of shared_kernel fit at once: the call is its start, which attend_kernel's waves,
   // each alone, do sooner (8 kv heads of 128, 4 heads each, us of both kernels and the join, attend and shared: 7 nodes of one
   // sequence of 100 tokens 11 and 15, of 1000 14 and 16, of 8000 21 and 21; of 4 of 1000 19 and 17, of 32 of 300 36 and 20, of
-  // 16 of 4000 55 and 39; where pieces are listed, 2 of 65 of 100 18 and 21, of 100 of 100 21 and 21, 4 of 100 of 300 42 and 29).  Many columns and more blocks than fit at a time: prompt_kernel, which brings codes to fp16 once for 128
-  // columns (prompt and shared: 24 nodes of 100 tokens 21 and 14; 128 of 1000 36 and 23, of 4000 48 and 39, of 8 of 300 46 and 39, of
-  // 16 of 300 50 and 68; 96 of 16 of 2000 122 and 151; 32 of 64 of up to 8000 573 and 332, 64 of those 638 and 587).
+  // 16 of 4000 55 and 39; where pieces are listed, 2 nodes of 65 of 100 18 and 21, of 100 of 100 21 and 21, 4 of 100 of 300 42 and
+  // 29).  Many columns and more blocks than fit at a time: prompt_kernel, which brings codes to fp16 once for 128 columns (prompt
+  // and shared: 24 nodes of 100 tokens 21 and 14; 128 of 1000 36 and 23, of 4000 48 and 39, of 8 of 300 46 and 39, of 16 of 300 50
+  // and 68; 96 of 16 of 2000 122 and 151; 32 of 64 of up to 8000 573 and 332, 64 of those 638 and 587).
   p.shared = p.prompt ? columns < 384 * seqs || total < 16384 : total >= (seqs > 64 ? 4096 : 1024);
   if (!p.shared) return p;
   p.prompt = false;
