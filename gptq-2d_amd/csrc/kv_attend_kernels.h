@@ -782,9 +782,8 @@ __global__ __launch_bounds__(64 * PWAVES, ND <= 2 ? 2 : 1) void prompt_kernel(Kv
     if (wave == 0) {  // lanes 0..31 the keys, 32..63 the values
       unsigned w = page && kb * 32 + (lane & 31) < len ? affine : FLAT;  // beyond the sequence: whatever the page holds
       const float s = __uint_as_float(w << 16), z = __builtin_fmaf(8.f, s, __uint_as_float(w & 0xffff0000u));
-      const unsigned bits = (w >> 7 & 255u) - 1;  // zeros, subnormal numbers, infinities and NaN are of no matter
-      const bool real = lane >= 32 && bits < 254u;
-      const int ex = real ? (int)bits - 125 : held;  // s in [2^(ex - 1), 2^ex)
+      const bool real = lane >= 32 && s > 0.f && s < __builtin_inff();  // -0, infinities and NaN are of no matter
+      const int ex = real ? exponent_of(s) + 1 : held;                  // s in [2^(ex - 1), 2^ex), subnormal or not
       if (__builtin_amdgcn_ballot_w64((unsigned)(held - ex) >= (unsigned)(held - least))) {
         int big = real ? ex : -1000, low = real ? ex : 1000;
 #pragma unroll

@@ -394,9 +394,8 @@ shared_kernel(KvCache c, Attend a) {
     const unsigned affine = *reinterpret_cast<const unsigned*>(ring[mine][stage] + 2048 * ND + 4 * lane);
     const unsigned w = (there >> stage & 1u) && kb * 32 + (lane & 31) < len ? affine : FLAT;  // beyond the sequence: whatever the page holds
     const float s = __uint_as_float(w << 16), zero = __uint_as_float(w & 0xffff0000u), z = PLAIN ? zero : __builtin_fmaf(8.f, s, zero);
-    const unsigned bits = (w >> 7 & 255u) - 1;  // zeros, subnormal numbers, infinities and NaN are of no matter
-    const bool real = lane >= 32 && bits < 254u;
-    const int ex = real ? (int)bits - 125 : held;  // s in [2^(ex - 1), 2^ex)
+    const bool real = lane >= 32 && s > 0.f && s < __builtin_inff();  // -0, infinities and NaN are of no matter
+    const int ex = real ? exponent_of(s) + 1 : held;                  // s in [2^(ex - 1), 2^ex), subnormal or not
     if (__builtin_amdgcn_ballot_w64((unsigned)(held - ex) >= (unsigned)(held - least))) {
       int big = real ? ex : -1000, low = real ? ex : 1000;
 #pragma unroll
