@@ -11,6 +11,9 @@ as near ones; sums are in 32 bits and rounded once.
 
     rotary = Rotary(128, base=500000., scaling=Bands(8., context=8192))
     q, k = rotary(q, k, positions=positions)        # one launch; differentiable in q and k
+
+Derivatives go backward and forward, of any order, and through `torch.func`'s transforms; the rotation is linear, so each of them
+is a rotation, by the angles or back.
 """
 
 from __future__ import annotations
@@ -19,11 +22,19 @@ import math
 from typing import NamedTuple, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 import _hip
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _NO_PART = (None, 0, 0, 0, None, 0, 0, 0, 0)
+# Whether a transform of torch.func is at work; a torch that does not say so is taken to be at it, which costs a node a call.
+_transformed = getattr(torch._C, "_are_functorch_transforms_active", lambda: True)
+
+
+def _followed(xs) -> bool:
+    """Whether forward derivatives of xs are wanted."""
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in xs)
 
 
 class Linear(NamedTuple):
@@ -137,8 +148,8 @@ class Rotary:
         if positions.shape != lead and (positions.dim() > len(lead) or
                                         any(a != b and a != 1 for a, b in zip(positions.shape[::-1], lead[::-1]))):
             raise ValueError(f"positions {tuple(positions.shape)} do not broadcast to {tuple(lead)}")
-        if grad and torch.is_grad_enabled():
-            out = _Rotation.apply(self, False, positions, *xs)
+        if (grad and torch.is_grad_enabled()) or _transformed() or _followed(xs):
+            out = _turned(self, False, positions, xs)
         else:
             out = self._rotate(xs, positions, False)
         return out[0] if len(xs) == 1 else out
@@ -172,21 +183,66 @@ class Rotary:
 
 
 class _Rotation(torch.autograd.Function):
-    """The rotation (or, `back`, its transpose), whose gradient is the other one."""
+    """The rotation (or, `back`, its transpose).  It is linear: its derivative along a direction is the direction rotated, its
+    gradient the other rotation."""
 
     @staticmethod
     def forward(ctx, rotary, back, positions, *xs):
-        ctx.set_materialize_grads(False)
-        ctx.rotary, ctx.back = rotary, back
-        ctx.save_for_backward(positions)
+        _Rotation._keep(ctx, rotary, back, positions, xs)
         return rotary._rotate(xs, positions, back)
+
+    @staticmethod
+    def _keep(ctx, rotary, back, positions, xs):
+        ctx.set_materialize_grads(False)
+        ctx.rotary, ctx.back, ctx.shapes = rotary, back, [x.shape for x in xs]
+        ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
 
     @staticmethod
     def backward(ctx, *grads):
         grads = [g if wanted else None for g, wanted in zip(grads, ctx.needs_input_grad[3:])]
         there, positions = [g for g in grads if g is not None], ctx.saved_tensors[0]
-        if torch.is_grad_enabled():  # of the gradient too
-            turned = iter(_Rotation.apply(ctx.rotary, not ctx.back, positions, *there) if there else ())
-        else:
-            turned = iter(ctx.rotary._rotate(there, positions, not ctx.back) if there else ())
+        turned = iter(_turned(ctx.rotary, not ctx.back, positions, there) if there else ())
         return (None, None, None, *(None if g is None else next(turned) for g in grads))
+
+    @staticmethod
+    def jvp(ctx, _rotary, _back, _positions, *tangents):
+        there, positions = [t for t in tangents if t is not None], ctx.saved_tensors[0]
+        turned = iter(_turned(ctx.rotary, ctx.back, positions, there))
+        return tuple(there[0].new_zeros(shape) if t is None else next(turned) for t, shape in zip(tangents, ctx.shapes))
+
+
+class _Mapped(_Rotation):
+    """The same in the form that torch.func's transforms take, of which a call costs more."""
+
+    @staticmethod
+    def forward(rotary, back, positions, *xs):
+        return rotary._rotate(xs, positions, back)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        _Rotation._keep(ctx, *inputs[:3], inputs[3:])
+
+    @staticmethod
+    def vmap(info, in_dims, rotary, back, positions, *xs):
+        """The mapped axis in front of a leading one, or one with the first of two."""
+        n = info.batch_size
+        xs = [x.expand(n, *x.shape) if at is None else x.movedim(at, 0) for x, at in zip(xs, in_dims[3:])]
+        lead = xs[0].shape[1:-2]
+        p = positions[None] if in_dims[2] is None else positions.movedim(in_dims[2], 0)
+        p = p.reshape(p.size(0), *[1] * (len(lead) - p.dim() + 1), *p.shape[1:]).expand(n, *lead)
+        if len(lead) == 2:
+            p, xs = p.flatten(0, 1), [x.flatten(0, 1) for x in xs]
+        out = _turned(rotary, back, p, xs)
+        if len(lead) == 2:
+            out = tuple(y.unflatten(0, (n, lead[0])) for y in out)
+        return out, (0,) * len(out)
+
+
+def _turned(rotary, back, positions, xs):
+    """The rotation of xs, which whatever follows them sees."""
+    if _transformed():
+        return _Mapped.apply(rotary, back, positions, *xs)
+    if torch.is_grad_enabled() or _followed(xs):
+        return _Rotation.apply(rotary, back, positions, *xs)
+    return rotary._rotate(xs, positions, back)
