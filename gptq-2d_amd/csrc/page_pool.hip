@@ -141,12 +141,15 @@ __device__ __forceinline__ void take(const Pool& p, const Sums& s, int left, int
     int position = 0;
     int64_t slot = -1;
     if (b < n) {
-      position = s.base[b] + ((int)r - before(s.rows, b));
-      const int at = position / p.page, fresh = at - s.keep[b], count = s.taken[b] - before(s.taken, b);
-      // an entry that this call takes may not be in the table yet
-      const int page = fresh < 0 ? p.table[b * p.table_stride + at]
-                                 : fresh < count ? taken_page(p, top, before(s.taken, b) + fresh) : -1;
-      if (page >= 0) slot = (int64_t)page * p.page + position % p.page;
+      const int64_t row = (int64_t)s.base[b] + (r - before(s.rows, b));  // of more rows than a sequence may hold past 32 bits
+      position = row < MOST ? (int)row : MOST;
+      if (row < MOST) {
+        const int at = position / p.page, fresh = at - s.keep[b], count = s.taken[b] - before(s.taken, b);
+        // an entry that this call takes may not be in the table yet
+        const int page = fresh < 0 ? p.table[b * p.table_stride + at]
+                                   : fresh < count ? taken_page(p, top, before(s.taken, b) + fresh) : -1;
+        if (page >= 0) slot = (int64_t)page * p.page + position % p.page;
+      }
     }
     if (p.positions) p.positions[r] = position;
     if (p.slots) p.slots[r] = slot;

@@ -29,7 +29,7 @@ class Rows(NamedTuple):
     """The packed rows of a call's new tokens: sequence b's are ``offsets[b]`` to ``offsets[b + 1] - 1`` [B + 1], at the
     positions from ``held[b]`` on [B]; each row's position [tokens] (all int32) and its place in the cache [tokens] (int64:
     page times page_size, plus its place in the page; -1 without a page).  Rows behind the last sequence's have position 0 and
-    no place."""
+    no place, those past the 2^30 tokens that a sequence may hold position 2^30 and none."""
     offsets: torch.Tensor
     held: torch.Tensor
     positions: torch.Tensor

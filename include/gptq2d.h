@@ -425,8 +425,9 @@ int gptq2d_rotary(const void* x0, int64_t x0_outer, int64_t x0_token, int64_t x0
  * last one first; then the missing ones, in order, are taken from its top while there are pages.
  * With extend, the call's tokens (optional, NULL: not given): offsets[seqs + 1] (sums of request, at most `tokens`), held[seqs] (lengths
  * before), positions[tokens] and slots[tokens] (page number times page plus the place in it; -1 without a page) of the packed
- * rows; rows that no sequence has: 0 and -1.  work: 4-byte aligned, gptq2d_page_pool_workspace bytes (-1 for seqs it does
- * not take), of no use afterwards.  seqs width and tokens are below 2^31, seqs at most 2^24. */
+ * rows; rows that no sequence has: 0 and -1; those past a sequence's 2^30 tokens: 2^30 and -1.  work: 4-byte aligned,
+ * gptq2d_page_pool_workspace bytes (-1 for seqs it does not take), of no use afterwards.  seqs width and tokens are below 2^31,
+ * seqs at most 2^24. */
 int64_t gptq2d_page_pool_workspace(int64_t seqs);
 int gptq2d_page_pool(int32_t* table, int64_t seqs, int64_t width, int64_t table_stride, int32_t page, int64_t pages,
                      int32_t* owned, int32_t* lengths, int32_t* missing, int32_t* free, int32_t* left, const int32_t* request,
