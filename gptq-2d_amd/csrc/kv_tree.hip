@@ -4,42 +4,14 @@
 
 namespace {
 
-// Some columns a sequence (its nodes times the heads that share a kv head).  Bound by vector instructions, so they are shared or
-// done without:
-//   - two waves share a ring of blocks in LDS, each with 16 columns of its own: a block's words are brought to LDS once, some by
-//     each, and its 64 scales and zeros are prepared by one of them, one block ahead, two blocks in turn;
-//   - codes are not centred for bf16 (PLAIN): a nibble is an fp16 number as it lies, c 2^-24 or 16 c 2^-24 (subnormal), after one
-//     mask: five instructions a word of eight, not nine.  The 16 is divided out of the other operand (of the queries' elements and
-//     of the values' scales where e & 2), 2^24 out of the sums.  A key is then (q . c) s + z sum q and a value c s + z.  A query's
-//     element is so held to 2^-27 of the largest where that is coarser, and the values' scales may lie 2^4 less apart.  The
-//     matrix cores align products by the exponents that operands are written with, so such sums are good to some 17 bits (fp32
-//     results measured 1e-5 off that way, 2e-5 with scores of 30; 1e-7 and 2e-6 with centred codes): eight bits finer than bf16,
-//     not enough for fp16 and fp32.
+// Some columns a sequence (its nodes times the heads that share a kv head).  Bound by vector instructions, so they are shared: two
+// waves share a ring of blocks in LDS, each with 16 columns of its own.  A block's words are brought to LDS once, some by each,
+// and its 64 scales and zeros are prepared by one of them, one block ahead, two blocks in turn.  Operands are attend_kernel's.
 // One barrier a block: after it, the stage that was read in the turn before is loaded again.  A workgroup has two rings, with
 // every second block each, whose results are joined at the end; four workgroups a CU.
 // Of up to 16 columns a sequence a ring has one wave (COLS): 64 sequences of 2 nodes and up to 8000 tokens 90 us (with two, one of
 // them without columns, 100), 100 of 4 nodes and 1000 46 (54).
 constexpr int RINGS = 2;
-
-template <bool PLAIN>
-__device__ __forceinline__ half8 codes_of(unsigned w) {
-  if constexpr (!PLAIN) return centred_codes(w);
-  union {
-    half2v h[4];
-    half8 v;
-  } r;
-  const unsigned x = w >> 8;
-  r.h[0] = as_half2(w & 0x000f000fu);
-  r.h[1] = as_half2(w & 0x00f000f0u);
-  r.h[2] = as_half2(x & 0x000f000fu);
-  r.h[3] = as_half2(x & 0x00f000f0u);
-  return r.v;
-}
-// log2 of what a code is held times, and of the 16 of every second pair.
-template <bool PLAIN>
-constexpr int CODE = PLAIN ? -24 : 0;
-template <bool PLAIN>
-constexpr int FOLD = PLAIN ? 4 : 0;
 
 template <int ND, int COLS>
 struct Shared {
@@ -57,31 +29,8 @@ __device__ __forceinline__ void wait_turn(int ct) {
     wait_loads<(R::S - 2) * R::LOADS[1]>();
 }
 
-// As query_operands, with the codes' 16 divided out.
-template <bool PLAIN, int TYPE, int ND, int QP>
-__device__ __forceinline__ void shared_operands(half8 (&q)[2 * ND][QP], float& sum, const Raw8<TYPE> (&x)[2 * ND], int ex) {
-  float total = 0.f;
-#pragma unroll
-  for (int s = 0; s < 2 * ND; ++s) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int fold = e & 2 ? FOLD<PLAIN> : 0;
-      const float v = __builtin_ldexpf(x[s][e], -ex - fold), times = (float)(1 << fold);
-      const _Float16 h = (_Float16)v;
-      q[s][0][e] = h;
-      total = __builtin_fmaf((float)h, times, total);
-      if constexpr (QP == 2) {
-        const _Float16 l = (_Float16)(v - (float)h);
-        q[s][1][e] = l;
-        total = __builtin_fmaf((float)l, times, total);
-      }
-    }
-  }
-  sum = quad_sum(total);
-}
-
-template <bool PLAIN, int ND, int QP, int PP>
-__device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[2 * ND][QP], const float (&qsum)[1],
+template <int ND, int QP, int PP>
+__device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[1][2 * ND][QP], const float (&qsum)[1],
                                              const char* stage, const float (*aff)[32], bool mask, int key0,
                                              const Column (&col)[1], int window, int len, int shift, bool apart, bool uneven,
                                              int down) {
@@ -95,9 +44,9 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
 #pragma unroll
     for (int i = 0; i < 4 * ND; ++i) {
       const int W = i / 2 + i % 2 * (2 * ND);  // the two tiles of keys in turn
-      const half8 k = codes_of<PLAIN>(w[W / 4][W % 4]);
+      const half8 k = centred_codes(w[W / 4][W % 4]);
 #pragma unroll
-      for (int p = 0; p < QP; ++p) s[0][i % 2] = mfma(k, q[i / 2][p], s[0][i % 2]);
+      for (int p = 0; p < QP; ++p) s[0][i % 2] = mfma(k, q[0][i / 2][p], s[0][i % 2]);
     }
   }
   float a0[8], a1[8], e[1][8];
@@ -117,8 +66,8 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
     for (int i = 0; i < 8; ++i) s[0][i / 4][i % 4] = __builtin_ldexpf(s[0][i / 4][i % 4], down);
   }
   exponents<true, ND, 1>(st, e, s, a0, a1, qsum, mask, key0, col, window, len, shift, apart, [&](int i) {
-    const float x = aff[2][16 * (i / 4) + 4 * g + i % 4];  // s 2^(ROOM - shift), less the codes' 16
-    return x > 0.f ? exponent_of(x) + 1 - ROOM + shift + (i & 2 ? FOLD<PLAIN> : 0) : -1000;
+    const float x = aff[2][16 * (i / 4) + 4 * g + i % 4];  // s 2^(ROOM - shift)
+    return x > 0.f ? exponent_of(x) + 1 - ROOM + shift : -1000;
   });
   half8 p[1][PP];
   read(a0, 2);
@@ -129,7 +78,7 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
   for (int i = 0; i < ND; ++i) w[i] = *reinterpret_cast<const uint4v*>(stage + 1024 * (ND + i) + 16 * lane);
 #pragma unroll
   for (int W = 0; W < 4 * ND; ++W) {
-    const half8 v = codes_of<PLAIN>(w[W / 4][W % 4]);
+    const half8 v = centred_codes(w[W / 4][W % 4]);
 #pragma unroll
     for (int r = 0; r < PP; ++r) st.o[0][W] = mfma(v, p[0][r], st.o[0][W]);
   }
@@ -309,7 +258,6 @@ shared_kernel(KvCache c, Attend a) {
   typedef typename Elem<TYPE>::T T;
   typedef Shared<ND, COLS> R;
   constexpr int SWAVES = COLS * RINGS, CT = 16 * COLS, DP = 64 * ND, QP = TYPE == TYPE_F32 ? 2 : 1, PP = TYPE == TYPE_BF16 ? 1 : 2, S = R::S;
-  constexpr bool PLAIN = TYPE == TYPE_BF16;
   alignas(16) __shared__ char ring[RINGS][S][R::STAGE];
   __shared__ float aff[RINGS][2][4][32];  // scale and zero of keys (times what scores share), of values
   __shared__ int shifts[RINGS][2];        // and whether columns part in the lowest bit
@@ -369,7 +317,7 @@ shared_kernel(KvCache c, Attend a) {
   // One exponent for all columns of the workgroup; a wave with a column whose largest element is 2^EVEN below the largest of all
   // gives each its own, and takes its scores to the common one.
   Raw8<TYPE> x[1][2 * ND];
-  half8 q[2 * ND][QP];
+  half8 q[1][2 * ND][QP];
   float top[1], qsum[1];
   read_queries<TYPE, ND, 1>(x, top, rows, {valid}, c.dim);
   float most = top[0];
@@ -383,7 +331,7 @@ shared_kernel(KvCache c, Attend a) {
   int down = top[0] > 0.f ? exponent_of(top[0]) - 14 - common : 0;
   const bool uneven = __builtin_amdgcn_ballot_w64(down < -EVEN);
   down = uneven ? down : 0;
-  shared_operands<PLAIN, TYPE, ND, QP>(q, qsum[0], x[0], common + down);
+  query_operands<TYPE, ND, 1, QP>(q, qsum, x, {common + down});
   qsum[0] = __builtin_ldexpf(qsum[0], down);
   const float factor = __builtin_ldexpf(a.scale, common);
   State<ND, 1> st;
@@ -393,7 +341,7 @@ shared_kernel(KvCache c, Attend a) {
   auto prepare = [&](int kb, int stage, int buf) {  // lanes 0..31 the keys, 32..63 the values
     const unsigned affine = *reinterpret_cast<const unsigned*>(ring[mine][stage] + 2048 * ND + 4 * lane);
     const unsigned w = (there >> stage & 1u) && kb * 32 + (lane & 31) < len ? affine : FLAT;  // beyond the sequence: whatever the page holds
-    const float s = __uint_as_float(w << 16), zero = __uint_as_float(w & 0xffff0000u), z = PLAIN ? zero : __builtin_fmaf(8.f, s, zero);
+    const float s = __uint_as_float(w << 16), z = __builtin_fmaf(8.f, s, __uint_as_float(w & 0xffff0000u));
     const bool real = lane >= 32 && s > 0.f && s < __builtin_inff();  // -0, infinities and NaN are of no matter
     const int ex = real ? exponent_of(s) + 1 : held;                  // s in [2^(ex - 1), 2^ex), subnormal or not
     if (__builtin_amdgcn_ballot_w64((unsigned)(held - ex) >= (unsigned)(held - least))) {
@@ -411,10 +359,9 @@ shared_kernel(KvCache c, Attend a) {
       }
     }
     float(*const to)[32] = aff[mine][buf];
-    to[lane >> 5 << 1][lane & 31] = lane < 32 ? __builtin_ldexpf(s * factor, -CODE<PLAIN>)
-                                                  : __builtin_ldexpf(s, ROOM - held - (lane & 2 ? FOLD<PLAIN> : 0));
+    to[lane >> 5 << 1][lane & 31] = lane < 32 ? s * factor : __builtin_ldexpf(s, ROOM - held);
     to[(lane >> 5 << 1) + 1][lane & 31] = lane < 32 ? z * factor : z;
-    if (lane == 0) shifts[mine][buf] = 2 * held + (least < held - SPREAD<PP> + FOLD<PLAIN>);
+    if (lane == 0) shifts[mine][buf] = 2 * held + (least < held - SPREAD<PP>);
   };
   if (ct == 0 && count) {
     if (S - 1 <= count)
@@ -442,7 +389,7 @@ shared_kernel(KvCache c, Attend a) {
       const int staged = __builtin_amdgcn_readfirstlane(shifts[mine][i % 2]), shift = staged >> 1;
       const bool page = there >> buf & 1u;
       const bool mask = !page || kb * 32 + 31 > all_to || kb * 32 < all_from;
-      shared_block<PLAIN, ND, QP, PP>(st, q, qsum, ring[mine][buf], aff[mine][i % 2], mask, kb * 32 + 4 * g, place, a.window,
+      shared_block<ND, QP, PP>(st, q, qsum, ring[mine][buf], aff[mine][i % 2], mask, kb * 32 + 4 * g, place, a.window,
                                page ? len : 0, shift, staged & 1, uneven, down);
     }
     buf = next;
@@ -454,7 +401,7 @@ shared_kernel(KvCache c, Attend a) {
 #pragma unroll
   for (int d = 0; d < 4 * ND; ++d)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) st.o[0][d][i] = __builtin_ldexpf(st.o[0][d][i], st.shift[0] - ROOM - CODE<PLAIN>) + z;
+    for (int i = 0; i < 4; ++i) st.o[0][d][i] = __builtin_ldexpf(st.o[0][d][i], st.shift[0] - ROOM) + z;
   floatx4* const other = reinterpret_cast<floatx4*>(&ring[1][0][0]) + ct * (4 * ND * 64);
   __syncthreads();
   if (mine == 1) {

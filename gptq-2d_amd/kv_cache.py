@@ -137,8 +137,7 @@ class KVCache4:
 
         ``tree``: the sequences' last tokens are the nodes of a `drafts.DraftTree` of the same ``offsets``, made with ``held`` =
         ``lengths[b]`` less the nodes. Each sees the tokens before the nodes -- with ``window``, which holds the tree's
-        `nodes` at least, the last `window` up to its own position -- and the nodes that it comes from. For bf16 a query's
-        elements then count to 2^-27 of its largest where that is coarser, scores and sums of values to some 17 bits."""
+        `nodes` at least, the last `window` up to its own position -- and the nodes that it comes from."""
         if q.dim() != 3 or q.size(1) % self.kv_heads or q.size(1) == 0:
             raise ValueError(f"q must be [tokens, heads, {self.head_dim}], heads a multiple of {self.kv_heads}")
         tokens, heads, dim = q.shape

@@ -365,8 +365,7 @@ int gptq2d_draft_accept(const int32_t* parents, const int32_t* offsets, int64_t 
 
 /* gptq2d_kv_attend of the nodes, that the cache holds as the last tokens (node i at length - T_b + i): each sees the tokens held
  * before them (with window > 0 those of positions > positions[row] - window), the nodes of its `ancestors` and no others.
- * window: 0, or at least `nodes`.  For bf16, a query's elements to 2^-27 of its largest where that is coarser, and scores and
- * sums of values to some 17 bits of their terms. */
+ * window: 0, or at least `nodes`. */
 int64_t gptq2d_kv_attend_tree_workspace(int64_t tokens, int64_t seqs, int32_t heads, int32_t group, int32_t dim, int64_t most,
                                         int64_t window, int64_t nodes);
 int gptq2d_kv_attend_tree(const void* pages, int64_t page_count, int32_t heads, int32_t dim, int32_t page, const void* q,
