@@ -84,6 +84,14 @@ class KVCache4:
             raise ValueError(f"{name} must be on the cache's device")
         return x if x.stride(2) == 1 or self.head_dim == 1 else x.contiguous()
 
+    # Refuses a tree that is not of the call's sequences; a block asks before it appends.
+    def _fits(self, tree, offsets, seqs, tokens, window):
+        if offsets is None or tree.seqs != seqs or tree.tokens != tokens or tree.device != self.device:
+            raise ValueError(f"the tree is one of {tree.tokens} tokens of {tree.seqs} sequences on {tree.device}, and takes "
+                             f"their offsets")
+        if window and window < tree.nodes:
+            raise ValueError(f"a window holds the tree's {tree.nodes} nodes at least")
+
     def _call(self, fn, name, *args):
         index = self.device.index
         if torch.cuda.current_device() == index:
@@ -151,11 +159,7 @@ class KVCache4:
         group, window = heads // self.kv_heads, window or 0
         name, nodes, of_tree = "attend", (), ()
         if tree is not None:
-            if offsets is None or tree.seqs != where[1] or tree.tokens != tokens or tree.device != self.device:
-                raise ValueError(f"the tree is one of {tree.tokens} tokens of {tree.seqs} sequences on {tree.device}, and takes "
-                                 f"their offsets")
-            if window and window < tree.nodes:
-                raise ValueError(f"a window holds the tree's {tree.nodes} nodes at least")
+            self._fits(tree, offsets, where[1], tokens, window)
             name, nodes = "attend_tree", (tree.nodes,)
             of_tree = (tree.ancestors.data_ptr(), tree.positions.data_ptr(), tree.nodes)
         out = torch.empty(tokens, heads, dim, dtype=q.dtype, device=self.device)

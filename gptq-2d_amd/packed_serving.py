@@ -92,6 +92,8 @@ class PackedAttention:
                 raise ValueError(f"{name} has {layer.words.size(0)} rows, its heads take {rows}")
         if out.columns not in (None, heads * dim):
             raise ValueError(f"out has {out.columns} columns, the heads give {heads * dim}")
+        if window is not None and not 1 <= window < 1 << 30:
+            raise ValueError("a window holds at least one token, and fewer than 2^30")
         if rotary is not None and (rotary.dim != dim or rotary.device != cache.device):
             raise ValueError(f"the rotation is of {rotary.dim} elements on {rotary.device}, the cache's heads are {dim} on {cache.device}")
         self.q, self.k, self.v, self.out, self.cache, self.heads, self.window = q, k, v, out, cache, heads, window
@@ -106,6 +108,8 @@ class PackedAttention:
         nodes of this tree, made with the same ``held`` and ``offsets``.  ``positions`` [tokens] of the rotation (int32 or int64):
         the tree's, or those that follow what is held, where they are not given."""
         of, dim = adapters or {}, self.cache.head_dim
+        if tree is not None:  # what attention would refuse, before the cache has the tokens
+            self.cache._fits(tree, offsets, table.size(0), x.size(0), self.window)
         q = self.q(x, of.get("q"), index).unflatten(-1, (self.heads, dim))
         k = self.k(x, of.get("k"), index).unflatten(-1, (self.cache.kv_heads, dim))
         v = self.v(x, of.get("v"), index).unflatten(-1, (self.cache.kv_heads, dim))
