@@ -540,13 +540,19 @@ inline TreePlan make_tree_plan(int64_t tokens, int64_t seqs, int heads, int grou
   const int64_t columns = tokens * group, tiles = cdiv(columns, 32) > seqs ? cdiv(columns, 32) : seqs;
   const int64_t total = p.blocks * tiles * heads;
   // Few columns, and fewer blocks than workgroups of shared_kernel fit at once: the call is its start, which attend_kernel's waves,
-  // each alone, do sooner (8 kv heads of 128, 4 heads each, us of both kernels and the join, attend and shared: 7 nodes of one
-  // sequence of 100 tokens 11 and 15, of 1000 14 and 16, of 8000 21 and 21; of 4 of 1000 19 and 17, of 32 of 300 36 and 20, of
-  // 16 of 4000 55 and 39; where pieces are listed, 2 nodes of 65 of 100 18 and 21, of 100 of 100 21 and 21, 4 of 100 of 300 42 and
-  // 29).  Many columns and more blocks than fit at a time: prompt_kernel, which brings codes to fp16 once for 128 columns (prompt
-  // and shared: 24 nodes of 100 tokens 21 and 14; 128 of 1000 36 and 23, of 4000 48 and 39, of 8 of 300 46 and 39, of 16 of 300 50
-  // and 68; 96 of 16 of 2000 122 and 151; 32 of 64 of up to 8000 573 and 332, 64 of those 638 and 587).
-  p.shared = p.prompt ? columns < 384 * seqs || total < 16384 : total >= (seqs > 64 ? 4096 : 1024);
+  // each alone, do sooner (bf16, 8 kv heads of 128, 4 heads each, us of all kernels, attend and shared: 7 nodes of one sequence of
+  // 100 tokens 10 and 15, of 1000 14 and 16, of 8000 23 and 23; of 4 of 1000 19 and 17, of 32 of 300 37 and 21, of 16 of 4000 56
+  // and 44; where pieces are listed, 2 nodes of 65 of 100 18 and 21, of 100 of 100 22 and 23, 4 of 100 of 300 43 and 30).  Up to 8
+  // columns a sequence attend_kernel is ahead of more work too where lengths are alike (2 nodes of one of 8000 16 and 20, of 100 of
+  // 4000 123 and 140, of 256 of 2000 149 and 170), which a call does not know, and behind where they differ (300 to 8000: 64
+  // sequences 122 and 94, 100 165 and 142, 256 365 and 331; 300 to 4000: 65 63 and 73, 256 193 and 187).
+  // Many columns and more blocks than fit at a time: prompt_kernel, which brings codes to fp16 once for 128 columns (shared and
+  // prompt: 24 nodes of 100 tokens 14 and 20; 128 of 1000 25 and 36, of 4000 42 and 47, of 8 of 300 43 and 46, of 16 of 300 73 and
+  // 50; of 64 of up to 8000 32 366 and 560, 48 538 and 597, 64 697 and 603, 80 838 and 757; of 16 of 2000 48 92 and 112, 64 117 and
+  // 115, 80 141 and 116; 32 of 4 of 131000, 8 heads each, 1151 and 989.  fp16 and fp32 64 of 16 of 2000 128 and 141, 142 and 154, else
+  // alike).  Heads past 128 leave it a wave a SIMD (of 256, 16 of 3000: 64 nodes 300 and 490, 96 414 and 502).
+  const int64_t many = p.nd <= 2 ? 256 : 384;
+  p.shared = p.prompt ? columns < many * seqs || total < 16384 : total >= (seqs > 64 ? 4096 : 1024);
   if (!p.shared) return p;
   p.prompt = false;
   p.ct = columns <= 16 * seqs ? 16 : 32;

@@ -19,7 +19,7 @@ def plan(tokens, seqs, heads, group, dim, most, window=0, nodes=0):
     if nodes:
         wide = max(cdiv(columns, 32), seqs)
         total = blocks * wide * heads
-        if columns < 384 * seqs or total < 16384 if prompt else total >= (4096 if seqs > 64 else 1024):
+        if columns < (256 if nd <= 2 else 384) * seqs or total < 16384 if prompt else total >= (4096 if seqs > 64 else 1024):
             cols = 16 if columns <= 16 * seqs else 32
             tiles, chunks = columns // cols + seqs, 3 * 1024 // heads + 1
             listed = 4 * (1 + 2 * tiles + chunks) if seqs > 64 else 0
