@@ -96,7 +96,8 @@ __device__ __forceinline__ unsigned* kv_head(const KvCache& c, int64_t b, int kb
   const int p = (int)__umulhi((unsigned)kb, c.mag);
   at = kb - p * c.blocks;
   if (c.blocks == 1) at = 0;
-  // a uniform index: through the scalar data cache (no kernel writes the table), whose loads wait for no others
+  // A uniform index: through the scalar data cache, whose loads wait for no others and which sees no store of its own launch.  No
+  // kernel that calls this writes the table; what does (page_pool.hip) is a launch before, and a launch begins with that cache empty.
   typedef const __attribute__((address_space(4))) int32_t* scalar;
   const int64_t id = ((scalar)(c.table + b * c.table_stride))[__builtin_amdgcn_readfirstlane(c.blocks == 1 ? kb : p)];
   if (id < 0 || id >= c.page_count) return nullptr;

@@ -9,8 +9,8 @@ namespace {
 // and its 64 scales and zeros are prepared by one of them, one block ahead, two blocks in turn.  Operands are attend_kernel's.
 // One barrier a block: after it, the stage that was read in the turn before is loaded again.  A workgroup has two rings, with
 // every second block each, whose results are joined at the end; four workgroups a CU.
-// Of up to 16 columns a sequence a ring has one wave (COLS): 64 sequences of 2 nodes and up to 8000 tokens 90 us (with two, one of
-// them without columns, 100), 100 of 4 nodes and 1000 46 (54).
+// Of up to 16 columns a sequence a ring has one wave (COLS): 64 sequences of 2 nodes and up to 8000 tokens 99 us (with two, one of
+// them without columns, 111), 100 of 4 nodes and 1000 51 (60).
 constexpr int RINGS = 2;
 
 template <int ND, int COLS>
@@ -85,13 +85,13 @@ __device__ __forceinline__ void shared_block(State<ND, 1>& st, const half8 (&q)[
 }
 
 // How a call's work is dealt.  A sequence has a tile for every CT (32 or 16) of its columns, and its keys are cut into as many
-// chunks as the lengths that there are make right, whatever the table has room for (64 sequences of 8 nodes, up to 8000 tokens,
-// 115 us; chunks made for a table of room for 32768 178); a piece is a chunk of a tile.  Pieces lie side by side, a chunk's tiles
-// next to each other, and the workgroups without one behind them: neighbours are dealt to an XCD's shader engines in turn, and
-// engines without work are what pieces that may or may not be there lead to (every second one of no columns 185 us; 64 empty
-// sequences at the end 163, so 119).  Up to 64 sequences every workgroup looks at all of them, a lane each, and finds its own
-// piece; more are looked at by one workgroup beforehand, which lists the pieces (some 5 us a call; done by every workgroup, 256
-// sequences 192 us for 141, 4096 8.6 ms for 0.65).
+// chunks as the lengths that there are make right, whatever the table has room for (chunks made for a table's room, four times the
+// longest of 64 sequences: half as long again); a piece is a chunk of a tile.  Pieces lie side by side, a chunk's tiles next to each
+// other, and the workgroups without one behind them: neighbours are dealt to an XCD's shader engines in turn, and engines without
+// work are what pieces that may or may not be there lead to (every second one of no columns: 1.7 times the time; 64 empty sequences
+// behind 64 others: 1.4).  Up to 64 sequences every workgroup looks at all of them, a lane each, and finds its own piece; more are
+// looked at by one workgroup beforehand, which lists the pieces (some 5 us a call; done by every workgroup, 256 sequences take 1.4
+// times as long, 4096 13 times).
 struct Work {
   bool any;
   int tile, tiles, chunk, chunks;  // of the sequence: the tile, how many; the chunk, how many
@@ -102,7 +102,7 @@ struct Work {
 
 // Three rounds of the workgroups that fit at once.  Of less work than makes chunks of 32 blocks so, whose starts and joining take
 // longer than uneven ends, half a round, of still less chunks of 8 or a quarter of a round; two blocks a ring at least (a round:
-// 32 sequences of 300 tokens, 7 nodes, 32 heads of 128, 25 us, so 20, 32 of 1000 34 and 31).  `total`: blocks of all tiles and heads.
+// 32 sequences of 300 tokens, 7 nodes, 32 heads of 128, 26 us, so 21, 32 of 1000 36 and 34).  `total`: blocks of all tiles and heads.
 constexpr int ROUND = 1024;  // four a CU
 __device__ __forceinline__ int chunk_size(float total) {
   const int thirds = 1 + (int)(total * (1.0001f / (3 * ROUND))), half = (int)(total * (2.f / ROUND));
@@ -251,7 +251,7 @@ __device__ __forceinline__ void clear_idle(const KvCache& c, const Attend& a, in
 }
 
 // (Workgroups a CU as registers are dealt: with one column tile four, as there is LDS for, made the compiler move sums to and fro,
-// 93 us for 89 with 64 sequences of 2 nodes.)
+// 104 us for 99 with 64 sequences of 2 nodes.)
 template <int TYPE, int ND, int COLS>
 __global__ __launch_bounds__(64 * COLS * RINGS, COLS == 1 ? 2 : ND <= 2 && TYPE != TYPE_F32 ? 4 : ND <= 2 ? 3 : 2) void
 shared_kernel(KvCache c, Attend a) {
@@ -449,9 +449,9 @@ shared_kernel(KvCache c, Attend a) {
 }
 
 // Joins the chunks' results of shared_kernel: a workgroup 8 columns of a tile and head, a wave's loads of 16 chunks on their way at
-// once: of few tiles, that many chunks share, it is the joining that is waited for.  One sequence of 8000 tokens, 7 nodes, 32 heads
-// of 128: both kernels 24 us (a workgroup all 32 columns, 4 loads at once: 34), of 32 nodes and 64 heads 37 (42), 4 of 131000 274
-// (294), 64 of up to 8000 111 (110).
+// once: of few tiles, that many chunks share, it is the joining that is waited for.  All kernels, bf16, 8 kv heads of 128, 4 heads
+// each (in brackets: a workgroup all 32 columns, 4 loads at once): 7 nodes of one sequence of 8000 tokens 22 us (28), of 4 of 131000
+// 220 (230), 8 of 64 of up to 8000 127 (126); 8 heads each, 32 of one of 8000 42 (44).
 constexpr int CJ = 8;
 template <int TYPE, int ND, int CT>
 __global__ __launch_bounds__(THREADS) void join_tile_kernel(KvCache c, Attend a) {

@@ -11,7 +11,8 @@
 //
 // Bound by latency.  Up to SMALL rows and sequences one workgroup does it all, with the sums in LDS; more take a second
 // launch, between the pages that come back and those that go out, and every workgroup of the first sums for itself.  No
-// kernel waits for another workgroup.
+// kernel waits for another workgroup.  The cache's kernels read the table in a way that sees earlier launches only (kv_head of
+// kv_cache.h): pages are dealt in launches of their own.
 #include "common.h"
 
 namespace {

@@ -4,8 +4,9 @@
 //   y1 = a (x1 cos t - x2 sin t),  y2 = a (x2 cos t + x1 sin t);  its transpose turns by -t.
 // The elements from r on are passed on.
 //
-// Frequencies are held as turns a position, in fp64: the product with a position of up to 2^31 leaves the fraction of a turn
-// good to 2^-53 of the turns made, where fp32 would leave nothing of far positions.  The fraction is brought to an eighth of
+// Frequencies are held as turns a position, in fp64: the product with a position leaves the fraction of a turn good to 2^-51 of
+// the turns made (three roundings, the frequency's among them: 10^-6 of a radian at a position of 2^31 and f_i = 1), where fp32 would
+// leave nothing of far positions.  The fraction is brought to an eighth of
 // a turn around the nearest quarter, exactly, and only then rounded to fp32, for which the Taylor series of sine (to x^9) and
 // cosine (to x^10) are good to 2^-28.  So an angle costs some 40 instructions and no memory (a table of 131072 positions and
 // 64 pairs is 64 MB, and as many reads a head's worth each token).

@@ -42,7 +42,9 @@ class PagePool:
     The state, on the device, all int32: ``table`` [seqs, width] (-1: no page), ``lengths`` [seqs] (tokens held), ``owned``
     [seqs] (pages, the first entries of the row), ``missing`` [seqs] (pages that the last call had none left for), ``free``
     [pages] and ``left`` [1] (the stack, and its height).  It is written by the calls alone, in the order of the stream that they
-    are made on.  Tokens past a sequence's last entry count in its length and have no place."""
+    are made on.  Tokens past a sequence's last entry count in its length and have no place; a page that it gets
+    later holds nothing of them, so a sequence with pages missing is taken back (`resize`) to what it has pages for, or those
+    tokens are appended again."""
 
     def __init__(self, pages: int, seqs: int, width: int, *, page_size: int = 64, device: torch.device | str = "cuda"):
         if not (0 <= pages < 1 << 31 and 0 <= seqs <= 1 << 24 and 0 <= width and seqs * width < 1 << 31 and width < 1 << 31 and

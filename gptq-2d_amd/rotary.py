@@ -6,8 +6,8 @@ turned by position times f_i:
     y1 = a (x1 cos t - x2 sin t),   y2 = a (x2 cos t + x1 sin t),   t = position f_i,   f_i = base^(-2 i / rotated)
 
 and the elements behind them are passed on.  Frequencies may be scaled for contexts longer than a model was trained on
-(`Linear`, `Ntk`, `Bands`, `Yarn`; a is 1 but for the last).  Angles are formed in 64 bits, so that far positions are as good
-as near ones; sums are in 32 bits and rounded once.
+(`Linear`, `Ntk`, `Bands`, `Yarn`; a is 1 but for the last).  Angles are formed in 64 bits: t is off by 2^-51 |t| at most, 10^-6 at
+2^31, before its sine and cosine are rounded to 32 bits.  Sums are in 32 bits and rounded once.
 
     rotary = Rotary(128, base=500000., scaling=Bands(8., context=8192))
     q, k = rotary(q, k, positions=positions)        # one launch; differentiable in q and k
@@ -128,7 +128,8 @@ class Rotary:
     def __call__(self, *xs: torch.Tensor, positions: torch.Tensor):
         """One or two tensors (queries, keys) [..., heads, dim] of one type (fp32, bf16 or fp16) rotated, each with its own
         number of heads, any strides.  ``positions`` (int32 or int64) broadcasts to their leading axes, of which there are one
-        or two ([tokens], [batch, tokens]); a position may be negative and counts to 2^53."""
+        or two ([tokens], [batch, tokens]); a position may be negative, and is held as it is up to 2^53, where the angle of a fast pair
+        is off by more than a radian."""
         if not 1 <= len(xs) <= 2:
             raise ValueError("one or two tensors are rotated in a call")
         lead, kind, device, grad = xs[0].shape[:-2], xs[0].dtype, self.device, False
